@@ -18,7 +18,7 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libgadeon_hip.so"
 
 GD_OK, GD_EINVAL, GD_ENODEV, GD_ENOMEM, GD_ELAUNCH, GD_EHIP, GD_ESTOPPED = 0, -1, -2, -3, -4, -5, -6
-F32, F16 = 0, 1
+F32, F16, I8 = 0, 1, 2
 
 _vp, _i, _i64, _u64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_size_t
 _fp = C.POINTER(C.c_float)
@@ -29,6 +29,18 @@ class Q2W(C.Structure):
     _fields_ = [("codes", _vp), ("scales", _vp), ("K", _i64), ("R", _i64)]
 
 
+class KV(C.Structure):
+    """A paged KV cache of one attention layer (gd_kv)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_exp", _vp), ("v_exp", _vp), ("n_pages", _i64),
+                ("dtype", _i), ("n_head_kv", _i), ("head_dim", _i), ("page_size", _i)]
+
+
+class Seqs(C.Structure):
+    """The rows of a call over many sequences, arrays in device memory (gd_seqs)."""
+    _fields_ = [("n_rows", _i64), ("row_start", _vp), ("pos", _vp), ("rope_shift", _vp),
+                ("page_table", _vp), ("n_seq", _i), ("max_pages", _i), ("max_len", _i)]
+
+
 class StackConfig(C.Structure):
     _fields_ = [(n, _i) for n in ("n_layer", "n_embd", "n_ff", "n_head", "n_head_kv", "head_dim",
                                   "n_rot")] + [("rope_base", _f), ("eps", _f)] + \
@@ -37,6 +49,7 @@ class StackConfig(C.Structure):
 
 
 _Q2WP = C.POINTER(Q2W)
+_KVP, _SEQSP = C.POINTER(KV), C.POINTER(Seqs)
 
 # name -> (restype, argtypes)
 _PROTOS = {
@@ -84,6 +97,12 @@ _PROTOS = {
                            _i, _i]),
     "gd_attn_batch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i64,
                            _i, _i]),
+    "gd_kv_alloc": (_i, [_vp, _i, _i, _i, _i, _i64, _KVP]),
+    "gd_kv_free": (_i, [_vp, _KVP]),
+    "gd_kv_append_rope": (_i, [_vp, _KVP, _SEQSP, _vp, _i64, _vp, _i, _vp, _i64, _vp, _i64, _i, _i,
+                               _f]),
+    "gd_kv_read": (_i, [_vp, _KVP, _SEQSP, _vp, _vp, _i]),
+    "gd_kv_attn": (_i, [_vp, _KVP, _SEQSP, _vp, _i64, _vp, _i64, _vp, _i, _i, _f, _i, _i]),
     "gd_gdn_gate": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64]),
     "gd_gdn_conv": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i64]),
     "gd_l2norm_rows": (_i, [_vp, _vp, _i, _i, _i64, _i64, _f]),

@@ -1,0 +1,626 @@
+// The paged KV cache of many sequences: appending rows with the rotation on the
+// way, reading rows back, and attention with a sliding window and sinks, over f16
+// values or 8-bit codes with a scale for each block of 16 positions and kv head.
+//
+// The reference serves one conversation at a time (MetalEnc.ropeBatch,
+// kvAppendBatch, attnPaged and attnBatch, MetalEnc.swift:560-706, 817-1025) and
+// keeps half pages; its attnBatch takes a window for another model family.  Here a
+// call serves the rows of many sequences (gd_seqs), each with a page table of its
+// own, as the batched GDN step does.
+//
+// Cache types:
+//   GD_F16: [page][slot][n_head_kv][head_dim], what gd_kv_append writes.
+//   GD_I8:  codes [page][n_head_kv][slot][head_dim] and, for each 16 slots of a
+//           head, one byte e + 127: a code c stands for c 2^e.  e is the least of
+//           -24 .. 9 that holds the block's largest value within 127 steps, so the
+//           type spans f16's range and every value it holds is an f16 exactly.
+#include "gd_internal.h"
+
+#include <algorithm>
+#include <math.h>
+
+namespace {
+
+constexpr int BLK = GD_KV_BLOCK;                 // positions of a scale
+constexpr int EXP_BIAS = 127;                    // of a stored exponent (an f32's)
+constexpr int EXP_MIN = -24, EXP_MAX = 9;        // f16's least step; 127 2^9 < f16's largest
+constexpr int EXP_NAN = 255;                     // a block that took a NaN: every value NaN
+
+// n / d for 0 <= n < 2^31 (d > 0) by a high product: q = (mulhi(mul, n) + n) >> shift.
+struct FastDiv {
+    uint32_t mul, shift;
+    explicit FastDiv(uint32_t d) {
+        shift = 0;
+        while (((uint64_t)1 << shift) < d) shift++;
+        mul = (uint32_t)(((((uint64_t)1 << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(mul, n) + n) >> shift; }
+};
+
+// What the kernels need of a gd_kv and a gd_seqs.  Page tables, positions and row
+// starts are device data: nothing here trusts them with an address.
+struct Cache {
+    void *k, *v;
+    uint8_t *kx, *vx;
+    uint32_t n_pages;
+    int HKV, P;
+    FastDiv by_page;
+};
+struct Rows {
+    const int32_t *row_start, *pos, *shift, *table;
+    int n_rows, n_seq, max_pages;
+    uint32_t cap;                                // positions that the tables hold
+};
+
+// Rows [r0, r1) of sequence b, the first at position pos (r0 = r1 where it is idle).
+struct Seq {
+    int r0, r1, pos;
+};
+__device__ __forceinline__ Seq seq_at(const Rows &s, int b) {
+    Seq q;
+    q.r0 = s.row_start ? min(max(s.row_start[b], 0), s.n_rows) : b;
+    q.r1 = s.row_start ? min(max(s.row_start[b + 1], q.r0), s.n_rows) : b + 1;
+    q.pos = s.pos[b];
+    if (q.pos < 0) q.r1 = q.r0;
+    return q;
+}
+
+// The sequence of row n, for the whole wave (-1: none).
+__device__ __forceinline__ int seq_of_row(const Rows &s, int n) {
+    if (!s.row_start) return n < s.n_seq ? n : -1;
+    const int lane = threadIdx.x & 63;
+    for (int c = 0; c < s.n_seq; c += 64) {
+        const int end = c + lane < s.n_seq ? s.row_start[c + lane + 1] : 0x7fffffff;
+        const int before = __popcll(__ballot(end <= n));
+        if (before < 64) return c + before < s.n_seq && n >= s.row_start[c + before] ? c + before : -1;
+    }
+    return -1;
+}
+
+// Unit u of the sequences' units, `count` of them each (count(Seq) lane by lane): its
+// sequence b and place k in it, for the whole wave.  False: fewer units than that.
+template <class F>
+__device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, int &b, int &k) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int c = 0; c < s.n_seq; c += 64) {
+        const int n = c + lane < s.n_seq ? count(seq_at(s, c + lane)) : 0;
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += o;
+        }
+        const uint64_t past = __ballot(base + sum > u);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            b = c + l;
+            k = u - (base + __shfl(sum - n, l, 64));
+            return k >= 0;
+        }
+        base += __shfl(sum, 63, 64);
+    }
+    return false;
+}
+
+// The page of position p of sequence b, -1 where there is none.
+__device__ __forceinline__ int page_of(const Cache &c, const Rows &s, int b, uint32_t p) {
+    if (p >= s.cap) return -1;
+    const int page = s.table[(int64_t)b * s.max_pages + c.by_page(p)];
+    return (uint32_t)page < c.n_pages ? page : -1;
+}
+__device__ __forceinline__ int slot_of(const Cache &c, uint32_t p) { return (int)(p - c.by_page(p) * c.P); }
+
+// Element offset of (page, slot, head) in a plane, and of its exponent.
+template <int HD> __device__ __forceinline__ int64_t f16_at(const Cache &c, int page, int slot, int h) {
+    return (((int64_t)page * c.P + slot) * c.HKV + h) * HD;
+}
+template <int HD> __device__ __forceinline__ int64_t i8_at(const Cache &c, int page, int slot, int h) {
+    return (((int64_t)page * c.HKV + h) * c.P + slot) * HD;
+}
+__device__ __forceinline__ int64_t exp_at(const Cache &c, int page, int slot, int h) {
+    return ((int64_t)page * c.HKV + h) * (c.P / BLK) + slot / BLK;
+}
+// 2^e of a stored exponent: 0 for a block never written, NaN for one that took a NaN.
+__device__ __forceinline__ float step_of(uint8_t x) {
+    return x == EXP_NAN ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)x << 23);
+}
+
+template <typename T> __device__ __forceinline__ float to_f32(T x);
+template <> __device__ __forceinline__ float to_f32(float x) { return x; }
+template <> __device__ __forceinline__ float to_f32(uint16_t x) { return gd_h2f(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32(float x) { return x; }
+template <> __device__ __forceinline__ uint16_t from_f32(float x) { return gd_f2h(x); }
+
+// A turned value, formed in 64 bits, as the row it would be in 32 (gd_rope's), in T.
+template <typename T> __device__ __forceinline__ T from_f64(double x) { return from_f32<T>((float)x); }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// ---------------------------------------------------------------- append
+
+// Turns per position of each rotated pair, as fractions of 2^64: the phase of
+// position p is p * turn[j] mod 2^64, without rounding whatever p is.
+struct Turns {
+    uint64_t t[128];
+};
+
+// Rotates and appends the rows that fall into one block of 16 positions of a
+// sequence (unit blockIdx.x), and turns its query rows: wave w of workgroup y takes
+// the heads 4 y + w of H query heads, then the kv heads' keys, then their values.
+// The cos and sin of the block's positions are formed once a workgroup, and rows turned,
+// in 64 bits: from turns in 32 one code in 40 000 came out on the other side of a
+// border, and one half in 700 a step off.
+template <int HD, bool I8, typename T>
+__global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, const T *q, int64_t q_stride, T *q_out,
+                                                int H, const T *kx, int64_t k_stride, const T *vx, int64_t v_stride,
+                                                int n_rot) {
+    constexpr int NP = HD / 128;                 // pairs of a lane
+    __shared__ double2 cs[BLK * (HD / 2)];
+    const int t = threadIdx.x, lane = t & 63, half = n_rot / 2;
+    int b, blk;
+    auto blocks = [](const Seq &q) {
+        return q.r1 > q.r0 ? (int)(((uint32_t)q.pos % BLK + (uint32_t)(q.r1 - q.r0) + BLK - 1) / BLK) : 0;
+    };
+    if (!unit_at(s, blockIdx.x, blocks, b, blk)) return;
+    const Seq sq = seq_at(s, b);
+    // The block's new rows: n of them from row r on, the first at slot `off` of it.
+    const int off = blk ? 0 : sq.pos % BLK;
+    const int skip = blk ? blk * BLK - sq.pos % BLK : 0;
+    const int r = sq.r0 + skip, n = min(BLK - off, sq.r1 - r);
+    const uint32_t p = (uint32_t)sq.pos + (uint32_t)skip;
+    const int64_t rp = (int64_t)p + (s.shift ? s.shift[b] : 0);
+    for (int i = t; i < n * half; i += 256) {
+        const int64_t turn = (int64_t)((uint64_t)(rp + i / half) * turns.t[i % half]);
+        double sn, cn;
+        sincospi((double)turn * 0x1p-63, &sn, &cn);
+        cs[i] = double2{cn, sn};
+    }
+    __syncthreads();
+    const int hs = blockIdx.y * 4 + (t >> 6);
+    if (hs >= H + 2 * c.HKV) return;
+    // Pair j of a head: the dims j and j + half, past the rotated ones two neighbours.
+    int d0[NP], d1[NP];
+#pragma unroll
+    for (int e = 0; e < NP; e++) {
+        const int j = lane + 64 * e;
+        d0[e] = j < half ? j : n_rot + 2 * (j - half);
+        d1[e] = j < half ? j + half : d0[e] + 1;
+    }
+    // Row i's pair e, turned where it is one of the rotated.
+    auto turned = [&](bool turn, int i, int e, float x0, float x1, double &a, double &z) {
+        a = x0, z = x1;
+        if (turn && lane + 64 * e < half && i < n) {
+            const double2 w = cs[i * half + lane + 64 * e];
+            const double o = a;
+            a = o * w.x - z * w.y;
+            z = o * w.y + z * w.x;
+        }
+    };
+    if (hs < H) {
+        for (int i = 0; i < n; i++) {
+            const T *x = q + (r + i) * q_stride + (int64_t)hs * HD;
+            T *y = q_out + ((int64_t)(r + i) * H + hs) * HD;
+#pragma unroll
+            for (int e = 0; e < NP; e++) {
+                double a, z;
+                turned(true, i, e, to_f32(x[d0[e]]), to_f32(x[d1[e]]), a, z);
+                y[d0[e]] = from_f64<T>(a);
+                y[d1[e]] = from_f64<T>(z);
+            }
+        }
+        return;
+    }
+    const bool is_k = hs < H + c.HKV;
+    const int h = hs - H - (is_k ? 0 : c.HKV);
+    const T *src = (is_k ? kx + r * k_stride : vx + r * v_stride) + (int64_t)h * HD;
+    const int64_t stride = is_k ? k_stride : v_stride;
+    void *plane = is_k ? c.k : c.v;
+    if (!I8) {
+        // A page may end inside the block.  Values past f16's range are held as its
+        // largest.
+        for (int i = 0; i < n; i++) {
+            const int page = page_of(c, s, b, p + i);
+            if (page < 0) continue;
+            uint16_t *y = (uint16_t *)plane + f16_at<HD>(c, page, slot_of(c, p + i), h);
+            auto f16_of = [](double x) { return from_f64<uint16_t>(x > 65504. ? 65504. : x < -65504. ? -65504. : x); };
+#pragma unroll
+            for (int e = 0; e < NP; e++) {
+                double a, z;
+                turned(is_k, i, e, to_f32(src[i * stride + d0[e]]), to_f32(src[i * stride + d1[e]]), a, z);
+                y[d0[e]] = f16_of(a);
+                y[d1[e]] = f16_of(z);
+            }
+        }
+        return;
+    }
+    const int page = page_of(c, s, b, p);
+    if (page < 0) return;
+    const int slot = slot_of(c, p);              // of the first new row; the block's is slot - off
+    float x0[BLK][NP], x1[BLK][NP];
+#pragma unroll
+    for (int i = 0; i < BLK; i++)
+#pragma unroll
+        for (int e = 0; e < NP; e++) {
+            x0[i][e] = i < n ? to_f32(src[i * stride + d0[e]]) : 0.f;
+            x1[i][e] = i < n ? to_f32(src[i * stride + d1[e]]) : 0.f;
+        }
+    float top = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < BLK; i++)
+#pragma unroll
+        for (int e = 0; e < NP; e++) {
+            double a, z;
+            turned(is_k, i, e, x0[i][e], x1[i][e], a, z);
+            top = fmaxf(top, fmaxf(fabsf((float)a), fabsf((float)z)));
+            nan |= a != a || z != z;
+        }
+    top = wave_max(top);
+    const uint32_t bits = __float_as_uint(top);
+    int ex = (int)(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u);   // 127 2^ex holds top
+    ex = min(max(ex, EXP_MIN), EXP_MAX);
+    uint8_t *xp = (is_k ? c.kx : c.vx) + exp_at(c, page, slot, h);
+    int8_t *y = (int8_t *)plane + i8_at<HD>(c, page, slot - off, h);
+    nan = __any(nan);
+    if (off) {
+        // The rows before these keep their codes, or take the greater step.
+        const int had = *xp;
+        nan |= had == EXP_NAN;
+        const int ex0 = min(max(had - EXP_BIAS, EXP_MIN), EXP_MAX);
+        if (ex > ex0) {
+            const float f = __uint_as_float((uint32_t)(127 + ex0 - ex) << 23);
+            for (int i = 0; i < off; i++)
+#pragma unroll
+                for (int e = 0; e < NP; e++) {
+                    y[i * HD + d0[e]] = (int8_t)rintf(y[i * HD + d0[e]] * f);
+                    y[i * HD + d1[e]] = (int8_t)rintf(y[i * HD + d1[e]] * f);
+                }
+        }
+        ex = max(ex, ex0);
+    }
+    if (lane == 0) *xp = nan ? EXP_NAN : (uint8_t)(ex + EXP_BIAS);
+    const double inv = __longlong_as_double((long long)(1023 - ex) << 52);
+    auto code = [&](double x) { return (int8_t)(int)fmin(fmax(rint(x * inv), -127.0), 127.0); };
+#pragma unroll
+    for (int i = 0; i < BLK; i++) {
+        if (i >= n) break;
+#pragma unroll
+        for (int e = 0; e < NP; e++) {
+            double a, z;
+            turned(is_k, i, e, x0[i][e], x1[i][e], a, z);
+            y[(off + i) * HD + d0[e]] = code(a);
+            y[(off + i) * HD + d1[e]] = code(z);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- read
+
+// Rows of the cache as values, eight dims a thread: thread i over [row][K then V]
+// [head][HD / 8].  Rows of pages that are not there come out as zeros.
+template <int HD, bool I8, typename T>
+__global__ __launch_bounds__(256) void k_read(Cache c, Rows s, T *k_out, T *v_out) {
+    const int per = 2 * c.HKV * (HD / 8), n = blockIdx.x;
+    const int b = seq_of_row(s, n);
+    if (b < 0) return;
+    const Seq sq = seq_at(s, b);
+    if (n < sq.r0 || n >= sq.r1) return;
+    const uint32_t p = (uint32_t)sq.pos + (uint32_t)(n - sq.r0);
+    const int page = page_of(c, s, b, p), slot = slot_of(c, p);
+    for (int i = threadIdx.x; i < per; i += 256) {
+        const int d = i % (HD / 8) * 8, hh = i / (HD / 8), h = hh % c.HKV;
+        const bool is_k = hh < c.HKV;
+        T *y = (is_k ? k_out : v_out) + ((int64_t)n * c.HKV + h) * HD + d;
+        float f[8] = {};
+        if (page >= 0) {
+            if constexpr (I8) {
+                const int8_t *x = (const int8_t *)(is_k ? c.k : c.v) + i8_at<HD>(c, page, slot, h) + d;
+                const float st = step_of((is_k ? c.kx : c.vx)[exp_at(c, page, slot, h)]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[e] = (float)x[e] * st;
+            } else {
+                const uint16_t *x = (const uint16_t *)(is_k ? c.k : c.v) + f16_at<HD>(c, page, slot, h) + d;
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[e] = gd_h2f(x[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = from_f32<T>(f[e]);
+    }
+}
+
+// ---------------------------------------------------------------- attention
+
+struct Mask {
+    int window, sinks;                           // window 0: every key up to the query's own
+};
+
+// A wave for each (row, query head), a key at a time: the visible keys are the
+// sinks [0, min(n_sink, lo)) and [lo, p], lo = max(0, p - window + 1).
+template <int HD, bool I8, typename T>
+__global__ __launch_bounds__(256) void k_attn(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate,
+                                              int64_t gate_stride, T *out, int H, float scale, Mask mask) {
+    constexpr int DPL = HD / 64;
+    const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, n = (int)(u / H), h = (int)(u % H);
+    if (n >= s.n_rows) return;
+    const int b = seq_of_row(s, n);
+    if (b < 0) return;
+    const Seq sq = seq_at(s, b);
+    if (n < sq.r0 || n >= sq.r1) return;
+    const uint32_t p = min((uint32_t)sq.pos + (uint32_t)(n - sq.r0), s.cap - 1);
+    const uint32_t at = (uint32_t)sq.pos + (uint32_t)(n - sq.r0);
+    const uint32_t lo = mask.window && at >= (uint32_t)mask.window ? at - mask.window + 1 : 0;
+    const uint32_t sinks = min((uint32_t)mask.sinks, lo);
+    const int kvh = h / (H / c.HKV);
+    float qv[DPL], acc[DPL], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < DPL; e++) {
+        qv[e] = to_f32(q[n * q_stride + (int64_t)h * HD + DPL * lane + e]) * scale;
+        acc[e] = 0.f;
+    }
+    for (uint32_t t = sinks ? 0 : lo; t <= p; t = t + 1 == sinks ? max(lo, sinks) : t + 1) {
+        const int page = page_of(c, s, b, t), slot = slot_of(c, t);
+        if (page < 0) continue;
+        float kf[DPL], vf[DPL];
+        if constexpr (I8) {
+            const int64_t at8 = i8_at<HD>(c, page, slot, kvh) + DPL * lane, x = exp_at(c, page, slot, kvh);
+            const float ks = step_of(c.kx[x]), vs = step_of(c.vx[x]);
+#pragma unroll
+            for (int e = 0; e < DPL; e++) {
+                kf[e] = (float)((const int8_t *)c.k)[at8 + e] * ks;
+                vf[e] = (float)((const int8_t *)c.v)[at8 + e] * vs;
+            }
+        } else {
+            const int64_t at16 = f16_at<HD>(c, page, slot, kvh) + DPL * lane;
+#pragma unroll
+            for (int e = 0; e < DPL; e++) {
+                kf[e] = gd_h2f(((const uint16_t *)c.k)[at16 + e]);
+                vf[e] = gd_h2f(((const uint16_t *)c.v)[at16 + e]);
+            }
+        }
+        float d = 0.f;
+#pragma unroll
+        for (int e = 0; e < DPL; e++) d += qv[e] * kf[e];
+        d = gd_wave_sum(d);
+        const float mn = fmaxf(m, d), al = m == -INFINITY ? 0.f : expf(m - mn);
+        const float w = d == -INFINITY ? 0.f : expf(d - mn);
+        l = l * al + w;
+#pragma unroll
+        for (int e = 0; e < DPL; e++) acc[e] = acc[e] * al + w * vf[e];
+        m = mn;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int64_t o = ((int64_t)n * H + h) * HD + DPL * lane;
+#pragma unroll
+    for (int e = 0; e < DPL; e++) {
+        float y = acc[e] * inv;
+        if (gate) y *= gd_sigmoid(to_f32(gate[n * gate_stride + (int64_t)h * HD + DPL * lane + e]));
+        out[o + e] = from_f32<T>(y);
+    }
+}
+
+// ---------------------------------------------------------------- checks
+
+int check_kv(gd_ctx *ctx, const char *fn, const gd_kv *kv, bool planes) {
+    GD_REQUIRE(ctx, kv, "%s: null cache", fn);
+    GD_REQUIRE(ctx, kv->dtype == GD_F16 || kv->dtype == GD_I8, "%s: cache dtype %d (GD_F16 or GD_I8)", fn, kv->dtype);
+    GD_REQUIRE(ctx, kv->head_dim == 128 || kv->head_dim == 256, "%s: head_dim %d (takes 128 or 256)", fn, kv->head_dim);
+    GD_REQUIRE(ctx, kv->n_head_kv > 0 && kv->n_head_kv <= 4096, "%s: n_head_kv %d", fn, kv->n_head_kv);
+    GD_REQUIRE(ctx, kv->page_size > 0 && kv->page_size <= (1 << 24), "%s: page size %d", fn, kv->page_size);
+    GD_REQUIRE(ctx, kv->dtype != GD_I8 || kv->page_size % GD_KV_BLOCK == 0,
+               "%s: page size %d of an 8-bit cache is not a multiple of %d", fn, kv->page_size, GD_KV_BLOCK);
+    // At most 2^62 elements, so that no byte offset of the kernels passes 63 bits.
+    const int64_t page = (int64_t)kv->page_size * kv->n_head_kv * kv->head_dim;
+    GD_REQUIRE(ctx, kv->n_pages > 0 && kv->n_pages < (1LL << 31) && kv->n_pages < (1LL << 60) / page,
+               "%s: %lld pages", fn, (long long)kv->n_pages);
+    if (!planes) return GD_OK;
+    GD_REQUIRE(ctx, kv->k && kv->v && (kv->dtype != GD_I8 || (kv->k_exp && kv->v_exp)), "%s: null cache plane", fn);
+    GD_REQUIRE(ctx, ((uintptr_t)kv->k | (uintptr_t)kv->v) % 16 == 0, "%s: cache planes must be 16-byte aligned", fn);
+    return GD_OK;
+}
+
+int check_seqs(gd_ctx *ctx, const char *fn, const gd_seqs *s) {
+    GD_REQUIRE(ctx, s, "%s: null sequences", fn);
+    GD_REQUIRE(ctx, s->n_seq >= 0 && s->n_rows >= 0 && s->n_rows < (1LL << 31), "%s: %d sequences, %lld rows", fn,
+               s->n_seq, (long long)s->n_rows);
+    GD_REQUIRE(ctx, s->row_start || s->n_rows == s->n_seq,
+               "%s: %lld rows of %d sequences need row_start (one row each without)", fn, (long long)s->n_rows, s->n_seq);
+    GD_REQUIRE(ctx, s->n_rows == 0 || s->n_seq == 0 || (s->pos && s->page_table), "%s: null positions or page table", fn);
+    GD_REQUIRE(ctx, s->max_pages > 0 && s->max_len >= 0, "%s: max_pages %d, max_len %d", fn, s->max_pages, s->max_len);
+    return GD_OK;
+}
+
+int check_x(gd_ctx *ctx, const char *fn, int dtype) {
+    GD_REQUIRE(ctx, dtype == GD_F32 || dtype == GD_F16, "%s: row dtype %d (GD_F32 or GD_F16)", fn, dtype);
+    return GD_OK;
+}
+
+Cache cache_of(const gd_kv *kv) {
+    return Cache{kv->k, kv->v, kv->k_exp, kv->v_exp, (uint32_t)kv->n_pages, kv->n_head_kv, kv->page_size,
+                 FastDiv((uint32_t)kv->page_size)};
+}
+Rows rows_of(const gd_kv *kv, const gd_seqs *s) {
+    const int64_t cap = std::min<int64_t>((int64_t)s->max_pages * kv->page_size, 0x7fffffff);
+    return Rows{s->row_start, s->pos, s->rope_shift, s->page_table, (int)s->n_rows, s->n_seq, s->max_pages, (uint32_t)cap};
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------- C ABI
+// Arguments are checked before the context is looked at, so that a null one shows
+// what is wrong with them too (gd_last_error(NULL)).
+
+static size_t exp_bytes(const gd_kv *kv) {
+    return (size_t)kv->n_pages * kv->n_head_kv * (kv->page_size / GD_KV_BLOCK);
+}
+
+extern "C" int gd_kv_alloc(gd_ctx *ctx, int dtype, int n_head_kv, int head_dim, int page_size, int64_t n_pages,
+                           gd_kv *kv) {
+    GD_REQUIRE(ctx, kv, "gd_kv_alloc: null out pointer");
+    *kv = gd_kv{nullptr, nullptr, nullptr, nullptr, n_pages, dtype, n_head_kv, head_dim, page_size};
+    int rc = check_kv(ctx, "gd_kv_alloc", kv, false);
+    if (rc) return rc;
+    GD_CHECK_CTX(ctx);
+    const size_t plane = (size_t)n_pages * page_size * n_head_kv * head_dim * (dtype == GD_F16 ? 2 : 1);
+    void *p[4] = {};
+    const int n = dtype == GD_I8 ? 4 : 2;
+    for (int i = 0; i < n && !rc; i++) {
+        const size_t bytes = ((i < 2 ? plane : exp_bytes(kv)) + 15) / 16 * 16;
+        rc = gd_alloc(ctx, bytes, &p[i]);
+        if (!rc) rc = gd_fill_u32(ctx, p[i], 0u, bytes / 4);
+    }
+    kv->k = p[0];
+    kv->v = p[1];
+    kv->k_exp = (uint8_t *)p[2];
+    kv->v_exp = (uint8_t *)p[3];
+    if (rc) {
+        const std::string why = ctx->err;
+        gd_kv_free(ctx, kv);
+        ctx->err = why;
+    }
+    return rc;
+}
+
+extern "C" int gd_kv_free(gd_ctx *ctx, gd_kv *kv) {
+    GD_CHECK_CTX(ctx);
+    if (!kv) return GD_OK;
+    int rc = GD_OK;
+    for (void *p : {kv->k, kv->v, (void *)kv->k_exp, (void *)kv->v_exp}) {
+        const int e = gd_free(ctx, p);
+        rc = rc ? rc : e;
+    }
+    kv->k = kv->v = nullptr;
+    kv->k_exp = kv->v_exp = nullptr;
+    return rc;
+}
+
+// The template of head dim, cache type and row type that a call runs.
+#define GD_KV_PICK(kv, x_dtype, GO) \
+    do { \
+        if ((kv)->head_dim == 128) { \
+            if ((kv)->dtype == GD_I8) { if ((x_dtype) == GD_F32) GO(128, true, float); else GO(128, true, uint16_t); } \
+            else { if ((x_dtype) == GD_F32) GO(128, false, float); else GO(128, false, uint16_t); } \
+        } else { \
+            if ((kv)->dtype == GD_I8) { if ((x_dtype) == GD_F32) GO(256, true, float); else GO(256, true, uint16_t); } \
+            else { if ((x_dtype) == GD_F32) GO(256, false, float); else GO(256, false, uint16_t); } \
+        } \
+    } while (0)
+
+extern "C" int gd_kv_append_rope(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const void *q, int64_t q_stride,
+                                 void *q_out, int n_head, const void *k, int64_t k_stride, const void *v,
+                                 int64_t v_stride, int x_dtype, int n_rot, float base) {
+    const char *fn = "gd_kv_append_rope";
+    int rc;
+    if ((rc = check_kv(ctx, fn, kv, true)) || (rc = check_seqs(ctx, fn, s)) || (rc = check_x(ctx, fn, x_dtype))) return rc;
+    const int hd = kv->head_dim;
+    GD_REQUIRE(ctx, k && v, "%s: null k or v", fn);
+    GD_REQUIRE(ctx, k_stride >= (int64_t)kv->n_head_kv * hd && v_stride >= (int64_t)kv->n_head_kv * hd,
+               "%s: k and v rows of %d heads overlap at strides %lld, %lld", fn, kv->n_head_kv, (long long)k_stride,
+               (long long)v_stride);
+    GD_REQUIRE(ctx, n_rot >= 0 && n_rot % 2 == 0 && n_rot <= hd, "%s: n_rot %d must be even and at most head_dim %d", fn,
+               n_rot, hd);
+    GD_REQUIRE(ctx, n_rot == 0 || (base > 0.f && std::isfinite(base)), "%s: rotation base %g", fn, (double)base);
+    if (q) {
+        GD_REQUIRE(ctx, q_out && n_head > 0 && n_head <= 65536, "%s: q of %d heads without q_out", fn, n_head);
+        GD_REQUIRE(ctx, q_stride >= (int64_t)n_head * hd, "%s: q rows of %d heads overlap at stride %lld", fn, n_head,
+                   (long long)q_stride);
+        const int64_t size = x_dtype == GD_F32 ? 4 : 2, row = (int64_t)n_head * hd;
+        const uintptr_t a = (uintptr_t)q, o = (uintptr_t)q_out;
+        GD_REQUIRE(ctx, (a == o && q_stride == row) || !s->n_rows || a + ((s->n_rows - 1) * q_stride + row) * size <= o ||
+                            o + s->n_rows * row * size <= a,
+                   "%s: q turned in place needs q_out = q and rows of n_head * head_dim (stride %lld)", fn,
+                   (long long)q_stride);
+    }
+    const int64_t widest = std::max({q ? q_stride : 0, k_stride, v_stride});
+    GD_REQUIRE(ctx, widest < (1LL << 31), "%s: row stride %lld", fn, (long long)widest);
+    GD_CHECK_CTX(ctx);
+    if (!s->n_rows || !s->n_seq) return GD_OK;
+    GD_HIP(ctx, hipSetDevice(ctx->device));
+    // base^(-2j / n_rot) / (2 pi) of each pair, by one power and its multiples: off by
+    // under 2^-57 of itself, which even position 2^31 turns into less than 2^-28 of a turn.
+    Turns turns;
+    long double turn = 0.159154943091895335768883763372514362L, by = n_rot ? powl(base, -2.0L / n_rot) : 0.0L;
+    for (int j = 0; j < n_rot / 2; j++, turn *= by) {
+        long double f = turn - floorl(turn);
+        turns.t[j] = f >= 1.0L - 0x1p-64L ? 0 : (uint64_t)(f * 0x1p64L);
+    }
+    const int H = q ? n_head : 0;
+    // Blocks of 16 positions that the rows can touch: rows / 16 and two ends a sequence.
+    const int64_t units = std::min<int64_t>(s->n_rows, s->n_rows / BLK + 2 * std::min<int64_t>(s->n_seq, s->n_rows));
+    const dim3 grid((unsigned)units, gd_blocks(H + 2 * kv->n_head_kv, 4));
+#define GD_GO(HD_, I8_, T_) \
+    hipLaunchKernelGGL((k_append<HD_, I8_, T_>), grid, dim3(256), 0, ctx->stream, cache_of(kv), rows_of(kv, s), turns, \
+                       (const T_ *)q, q_stride, (T_ *)q_out, H, (const T_ *)k, k_stride, (const T_ *)v, v_stride, n_rot)
+    GD_KV_PICK(kv, x_dtype, GD_GO);
+#undef GD_GO
+    GD_LAUNCHED(ctx, fn);
+    return GD_OK;
+}
+
+extern "C" int gd_kv_read(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, void *k_out, void *v_out, int dtype) {
+    const char *fn = "gd_kv_read";
+    int rc;
+    if ((rc = check_kv(ctx, fn, kv, true)) || (rc = check_seqs(ctx, fn, s)) || (rc = check_x(ctx, fn, dtype))) return rc;
+    GD_REQUIRE(ctx, k_out && v_out, "%s: null output", fn);
+    GD_REQUIRE(ctx, ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0, "%s: outputs must be 16-byte aligned", fn);
+    GD_CHECK_CTX(ctx);
+    if (!s->n_rows || !s->n_seq) return GD_OK;
+    GD_HIP(ctx, hipSetDevice(ctx->device));
+    const dim3 grid((unsigned)s->n_rows);
+#define GD_GO(HD_, I8_, T_) \
+    hipLaunchKernelGGL((k_read<HD_, I8_, T_>), grid, dim3(256), 0, ctx->stream, cache_of(kv), rows_of(kv, s), \
+                       (T_ *)k_out, (T_ *)v_out)
+    GD_KV_PICK(kv, dtype, GD_GO);
+#undef GD_GO
+    GD_LAUNCHED(ctx, fn);
+    return GD_OK;
+}
+
+extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const void *q, int64_t q_stride,
+                          const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
+                          int window, int n_sink) {
+    const char *fn = "gd_kv_attn";
+    int rc;
+    if ((rc = check_kv(ctx, fn, kv, true)) || (rc = check_seqs(ctx, fn, s)) || (rc = check_x(ctx, fn, x_dtype))) return rc;
+    const int hd = kv->head_dim, size = x_dtype == GD_F32 ? 4 : 2;
+    GD_REQUIRE(ctx, q && out, "%s: null q or out", fn);
+    GD_REQUIRE(ctx, n_head > 0 && n_head <= 65536 && n_head % kv->n_head_kv == 0,
+               "%s: n_head %d not a multiple of n_head_kv %d", fn, n_head, kv->n_head_kv);
+    const int64_t row = (int64_t)n_head * hd;
+    GD_REQUIRE(ctx, q_stride >= row && (!gate || gate_stride >= row) && q_stride < (1LL << 31) &&
+                        (!gate || gate_stride < (1LL << 31)),
+               "%s: rows of %d heads at strides %lld, %lld", fn, n_head, (long long)q_stride, (long long)gate_stride);
+    GD_REQUIRE(ctx, ((uintptr_t)q | (uintptr_t)out | (uintptr_t)gate) % 16 == 0 && q_stride * size % 16 == 0 &&
+                        (!gate || gate_stride * size % 16 == 0),
+               "%s: q, gate and out must be 16-byte aligned, and their rows", fn);
+    GD_REQUIRE(ctx, window >= 0 && n_sink >= 0, "%s: window %d, n_sink %d", fn, window, n_sink);
+    GD_REQUIRE(ctx, std::isfinite(scale), "%s: scale %g", fn, (double)scale);
+    GD_REQUIRE(ctx, s->n_rows * n_head < (1LL << 31), "%s: %lld rows of %d heads", fn, (long long)s->n_rows, n_head);
+    // Workgroups read their q and gate before they write: in place only row on row.
+    const size_t span = (size_t)s->n_rows * row * size;
+    auto apart = [&](const void *x, int64_t stride) {
+        const uintptr_t a = (uintptr_t)x, o = (uintptr_t)out, end = a + ((s->n_rows - 1) * stride + row) * size;
+        return !x || !span || (a == o && stride == row) || end <= o || o + span <= a;
+    };
+    GD_REQUIRE(ctx, apart(q, q_stride) && apart(gate, gate_stride),
+               "%s: out in place of q or gate needs their place and rows of n_head * head_dim", fn);
+    GD_CHECK_CTX(ctx);
+    if (!s->n_rows || !s->n_seq) return GD_OK;
+    GD_HIP(ctx, hipSetDevice(ctx->device));
+    const Mask mask{window, window ? n_sink : 0};
+    const dim3 grid(gd_blocks(s->n_rows * n_head, 4));
+#define GD_GO(HD_, I8_, T_) \
+    hipLaunchKernelGGL((k_attn<HD_, I8_, T_>), grid, dim3(256), 0, ctx->stream, cache_of(kv), rows_of(kv, s), \
+                       (const T_ *)q, q_stride, (const T_ *)gate, gate_stride, (T_ *)out, n_head, scale, mask)
+    GD_KV_PICK(kv, x_dtype, GD_GO);
+#undef GD_GO
+    GD_LAUNCHED(ctx, fn);
+    return GD_OK;
+}

@@ -47,6 +47,7 @@ extern "C" {
 
 #define GD_F32 0
 #define GD_F16 1
+#define GD_I8  2         /* KV caches only (gd_kv) */
 
 /* Q2_0 block geometry: 128 weights in 34 bytes {f16 d; u8 qs[32]}.
  * Reference: Quant.swift:2-12, GGUF.swift:13 (type 42), Kernels.metal:2484-2490. */
@@ -370,6 +371,106 @@ int gd_attn_batch(gd_ctx *ctx, const float *q, const uint16_t *k_cache,
                   const uint16_t *v_cache, const int32_t *page_table, const float *gate,
                   float *out, int head_dim, int n_head, int n_head_kv, int kv_dim,
                   int page_size, float scale, int base_pos, int64_t N, int gated, int window);
+
+/* ---- a paged KV cache for many sequences ---------------------------------------
+ * The attention of a batch of sequences, single tokens or prompt chunks, beside
+ * the batched GDN step: rows are appended with their rotation, and attended to,
+ * in one call each, over f16 values or 8-bit codes.  The reference serves one
+ * conversation at a time from half pages (MetalKVPool.swift; ropeBatch,
+ * kvAppendBatch, attnPaged, attnBatch, MetalEnc.swift:560-706, 817-1025).
+ *
+ * gd_kv: one attention layer's cache, `n_pages` pages of `page_size` positions.
+ *   GD_F16: k and v [page][slot][n_head_kv][head_dim] halves, the cache of
+ *     gd_kv_append, gd_attn_paged and gd_attn_batch; any page size.
+ *   GD_I8: k and v int8 codes [page][n_head_kv][slot][head_dim]; k_exp and v_exp
+ *     one byte for each GD_KV_BLOCK positions of a page and head, [page]
+ *     [n_head_kv][page_size / GD_KV_BLOCK]: code c with byte x stands for
+ *     c 2^(x - 127), x - 127 in -24 .. 9 (each value an f16 exactly); x = 255
+ *     marks a block that took a NaN, whose values are all NaN; 0 one never
+ *     written.  page_size a multiple of GD_KV_BLOCK.
+ * Planes are 16-byte aligned device memory, from gd_kv_alloc or the caller's own.
+ *
+ * gd_seqs: the rows of a call and where they belong.  Sequence b has the rows
+ * row_start[b] .. row_start[b+1]-1 (row_start ascending, [n_seq + 1]; null: one
+ * row each, n_rows == n_seq), at the positions pos[b], pos[b]+1, ..; position p is
+ * at slot p % page_size of page page_table[b][p / page_size].  All four arrays are
+ * device memory read by the kernels, so a recorded graph may be replayed on
+ * changed positions, rows and tables.  A sequence with a negative pos is idle: its
+ * rows are not touched, and neither are rows that no sequence has (before
+ * row_start[0], from row_start[n_seq] on).  A table entry outside [0, n_pages),
+ * and a position past max_pages * page_size, is a page that is not there: rows for
+ * it are not kept and its keys are not seen (so a program with a window may drop
+ * pages that left it).  No two rows of a call may name the same slot, and of an
+ * 8-bit cache no two sequences the same block. */
+#define GD_KV_BLOCK 16
+
+typedef struct gd_kv {
+    void *k, *v;
+    uint8_t *k_exp, *v_exp;      /* GD_I8 only */
+    int64_t n_pages;
+    int dtype;                   /* GD_F16 or GD_I8 */
+    int n_head_kv, head_dim;     /* head_dim 128 or 256 */
+    int page_size;
+} gd_kv;
+
+typedef struct gd_seqs {
+    int64_t n_rows;              /* rows of q, k, v and out */
+    const int32_t *row_start;    /* [n_seq + 1] or null */
+    const int32_t *pos;          /* [n_seq] */
+    const int32_t *rope_shift;   /* [n_seq] or null: rows are rotated at position + shift */
+    const int32_t *page_table;   /* [n_seq][max_pages] */
+    int n_seq, max_pages;
+    int max_len;                 /* most positions of a sequence with this call's rows, as far as the
+                                    caller knows (0: max_pages * page_size): how finely the keys
+                                    are split goes by it, no result depends on it */
+} gd_seqs;
+
+/* Allocate a cache's planes, zeroed (free with gd_kv_free). */
+int gd_kv_alloc(gd_ctx *ctx, int dtype, int n_head_kv, int head_dim, int page_size, int64_t n_pages,
+                gd_kv *kv);
+int gd_kv_free(gd_ctx *ctx, gd_kv *kv);
+
+/* Append the rows k, v [n_rows][n_head_kv][head_dim] (x_dtype GD_F32 or GD_F16; row
+ * strides in elements) to the cache at their positions, k turned as gd_rope turns it
+ * (n_rot even, 0 for none; here the angle's phase is exact at any position and its
+ * cos and sin are formed in 64 bits).  With q not null, q [n_rows][n_head]
+ * [head_dim] is turned likewise into q_out (contiguous rows, x_dtype; q_out may be
+ * q where q_stride is n_head * head_dim).  One launch; the result of gd_rope twice
+ * and gd_kv_append for each sequence (MetalEnc.ropeBatch, kvAppendBatch,
+ * MetalEnc.swift:817-847).
+ *   GD_F16: rounded to nearest; values past f16's range are held as its largest.
+ *   GD_I8: per block and head x = c 2^e, c = x 2^-e rounded to nearest (ties to
+ *     even), e the least of -24 .. 9 that holds the largest |x| of the block's rows
+ *     so far within 127 2^e, values past 127 2^9 held as that.  e is never lowered
+ *     by later rows of the block; where they raise it by d, the codes before them
+ *     become c 2^-d, rounded alike.  Rows of a block behind the last one appended are
+ *     dead: a row appended again at an earlier position (after a rewind) leaves
+ *     theirs as they were, whatever its exponent. */
+int gd_kv_append_rope(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const void *q, int64_t q_stride,
+                      void *q_out, int n_head, const void *k, int64_t k_stride, const void *v,
+                      int64_t v_stride, int x_dtype, int n_rot, float base);
+
+/* The cached rows at the sequences' positions as values: k_out, v_out [n_rows]
+ * [n_head_kv][head_dim] (GD_F32, or GD_F16: exact), zeros for pages that are not
+ * there.  What MetalEngine.serialize widens its half pages for
+ * (MetalEngine.swift:492-530). */
+int gd_kv_read(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, void *k_out, void *v_out, int dtype);
+
+/* Causal attention of the rows q [n_rows][n_head][head_dim] over their sequences'
+ * cached positions (their own k, v appended first): the row at position p sees
+ * the positions t <= p with window == 0, t > p - window or t < n_sink, whose pages
+ * are there: out[h] = softmax((q_h . k_t) * scale) . v_t, h's kv head h / (n_head /
+ * n_head_kv), times sigmoid(gate[h]) where gate is not null; zeros where it sees no
+ * position.  q, gate and out have x_dtype (GD_F32 or GD_F16), out contiguous rows, all
+ * 16-byte aligned, row strides (in elements) too; out may be q or gate.  f32 rows
+ * are worked as f16 hi + lo pairs (about 22 bits), f16 ones in f16 products with f32
+ * sums.  A NaN or infinity in the cache reaches only the rows that see it, which
+ * are then not to be relied on.  Two launches where the keys are split; partials go to
+ * the context's or the recording's scratch as gd_attn_paged's.  MetalEnc.attnPaged and
+ * attnBatch (MetalEnc.swift:679-706, 966-1025), the latter's window included. */
+int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const void *q, int64_t q_stride,
+               const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
+               int window, int n_sink);
 
 /* ---- GDN recurrence -----------------------------------------------------------
  * State S[nV][dS][dS] f32, key-major: S[h][i*dS + j], i = key, j = value
