@@ -134,7 +134,12 @@ template <> __device__ __forceinline__ float from_f32(float x) { return x; }
 template <> __device__ __forceinline__ uint16_t from_f32(float x) { return gd_f2h(x); }
 
 // A turned value, formed in 64 bits, as the row it would be in 32 (gd_rope's), in T.
-template <typename T> __device__ __forceinline__ T from_f64(double x) { return from_f32<T>((float)x); }
+// (Opaque: the compiler otherwise rounds the 64 bits to f16 in one step.)
+template <typename T> __device__ __forceinline__ T from_f64(double x) {
+    float f = (float)x;
+    asm("" : "+v"(f));
+    return from_f32<T>(f);
+}
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
