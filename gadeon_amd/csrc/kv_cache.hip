@@ -111,15 +111,10 @@ __device__ __forceinline__ int page_of(const Cache &c, const Rows &s, int b, uin
 }
 __device__ __forceinline__ int slot_of(const Cache &c, uint32_t p) { return (int)(p - c.by_page(p) * c.P); }
 
-// Element offset of (page, slot, head) in a plane, and of its exponent.
-template <int HD> __device__ __forceinline__ int64_t f16_at(const Cache &c, int page, int slot, int h) {
-    return (((int64_t)page * c.P + slot) * c.HKV + h) * HD;
-}
-template <int HD> __device__ __forceinline__ int64_t i8_at(const Cache &c, int page, int slot, int h) {
-    return (((int64_t)page * c.HKV + h) * c.P + slot) * HD;
-}
-__device__ __forceinline__ int64_t exp_at(const Cache &c, int page, int slot, int h) {
-    return ((int64_t)page * c.HKV + h) * (c.P / BLK) + slot / BLK;
+// Head h's row of (page, slot) in the planes, in rows of head_dim elements (fewer than
+// 2^32, check_kv); its exponent is the one of row / 16.
+template <bool I8> __device__ __forceinline__ uint32_t row_at(const Cache &c, int page, int slot, int h) {
+    return I8 ? ((uint32_t)page * c.HKV + h) * c.P + slot : ((uint32_t)page * c.P + slot) * c.HKV + h;
 }
 // 2^e of a stored exponent: 0 for a block never written, NaN for one that took a NaN.
 __device__ __forceinline__ float step_of(uint8_t x) {
@@ -232,7 +227,7 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
         for (int i = 0; i < n; i++) {
             const int page = page_of(c, s, b, p + i);
             if (page < 0) continue;
-            uint16_t *y = (uint16_t *)plane + f16_at<HD>(c, page, slot_of(c, p + i), h);
+            uint16_t *y = (uint16_t *)plane + (uint64_t)row_at<false>(c, page, slot_of(c, p + i), h) * HD;
             auto f16_of = [](double x) { return from_f64<uint16_t>(x > 65504. ? 65504. : x < -65504. ? -65504. : x); };
 #pragma unroll
             for (int e = 0; e < NP; e++) {
@@ -270,8 +265,9 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
     const uint32_t bits = __float_as_uint(top);
     int ex = (int)(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u);   // 127 2^ex holds top
     ex = min(max(ex, EXP_MIN), EXP_MAX);
-    uint8_t *xp = (is_k ? c.kx : c.vx) + exp_at(c, page, slot, h);
-    int8_t *y = (int8_t *)plane + i8_at<HD>(c, page, slot - off, h);
+    const uint32_t row = row_at<true>(c, page, slot - off, h);
+    uint8_t *xp = (is_k ? c.kx : c.vx) + row / BLK;
+    int8_t *y = (int8_t *)plane + (uint64_t)row * HD;
     nan = __any(nan);
     if (off) {
         // The rows before these keep their codes, or take the greater step.
@@ -324,13 +320,14 @@ __global__ __launch_bounds__(256) void k_read(Cache c, Rows s, T *k_out, T *v_ou
         T *y = (is_k ? k_out : v_out) + ((int64_t)n * c.HKV + h) * HD + d;
         float f[8] = {};
         if (page >= 0) {
+            const uint32_t row = row_at<I8>(c, page, slot, h);
             if constexpr (I8) {
-                const int8_t *x = (const int8_t *)(is_k ? c.k : c.v) + i8_at<HD>(c, page, slot, h) + d;
-                const float st = step_of((is_k ? c.kx : c.vx)[exp_at(c, page, slot, h)]);
+                const int8_t *x = (const int8_t *)(is_k ? c.k : c.v) + (uint64_t)row * HD + d;
+                const float st = step_of((is_k ? c.kx : c.vx)[row / BLK]);
 #pragma unroll
                 for (int e = 0; e < 8; e++) f[e] = (float)x[e] * st;
             } else {
-                const uint16_t *x = (const uint16_t *)(is_k ? c.k : c.v) + f16_at<HD>(c, page, slot, h) + d;
+                const uint16_t *x = (const uint16_t *)(is_k ? c.k : c.v) + (uint64_t)row * HD + d;
 #pragma unroll
                 for (int e = 0; e < 8; e++) f[e] = gd_h2f(x[e]);
             }
@@ -374,16 +371,17 @@ __global__ __launch_bounds__(256) void k_attn(Cache c, Rows s, const T *q, int64
         const int page = page_of(c, s, b, t), slot = slot_of(c, t);
         if (page < 0) continue;
         float kf[DPL], vf[DPL];
+        const uint32_t row = row_at<I8>(c, page, slot, kvh);
         if constexpr (I8) {
-            const int64_t at8 = i8_at<HD>(c, page, slot, kvh) + DPL * lane, x = exp_at(c, page, slot, kvh);
-            const float ks = step_of(c.kx[x]), vs = step_of(c.vx[x]);
+            const uint64_t at8 = (uint64_t)row * HD + DPL * lane;
+            const float ks = step_of(c.kx[row / BLK]), vs = step_of(c.vx[row / BLK]);
 #pragma unroll
             for (int e = 0; e < DPL; e++) {
                 kf[e] = (float)((const int8_t *)c.k)[at8 + e] * ks;
                 vf[e] = (float)((const int8_t *)c.v)[at8 + e] * vs;
             }
         } else {
-            const int64_t at16 = f16_at<HD>(c, page, slot, kvh) + DPL * lane;
+            const uint64_t at16 = (uint64_t)row * HD + DPL * lane;
 #pragma unroll
             for (int e = 0; e < DPL; e++) {
                 kf[e] = gd_h2f(((const uint16_t *)c.k)[at16 + e]);
@@ -411,6 +409,319 @@ __global__ __launch_bounds__(256) void k_attn(Cache c, Rows s, const T *q, int64
     }
 }
 
+// Four codes as two pairs of halves: byte c ^ 0x80 below 0x64 is the half 1152 + c.
+__device__ __forceinline__ void halves(uint32_t codes, f16x2 &a, f16x2 &b) {
+    const uint32_t x = codes ^ 0x80808080u;
+    const f16x2 off = {(f16)1152.f, (f16)1152.f};
+    a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - off;
+    b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - off;
+}
+__device__ __forceinline__ f16x8 halves(uint32_t lo, uint32_t hi) {
+    f16x2 a, b, c, d;
+    halves(lo, a, b);
+    halves(hi, c, d);
+    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// The visible keys of the query at position p as blocks of W keys that start at a
+// multiple of W: first those of the sinks, then those from the window's first key lo on.
+// Key t of a block is seen where t <= p and (t >= lo or t < sinks).
+template <int W> struct KeyBlocks {
+    uint32_t lo, sinks;
+    int ns, n;                                   // blocks of sinks, blocks in all
+    // Window of the query at `first` and on, keys up to `last`.
+    __device__ __forceinline__ KeyBlocks(const Mask &m, uint32_t first, uint32_t last) {
+        lo = m.window && first >= (uint32_t)m.window ? first - m.window + 1 : 0;
+        sinks = min((uint32_t)m.sinks, lo);
+        ns = (int)min((sinks + W - 1) / W, lo / W);
+        n = ns + (lo <= last ? (int)(last / W - lo / W + 1) : 0);
+    }
+    __device__ __forceinline__ uint32_t start(int j) const { return (uint32_t)(j < ns ? j : j - ns + (int)(lo / W)) * W; }
+};
+
+// Attention of single tokens: workgroup (row, kv head and eight of its query heads;
+// split sp of ns) reads the split's keys once for its heads.  Wave w takes the blocks
+// of 32 keys sp + ns (w + TW i): S = K Q^T with K straight from the cache as the A
+// operand, and O^T += V^T P^T with V staged in the wave's own LDS rows and read by the
+// transposing LDS read (no barrier in the loop).  The 16 columns of an MFMA are the
+// heads' q as f16 hi (0..7) and lo (8..15), and P likewise: both halves of a product
+// come from one instruction and are added across lanes lr, lr ^ 8.  q is brought to
+// 2^14 .. 2^15 by a power of two and weights to 2^14, so that no low half leaves f16's
+// normal range; scores are in units of log2.  8-bit keys enter as whole numbers, their
+// steps scaling the scores; 8-bit values as the halves they are.  Keys that are not
+// seen have the weight 0 and zeros for values.  A block's rows are requested one
+// block ahead, its page-table entries two.
+constexpr int TW = 4;                            // waves
+constexpr int MAX_SPLITS = 64;                   // what the combine weighs in one wave
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int HD, bool I8, typename T>
+__global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_tokens(
+        Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, float *part, int ns,
+        int H, float scale, Mask mask) {
+    constexpr int KS = HD / 32, DT = HD / 16, VP = HD + 16;
+    constexpr int KL = I8 ? KS / 2 : KS;         // 16-byte loads of a key tile, per lane
+    constexpr int CPK = I8 ? HD / 16 : HD / 8;   // 16-byte chunks of a value row
+    constexpr int VCH = 32 * CPK / 64;           // of a block's values, per lane
+    constexpr int EL = I8 ? 16 : 8;              // elements of 16 bytes
+    __shared__ __attribute__((aligned(16))) f16 Vs[TW][32][VP];
+    __shared__ f16x8 Qs[KS][64];
+    __shared__ float wm[TW][8], wl[TW][8];
+    static_assert(sizeof(Vs) >= (size_t)TW * 8 * HD * 4, "the merge reuses Vs");
+    const int G = H / c.HKV, groups = c.HKV * ((G + 7) / 8);
+    const int n = blockIdx.x / groups, gr = blockIdx.x % groups, sp = blockIdx.y;
+    const int kvh = gr / ((G + 7) / 8), g8 = 8 * (gr % ((G + 7) / 8)), h0 = kvh * G + g8, nh = min(8, G - g8);
+    const int pos = s.pos[n];
+    if (pos < 0) return;
+    const KeyBlocks<32> kb(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int lr = lane & 15, g = lane >> 4, col = lr & 7;
+    // Key lane % 32 of block j: its row in the planes (any, where it is not seen), its
+    // steps as exponents, and whether it is seen.
+    struct Key {
+        uint32_t row;
+        bool seen;
+    };
+    auto key_of = [&](int j) {
+        const uint32_t kp = kb.start(min(j, kb.n - 1)) + (lane & 31);
+        const int page = page_of(c, s, n, kp);
+        const bool seen = page >= 0 && kp <= (uint32_t)pos && (kp >= kb.lo || kp < kb.sinks);
+        return Key{page >= 0 ? row_at<I8>(c, page, slot_of(c, kp), kvh) : (uint32_t)(I8 ? 0 : kvh), seen};
+    };
+    u32x4 kreg[2][KL], vreg[VCH];
+    uint8_t kx = 0, vx = 0;
+    auto fetch = [&](const Key &k) {
+        if constexpr (I8) {
+            kx = c.kx[k.row / BLK];
+            vx = c.vx[k.row / BLK];
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+            const uint64_t row = (uint32_t)__shfl((int)k.row, 16 * kt + lr, 64);
+#pragma unroll
+            for (int i = 0; i < KL; i++)
+                kreg[kt][i] = *(const u32x4 *)((const char *)c.k + row * (HD * (I8 ? 1 : 2)) + 64 * i + 16 * g);
+        }
+#pragma unroll
+        for (int i = 0; i < VCH; i++) {
+            const uint64_t row = (uint32_t)__shfl((int)k.row, (i * 64 + lane) / CPK, 64);
+            vreg[i] = *(const u32x4 *)((const char *)c.v + row * (HD * (I8 ? 1 : 2)) + 16 * (lane % CPK));
+        }
+    };
+    const int step = ns * TW;
+    int j = sp + ns * w;
+    Key kc = key_of(j), kn = key_of(j + step);
+    float sf;                                    // score factor of this lane's head
+    {
+        const T *qrow = q + n * q_stride + (int64_t)(h0 + min(col, nh - 1)) * HD;
+        // Dim of element e of k step ks: as the cache's 16-byte loads give them.
+        auto dim = [&](int ks) { return I8 ? 64 * (ks / 2) + 16 * g + 8 * (ks % 2) : 32 * ks + 8 * g; };
+        float qv[KS][8], mx = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                qv[ks][e] = to_f32(qrow[dim(ks) + e]);
+                mx = fmaxf(mx, fabsf(qv[ks][e]));
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const int ex = min(max((int)(__float_as_uint(mx) >> 23), 40), 254) - 127;
+        const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+        sf = scale * LOG2E * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+        if (fabsf(sf) < 0x1p-126f) sf = 0x1p-126f;         // weights of 1 alike; times inf not NaN
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            if (ks % TW != w) continue;
+            f16x8 qf;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f16 hi, lo;
+                gd_split_f16(col < nh ? qv[ks][e] * up : 0.f, hi, lo);
+                qf[e] = lr < 8 ? hi : lo;
+            }
+            Qs[ks][lane] = qf;
+        }
+    }
+    if (kb.n) fetch(kc);
+    const float none = sf < 0.f ? INFINITY : -INFINITY;    // the score of no key
+    f32x4 acc[DT];                               // O^T rows 16 dt + 4 g + v
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;                // l: this lane's keys only
+    __syncthreads();
+    for (; j < kb.n; j += step) {
+        // Four chains a key tile: shorter sums round less (and wait less).
+        f32x4 st[2][4];
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const f16x8 qf = Qs[ks][lane];
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                f16x8 kf;
+                if constexpr (I8) kf = halves(kreg[kt][ks / 2][2 * (ks % 2)], kreg[kt][ks / 2][2 * (ks % 2) + 1]);
+                else kf = __builtin_bit_cast(f16x8, kreg[kt][ks]);
+                st[kt][ks & 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        kf, qf, ks < 4 ? f32x4{0.f, 0.f, 0.f, 0.f} : st[kt][ks & 3], 0, 0, 0);
+            }
+        }
+        const uint32_t seen = (uint32_t)__ballot(kc.seen);
+        const int ks_all = kx, vs_all = vx;
+        f32x4 sc[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) sc[kt] = (st[kt][0] + st[kt][1]) + (st[kt][2] + st[kt][3]);
+        // Values to LDS, then the next block's loads.
+#pragma unroll
+        for (int i = 0; i < VCH; i++) {
+            const int k = (i * 64 + lane) / CPK;
+            u32x4 v = vreg[i];
+            if (seen != 0xffffffffu && !(seen >> k & 1)) v = u32x4{0u, 0u, 0u, 0u};
+            f16 *row = &Vs[w][k][EL * (lane % CPK)];
+            if constexpr (I8) {
+                const f16 step = (f16)step_of((uint8_t)__shfl(vs_all, k, 64));
+                const f16 sv = seen >> k & 1 ? step : (f16)0.f;
+                *(f16x8 *)row = halves(v[0], v[1]) * sv;
+                *(f16x8 *)(row + 8) = halves(v[2], v[3]) * sv;
+            } else {
+                *(u32x4 *)row = v;
+            }
+        }
+        const Key k2 = key_of(j + 2 * step);
+        fetch(kn);
+        kc = kn;
+        kn = k2;
+        __builtin_amdgcn_sched_barrier(0);
+        if (!seen) continue;
+        // hi + lo of a head's score; keys 16 kt + 4 g + v of the block.  (Unscaled:
+        // a weight's exponent is rounded once.)
+        float bmax = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const int k = 16 * kt + 4 * g + v;
+                sc[kt][v] += gd_dpp<GD_DPP_ROR8>(sc[kt][v]);
+                if constexpr (I8) sc[kt][v] *= step_of((uint8_t)__shfl(ks_all, k, 64));
+                if (!(seen >> k & 1)) sc[kt][v] = none;
+                bmax = fmaxf(bmax, sc[kt][v] * sf);
+            }
+        bmax = fmaxf(bmax, __shfl_xor(bmax, 16, 64));
+        bmax = fmaxf(bmax, __shfl_xor(bmax, 32, 64));
+        const float mn = fmaxf(m, bmax);
+        if (__any(mn > m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) acc[dt] *= alpha;
+            m = mn;
+        }
+        f16x8 pf;                                // weights times 2^14, and so are l and the sums
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                float p = __builtin_amdgcn_exp2f(fmaf(sc[kt][v], sf, -m)) * 16384.f;
+                asm("" : "+v"(p));
+                l += p;
+                const f16 hi = (f16)p;
+                pf[4 * kt + v] = lr < 8 ? hi : (f16)(p - (float)hi);
+            }
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+            const f16 *vr = &Vs[w][4 * g + (lr >> 2)][16 * dt + 4 * (lr & 3)];
+            const f16x4 v0 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)vr));
+            const f16x4 v1 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 16 * VP)));
+            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]}, pf, acc[dt], 0, 0, 0);
+        }
+    }
+    // Merge the waves: each scales its sums to the common maximum.
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (lane < 8) {
+        wm[w][lane] = m;
+        wl[w][lane] = l;
+    }
+    __syncthreads();
+    float M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < TW; i++) M = fmaxf(M, wm[i][col]);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    float *red = (float *)Vs;                    // [TW][8][HD]
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+        for (int v = 0; v < 4; v++) acc[dt][v] += gd_dpp<GD_DPP_ROR8>(acc[dt][v]);
+        if (lr < 8) *(f32x4 *)&red[(w * 8 + lr) * HD + 16 * dt + 4 * g] = acc[dt] * f;
+    }
+    __syncthreads();
+    auto weight = [&](int i, int hh) { return wm[i][hh] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wm[i][hh] - fmaxf(fmaxf(wm[0][hh], wm[1][hh]), fmaxf(wm[2][hh], wm[3][hh]))); };
+    static_assert(TW == 4, "the waves' maxima");
+    for (int e = t; e < nh * HD; e += 64 * TW) {
+        const int hh = e / HD, d = e % HD;
+        float A = 0.f, L = 0.f;
+#pragma unroll
+        for (int i = 0; i < TW; i++) {
+            A += red[(i * 8 + hh) * HD + d];
+            L += wl[i][hh] * weight(i, hh);
+        }
+        const int64_t row = (int64_t)n * H + h0 + hh;
+        if (ns == 1) {
+            float y = L == 0.f ? 0.f : A / L;
+            if (gate) y *= gd_sigmoid(to_f32(gate[n * gate_stride + (int64_t)(h0 + hh) * HD + d]));
+            out[row * HD + d] = from_f32<T>(y);
+        } else {
+            float *p = part + (row * ns + sp) * (HD + 2);
+            p[d] = A;
+            if (d == 0) {
+                p[HD] = fmaxf(fmaxf(wm[0][hh], wm[1][hh]), fmaxf(wm[2][hh], wm[3][hh]));
+                p[HD + 1] = L;
+            }
+        }
+    }
+}
+
+// Merges the ns <= MAX_SPLITS partials of head h of row n (maxima in units of log2):
+// thread (d, r) takes the splits r, r + NR, .. of one dim, beside the splits' weights,
+// once a workgroup.
+template <int HD, typename T>
+__global__ __launch_bounds__(512) void k_attn_merge(const float *part, int ns, Rows s, const T *gate, int64_t gate_stride,
+                                                    T *out, int H) {
+    constexpr int NR = 512 / HD;
+    __shared__ float fs[MAX_SPLITS], sum[NR][HD];
+    const int n = blockIdx.x / H, h = blockIdx.x % H, t = threadIdx.x, d = t % HD, r = t / HD;
+    if (s.pos[n] < 0) return;
+    const float *p = part + (int64_t)blockIdx.x * ns * (HD + 2);
+    float a[MAX_SPLITS / NR];
+#pragma unroll
+    for (int i = 0; i < MAX_SPLITS / NR; i++) a[i] = r + NR * i < ns ? p[(r + NR * i) * (HD + 2) + d] : 0.f;
+    float inv;
+    {
+        const int lane = t & 63;                 // every wave: the weight of split lane
+        const float ms = lane < ns ? p[lane * (HD + 2) + HD] : -INFINITY;
+        const float ls = lane < ns ? p[lane * (HD + 2) + HD + 1] : 0.f;
+        const float M = wave_max(ms);
+        const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - M);
+        const float L = gd_wave_sum(ls * f);
+        inv = L == 0.f ? 0.f : 1.0f / L;
+        if (t < MAX_SPLITS) fs[t] = f;
+    }
+    __syncthreads();
+    float A = 0.f;
+#pragma unroll
+    for (int i = 0; i < MAX_SPLITS / NR; i++) A += a[i] * fs[r + NR * i];
+    sum[r][d] = A;
+    __syncthreads();
+    if (r) return;
+#pragma unroll
+    for (int i = 1; i < NR; i++) A += sum[i][d];
+    float y = A * inv;
+    if (gate) y *= gd_sigmoid(to_f32(gate[n * gate_stride + (int64_t)h * HD + d]));
+    out[(int64_t)blockIdx.x * HD + d] = from_f32<T>(y);
+}
+
 // ---------------------------------------------------------------- checks
 
 int check_kv(gd_ctx *ctx, const char *fn, const gd_kv *kv, bool planes) {
@@ -421,9 +732,9 @@ int check_kv(gd_ctx *ctx, const char *fn, const gd_kv *kv, bool planes) {
     GD_REQUIRE(ctx, kv->page_size > 0 && kv->page_size <= (1 << 24), "%s: page size %d", fn, kv->page_size);
     GD_REQUIRE(ctx, kv->dtype != GD_I8 || kv->page_size % GD_KV_BLOCK == 0,
                "%s: page size %d of an 8-bit cache is not a multiple of %d", fn, kv->page_size, GD_KV_BLOCK);
-    // At most 2^62 elements, so that no byte offset of the kernels passes 63 bits.
-    const int64_t page = (int64_t)kv->page_size * kv->n_head_kv * kv->head_dim;
-    GD_REQUIRE(ctx, kv->n_pages > 0 && kv->n_pages < (1LL << 31) && kv->n_pages < (1LL << 60) / page,
+    // Rows of head_dim are counted in 32 bits: 512 GiB of codes, more than the card has.
+    const int64_t page = (int64_t)kv->page_size * kv->n_head_kv;
+    GD_REQUIRE(ctx, kv->n_pages > 0 && kv->n_pages < (1LL << 31) && kv->n_pages < (1LL << 32) / page,
                "%s: %lld pages", fn, (long long)kv->n_pages);
     if (!planes) return GD_OK;
     GD_REQUIRE(ctx, kv->k && kv->v && (kv->dtype != GD_I8 || (kv->k_exp && kv->v_exp)), "%s: null cache plane", fn);
@@ -510,11 +821,11 @@ extern "C" int gd_kv_free(gd_ctx *ctx, gd_kv *kv) {
 #define GD_KV_PICK(kv, x_dtype, GO) \
     do { \
         if ((kv)->head_dim == 128) { \
-            if ((kv)->dtype == GD_I8) { if ((x_dtype) == GD_F32) GO(128, true, float); else GO(128, true, uint16_t); } \
-            else { if ((x_dtype) == GD_F32) GO(128, false, float); else GO(128, false, uint16_t); } \
+            if ((kv)->dtype == GD_I8) { if ((x_dtype) == GD_F32) { GO(128, true, float); } else { GO(128, true, uint16_t); } } \
+            else { if ((x_dtype) == GD_F32) { GO(128, false, float); } else { GO(128, false, uint16_t); } } \
         } else { \
-            if ((kv)->dtype == GD_I8) { if ((x_dtype) == GD_F32) GO(256, true, float); else GO(256, true, uint16_t); } \
-            else { if ((x_dtype) == GD_F32) GO(256, false, float); else GO(256, false, uint16_t); } \
+            if ((kv)->dtype == GD_I8) { if ((x_dtype) == GD_F32) { GO(256, true, float); } else { GO(256, true, uint16_t); } } \
+            else { if ((x_dtype) == GD_F32) { GO(256, false, float); } else { GO(256, false, uint16_t); } } \
         } \
     } while (0)
 
@@ -620,6 +931,33 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     if (!s->n_rows || !s->n_seq) return GD_OK;
     GD_HIP(ctx, hipSetDevice(ctx->device));
     const Mask mask{window, window ? n_sink : 0};
+    if (!s->row_start) {
+        const int G = n_head / kv->n_head_kv, groups = kv->n_head_kv * ((G + 7) / 8);
+        const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
+        const Rows rows = rows_of(kv, s);
+        int64_t keys = s->max_len ? std::min<int64_t>(s->max_len, rows.cap) : rows.cap;
+        if (window) keys = std::min(keys, (int64_t)window + 31 + (n_sink + 31) / 32 * 32);
+        const int64_t blocks = (keys + 31) / 32, wgs = s->n_rows * groups;
+        int64_t ns = std::min({blocks, (int64_t)MAX_SPLITS, std::max<int64_t>(1, 2 * cus / wgs),
+                               (int64_t)(GD_ATTN_SCRATCH_BYTES / ((size_t)s->n_rows * n_head * (hd + 2) * sizeof(float)))});
+        float *part = ns > 1 ? gd_attn_scratch(ctx) : nullptr;
+        if (!part) ns = 1;
+#define GD_GO(HD_, I8_, T_) \
+    do { \
+        hipLaunchKernelGGL((k_attn_tokens<HD_, I8_, T_>), dim3((unsigned)wgs, (unsigned)ns), dim3(64 * TW), 0, ctx->stream, \
+                           cache_of(kv), rows, (const T_ *)q, q_stride, (const T_ *)gate, gate_stride, (T_ *)out, part, \
+                           (int)ns, n_head, scale, mask); \
+        if (ns > 1) { \
+            GD_LAUNCHED(ctx, fn); \
+            hipLaunchKernelGGL((k_attn_merge<HD_, T_>), dim3((unsigned)(s->n_rows * n_head)), dim3(512), 0, ctx->stream, \
+                               part, (int)ns, rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head); \
+        } \
+    } while (0)
+        GD_KV_PICK(kv, x_dtype, GD_GO);
+#undef GD_GO
+        GD_LAUNCHED(ctx, fn);
+        return GD_OK;
+    }
     const dim3 grid(gd_blocks(s->n_rows * n_head, 4));
 #define GD_GO(HD_, I8_, T_) \
     hipLaunchKernelGGL((k_attn<HD_, I8_, T_>), grid, dim3(256), 0, ctx->stream, cache_of(kv), rows_of(kv, s), \

@@ -475,6 +475,35 @@ def test_scales(ctx, dtype, scale):
         check_attention(ctx, ATTN[which], dtype, False, 128, 4, 2, 16, 0, 0, False, row_start=which == "later", scale=scale)
 
 
+@pytest.mark.parametrize("x16", [False, True], ids=["f32rows", "f16rows"])
+@pytest.mark.parametrize("which", ["tokens", "ragged"])
+@pytest.mark.parametrize("ks,vs", [((-24, -20), (5, 10)), ((8, 10), (-24, -19)), ((-24, 10), (-24, 10))])
+def test_steps_of_the_whole_range(ctx, x16, which, ks, vs):
+    """8-bit blocks of all steps, every code among them, beside each other."""
+    hd, H, hkv, seqs = 128, 4, 2, ATTN[which]
+    with Batch(ctx, seqs, ga.I8, hkv, hd, 16, row_start=which == "ragged") as bt:
+        rng, KV = bt.rng, [[], []]
+        planes = [rng.integers(-127, 128, (bt.pages, hkv, 16, hd)).astype(np.int8) for _ in "kv"]
+        planes += [(127 + rng.integers(*e, (bt.pages, hkv, 1))).astype(np.uint8) for e in (ks, vs)]
+        for p, a in zip((bt.kv.k, bt.kv.v, bt.kv.k_exp, bt.kv.v_exp), planes):
+            ctx.set(p, a)
+        q = rows_of(rng, (bt.n, H, hd), x16)
+        dq, do = bt.put(raw(q)), bt.put(raw(np.zeros_like(q)))
+        # Scores of up to some tens, whatever the keys' steps.
+        scale = float(np.float32(2.0 ** (-ks[1] - 6)))
+        ctx.gd_kv_attn(*bt.ref, dq, H * hd, None, 0, do, ga.F16 if x16 else ga.F32, H, scale, 0, 0)
+        got = ctx.get(do, q.shape, q.dtype)
+        for b, (p, r) in enumerate(seqs):
+            t = np.arange(max(p + r, 0))
+            K, V = (planes[c][bt.table[b, t // 16], :, t % 16] * 2.0 ** (
+                planes[2 + c][bt.table[b, t // 16], :, 0].astype(np.float64)[..., None] - 127) for c in range(2))
+            rows = slice(bt.start[b], bt.start[b] + (r if p >= 0 else 0))
+            want = attend(q[rows], K, V, p, scale, 0, 0, None)
+            err = np.abs(got[rows] - want).max(initial=0)
+            # f16 rows: results under 2^-14 are rounded to steps of 2^-24
+            assert err <= bound(q[rows], K, V, scale, x16) + (2.0 ** -25 if x16 else 0), (b, err)
+
+
 @pytest.mark.parametrize("dtype", [ga.I8, ga.F16], ids=["i8", "f16"])
 @pytest.mark.parametrize("x16", [False, True], ids=["f32rows", "f16rows"])
 @pytest.mark.parametrize("hd", [128, 256])
