@@ -437,11 +437,14 @@ template <int W> struct KeyBlocks {
         n = ns + (lo <= last ? (int)(last / W - lo / W + 1) : 0);
     }
     __device__ __forceinline__ uint32_t start(int j) const { return (uint32_t)(j < ns ? j : j - ns + (int)(lo / W)) * W; }
+    // Splits that these blocks are worked in: of `least` blocks or more, `most` at most.
+    __device__ __forceinline__ int splits(int most, int least) const { return max(1, min(most, (n + least - 1) / least)); }
 };
 
 // Attention of single tokens: workgroup (row, kv head and eight of its query heads;
-// split sp of ns) reads the split's keys once for its heads.  Wave w takes the blocks
-// of 32 keys sp + ns (w + TW i): S = K Q^T with K straight from the cache as the A
+// split sp) reads the split's keys once for its heads.  A row's blocks of 32 keys go to
+// as many of the `most` splits as leave each `least` of them (the other workgroups end
+// at once): ns splits, and wave w of split sp takes the blocks sp + ns (w + TW i): S = K Q^T with K straight from the cache as the A
 // operand, and O^T += V^T P^T with V staged in the wave's own LDS rows and read by the
 // transposing LDS read (no barrier in the loop).  The 16 columns of an MFMA are the
 // heads' q as f16 hi (0..7) and lo (8..15), and P likewise: both halves of a product
@@ -455,10 +458,10 @@ constexpr int TW = 4;                            // waves
 constexpr int MAX_SPLITS = 64;                   // what the combine weighs in one wave
 constexpr float LOG2E = 1.4426950408889634f;
 
-template <int HD, bool I8, typename T>
+template <int HD, bool I8, bool TILED, typename T>
 __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_tokens(
-        Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, float *part, int ns,
-        int H, float scale, Mask mask) {
+        Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, float *part, int most,
+        int least, int H, float scale, Mask mask) {
     constexpr int KS = HD / 32, DT = HD / 16, VP = HD + 16;
     constexpr int KL = I8 ? KS / 2 : KS;         // 16-byte loads of a key tile, per lane
     constexpr int CPK = I8 ? HD / 16 : HD / 8;   // 16-byte chunks of a value row
@@ -474,20 +477,36 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int pos = s.pos[n];
     if (pos < 0) return;
     const KeyBlocks<32> kb(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
+    const int ns = kb.splits(most, least);
+    if (sp >= ns) return;
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int lr = lane & 15, g = lane >> 4, col = lr & 7;
-    // Key lane % 32 of block j: its row in the planes (any, where it is not seen), its
-    // steps as exponents, and whether it is seen.
+    // Key lane % 32 of block j: its page-table entry (a load, used a block later), then its
+    // row in the planes (any, where there is none) and whether it is seen.
+    struct Entry {
+        uint32_t kp;
+        int page;
+    };
     struct Key {
         uint32_t row;
         bool seen;
     };
-    auto key_of = [&](int j) {
+    const int32_t *table = s.table + (int64_t)n * s.max_pages;
+    auto entry_of = [&](int j) {
         const uint32_t kp = kb.start(min(j, kb.n - 1)) + (lane & 31);
-        const int page = page_of(c, s, n, kp);
-        const bool seen = page >= 0 && kp <= (uint32_t)pos && (kp >= kb.lo || kp < kb.sinks);
-        return Key{page >= 0 ? row_at<I8>(c, page, slot_of(c, kp), kvh) : (uint32_t)(I8 ? 0 : kvh), seen};
+        return Entry{kp, table[c.by_page(min(kp, s.cap - 1))]};
     };
+    auto key_of = [&](const Entry &e) {
+        const bool there = (uint32_t)e.page < c.n_pages && e.kp < s.cap;
+        return Key{there ? row_at<I8>(c, e.page, slot_of(c, e.kp), kvh) : (uint32_t)(I8 ? 0 : kvh),
+                   there && e.kp <= (uint32_t)pos && (e.kp >= kb.lo || e.kp < kb.sinks)};
+    };
+    // Bytes from a row to the next position's, and this lane's place in the 16 keys of a
+    // tile (keys) and in those of a load of values: with pages of whole tiles a tile has one
+    // page and one step, so that its loads take a uniform base.
+    constexpr int ES = I8 ? 1 : 2, KPV = 64 / CPK;
+    const uint32_t pitch = HD * ES * (I8 ? 1 : c.HKV);
+    const uint32_t kplace = lr * pitch + 16 * g, vplace = lane / CPK * pitch + 16 * (lane % CPK);
     u32x4 kreg[2][KL], vreg[VCH];
     uint8_t kx = 0, vx = 0;
     auto fetch = [&](const Key &k) {
@@ -495,22 +514,36 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             kx = c.kx[k.row / BLK];
             vx = c.vx[k.row / BLK];
         }
+        if constexpr (TILED) {
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-            const uint64_t row = (uint32_t)__shfl((int)k.row, 16 * kt + lr, 64);
+            for (int kt = 0; kt < 2; kt++) {
+                const uint64_t row = (uint32_t)__builtin_amdgcn_readlane((int)k.row, 16 * kt);
+                const char *kp = (const char *)c.k + row * (HD * ES), *vp = (const char *)c.v + row * (HD * ES);
 #pragma unroll
-            for (int i = 0; i < KL; i++)
-                kreg[kt][i] = *(const u32x4 *)((const char *)c.k + row * (HD * (I8 ? 1 : 2)) + 64 * i + 16 * g);
-        }
+                for (int i = 0; i < KL; i++) kreg[kt][i] = *(const u32x4 *)(kp + kplace + 64 * i);
 #pragma unroll
-        for (int i = 0; i < VCH; i++) {
-            const uint64_t row = (uint32_t)__shfl((int)k.row, (i * 64 + lane) / CPK, 64);
-            vreg[i] = *(const u32x4 *)((const char *)c.v + row * (HD * (I8 ? 1 : 2)) + 16 * (lane % CPK));
+                for (int i = kt * VCH / 2; i < (kt + 1) * VCH / 2; i++)
+                    vreg[i] = *(const u32x4 *)(vp + (uint32_t)(vplace + i * KPV % 16 * pitch));
+            }
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                const uint64_t row = (uint32_t)__shfl((int)k.row, 16 * kt + lr, 64);
+#pragma unroll
+                for (int i = 0; i < KL; i++) kreg[kt][i] = *(const u32x4 *)((const char *)c.k + row * (HD * ES) + 64 * i + 16 * g);
+            }
+#pragma unroll
+            for (int i = 0; i < VCH; i++) {
+                const uint64_t row = (uint32_t)__shfl((int)k.row, i * KPV + lane / CPK, 64);
+                vreg[i] = *(const u32x4 *)((const char *)c.v + row * (HD * ES) + 16 * (lane % CPK));
+            }
         }
     };
     const int step = ns * TW;
     int j = sp + ns * w;
-    Key kc = key_of(j), kn = key_of(j + step);
+    Entry en = entry_of(j);
+    Key kc = key_of(en);
+    en = entry_of(j + step);
     float sf;                                    // score factor of this lane's head
     {
         const T *qrow = q + n * q_stride + (int64_t)(h0 + min(col, nh - 1)) * HD;
@@ -566,30 +599,37 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             }
         }
         const uint32_t seen = (uint32_t)__ballot(kc.seen);
-        const int ks_all = kx, vs_all = vx;
+        float kstep[2];
+        f16 vstep[2];
+#pragma unroll
+        for (int kt = 0; kt < (I8 ? 2 : 0); kt++) {
+            kstep[kt] = step_of((uint8_t)__builtin_amdgcn_readlane(kx, 16 * kt));
+            vstep[kt] = (f16)step_of((uint8_t)__builtin_amdgcn_readlane(vx, 16 * kt));
+        }
         f32x4 sc[2];
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) sc[kt] = (st[kt][0] + st[kt][1]) + (st[kt][2] + st[kt][3]);
         // Values to LDS, then the next block's loads.
 #pragma unroll
         for (int i = 0; i < VCH; i++) {
-            const int k = (i * 64 + lane) / CPK;
-            u32x4 v = vreg[i];
-            if (seen != 0xffffffffu && !(seen >> k & 1)) v = u32x4{0u, 0u, 0u, 0u};
+            const int k = i * KPV + lane / CPK;
             f16 *row = &Vs[w][k][EL * (lane % CPK)];
+            f16x8 v[I8 ? 2 : 1];
             if constexpr (I8) {
-                const f16 step = (f16)step_of((uint8_t)__shfl(vs_all, k, 64));
-                const f16 sv = seen >> k & 1 ? step : (f16)0.f;
-                *(f16x8 *)row = halves(v[0], v[1]) * sv;
-                *(f16x8 *)(row + 8) = halves(v[2], v[3]) * sv;
+                v[0] = halves(vreg[i][0], vreg[i][1]) * vstep[2 * i / VCH];
+                v[1] = halves(vreg[i][2], vreg[i][3]) * vstep[2 * i / VCH];
             } else {
-                *(u32x4 *)row = v;
+                v[0] = __builtin_bit_cast(f16x8, vreg[i]);
             }
+            if (seen != 0xffffffffu && !(seen >> k & 1))
+#pragma unroll
+                for (int x = 0; x < (I8 ? 2 : 1); x++) v[x] = f16x8{};
+#pragma unroll
+            for (int x = 0; x < (I8 ? 2 : 1); x++) *(f16x8 *)(row + 8 * x) = v[x];
         }
-        const Key k2 = key_of(j + 2 * step);
-        fetch(kn);
-        kc = kn;
-        kn = k2;
+        kc = key_of(en);
+        en = entry_of(j + 2 * step);
+        fetch(kc);
         __builtin_amdgcn_sched_barrier(0);
         if (!seen) continue;
         // hi + lo of a head's score; keys 16 kt + 4 g + v of the block.  (Unscaled:
@@ -601,8 +641,8 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             for (int v = 0; v < 4; v++) {
                 const int k = 16 * kt + 4 * g + v;
                 sc[kt][v] += gd_dpp<GD_DPP_ROR8>(sc[kt][v]);
-                if constexpr (I8) sc[kt][v] *= step_of((uint8_t)__shfl(ks_all, k, 64));
-                if (!(seen >> k & 1)) sc[kt][v] = none;
+                if constexpr (I8) sc[kt][v] *= kstep[kt];
+                if (seen != 0xffffffffu && !(seen >> k & 1)) sc[kt][v] = none;
                 bmax = fmaxf(bmax, sc[kt][v] * sf);
             }
         bmax = fmaxf(bmax, __shfl_xor(bmax, 16, 64));
@@ -673,7 +713,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             if (gate) y *= gd_sigmoid(to_f32(gate[n * gate_stride + (int64_t)(h0 + hh) * HD + d]));
             out[row * HD + d] = from_f32<T>(y);
         } else {
-            float *p = part + (row * ns + sp) * (HD + 2);
+            float *p = part + (row * most + sp) * (HD + 2);
             p[d] = A;
             if (d == 0) {
                 p[HD] = fmaxf(fmaxf(wm[0][hh], wm[1][hh]), fmaxf(wm[2][hh], wm[3][hh]));
@@ -683,17 +723,20 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
 }
 
-// Merges the ns <= MAX_SPLITS partials of head h of row n (maxima in units of log2):
+// Merges the partials (up to `most` <= MAX_SPLITS) of head h of row n (maxima in units of log2):
 // thread (d, r) takes the splits r, r + NR, .. of one dim, beside the splits' weights,
 // once a workgroup.
 template <int HD, typename T>
-__global__ __launch_bounds__(512) void k_attn_merge(const float *part, int ns, Rows s, const T *gate, int64_t gate_stride,
-                                                    T *out, int H) {
+__global__ __launch_bounds__(512) void k_attn_merge(const float *part, int most, int least, Rows s, const T *gate,
+                                                    int64_t gate_stride, T *out, int H, Mask mask) {
     constexpr int NR = 512 / HD;
     __shared__ float fs[MAX_SPLITS], sum[NR][HD];
     const int n = blockIdx.x / H, h = blockIdx.x % H, t = threadIdx.x, d = t % HD, r = t / HD;
-    if (s.pos[n] < 0) return;
-    const float *p = part + (int64_t)blockIdx.x * ns * (HD + 2);
+    const int pos = s.pos[n];
+    if (pos < 0) return;
+    const int ns = KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1)).splits(most, least);
+    if (ns == 1) return;
+    const float *p = part + (int64_t)blockIdx.x * most * (HD + 2);
     float a[MAX_SPLITS / NR];
 #pragma unroll
     for (int i = 0; i < MAX_SPLITS / NR; i++) a[i] = r + NR * i < ns ? p[(r + NR * i) * (HD + 2) + d] : 0.f;
@@ -938,19 +981,21 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
         int64_t keys = s->max_len ? std::min<int64_t>(s->max_len, rows.cap) : rows.cap;
         if (window) keys = std::min(keys, (int64_t)window + 31 + (n_sink + 31) / 32 * 32);
         const int64_t blocks = (keys + 31) / 32, wgs = s->n_rows * groups;
-        int64_t ns = std::min({blocks, (int64_t)MAX_SPLITS, std::max<int64_t>(1, 2 * cus / wgs),
+        const int64_t least = std::max<int64_t>(TW, wgs * blocks / (8 * cus));
+        int64_t ns = std::min({(blocks + least - 1) / least, (int64_t)MAX_SPLITS,
                                (int64_t)(GD_ATTN_SCRATCH_BYTES / ((size_t)s->n_rows * n_head * (hd + 2) * sizeof(float)))});
         float *part = ns > 1 ? gd_attn_scratch(ctx) : nullptr;
         if (!part) ns = 1;
 #define GD_GO(HD_, I8_, T_) \
     do { \
-        hipLaunchKernelGGL((k_attn_tokens<HD_, I8_, T_>), dim3((unsigned)wgs, (unsigned)ns), dim3(64 * TW), 0, ctx->stream, \
-                           cache_of(kv), rows, (const T_ *)q, q_stride, (const T_ *)gate, gate_stride, (T_ *)out, part, \
-                           (int)ns, n_head, scale, mask); \
+        auto kernel = I8_ || kv->page_size % 16 == 0 ? k_attn_tokens<HD_, I8_, true, T_> : k_attn_tokens<HD_, I8_, I8_, T_>; \
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs, (unsigned)ns), dim3(64 * TW), 0, ctx->stream, cache_of(kv), rows, \
+                           (const T_ *)q, q_stride, (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)least, \
+                           n_head, scale, mask); \
         if (ns > 1) { \
             GD_LAUNCHED(ctx, fn); \
             hipLaunchKernelGGL((k_attn_merge<HD_, T_>), dim3((unsigned)(s->n_rows * n_head)), dim3(512), 0, ctx->stream, \
-                               part, (int)ns, rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head); \
+                               part, (int)ns, (int)least, rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head, mask); \
         } \
     } while (0)
         GD_KV_PICK(kv, x_dtype, GD_GO);
