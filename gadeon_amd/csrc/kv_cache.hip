@@ -343,72 +343,6 @@ struct Mask {
     int window, sinks;                           // window 0: every key up to the query's own
 };
 
-// A wave for each (row, query head), a key at a time: the visible keys are the
-// sinks [0, min(n_sink, lo)) and [lo, p], lo = max(0, p - window + 1).
-template <int HD, bool I8, typename T>
-__global__ __launch_bounds__(256) void k_attn(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate,
-                                              int64_t gate_stride, T *out, int H, float scale, Mask mask) {
-    constexpr int DPL = HD / 64;
-    const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, n = (int)(u / H), h = (int)(u % H);
-    if (n >= s.n_rows) return;
-    const int b = seq_of_row(s, n);
-    if (b < 0) return;
-    const Seq sq = seq_at(s, b);
-    if (n < sq.r0 || n >= sq.r1) return;
-    const uint32_t p = min((uint32_t)sq.pos + (uint32_t)(n - sq.r0), s.cap - 1);
-    const uint32_t at = (uint32_t)sq.pos + (uint32_t)(n - sq.r0);
-    const uint32_t lo = mask.window && at >= (uint32_t)mask.window ? at - mask.window + 1 : 0;
-    const uint32_t sinks = min((uint32_t)mask.sinks, lo);
-    const int kvh = h / (H / c.HKV);
-    float qv[DPL], acc[DPL], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < DPL; e++) {
-        qv[e] = to_f32(q[n * q_stride + (int64_t)h * HD + DPL * lane + e]) * scale;
-        acc[e] = 0.f;
-    }
-    for (uint32_t t = sinks ? 0 : lo; t <= p; t = t + 1 == sinks ? max(lo, sinks) : t + 1) {
-        const int page = page_of(c, s, b, t), slot = slot_of(c, t);
-        if (page < 0) continue;
-        float kf[DPL], vf[DPL];
-        const uint32_t row = row_at<I8>(c, page, slot, kvh);
-        if constexpr (I8) {
-            const uint64_t at8 = (uint64_t)row * HD + DPL * lane;
-            const float ks = step_of(c.kx[row / BLK]), vs = step_of(c.vx[row / BLK]);
-#pragma unroll
-            for (int e = 0; e < DPL; e++) {
-                kf[e] = (float)((const int8_t *)c.k)[at8 + e] * ks;
-                vf[e] = (float)((const int8_t *)c.v)[at8 + e] * vs;
-            }
-        } else {
-            const uint64_t at16 = (uint64_t)row * HD + DPL * lane;
-#pragma unroll
-            for (int e = 0; e < DPL; e++) {
-                kf[e] = gd_h2f(((const uint16_t *)c.k)[at16 + e]);
-                vf[e] = gd_h2f(((const uint16_t *)c.v)[at16 + e]);
-            }
-        }
-        float d = 0.f;
-#pragma unroll
-        for (int e = 0; e < DPL; e++) d += qv[e] * kf[e];
-        d = gd_wave_sum(d);
-        const float mn = fmaxf(m, d), al = m == -INFINITY ? 0.f : expf(m - mn);
-        const float w = d == -INFINITY ? 0.f : expf(d - mn);
-        l = l * al + w;
-#pragma unroll
-        for (int e = 0; e < DPL; e++) acc[e] = acc[e] * al + w * vf[e];
-        m = mn;
-    }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    const int64_t o = ((int64_t)n * H + h) * HD + DPL * lane;
-#pragma unroll
-    for (int e = 0; e < DPL; e++) {
-        float y = acc[e] * inv;
-        if (gate) y *= gd_sigmoid(to_f32(gate[n * gate_stride + (int64_t)h * HD + DPL * lane + e]));
-        out[o + e] = from_f32<T>(y);
-    }
-}
-
 // Four codes as two pairs of halves: byte c ^ 0x80 below 0x64 is the half 1152 + c.
 __device__ __forceinline__ void halves(uint32_t codes, f16x2 &a, f16x2 &b) {
     const uint32_t x = codes ^ 0x80808080u;
@@ -441,6 +375,13 @@ template <int W> struct KeyBlocks {
     __device__ __forceinline__ int splits(int most, int least) const { return max(1, min(most, (n + least - 1) / least)); }
 };
 
+// Partials of the key splits: sums of head h of row n, split z, at acc [n H + h][most][HD]
+// and its (maximum, sum of weights) at ml [n H + h][most], maxima in units of log2.
+struct Part {
+    float *acc;
+    float2 *ml;
+};
+
 // Attention of single tokens: workgroup (row, kv head and eight of its query heads;
 // split sp) reads the split's keys once for its heads.  A row's blocks of 32 keys go to
 // as many of the `most` splits as leave each `least` of them (the other workgroups end
@@ -460,7 +401,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 template <int HD, bool I8, bool TILED, typename T>
 __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_tokens(
-        Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, float *part, int most,
+        Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part, int most,
         int least, int H, float scale, Mask mask) {
     constexpr int KS = HD / 32, DT = HD / 16, VP = HD + 16;
     constexpr int KL = I8 ? KS / 2 : KS;         // 16-byte loads of a key tile, per lane
@@ -713,41 +654,363 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             if (gate) y *= gd_sigmoid(to_f32(gate[n * gate_stride + (int64_t)(h0 + hh) * HD + d]));
             out[row * HD + d] = from_f32<T>(y);
         } else {
-            float *p = part + (row * most + sp) * (HD + 2);
-            p[d] = A;
-            if (d == 0) {
-                p[HD] = fmaxf(fmaxf(wm[0][hh], wm[1][hh]), fmaxf(wm[2][hh], wm[3][hh]));
-                p[HD + 1] = L;
-            }
+            part.acc[(row * most + sp) * HD + d] = A;
+            if (d == 0)
+                part.ml[row * most + sp] = make_float2(fmaxf(fmaxf(wm[0][hh], wm[1][hh]), fmaxf(wm[2][hh], wm[3][hh])), L);
         }
     }
 }
 
-// Merges the partials (up to `most` <= MAX_SPLITS) of head h of row n (maxima in units of log2):
-// thread (d, r) takes the splits r, r + NR, .. of one dim, beside the splits' weights,
-// once a workgroup.
+// Attention of prompt chunks (rows of any length): a unit is PC columns of a sequence
+// and kv head, a column being one (row, query head) of the kv head's G heads, row by
+// row, so that a tile of keys read once serves all of them; wave w owns columns 32 w ..
+// Keys stream through LDS as halves in tiles of AK, requested a tile ahead; per tile a
+// wave forms S^T = K Q^T (v_mfma_f32_32x32x16_f16: lane = a column and 16 of each 32 keys),
+// its columns' online softmax, and O^T += V^T P^T, the C layout of S^T being the B operand
+// of P^T once the MFMA's K index 8 h + e (h = lane / 32) stands for key 4 h + e (e < 4) or
+// 8 + 4 h + e - 4 of its 16; V^T is read by the transposing LDS read.  f32 rows enter as
+// f16 hi + lo pairs (q brought to 2^14 .. 2^15 by a power of two a column, weights to
+// 2^14), f16 rows as they are, with weights rounded to f16: 2^-12 of each, less than the
+// result's own rounding.  A tile that some column does not see whole goes key by key: a
+// mask, and where V holds a NaN or infinity its finite part and, apart, which columns see
+// the others (0 x NaN would reach them all).
+constexpr int PC = 128;                          // columns of a unit
+template <int HD> constexpr int tile_keys() { return HD == 128 ? 64 : 32; }
+
+struct Tile {
+    int i0, i1;                                  // the unit's first and last row of its sequence
+};
+__device__ __forceinline__ Tile tile_at(int k, int rows, int G) {
+    return Tile{k * PC / G, min((k * PC + PC - 1) / G, rows - 1)};
+}
+
+template <int HD, bool I8, bool TILED, typename T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 && sizeof(T) == 4 ? 1 : 2)))
+void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part,
+                 int most, int least, int H, float scale, Mask mask) {
+    constexpr bool HL = sizeof(T) == 4;          // hi + lo
+    constexpr int AK = tile_keys<HD>(), NT = AK / 32, KS = HD / 16, DT = HD / 32;
+    constexpr int ES = I8 ? 1 : 2, CPR = HD * ES / 16;   // 16-byte chunks of a row
+    constexpr int CH = AK * CPR / 256, KPP = 256 / CPR;  // chunks a thread stages of K (and of V); keys of a pass
+    constexpr int KP = HD + 8, VP = HD + 16;
+    __shared__ __attribute__((aligned(16))) f16 Ks[AK][KP];
+    __shared__ __attribute__((aligned(16))) f16 Vs[AK][VP];
+    __shared__ int bad[2];
+    const int G = H / c.HKV, kvh = blockIdx.x % c.HKV;
+    int b, k;
+    auto units = [&](const Seq &q) { return (int)(((int64_t)(q.r1 - q.r0) * G + PC - 1) / PC); };
+    if (!unit_at(s, blockIdx.x / c.HKV, units, b, k)) return;
+    const Seq sq = seq_at(s, b);
+    const int rows = sq.r1 - sq.r0;
+    k = units(sq) - 1 - k;                       // the units that see the most keys first
+    const Tile tl = tile_at(k, rows, G);
+    const uint32_t p0 = (uint32_t)sq.pos, cap1 = s.cap - 1;
+    const KeyBlocks<AK> kb(mask, p0 + tl.i0, min(p0 + tl.i1, cap1));
+    const int nz = kb.splits(most, least), z = blockIdx.y;
+    if (z >= nz) return;
+    const int per = (kb.n + nz - 1) / nz, jend = min(kb.n, (z + 1) * per);
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int lc = lane & 31, h = lane >> 5;
+    // This lane's column, and the positions that the wave's columns stand at.
+    const int col = k * PC + 32 * w + lc, i = min(col / G, rows - 1);
+    const bool valid = col < rows * G;
+    const int head = kvh * G + (valid ? col % G : G - 1);
+    const int64_t n = sq.r0 + i;
+    const uint32_t p = p0 + i;
+    const bool busy = k * PC + 32 * w < rows * G;
+    const uint32_t plo = p0 + min((k * PC + 32 * w) / G, rows - 1), phi = p0 + min((k * PC + 32 * w + 31) / G, rows - 1);
+    // Staging: key lane % AK's page-table entry a tile ahead of its row, that a tile ahead of use.
+    const int32_t *table = s.table + (int64_t)b * s.max_pages;
+    struct Entry {
+        uint32_t kp;
+        int page;
+    };
+    auto entry_of = [&](int j) {
+        const uint32_t kp = kb.start(min(j, kb.n - 1)) + (lane & (AK - 1));
+        return Entry{kp, table[c.by_page(min(kp, cap1))]};
+    };
+    u32x4 kr[CH], vr[CH];
+    int kx[I8 ? CH : 1], vx[I8 ? CH : 1];
+    uint64_t here;                               // keys of the tile whose pages are there
+    auto fetch = [&](const Entry &e) {
+        const bool there = (uint32_t)e.page < c.n_pages && e.kp < s.cap && e.kp <= p0 + tl.i1;
+        const uint32_t row = there ? row_at<I8>(c, e.page, slot_of(c, e.kp), kvh) : (uint32_t)(I8 ? 0 : kvh);
+        here = __ballot(there);
+#pragma unroll
+        for (int x = 0; x < CH; x++) {
+            const int key = x * KPP + t / CPR;
+            const uint64_t kr_ = (uint32_t)__shfl((int)row, key, 64);
+            kr[x] = *(const u32x4 *)((const char *)c.k + kr_ * (HD * ES) + 16 * (t % CPR));
+            vr[x] = *(const u32x4 *)((const char *)c.v + kr_ * (HD * ES) + 16 * (t % CPR));
+            if constexpr (I8) {
+                kx[x] = c.kx[kr_ / BLK];
+                vx[x] = c.vx[kr_ / BLK];
+            }
+        }
+    };
+    if (t < 2) bad[t] = 0;
+    int j = z * per;
+    Entry en = entry_of(j);
+    if (j < jend) fetch(en);
+    en = entry_of(j + 1);
+    // B operand of S^T: dims 16 ks + 8 h + e of the lane's column; the sign of the scale
+    // goes into it, so that the greatest product is the greatest score.
+    f16x8 qh[KS], ql[HL ? KS : 1];
+    float sf = fabsf(scale) * LOG2E;
+    {
+        const T *qrow = q + n * q_stride + (int64_t)head * HD + 8 * h;
+        const bool neg = scale < 0.f;
+        if constexpr (HL) {
+            f32x4 x[KS][2];
+            float mx = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    x[ks][y] = *(const f32x4 *)(qrow + 16 * ks + 4 * y);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[ks][y][e]));
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const int ex = min(max((int)(__float_as_uint(mx) >> 23), 40), 254) - 127;
+            const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23) * (neg ? -1.f : 1.f);
+            sf *= __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    f16 hi, lo;
+                    gd_split_f16(x[ks][e >> 2][e & 3] * up, hi, lo);
+                    qh[ks][e] = hi;
+                    ql[ks][e] = lo;
+                }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                u32x4 x = *(const u32x4 *)(qrow + 16 * ks);
+                if (neg) x ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+                qh[ks] = __builtin_bit_cast(f16x8, x);
+            }
+        }
+    }
+    f32x16 acc[DT];                              // O^T dims 32 dt + 8 (v / 4) + 4 h + v % 4
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) acc[dt] = f32x16{};
+    float m = -INFINITY, l = 0.f;                // l: this lane's keys only
+    for (; j < jend; j++) {
+        const uint32_t k0 = kb.start(j);
+        const uint64_t all = AK == 64 ? ~0ull : 0xffffffffull;
+        const uint64_t now = here & all;
+        // Whether every column of the unit sees the whole tile; else keys may be masked.
+        const bool whole = now == all && k0 + AK - 1 <= p0 + tl.i0 &&
+                           (!mask.window || k0 + mask.window > p0 + tl.i1 || k0 + AK <= (uint32_t)mask.sinks);
+        __syncthreads();
+        bool odd = false;
+#pragma unroll
+        for (int x = 0; x < CH; x++) {
+            const int key = x * KPP + t / CPR, d = t % CPR * (16 / ES);
+            const bool in = now >> key & 1;
+            if constexpr (I8) {
+                const f16 ka = (f16)step_of((uint8_t)kx[x]), va = (f16)step_of((uint8_t)vx[x]);
+                *(f16x8 *)&Ks[key][d] = halves(kr[x][0], kr[x][1]) * ka;
+                *(f16x8 *)&Ks[key][d + 8] = halves(kr[x][2], kr[x][3]) * ka;
+                *(f16x8 *)&Vs[key][d] = in ? halves(vr[x][0], vr[x][1]) * va : f16x8{};
+                *(f16x8 *)&Vs[key][d + 8] = in ? halves(vr[x][2], vr[x][3]) * va : f16x8{};
+                odd |= in && vx[x] == EXP_NAN;
+            } else {
+                *(u32x4 *)&Ks[key][d] = kr[x];
+                *(u32x4 *)&Vs[key][d] = in ? vr[x] : u32x4{0u, 0u, 0u, 0u};
+                if (!whole)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) odd |= in && (((vr[x][e] & 0x7c007c00u) + 0x04000400u) & 0x80008000u);
+            }
+        }
+        if (!whole && odd) bad[j & 1] = 1;
+        __syncthreads();
+        const bool nan_tile = !whole && bad[j & 1];
+        if (t == 0) bad[~j & 1] = 0;
+        fetch(en);
+        en = entry_of(j + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        // The wave's own view of the tile.
+        if (!busy || k0 > phi) continue;
+        if (mask.window && k0 + AK - 1 + mask.window <= plo && k0 >= (uint32_t)mask.sinks) continue;
+        const bool full = now == all && k0 + AK - 1 <= plo &&
+                          (!mask.window || k0 + mask.window > phi || k0 + AK <= (uint32_t)mask.sinks);
+        f32x16 st[NT];
+#pragma unroll
+        for (int kt = 0; kt < NT; kt++) {
+            st[kt] = f32x16{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const f16x8 ka = *(const f16x8 *)&Ks[32 * kt + lc][16 * ks + 8 * h];
+                st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[ks], st[kt], 0, 0, 0);
+                if constexpr (HL) st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[ks], st[kt], 0, 0, 0);
+            }
+        }
+        // Keys 32 kt + 8 (v / 4) + 4 h + v % 4 that this column sees, a bit each.
+        uint32_t sees[NT];
+#pragma unroll
+        for (int kt = 0; kt < NT; kt++) {
+            sees[kt] = 0xffffu;
+            if (!full) {
+                sees[kt] = 0;
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int key = 32 * kt + 8 * (v / 4) + 4 * h + v % 4;
+                    const uint32_t kp = k0 + key;
+                    const bool see = kp <= p && (!mask.window || kp + mask.window > p || kp < (uint32_t)mask.sinks) &&
+                                     (now >> key & 1);
+                    sees[kt] |= (uint32_t)see << v;
+                    if (!see) st[kt][v] = -INFINITY;
+                }
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < NT; kt++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) top = fmaxf(top, st[kt][v]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mn = fmaxf(m, top == -INFINITY ? -INFINITY : top * sf);
+        if (__any(mn > m)) {
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) acc[dt] *= alpha;
+            m = mn;
+        }
+        // Weights times 2^14 (f16 rows: in the exponent, where 32-bit rows would lose bits).
+        const float off = m == -INFINITY ? 0.f : HL ? -m : 14.f - m;
+        f16x8 ph[2 * NT], pl[HL ? 2 * NT : 1];
+#pragma unroll
+        for (int kt = 0; kt < NT; kt++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                float w_ = __builtin_amdgcn_exp2f(fmaf(st[kt][v], sf, off));
+                if (!full && !(sees[kt] >> v & 1)) w_ = 0.f;
+                if constexpr (HL) {
+                    w_ *= 16384.f;
+                    asm("" : "+v"(w_));
+                }
+                l += w_;
+                const f16 hi = (f16)w_;
+                ph[2 * kt + v / 8][v % 8] = hi;
+                if constexpr (HL) pl[2 * kt + v / 8][v % 8] = (f16)(w_ - (float)hi);
+            }
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        auto values = [&](int kk, int dt) {      // V^T of keys 16 kk .., dims 32 dt + lane % 32
+            const f16 *v = &Vs[16 * kk + 4 * h + (lane >> 2 & 3)][32 * dt + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
+            const f16x4 v0 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v));
+            const f16x4 v1 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 8 * VP)));
+            return f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        };
+        if (!nan_tile || full) {
+#pragma unroll
+            for (int kk = 0; kk < 2 * NT; kk++)
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    const f16x8 va = values(kk, dt);
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[kk], acc[dt], 0, 0, 0);
+                    if constexpr (HL) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[kk], acc[dt], 0, 0, 0);
+                }
+            continue;
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2 * NT; kk++) {
+            f16x8 see;
+#pragma unroll
+            for (int e = 0; e < 8; e++) see[e] = sees[kk / 2] >> (8 * (kk & 1) + e) & 1 ? (f16)1.f : (f16)0.f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                f16x8 va = values(kk, dt), vn;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const bool fin = (__builtin_bit_cast(uint16_t, (f16)va[e]) & 0x7c00u) != 0x7c00u;
+                    vn[e] = fin ? (f16)0.f : (f16)1.f;
+                    va[e] = fin ? va[e] : (f16)0.f;
+                }
+                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[kk], acc[dt], 0, 0, 0);
+                if constexpr (HL) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[kk], acc[dt], 0, 0, 0);
+                const f32x16 count = __builtin_amdgcn_mfma_f32_32x32x16_f16(vn, see, f32x16{}, 0, 0, 0);
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    if (count[v] > 0.f) acc[dt][v] = __uint_as_float(0x7fc00000u);
+            }
+        }
+    }
+    if (!valid) return;
+    l += __shfl_xor(l, 32, 64);
+    const int64_t row = n * H + head;
+    if (nz > 1) {
+        float *y = part.acc + (row * most + z) * HD + 4 * h;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4)
+                *(f32x4 *)(y + 32 * dt + 2 * v) = f32x4{acc[dt][v], acc[dt][v + 1], acc[dt][v + 2], acc[dt][v + 3]};
+        if (h == 0) part.ml[row * most + z] = make_float2(m, l);
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+            const int d = 32 * dt + 2 * v + 4 * h;
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = acc[dt][v + e] * inv;
+            if (gate) {
+                const T *gr = gate + n * gate_stride + (int64_t)head * HD + d;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] *= gd_sigmoid(to_f32(gr[e]));
+            }
+            if constexpr (HL)
+                *(f32x4 *)(out + row * HD + d) = f32x4{y[0], y[1], y[2], y[3]};
+            else
+                *(uint64_t *)(out + row * HD + d) = (uint64_t)gd_f2h(y[0]) | ((uint64_t)gd_f2h(y[1]) << 16) |
+                                                    ((uint64_t)gd_f2h(y[2]) << 32) | ((uint64_t)gd_f2h(y[3]) << 48);
+        }
+}
+
+// Merges the partials (up to `most` <= MAX_SPLITS) of head h of row n: thread (d, r)
+// takes the splits r, r + NR, .. of one dim, beside the splits' weights, once a
+// workgroup.
 template <int HD, typename T>
-__global__ __launch_bounds__(512) void k_attn_merge(const float *part, int most, int least, Rows s, const T *gate,
+__global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, int least, Cache c, Rows s, const T *gate,
                                                     int64_t gate_stride, T *out, int H, Mask mask) {
-    constexpr int NR = 512 / HD;
+    constexpr int NR = 512 / HD, AK = tile_keys<HD>();
     __shared__ float fs[MAX_SPLITS], sum[NR][HD];
     const int n = blockIdx.x / H, h = blockIdx.x % H, t = threadIdx.x, d = t % HD, r = t / HD;
-    const int pos = s.pos[n];
-    if (pos < 0) return;
-    const int ns = KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1)).splits(most, least);
+    int ns;
+    if (s.row_start) {
+        const int b = seq_of_row(s, n);
+        if (b < 0) return;
+        const Seq sq = seq_at(s, b);
+        if (n < sq.r0 || n >= sq.r1) return;
+        const int G = H / c.HKV;
+        const Tile tl = tile_at(((n - sq.r0) * G + h % G) / PC, sq.r1 - sq.r0, G);
+        const uint32_t p0 = (uint32_t)sq.pos;
+        ns = KeyBlocks<AK>(mask, p0 + tl.i0, min(p0 + tl.i1, s.cap - 1)).splits(most, least);
+    } else {
+        const int pos = s.pos[n];
+        if (pos < 0) return;
+        ns = KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1)).splits(most, least);
+    }
     if (ns == 1) return;
-    const float *p = part + (int64_t)blockIdx.x * most * (HD + 2);
+    const float *p = part.acc + (int64_t)blockIdx.x * most * HD;
     float a[MAX_SPLITS / NR];
 #pragma unroll
-    for (int i = 0; i < MAX_SPLITS / NR; i++) a[i] = r + NR * i < ns ? p[(r + NR * i) * (HD + 2) + d] : 0.f;
+    for (int i = 0; i < MAX_SPLITS / NR; i++) a[i] = r + NR * i < ns ? p[(r + NR * i) * HD + d] : 0.f;
     float inv;
     {
         const int lane = t & 63;                 // every wave: the weight of split lane
-        const float ms = lane < ns ? p[lane * (HD + 2) + HD] : -INFINITY;
-        const float ls = lane < ns ? p[lane * (HD + 2) + HD + 1] : 0.f;
-        const float M = wave_max(ms);
-        const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - M);
-        const float L = gd_wave_sum(ls * f);
+        const float2 ml = lane < ns ? part.ml[(int64_t)blockIdx.x * most + lane] : make_float2(-INFINITY, 0.f);
+        const float M = wave_max(ml.x);
+        const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
+        const float L = gd_wave_sum(ml.y * f);
         inv = L == 0.f ? 0.f : 1.0f / L;
         if (t < MAX_SPLITS) fs[t] = f;
     }
@@ -961,7 +1224,7 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
                "%s: q, gate and out must be 16-byte aligned, and their rows", fn);
     GD_REQUIRE(ctx, window >= 0 && n_sink >= 0, "%s: window %d, n_sink %d", fn, window, n_sink);
     GD_REQUIRE(ctx, std::isfinite(scale), "%s: scale %g", fn, (double)scale);
-    GD_REQUIRE(ctx, s->n_rows * n_head < (1LL << 31), "%s: %lld rows of %d heads", fn, (long long)s->n_rows, n_head);
+    GD_REQUIRE(ctx, s->n_rows * n_head < (1LL << 31) - 256, "%s: %lld rows of %d heads", fn, (long long)s->n_rows, n_head);
     // Workgroups read their q and gate before they write: in place only row on row.
     const size_t span = (size_t)s->n_rows * row * size;
     auto apart = [&](const void *x, int64_t stride) {
@@ -974,39 +1237,36 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     if (!s->n_rows || !s->n_seq) return GD_OK;
     GD_HIP(ctx, hipSetDevice(ctx->device));
     const Mask mask{window, window ? n_sink : 0};
-    if (!s->row_start) {
-        const int G = n_head / kv->n_head_kv, groups = kv->n_head_kv * ((G + 7) / 8);
-        const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
-        const Rows rows = rows_of(kv, s);
-        int64_t keys = s->max_len ? std::min<int64_t>(s->max_len, rows.cap) : rows.cap;
-        if (window) keys = std::min(keys, (int64_t)window + 31 + (n_sink + 31) / 32 * 32);
-        const int64_t blocks = (keys + 31) / 32, wgs = s->n_rows * groups;
-        const int64_t least = std::max<int64_t>(TW, wgs * blocks / (8 * cus));
-        int64_t ns = std::min({(blocks + least - 1) / least, (int64_t)MAX_SPLITS,
-                               (int64_t)(GD_ATTN_SCRATCH_BYTES / ((size_t)s->n_rows * n_head * (hd + 2) * sizeof(float)))});
-        float *part = ns > 1 ? gd_attn_scratch(ctx) : nullptr;
-        if (!part) ns = 1;
+    const int G = n_head / kv->n_head_kv, cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
+    const Rows rows = rows_of(kv, s);
+    int64_t keys = s->max_len ? std::min<int64_t>(s->max_len, rows.cap) : rows.cap;
+    const bool tokens = !s->row_start;
+    const int width = tokens ? 32 : hd == 128 ? tile_keys<128>() : tile_keys<256>();
+    if (window) keys = std::min(keys, (int64_t)window + (tokens ? 0 : PC / G) + width - 1 + (n_sink + width - 1) / width * width);
+    // Blocks of keys of the longest row, workgroups without a split, and splits.
+    const int64_t blocks = (keys + width - 1) / width;
+    const int64_t wgs = tokens ? s->n_rows * kv->n_head_kv * ((G + 7) / 8)
+                               : (s->n_rows * G / PC + std::min<int64_t>(s->n_seq, s->n_rows)) * kv->n_head_kv;
+    const int64_t least = tokens ? std::max<int64_t>(TW, wgs * blocks / (8 * cus)) : std::max<int64_t>(4, wgs * blocks / (4 * cus));
+    int64_t ns = std::min({(blocks + least - 1) / least, (int64_t)MAX_SPLITS,
+                           (int64_t)(GD_ATTN_SCRATCH_BYTES / ((size_t)s->n_rows * n_head * (hd + 2) * sizeof(float)))});
+    float *scratch = ns > 1 ? gd_attn_scratch(ctx) : nullptr;
+    if (!scratch) ns = 1;
+    const Part part{scratch, (float2 *)(scratch + s->n_rows * n_head * ns * hd)};
 #define GD_GO(HD_, I8_, T_) \
     do { \
-        auto kernel = I8_ || kv->page_size % 16 == 0 ? k_attn_tokens<HD_, I8_, true, T_> : k_attn_tokens<HD_, I8_, I8_, T_>; \
-        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs, (unsigned)ns), dim3(64 * TW), 0, ctx->stream, cache_of(kv), rows, \
+        auto kernel = tokens ? (I8_ || kv->page_size % 16 == 0 ? k_attn_tokens<HD_, I8_, true, T_> : k_attn_tokens<HD_, I8_, I8_, T_>) \
+                             : k_attn_rows<HD_, I8_, I8_, T_>; \
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs, (unsigned)ns), dim3(256), 0, ctx->stream, cache_of(kv), rows, \
                            (const T_ *)q, q_stride, (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)least, \
                            n_head, scale, mask); \
         if (ns > 1) { \
             GD_LAUNCHED(ctx, fn); \
             hipLaunchKernelGGL((k_attn_merge<HD_, T_>), dim3((unsigned)(s->n_rows * n_head)), dim3(512), 0, ctx->stream, \
-                               part, (int)ns, (int)least, rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head, mask); \
+                               part, (int)ns, (int)least, cache_of(kv), rows, (const T_ *)gate, gate_stride, (T_ *)out, \
+                               n_head, mask); \
         } \
     } while (0)
-        GD_KV_PICK(kv, x_dtype, GD_GO);
-#undef GD_GO
-        GD_LAUNCHED(ctx, fn);
-        return GD_OK;
-    }
-    const dim3 grid(gd_blocks(s->n_rows * n_head, 4));
-#define GD_GO(HD_, I8_, T_) \
-    hipLaunchKernelGGL((k_attn<HD_, I8_, T_>), grid, dim3(256), 0, ctx->stream, cache_of(kv), rows_of(kv, s), \
-                       (const T_ *)q, q_stride, (const T_ *)gate, gate_stride, (T_ *)out, n_head, scale, mask)
     GD_KV_PICK(kv, x_dtype, GD_GO);
 #undef GD_GO
     GD_LAUNCHED(ctx, fn);
