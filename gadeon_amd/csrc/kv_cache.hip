@@ -693,9 +693,10 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     constexpr int ES = I8 ? 1 : 2, CPR = HD * ES / 16;   // 16-byte chunks of a row
     constexpr int CH = AK * CPR / 256, KPP = 256 / CPR;  // chunks a thread stages of K (and of V); keys of a pass
     constexpr int KP = HD + 8, VP = HD + 16;
-    __shared__ __attribute__((aligned(16))) f16 Ks[AK][KP];
-    __shared__ __attribute__((aligned(16))) f16 Vs[AK][VP];
-    __shared__ int bad[2];
+    __shared__ __attribute__((aligned(16))) f16 Ks[2][AK][KP];
+    __shared__ __attribute__((aligned(16))) f16 Vs[2][AK][VP];
+    __shared__ uint8_t odd[2][AK][HD / 8];       // which values of V are no numbers, a bit each
+    __shared__ int any_odd[2];
     const int G = H / c.HKV, kvh = blockIdx.x % c.HKV;
     int b, k;
     auto units = [&](const Seq &q) { return (int)(((int64_t)(q.r1 - q.r0) * G + PC - 1) / PC); };
@@ -719,7 +720,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     const uint32_t p = p0 + i;
     const bool busy = k * PC + 32 * w < rows * G;
     const uint32_t plo = p0 + min((k * PC + 32 * w) / G, rows - 1), phi = p0 + min((k * PC + 32 * w + 31) / G, rows - 1);
-    // Staging: key lane % AK's page-table entry a tile ahead of its row, that a tile ahead of use.
+    // Staging: key lane % AK's page-table entry a tile ahead of its row, that a tile ahead
+    // of the halves in LDS, those a tile ahead of use.
     const int32_t *table = s.table + (int64_t)b * s.max_pages;
     struct Entry {
         uint32_t kp;
@@ -729,30 +731,85 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         const uint32_t kp = kb.start(min(j, kb.n - 1)) + (lane & (AK - 1));
         return Entry{kp, table[c.by_page(min(kp, cap1))]};
     };
+    const uint32_t pitch = HD * ES * (I8 ? 1 : c.HKV);   // bytes from a row to the next position's
     u32x4 kr[CH], vr[CH];
-    int kx[I8 ? CH : 1], vx[I8 ? CH : 1];
-    uint64_t here;                               // keys of the tile whose pages are there
+    int kx = 0, vx = 0;
+    uint64_t here = 0;                           // keys of the tile whose pages are there
     auto fetch = [&](const Entry &e) {
         const bool there = (uint32_t)e.page < c.n_pages && e.kp < s.cap && e.kp <= p0 + tl.i1;
         const uint32_t row = there ? row_at<I8>(c, e.page, slot_of(c, e.kp), kvh) : (uint32_t)(I8 ? 0 : kvh);
         here = __ballot(there);
+        if constexpr (I8) {
+            kx = c.kx[row / BLK];
+            vx = c.vx[row / BLK];
+        }
 #pragma unroll
         for (int x = 0; x < CH; x++) {
-            const int key = x * KPP + t / CPR;
-            const uint64_t kr_ = (uint32_t)__shfl((int)row, key, 64);
-            kr[x] = *(const u32x4 *)((const char *)c.k + kr_ * (HD * ES) + 16 * (t % CPR));
-            vr[x] = *(const u32x4 *)((const char *)c.v + kr_ * (HD * ES) + 16 * (t % CPR));
-            if constexpr (I8) {
-                kx[x] = c.kx[kr_ / BLK];
-                vx[x] = c.vx[kr_ / BLK];
+            uint64_t at;
+            if constexpr (TILED) {               // 16 keys of a page: those of this wave's pass start at a uniform row
+                const int tile = (x * KPP + w * (64 / CPR)) & ~15;
+                const uint64_t first = (uint32_t)__builtin_amdgcn_readlane((int)row, tile);
+                const bool in = here >> tile & 1;                // (row 0, and that one alone, where there is none)
+                at = first * (HD * ES) + (in ? (uint32_t)((x * KPP + t / CPR) & 15) * pitch : 0u);
+            } else {
+                at = (uint64_t)(uint32_t)__shfl((int)row, x * KPP + t / CPR, 64) * (HD * ES);
             }
+            kr[x] = *(const u32x4 *)((const char *)c.k + at + 16 * (t % CPR));
+            vr[x] = *(const u32x4 *)((const char *)c.v + at + 16 * (t % CPR));
         }
     };
-    if (t < 2) bad[t] = 0;
+    constexpr uint64_t ALL = AK == 64 ? ~0ull : 0xffffffffull;
+    // The fetched tile (block j) to LDS.  Where some column does not see all of it, what is
+    // no number in V goes into bits beside it, and a zero in its place.
+    auto stage = [&](int j) {
+        const uint32_t k0 = kb.start(j);
+        const uint64_t in = here & ALL;
+        const bool whole = in == ALL && k0 + AK - 1 <= p0 + tl.i0 &&
+                           (!mask.window || k0 + mask.window > p0 + tl.i1 || k0 + AK <= (uint32_t)mask.sinks);
+        const int s2 = j & 1;
+        if (t == 0) any_odd[s2] = 0;             // (set, if at all, after the barrier below)
+        bool some = false;
+#pragma unroll
+        for (int x = 0; x < CH; x++) {
+            const int key = x * KPP + t / CPR, d = t % CPR * (16 / ES);
+            f16x8 kv[I8 ? 2 : 1], vv[I8 ? 2 : 1];
+            if constexpr (I8) {
+                const int tile = (x * KPP + w * (64 / CPR)) & ~15;
+                const f16 ka = (f16)step_of((uint8_t)__builtin_amdgcn_readlane(kx, tile));
+                const f16 va = (f16)step_of((uint8_t)__builtin_amdgcn_readlane(vx, tile));
+                kv[0] = halves(kr[x][0], kr[x][1]) * ka;
+                kv[1] = halves(kr[x][2], kr[x][3]) * ka;
+                vv[0] = halves(vr[x][0], vr[x][1]) * va;
+                vv[1] = halves(vr[x][2], vr[x][3]) * va;
+            } else {
+                kv[0] = __builtin_bit_cast(f16x8, kr[x]);
+                vv[0] = __builtin_bit_cast(f16x8, vr[x]);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int y = 0; y < (I8 ? 2 : 1); y++) {
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const bool no = (__builtin_bit_cast(uint16_t, (f16)vv[y][e]) & 0x7c00u) == 0x7c00u;
+                        bits |= (uint32_t)no << e;
+                        if (no || !(in >> key & 1)) vv[y][e] = (f16)0.f;
+                    }
+                    bits = in >> key & 1 ? bits : 0;
+                    odd[s2][key][d / 8 + y] = (uint8_t)bits;
+                    some |= bits != 0;
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < (I8 ? 2 : 1); y++) {
+                *(f16x8 *)&Ks[s2][key][d + 8 * y] = kv[y];
+                *(f16x8 *)&Vs[s2][key][d + 8 * y] = vv[y];
+            }
+        }
+        return some;
+    };
     int j = z * per;
     Entry en = entry_of(j);
-    if (j < jend) fetch(en);
-    en = entry_of(j + 1);
     // B operand of S^T: dims 16 ks + 8 h + e of the lane's column; the sign of the scale
     // goes into it, so that the greatest product is the greatest score.
     f16x8 qh[KS], ql[HL ? KS : 1];
@@ -793,152 +850,124 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             }
         }
     }
+    if (sf < 0x1p-126f) sf = 0x1p-126f;          // weights of 1 alike; times -inf not NaN
+    if (j < jend) fetch(en);
+    en = entry_of(j + 1);
     f32x16 acc[DT];                              // O^T dims 32 dt + 8 (v / 4) + 4 h + v % 4
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) acc[dt] = f32x16{};
     float m = -INFINITY, l = 0.f;                // l: this lane's keys only
+    bool some = j < jend && stage(j);
+    uint64_t now = here & ALL;
+    if (j + 1 < jend) fetch(en);
+    en = entry_of(j + 2);
+    __syncthreads();
     for (; j < jend; j++) {
         const uint32_t k0 = kb.start(j);
-        const uint64_t all = AK == 64 ? ~0ull : 0xffffffffull;
-        const uint64_t now = here & all;
-        // Whether every column of the unit sees the whole tile; else keys may be masked.
-        const bool whole = now == all && k0 + AK - 1 <= p0 + tl.i0 &&
-                           (!mask.window || k0 + mask.window > p0 + tl.i1 || k0 + AK <= (uint32_t)mask.sinks);
-        __syncthreads();
-        bool odd = false;
-#pragma unroll
-        for (int x = 0; x < CH; x++) {
-            const int key = x * KPP + t / CPR, d = t % CPR * (16 / ES);
-            const bool in = now >> key & 1;
-            if constexpr (I8) {
-                const f16 ka = (f16)step_of((uint8_t)kx[x]), va = (f16)step_of((uint8_t)vx[x]);
-                *(f16x8 *)&Ks[key][d] = halves(kr[x][0], kr[x][1]) * ka;
-                *(f16x8 *)&Ks[key][d + 8] = halves(kr[x][2], kr[x][3]) * ka;
-                *(f16x8 *)&Vs[key][d] = in ? halves(vr[x][0], vr[x][1]) * va : f16x8{};
-                *(f16x8 *)&Vs[key][d + 8] = in ? halves(vr[x][2], vr[x][3]) * va : f16x8{};
-                odd |= in && vx[x] == EXP_NAN;
-            } else {
-                *(u32x4 *)&Ks[key][d] = kr[x];
-                *(u32x4 *)&Vs[key][d] = in ? vr[x] : u32x4{0u, 0u, 0u, 0u};
-                if (!whole)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) odd |= in && (((vr[x][e] & 0x7c007c00u) + 0x04000400u) & 0x80008000u);
-            }
+        const int s2 = j & 1;
+        if (some) any_odd[s2] = 1;
+        // The next tile to the other half of LDS, the one after it requested.
+        const uint64_t next = here & ALL;
+        if (j + 1 < jend) {
+            some = stage(j + 1);
+            fetch(en);
+            en = entry_of(j + 3);
         }
-        if (!whole && odd) bad[j & 1] = 1;
-        __syncthreads();
-        const bool nan_tile = !whole && bad[j & 1];
-        if (t == 0) bad[~j & 1] = 0;
-        fetch(en);
-        en = entry_of(j + 2);
         __builtin_amdgcn_sched_barrier(0);
         // The wave's own view of the tile.
-        if (!busy || k0 > phi) continue;
-        if (mask.window && k0 + AK - 1 + mask.window <= plo && k0 >= (uint32_t)mask.sinks) continue;
-        const bool full = now == all && k0 + AK - 1 <= plo &&
-                          (!mask.window || k0 + mask.window > phi || k0 + AK <= (uint32_t)mask.sinks);
-        f32x16 st[NT];
+        if (busy && k0 <= phi && !(mask.window && k0 + AK - 1 + mask.window <= plo && k0 >= (uint32_t)mask.sinks)) {
+            const bool full = now == ALL && k0 + AK - 1 <= plo &&
+                              (!mask.window || k0 + mask.window > phi || k0 + AK <= (uint32_t)mask.sinks);
+            f32x16 st[NT];
 #pragma unroll
-        for (int kt = 0; kt < NT; kt++) {
-            st[kt] = f32x16{};
+            for (int kt = 0; kt < NT; kt++) {
+                st[kt] = f32x16{};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const f16x8 ka = *(const f16x8 *)&Ks[32 * kt + lc][16 * ks + 8 * h];
-                st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[ks], st[kt], 0, 0, 0);
-                if constexpr (HL) st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[ks], st[kt], 0, 0, 0);
-            }
-        }
-        // Keys 32 kt + 8 (v / 4) + 4 h + v % 4 that this column sees, a bit each.
-        uint32_t sees[NT];
-#pragma unroll
-        for (int kt = 0; kt < NT; kt++) {
-            sees[kt] = 0xffffu;
-            if (!full) {
-                sees[kt] = 0;
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int key = 32 * kt + 8 * (v / 4) + 4 * h + v % 4;
-                    const uint32_t kp = k0 + key;
-                    const bool see = kp <= p && (!mask.window || kp + mask.window > p || kp < (uint32_t)mask.sinks) &&
-                                     (now >> key & 1);
-                    sees[kt] |= (uint32_t)see << v;
-                    if (!see) st[kt][v] = -INFINITY;
+                for (int ks = 0; ks < KS; ks++) {
+                    const f16x8 ka = *(const f16x8 *)&Ks[s2][32 * kt + lc][16 * ks + 8 * h];
+                    st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[ks], st[kt], 0, 0, 0);
+                    if constexpr (HL) st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[ks], st[kt], 0, 0, 0);
                 }
             }
-        }
-        float top = -INFINITY;
+            // Keys 32 kt + 8 (v / 4) + 4 h + v % 4.
+            auto sees = [&](int key) {
+                const uint32_t kp = k0 + key;
+                return kp <= p && (!mask.window || kp + mask.window > p || kp < (uint32_t)mask.sinks) && (now >> key & 1);
+            };
+            if (!full)
 #pragma unroll
-        for (int kt = 0; kt < NT; kt++)
+                for (int kt = 0; kt < NT; kt++)
 #pragma unroll
-            for (int v = 0; v < 16; v++) top = fmaxf(top, st[kt][v]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float mn = fmaxf(m, top == -INFINITY ? -INFINITY : top * sf);
-        if (__any(mn > m)) {
-            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-            l *= alpha;
+                    for (int v = 0; v < 16; v++)
+                        if (!sees(32 * kt + 8 * (v / 4) + 4 * h + v % 4)) st[kt][v] = -INFINITY;
+            float top = -INFINITY;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) acc[dt] *= alpha;
-            m = mn;
-        }
-        // Weights times 2^14 (f16 rows: in the exponent, where 32-bit rows would lose bits).
-        const float off = m == -INFINITY ? 0.f : HL ? -m : 14.f - m;
-        f16x8 ph[2 * NT], pl[HL ? 2 * NT : 1];
+            for (int kt = 0; kt < NT; kt++)
 #pragma unroll
-        for (int kt = 0; kt < NT; kt++)
+                for (int v = 0; v < 16; v++) top = fmaxf(top, st[kt][v]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = fmaxf(m, top * sf);
+            if (__any(mn > m)) {
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+                l *= alpha;
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                float w_ = __builtin_amdgcn_exp2f(fmaf(st[kt][v], sf, off));
-                if (!full && !(sees[kt] >> v & 1)) w_ = 0.f;
-                if constexpr (HL) {
-                    w_ *= 16384.f;
-                    asm("" : "+v"(w_));
-                }
-                l += w_;
-                const f16 hi = (f16)w_;
-                ph[2 * kt + v / 8][v % 8] = hi;
-                if constexpr (HL) pl[2 * kt + v / 8][v % 8] = (f16)(w_ - (float)hi);
+                for (int dt = 0; dt < DT; dt++) acc[dt] *= alpha;
+                m = mn;
             }
-        typedef short s16x4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        auto values = [&](int kk, int dt) {      // V^T of keys 16 kk .., dims 32 dt + lane % 32
-            const f16 *v = &Vs[16 * kk + 4 * h + (lane >> 2 & 3)][32 * dt + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
-            const f16x4 v0 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v));
-            const f16x4 v1 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 8 * VP)));
-            return f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-        };
-        if (!nan_tile || full) {
+            // Weights times 2^14 (f16 rows: in the exponent, where 32-bit rows would lose bits).
+            const float off = m == -INFINITY ? 0.f : HL ? -m : 14.f - m;
+            f16x8 ph[2 * NT], pl[HL ? 2 * NT : 1];
+#pragma unroll
+            for (int kt = 0; kt < NT; kt++)
+#pragma unroll
+                for (int v = 0; v < 16; v += 2) {
+                    float w0 = __builtin_amdgcn_exp2f(fmaf(st[kt][v], sf, off));
+                    float w1 = __builtin_amdgcn_exp2f(fmaf(st[kt][v + 1], sf, off));
+                    f16x2 hi, lo;
+                    if constexpr (HL) {
+                        w0 *= 16384.f;
+                        w1 *= 16384.f;
+                        gd_split2_f16(w0, w1, hi, lo);
+                        pl[2 * kt + v / 8][v % 8] = lo[0];
+                        pl[2 * kt + v / 8][v % 8 + 1] = lo[1];
+                    } else {
+                        typedef float f32x2 __attribute__((ext_vector_type(2)));
+                        hi = __builtin_convertvector((f32x2{w0, w1}), f16x2);
+                    }
+                    l += w0;
+                    l += w1;
+                    ph[2 * kt + v / 8][v % 8] = hi[0];
+                    ph[2 * kt + v / 8][v % 8 + 1] = hi[1];
+                }
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 #pragma unroll
             for (int kk = 0; kk < 2 * NT; kk++)
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
-                    const f16x8 va = values(kk, dt);
+                    // V^T of keys 16 kk .., dims 32 dt + lane % 32.
+                    const f16 *v = &Vs[s2][16 * kk + 4 * h + (lane >> 2 & 3)][32 * dt + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
+                    const f16x4 v0 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v));
+                    const f16x4 v1 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 8 * VP)));
+                    const f16x8 va = f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
                     acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[kk], acc[dt], 0, 0, 0);
                     if constexpr (HL) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[kk], acc[dt], 0, 0, 0);
                 }
-            continue;
         }
+        __syncthreads();
+        if (any_odd[s2]) {
+            // What is no number reaches the columns that see it.
+            for (int key = 0; key < AK; key++)
+                if (kb.start(j) + key <= p && (now >> key & 1) &&
+                    (!mask.window || k0 + key + mask.window > p || k0 + key < (uint32_t)mask.sinks))
 #pragma unroll
-        for (int kk = 0; kk < 2 * NT; kk++) {
-            f16x8 see;
+                    for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) see[e] = sees[kk / 2] >> (8 * (kk & 1) + e) & 1 ? (f16)1.f : (f16)0.f;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                f16x8 va = values(kk, dt), vn;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const bool fin = (__builtin_bit_cast(uint16_t, (f16)va[e]) & 0x7c00u) != 0x7c00u;
-                    vn[e] = fin ? (f16)0.f : (f16)1.f;
-                    va[e] = fin ? va[e] : (f16)0.f;
-                }
-                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[kk], acc[dt], 0, 0, 0);
-                if constexpr (HL) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[kk], acc[dt], 0, 0, 0);
-                const f32x16 count = __builtin_amdgcn_mfma_f32_32x32x16_f16(vn, see, f32x16{}, 0, 0, 0);
-#pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (count[v] > 0.f) acc[dt][v] = __uint_as_float(0x7fc00000u);
-            }
+                        for (int v = 0; v < 16; v++)
+                            if (odd[s2][key][4 * dt + v / 4] >> (4 * h + v % 4) & 1) acc[dt][v] = __uint_as_float(0x7fc00000u);
+            __syncthreads();
         }
+        now = next;
     }
     if (!valid) return;
     l += __shfl_xor(l, 32, 64);
@@ -1255,8 +1284,9 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const Part part{scratch, (float2 *)(scratch + s->n_rows * n_head * ns * hd)};
 #define GD_GO(HD_, I8_, T_) \
     do { \
-        auto kernel = tokens ? (I8_ || kv->page_size % 16 == 0 ? k_attn_tokens<HD_, I8_, true, T_> : k_attn_tokens<HD_, I8_, I8_, T_>) \
-                             : k_attn_rows<HD_, I8_, I8_, T_>; \
+        const bool tiled = I8_ || kv->page_size % 16 == 0; \
+        auto kernel = tokens ? (tiled ? k_attn_tokens<HD_, I8_, true, T_> : k_attn_tokens<HD_, I8_, I8_, T_>) \
+                             : (tiled ? k_attn_rows<HD_, I8_, true, T_> : k_attn_rows<HD_, I8_, I8_, T_>); \
         hipLaunchKernelGGL(kernel, dim3((unsigned)wgs, (unsigned)ns), dim3(256), 0, ctx->stream, cache_of(kv), rows, \
                            (const T_ *)q, q_stride, (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)least, \
                            n_head, scale, mask); \
