@@ -692,7 +692,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     constexpr int AK = tile_keys<HD>(), NT = AK / 32, KS = HD / 16, DT = HD / 32;
     constexpr int ES = I8 ? 1 : 2, CPR = HD * ES / 16;   // 16-byte chunks of a row
     constexpr int CH = AK * CPR / 256, KPP = 256 / CPR;  // chunks a thread stages of K (and of V); keys of a pass
-    constexpr int KP = HD + 8, VP = HD + 16;
+    constexpr int KP = HD + 8, VP = HD + 16, FD = 4;
     __shared__ __attribute__((aligned(16))) f16 Ks[2][AK][KP];
     __shared__ __attribute__((aligned(16))) f16 Vs[2][AK][VP];
     __shared__ uint8_t odd[2][AK][HD / 8];       // which values of V are no numbers, a bit each
@@ -788,16 +788,23 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             if (!whole) {
 #pragma unroll
                 for (int y = 0; y < (I8 ? 2 : 1); y++) {
-                    uint32_t bits = 0;
+                    u32x4 v = __builtin_bit_cast(u32x4, vv[y]);
+                    if (!(in >> key & 1)) v = u32x4{0u, 0u, 0u, 0u};
+                    uint32_t no = 0;             // a half's top bit: all exponent bits set
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const bool no = (__builtin_bit_cast(uint16_t, (f16)vv[y][e]) & 0x7c00u) == 0x7c00u;
-                        bits |= (uint32_t)no << e;
-                        if (no || !(in >> key & 1)) vv[y][e] = (f16)0.f;
+                    for (int e = 0; e < 4; e++) no |= (v[e] & 0x7c007c00u) + 0x04000400u;
+                    uint32_t bits = 0;
+                    if (no & 0x80008000u) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t x = (v[e] & 0x7c007c00u) + 0x04000400u;
+                            bits |= (x >> 15 & 1u) << 2 * e | (x >> 31) << (2 * e + 1);
+                            v[e] &= ((x >> 15 & 1u) ? 0u : 0xffffu) | (x >> 31 ? 0u : 0xffff0000u);
+                        }
+                        some = true;
                     }
-                    bits = in >> key & 1 ? bits : 0;
                     odd[s2][key][d / 8 + y] = (uint8_t)bits;
-                    some |= bits != 0;
+                    vv[y] = __builtin_bit_cast(f16x8, v);
                 }
             }
 #pragma unroll
@@ -879,27 +886,39 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             const bool full = now == ALL && k0 + AK - 1 <= plo &&
                               (!mask.window || k0 + mask.window > phi || k0 + AK <= (uint32_t)mask.sinks);
             f32x16 st[NT];
+            {
+                // A operands FD reads ahead of their products.
+                auto keys = [&](int x) { return *(const f16x8 *)&Ks[s2][x / KS * 32 + lc][x % KS * 16 + 8 * h]; };
+                f16x8 ka[FD];
 #pragma unroll
-            for (int kt = 0; kt < NT; kt++) {
-                st[kt] = f32x16{};
+                for (int x = 0; x < FD; x++) ka[x] = keys(x);
+                __builtin_amdgcn_sched_group_barrier(0x100, FD, 0);
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    const f16x8 ka = *(const f16x8 *)&Ks[s2][32 * kt + lc][16 * ks + 8 * h];
-                    st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[ks], st[kt], 0, 0, 0);
-                    if constexpr (HL) st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[ks], st[kt], 0, 0, 0);
+                for (int x = 0; x < NT * KS; x++) {
+                    const int kt = x / KS, ks = x % KS;
+                    st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[x % FD], qh[ks], ks ? st[kt] : f32x16{}, 0, 0, 0);
+                    if constexpr (HL) st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[x % FD], ql[ks], st[kt], 0, 0, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, HL ? 2 : 1, 0);
+                    if (x + FD < NT * KS) {
+                        ka[x % FD] = keys(x + FD);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    }
                 }
             }
-            // Keys 32 kt + 8 (v / 4) + 4 h + v % 4.
-            auto sees = [&](int key) {
-                const uint32_t kp = k0 + key;
-                return kp <= p && (!mask.window || kp + mask.window > p || kp < (uint32_t)mask.sinks) && (now >> key & 1);
-            };
-            if (!full)
+            if (!full) {
+                // Bit 8 (v / 4) + v % 4 of a 32-key half: key 4 h on, as this column sees it.
+                auto below = [](int64_t x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; };
+                uint64_t see = below((int64_t)p - k0 + 1);
+                if (mask.window) see &= ~below((int64_t)p - mask.window + 1 - k0) | below((int64_t)mask.sinks - k0);
+                see = (see & now) >> (4 * h);
 #pragma unroll
-                for (int kt = 0; kt < NT; kt++)
+                for (int kt = 0; kt < NT; kt++) {
+                    const uint32_t bits = (uint32_t)(see >> (32 * kt));
 #pragma unroll
                     for (int v = 0; v < 16; v++)
-                        if (!sees(32 * kt + 8 * (v / 4) + 4 * h + v % 4)) st[kt][v] = -INFINITY;
+                        st[kt][v] = bits & (1u << (8 * (v / 4) + v % 4)) ? st[kt][v] : -INFINITY;
+                }
+            }
             float top = -INFINITY;
 #pragma unroll
             for (int kt = 0; kt < NT; kt++)
@@ -939,20 +958,32 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                     ph[2 * kt + v / 8][v % 8] = hi[0];
                     ph[2 * kt + v / 8][v % 8 + 1] = hi[1];
                 }
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-#pragma unroll
-            for (int kk = 0; kk < 2 * NT; kk++)
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    // V^T of keys 16 kk .., dims 32 dt + lane % 32.
-                    const f16 *v = &Vs[s2][16 * kk + 4 * h + (lane >> 2 & 3)][32 * dt + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
+            {
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                // V^T of keys 16 (x / DT) .., dims 32 (x % DT) + lane % 32.
+                auto values = [&](int x) {
+                    const f16 *v = &Vs[s2][x / DT * 16 + 4 * h + (lane >> 2 & 3)][x % DT * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
                     const f16x4 v0 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v));
                     const f16x4 v1 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 8 * VP)));
-                    const f16x8 va = f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[kk], acc[dt], 0, 0, 0);
-                    if constexpr (HL) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[kk], acc[dt], 0, 0, 0);
+                    return f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                };
+                f16x8 va[FD];
+#pragma unroll
+                for (int x = 0; x < FD; x++) va[x] = values(x);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2 * FD, 1);
+#pragma unroll
+                for (int x = 0; x < 2 * NT * DT; x++) {
+                    const int kk = x / DT, dt = x % DT;
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[x % FD], ph[kk], acc[dt], 0, 0, 0);
+                    if constexpr (HL) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[x % FD], pl[kk], acc[dt], 0, 0, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, HL ? 2 : 1, 1);
+                    if (x + FD < 2 * NT * DT) {
+                        va[x % FD] = values(x + FD);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+                    }
                 }
+            }
         }
         __syncthreads();
         if (any_odd[s2]) {
