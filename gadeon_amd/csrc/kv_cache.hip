@@ -670,11 +670,12 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // of P^T once the MFMA's K index 8 h + e (h = lane / 32) stands for key 4 h + e (e < 4) or
 // 8 + 4 h + e - 4 of its 16; V^T is read by the transposing LDS read.  f32 rows enter as
 // f16 hi + lo pairs (q brought to 2^14 .. 2^15 by a power of two a column, weights to
-// 2^14), f16 rows as they are, with weights rounded to f16: 2^-12 of each, less than the
+// 2^8), f16 rows as they are, with weights rounded to f16: 2^-12 of each, less than the
 // result's own rounding.  A tile that some column does not see whole goes key by key: a
 // mask, and where V holds a NaN or infinity its finite part and, apart, which columns see
 // the others (0 x NaN would reach them all).
 constexpr int PC = 128;                          // columns of a unit
+constexpr float LAZY = 7.f;
 template <int HD> constexpr int tile_keys() { return HD == 128 ? 64 : 32; }
 
 struct Tile {
@@ -692,7 +693,9 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     constexpr int AK = tile_keys<HD>(), NT = AK / 32, KS = HD / 16, DT = HD / 32;
     constexpr int ES = I8 ? 1 : 2, CPR = HD * ES / 16;   // 16-byte chunks of a row
     constexpr int CH = AK * CPR / 256, KPP = 256 / CPR;  // chunks a thread stages of K (and of V); keys of a pass
-    constexpr int KP = HD + 8, VP = HD + 16, FD = 4;
+    // V rows padded by 64 bytes: the four rows and 32 dims of a transposing read's 32 lanes
+    // then lie in 64 different banks.
+    constexpr int KP = HD + 8, VP = HD + 32, FD = 4;
     __shared__ __attribute__((aligned(16))) f16 Ks[2][AK][KP];
     __shared__ __attribute__((aligned(16))) f16 Vs[2][AK][VP];
     __shared__ uint8_t odd[2][AK][HD / 8];       // which values of V are no numbers, a bit each
@@ -886,16 +889,17 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             const bool full = now == ALL && k0 + AK - 1 <= plo &&
                               (!mask.window || k0 + mask.window > phi || k0 + AK <= (uint32_t)mask.sinks);
             f32x16 st[NT];
+            __builtin_amdgcn_s_setprio(1);
             {
                 // A operands FD reads ahead of their products.
-                auto keys = [&](int x) { return *(const f16x8 *)&Ks[s2][x / KS * 32 + lc][x % KS * 16 + 8 * h]; };
+                auto keys = [&](int x) { return *(const f16x8 *)&Ks[s2][x % NT * 32 + lc][x / NT * 16 + 8 * h]; };
                 f16x8 ka[FD];
 #pragma unroll
                 for (int x = 0; x < FD; x++) ka[x] = keys(x);
                 __builtin_amdgcn_sched_group_barrier(0x100, FD, 0);
 #pragma unroll
                 for (int x = 0; x < NT * KS; x++) {
-                    const int kt = x / KS, ks = x % KS;
+                    const int kt = x % NT, ks = x / NT;
                     st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[x % FD], qh[ks], ks ? st[kt] : f32x16{}, 0, 0, 0);
                     if constexpr (HL) st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[x % FD], ql[ks], st[kt], 0, 0, 0);
                     __builtin_amdgcn_sched_group_barrier(0x008, HL ? 2 : 1, 0);
@@ -905,6 +909,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                     }
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
             if (!full) {
                 // Bit 8 (v / 4) + v % 4 of a 32-key half: key 4 h on, as this column sees it.
                 auto below = [](int64_t x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; };
@@ -925,16 +930,19 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 #pragma unroll
                 for (int v = 0; v < 16; v++) top = fmaxf(top, st[kt][v]);
             top = fmaxf(top, __shfl_xor(top, 32, 64));
+            // Sums are brought to a new maximum only where it is over 2^LAZY of the one they
+            // stand at (random scores: hardly after the first tiles).
             const float mn = fmaxf(m, top * sf);
-            if (__any(mn > m)) {
+            if (__any(mn > m + LAZY)) {
                 const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
                 l *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) acc[dt] *= alpha;
                 m = mn;
             }
-            // Weights times 2^14 (f16 rows: in the exponent, where 32-bit rows would lose bits).
-            const float off = m == -INFINITY ? 0.f : HL ? -m : 14.f - m;
+            // Weights times 2^8, under 2^15 (f16 rows: in the exponent, where 32-bit rows would
+            // lose bits).
+            const float off = m == -INFINITY ? 0.f : HL ? -m : 8.f - m;
             f16x8 ph[2 * NT], pl[HL ? 2 * NT : 1];
 #pragma unroll
             for (int kt = 0; kt < NT; kt++)
@@ -944,8 +952,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                     float w1 = __builtin_amdgcn_exp2f(fmaf(st[kt][v + 1], sf, off));
                     f16x2 hi, lo;
                     if constexpr (HL) {
-                        w0 *= 16384.f;
-                        w1 *= 16384.f;
+                        w0 *= 256.f;
+                        w1 *= 256.f;
                         gd_split2_f16(w0, w1, hi, lo);
                         pl[2 * kt + v / 8][v % 8] = lo[0];
                         pl[2 * kt + v / 8][v % 8 + 1] = lo[1];
@@ -953,8 +961,12 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                         typedef float f32x2 __attribute__((ext_vector_type(2)));
                         hi = __builtin_convertvector((f32x2{w0, w1}), f16x2);
                     }
-                    l += w0;
-                    l += w1;
+                    if constexpr (HL) {
+                        l += w0;
+                        l += w1;
+                    } else {
+                        l = __builtin_amdgcn_fdot2(hi, f16x2{(f16)1.f, (f16)1.f}, l, false);
+                    }
                     ph[2 * kt + v / 8][v % 8] = hi[0];
                     ph[2 * kt + v / 8][v % 8 + 1] = hi[1];
                 }
@@ -1025,7 +1037,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             if (gate) {
                 const T *gr = gate + n * gate_stride + (int64_t)head * HD + d;
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] *= gd_sigmoid(to_f32(gr[e]));
+                for (int e = 0; e < 4; e++)
+                    y[e] *= HL ? gd_sigmoid(to_f32(gr[e])) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * to_f32(gr[e])));
             }
             if constexpr (HL)
                 *(f32x4 *)(out + row * HD + d) = f32x4{y[0], y[1], y[2], y[3]};
@@ -1035,31 +1048,38 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         }
 }
 
-// Merges the partials (up to `most` <= MAX_SPLITS) of head h of row n: thread (d, r)
-// takes the splits r, r + NR, .. of one dim, beside the splits' weights, once a
+// The splits that row n's keys were worked in for query head h (0: the row has no sequence).
+template <int HD>
+__device__ __forceinline__ int splits_of(const Cache &c, const Rows &s, const Mask &mask, int n, int h, int H, int most, int least) {
+    if (!s.row_start) {
+        const int pos = s.pos[n];
+        return pos < 0 ? 0 : KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1)).splits(most, least);
+    }
+    const int b = seq_of_row(s, n);
+    if (b < 0) return 0;
+    const Seq sq = seq_at(s, b);
+    if (n < sq.r0 || n >= sq.r1) return 0;
+    const int G = H / c.HKV;
+    const Tile tl = tile_at(((n - sq.r0) * G + h % G) / PC, sq.r1 - sq.r0, G);
+    const uint32_t p0 = (uint32_t)sq.pos;
+    return KeyBlocks<tile_keys<HD>()>(mask, p0 + tl.i0, min(p0 + tl.i1, s.cap - 1)).splits(most, least);
+}
+
+template <typename T> __device__ __forceinline__ float gated(float y, const T *gate) {
+    return y * gd_sigmoid(to_f32(*gate));
+}
+
+// Merges the partials (up to `most` <= MAX_SPLITS) of head h of row n, few rows: thread
+// (d, r) takes the splits r, r + NR, .. of one dim, beside the splits' weights, once a
 // workgroup.
 template <int HD, typename T>
 __global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, int least, Cache c, Rows s, const T *gate,
                                                     int64_t gate_stride, T *out, int H, Mask mask) {
-    constexpr int NR = 512 / HD, AK = tile_keys<HD>();
+    constexpr int NR = 512 / HD;
     __shared__ float fs[MAX_SPLITS], sum[NR][HD];
     const int n = blockIdx.x / H, h = blockIdx.x % H, t = threadIdx.x, d = t % HD, r = t / HD;
-    int ns;
-    if (s.row_start) {
-        const int b = seq_of_row(s, n);
-        if (b < 0) return;
-        const Seq sq = seq_at(s, b);
-        if (n < sq.r0 || n >= sq.r1) return;
-        const int G = H / c.HKV;
-        const Tile tl = tile_at(((n - sq.r0) * G + h % G) / PC, sq.r1 - sq.r0, G);
-        const uint32_t p0 = (uint32_t)sq.pos;
-        ns = KeyBlocks<AK>(mask, p0 + tl.i0, min(p0 + tl.i1, s.cap - 1)).splits(most, least);
-    } else {
-        const int pos = s.pos[n];
-        if (pos < 0) return;
-        ns = KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1)).splits(most, least);
-    }
-    if (ns == 1) return;
+    const int ns = splits_of<HD>(c, s, mask, n, h, H, most, least);
+    if (ns <= 1) return;
     const float *p = part.acc + (int64_t)blockIdx.x * most * HD;
     float a[MAX_SPLITS / NR];
 #pragma unroll
@@ -1084,8 +1104,42 @@ __global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, int lea
 #pragma unroll
     for (int i = 1; i < NR; i++) A += sum[i][d];
     float y = A * inv;
-    if (gate) y *= gd_sigmoid(to_f32(gate[n * gate_stride + (int64_t)h * HD + d]));
+    if (gate) y = gated(y, gate + n * gate_stride + (int64_t)h * HD + d);
     out[(int64_t)blockIdx.x * HD + d] = from_f32<T>(y);
+}
+
+// The same for many rows: HD / 4 threads a (row, head), four dims each, a split at a time.
+template <int HD, typename T>
+__global__ __launch_bounds__(256) void k_attn_merge_many(Part part, int most, int least, Cache c, Rows s, const T *gate,
+                                                         int64_t gate_stride, T *out, int H, Mask mask) {
+    constexpr int TPR = HD / 4, RPW = 256 / TPR;
+    const int groups = (H + RPW - 1) / RPW, n = blockIdx.x / groups;
+    const int h = min((int)(blockIdx.x % groups) * RPW + (int)threadIdx.x / TPR, H - 1), d = 4 * (threadIdx.x % TPR);
+    const int ns = splits_of<HD>(c, s, mask, n, h, H, most, least);
+    if (ns <= 1) return;
+    const int64_t row = (int64_t)n * H + h;
+    const float2 *ml = part.ml + row * most;
+    const float *p = part.acc + row * most * HD + d;
+    float M = -INFINITY, L = 0.f;
+    for (int z = 0; z < ns; z++) M = fmaxf(M, ml[z].x);
+    f32x4 A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int z = 0; z < ns; z++) {
+        const float2 x = ml[z];
+        const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - M);
+        L += x.y * f;
+        A += *(const f32x4 *)(p + (int64_t)z * HD) * f;
+    }
+    A *= L == 0.f ? 0.f : 1.0f / L;
+    if (gate)
+#pragma unroll
+        for (int e = 0; e < 4; e++) A[e] = gated(A[e], gate + n * gate_stride + (int64_t)h * HD + d + e);
+    T *y = out + row * HD + d;
+    if constexpr (sizeof(T) == 4)
+        *(f32x4 *)y = A;
+    else
+        *(uint64_t *)y = (uint64_t)gd_f2h(A[0]) | ((uint64_t)gd_f2h(A[1]) << 16) | ((uint64_t)gd_f2h(A[2]) << 32) |
+                         ((uint64_t)gd_f2h(A[3]) << 48);
 }
 
 // ---------------------------------------------------------------- checks
@@ -1116,6 +1170,29 @@ int check_seqs(gd_ctx *ctx, const char *fn, const gd_seqs *s) {
                "%s: %lld rows of %d sequences need row_start (one row each without)", fn, (long long)s->n_rows, s->n_seq);
     GD_REQUIRE(ctx, s->n_rows == 0 || s->n_seq == 0 || (s->pos && s->page_table), "%s: null positions or page table", fn);
     GD_REQUIRE(ctx, s->max_pages > 0 && s->max_len >= 0, "%s: max_pages %d, max_len %d", fn, s->max_pages, s->max_len);
+    return GD_OK;
+}
+
+// Memory for the partials of ns key splits, `bytes` each: the attention scratch where it
+// holds them, else the context's workspace, up to WS_BYTES; ns becomes what there is memory
+// for (1: none needed).  A recording takes the workspace as it is.
+constexpr size_t WS_BYTES = 256u << 20;
+int split_scratch(gd_ctx *ctx, size_t bytes, int64_t &ns, float **scratch) {
+    size_t most = GD_ATTN_SCRATCH_BYTES;
+    void *p = nullptr;
+    if (ns > 1 && ns * bytes > most) {
+        const size_t want = std::min<size_t>(ns * bytes, std::max(bytes, WS_BYTES / bytes * bytes));
+        const size_t have = ctx->recording ? std::min(want, ctx->ws_bytes) : want;
+        if (have / bytes > most / bytes && have / bytes > 1) {
+            const int rc = gd_ctx_workspace(ctx, have, &p);
+            if (rc) return rc;
+            most = have;
+        }
+    }
+    ns = std::max<int64_t>(1, std::min<int64_t>(ns, most / bytes));
+    if (ns > 1 && !p) p = gd_attn_scratch(ctx);
+    if (!p) ns = 1;
+    *scratch = (float *)p;
     return GD_OK;
 }
 
@@ -1307,11 +1384,10 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const int64_t blocks = (keys + width - 1) / width;
     const int64_t wgs = tokens ? s->n_rows * kv->n_head_kv * ((G + 7) / 8)
                                : (s->n_rows * G / PC + std::min<int64_t>(s->n_seq, s->n_rows)) * kv->n_head_kv;
-    const int64_t least = tokens ? std::max<int64_t>(TW, wgs * blocks / (8 * cus)) : std::max<int64_t>(4, wgs * blocks / (4 * cus));
-    int64_t ns = std::min({(blocks + least - 1) / least, (int64_t)MAX_SPLITS,
-                           (int64_t)(GD_ATTN_SCRATCH_BYTES / ((size_t)s->n_rows * n_head * (hd + 2) * sizeof(float)))});
-    float *scratch = ns > 1 ? gd_attn_scratch(ctx) : nullptr;
-    if (!scratch) ns = 1;
+    const int64_t least = tokens ? std::max<int64_t>(TW, wgs * blocks / (8 * cus)) : std::max<int64_t>(8, wgs * blocks / (4 * cus));
+    int64_t ns = std::min<int64_t>((blocks + least - 1) / least, MAX_SPLITS);
+    float *scratch = nullptr;
+    if ((rc = split_scratch(ctx, (size_t)s->n_rows * n_head * (hd + 2) * sizeof(float), ns, &scratch))) return rc;
     const Part part{scratch, (float2 *)(scratch + s->n_rows * n_head * ns * hd)};
 #define GD_GO(HD_, I8_, T_) \
     do { \
@@ -1323,9 +1399,12 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
                            n_head, scale, mask); \
         if (ns > 1) { \
             GD_LAUNCHED(ctx, fn); \
-            hipLaunchKernelGGL((k_attn_merge<HD_, T_>), dim3((unsigned)(s->n_rows * n_head)), dim3(512), 0, ctx->stream, \
-                               part, (int)ns, (int)least, cache_of(kv), rows, (const T_ *)gate, gate_stride, (T_ *)out, \
-                               n_head, mask); \
+            const bool many = s->n_rows * n_head >= 1024; \
+            const int per = 1024 / HD_, merges = many ? (n_head + per - 1) / per : n_head; \
+            auto merge = many ? k_attn_merge_many<HD_, T_> : k_attn_merge<HD_, T_>; \
+            hipLaunchKernelGGL(merge, dim3((unsigned)(s->n_rows * merges)), dim3(many ? 256 : 512), 0, ctx->stream, part, \
+                               (int)ns, (int)least, cache_of(kv), rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head, \
+                               mask); \
         } \
     } while (0)
     GD_KV_PICK(kv, x_dtype, GD_GO);
