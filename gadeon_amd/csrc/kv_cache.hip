@@ -81,6 +81,11 @@ __device__ __forceinline__ int seq_of_row(const Rows &s, int n) {
 // sequence b and place k in it, for the whole wave.  False: fewer units than that.
 template <class F>
 __device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, int &b, int &k) {
+    if (!s.row_start) {                          // a row, and a unit, each
+        b = u;
+        k = 0;
+        return u < s.n_seq && s.pos[u] >= 0;
+    }
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int c = 0; c < s.n_seq; c += 64) {
@@ -150,17 +155,30 @@ struct Turns {
     uint64_t t[128];
 };
 
+// Four elements at x as floats, and back.
+template <typename T, bool VEC> __device__ __forceinline__ f32x4 load4(const T *x) {
+    if constexpr (!VEC) return f32x4{to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3])};
+    else if constexpr (sizeof(T) == 4) return *(const f32x4 *)x;
+    else return __builtin_convertvector(*(const f16x4 *)x, f32x4);
+}
+
 // Rotates and appends the rows that fall into one block of 16 positions of a
 // sequence (unit blockIdx.x), and turns its query rows: wave w of workgroup y takes
 // the heads 4 y + w of H query heads, then the kv heads' keys, then their values.
-// The cos and sin of the block's positions are formed once a workgroup, and rows turned,
+//   A lane holds eight elements of a row as two fours, whose elements make four of the
+// rotated pairs (j and j + n_rot / 2, n_rot a multiple of 8) or eight of the dims behind
+// them: 64 lanes are four rows of head dim 128 or two of 256, the block's 16 rows that
+// many steps, all requested at once (a row at a time 46 us for 2175 rows of 24 / 4 x
+// 256, its loads one after the other).
+//   The cos and sin of the block's positions are formed once a workgroup, and rows turned,
 // in 64 bits: from turns in 32 one code in 40 000 came out on the other side of a
 // border, and one half in 700 a step off.
-template <int HD, bool I8, typename T>
+template <int HD, bool I8, bool VEC, typename T>
 __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, const T *q, int64_t q_stride, T *q_out,
                                                 int H, const T *kx, int64_t k_stride, const T *vx, int64_t v_stride,
                                                 int n_rot) {
-    constexpr int NP = HD / 128;                 // pairs of a lane
+    // Lanes of a row, rows of a step, steps; pairs of a lane are VEC ? 4 : 1 wide.
+    constexpr int LPR = HD / 8, RPS = 64 / LPR, ST = BLK / RPS;
     __shared__ double2 cs[BLK * (HD / 2)];
     const int t = threadIdx.x, lane = t & 63, half = n_rot / 2;
     int b, blk;
@@ -174,6 +192,44 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
     const int skip = blk ? blk * BLK - sq.pos % BLK : 0;
     const int r = sq.r0 + skip, n = min(BLK - off, sq.r1 - r);
     const uint32_t p = (uint32_t)sq.pos + (uint32_t)skip;
+    const int hs = blockIdx.y * 4 + (t >> 6), H2 = H + 2 * c.HKV;
+    const bool is_q = hs < H, is_k = !is_q && hs < H + c.HKV;
+    const int h = is_q ? hs : hs - H - (is_k ? 0 : c.HKV);
+    // This lane's place: row `lr` of a step's, elements d0 .. and d1 .. of it.  Without VEC
+    // (any n_rot, any alignment) element e of both is a pair of its own.
+    const int lr = lane / LPR, j0 = 4 * (lane % LPR);
+    auto dims = [&](int e, int &d0, int &d1) {
+        const int j = j0 + e;
+        d0 = j < half ? j : n_rot + 2 * (j - half);
+        d1 = j < half ? j + half : d0 + 1;
+        if (VEC && j0 >= half) {
+            d0 = n_rot + 2 * (j0 - half) + e;
+            d1 = d0 + 4;
+        }
+    };
+    f32x4 x0[ST], x1[ST];
+    if (hs < H2) {
+        const T *src = (is_q ? q + r * q_stride : is_k ? kx + r * k_stride : vx + r * v_stride) + (int64_t)h * HD;
+        const int64_t stride = is_q ? q_stride : is_k ? k_stride : v_stride;
+#pragma unroll
+        for (int i = 0; i < ST; i++) {
+            const T *row = src + min(i * RPS + lr, n - 1) * stride;
+            if constexpr (VEC) {
+                int d0, d1;
+                dims(0, d0, d1);
+                x0[i] = load4<T, true>(row + d0);
+                x1[i] = load4<T, true>(row + d1);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    int d0, d1;
+                    dims(e, d0, d1);
+                    x0[i][e] = to_f32(row[d0]);
+                    x1[i][e] = to_f32(row[d1]);
+                }
+            }
+        }
+    }
     const int64_t rp = (int64_t)p + (s.shift ? s.shift[b] : 0);
     for (int i = t; i < n * half; i += 256) {
         const int64_t turn = (int64_t)((uint64_t)(rp + i / half) * turns.t[i % half]);
@@ -182,121 +238,142 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
         cs[i] = double2{cn, sn};
     }
     __syncthreads();
-    const int hs = blockIdx.y * 4 + (t >> 6);
-    if (hs >= H + 2 * c.HKV) return;
-    // Pair j of a head: the dims j and j + half, past the rotated ones two neighbours.
-    int d0[NP], d1[NP];
-#pragma unroll
-    for (int e = 0; e < NP; e++) {
-        const int j = lane + 64 * e;
-        d0[e] = j < half ? j : n_rot + 2 * (j - half);
-        d1[e] = j < half ? j + half : d0[e] + 1;
-    }
-    // Row i's pair e, turned where it is one of the rotated.
-    auto turned = [&](bool turn, int i, int e, float x0, float x1, double &a, double &z) {
-        a = x0, z = x1;
-        if (turn && lane + 64 * e < half && i < n) {
-            const double2 w = cs[i * half + lane + 64 * e];
+    if (hs >= H2) return;
+    const bool turn = is_q || is_k;
+    // Element e of step i, turned where it is one of the rotated.
+    auto turned = [&](int i, int e, double &a, double &z) {
+        a = x0[i][e], z = x1[i][e];
+        const int row = i * RPS + lr, j = j0 + e;
+        if (turn && j < half && row < n) {
+            const double2 w = cs[row * half + j];
             const double o = a;
             a = o * w.x - z * w.y;
             z = o * w.y + z * w.x;
         }
     };
-    if (hs < H) {
-        for (int i = 0; i < n; i++) {
-            const T *x = q + (r + i) * q_stride + (int64_t)hs * HD;
-            T *y = q_out + ((int64_t)(r + i) * H + hs) * HD;
+    // Four results at d0 and four at d1 of a row in memory.
+    auto put = [&](auto *y, auto a, auto z) {
+        if constexpr (VEC) {
+            int d0, d1;
+            dims(0, d0, d1);
+            *(decltype(a) *)(y + d0) = a;
+            *(decltype(z) *)(y + d1) = z;
+        } else {
 #pragma unroll
-            for (int e = 0; e < NP; e++) {
-                double a, z;
-                turned(true, i, e, to_f32(x[d0[e]]), to_f32(x[d1[e]]), a, z);
-                y[d0[e]] = from_f64<T>(a);
-                y[d1[e]] = from_f64<T>(z);
+            for (int e = 0; e < 4; e++) {
+                int d0, d1;
+                dims(e, d0, d1);
+                y[d0] = a[e];
+                y[d1] = z[e];
             }
+        }
+    };
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+    typedef int8_t i8x4 __attribute__((ext_vector_type(4)));
+    if (is_q) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) {
+            const int row = i * RPS + lr;
+            if (row >= n) break;
+            T4 a4, z4;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                double a, z;
+                turned(i, e, a, z);
+                a4[e] = from_f64<T>(a);
+                z4[e] = from_f64<T>(z);
+            }
+            put(q_out + ((int64_t)(r + row) * H + h) * HD, a4, z4);
         }
         return;
     }
-    const bool is_k = hs < H + c.HKV;
-    const int h = hs - H - (is_k ? 0 : c.HKV);
-    const T *src = (is_k ? kx + r * k_stride : vx + r * v_stride) + (int64_t)h * HD;
-    const int64_t stride = is_k ? k_stride : v_stride;
     void *plane = is_k ? c.k : c.v;
-    if (!I8) {
+    if constexpr (!I8) {
         // A page may end inside the block.  Values past f16's range are held as its
         // largest.
-        for (int i = 0; i < n; i++) {
-            const int page = page_of(c, s, b, p + i);
-            if (page < 0) continue;
-            uint16_t *y = (uint16_t *)plane + (uint64_t)row_at<false>(c, page, slot_of(c, p + i), h) * HD;
-            auto f16_of = [](double x) { return from_f64<uint16_t>(x > 65504. ? 65504. : x < -65504. ? -65504. : x); };
+        auto f16_of = [](double x) { return from_f64<uint16_t>(x > 65504. ? 65504. : x < -65504. ? -65504. : x); };
+        int page[ST];
 #pragma unroll
-            for (int e = 0; e < NP; e++) {
+        for (int i = 0; i < ST; i++) page[i] = page_of(c, s, b, p + i * RPS + lr);
+#pragma unroll
+        for (int i = 0; i < ST; i++) {
+            const int row = i * RPS + lr;
+            if (row >= n) break;
+            if (page[i] < 0) continue;
+            u16x4 a4, z4;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
                 double a, z;
-                turned(is_k, i, e, to_f32(src[i * stride + d0[e]]), to_f32(src[i * stride + d1[e]]), a, z);
-                y[d0[e]] = f16_of(a);
-                y[d1[e]] = f16_of(z);
+                turned(i, e, a, z);
+                a4[e] = f16_of(a);
+                z4[e] = f16_of(z);
             }
+            put((uint16_t *)plane + (uint64_t)row_at<false>(c, page[i], slot_of(c, p + row), h) * HD, a4, z4);
         }
         return;
-    }
-    const int page = page_of(c, s, b, p);
-    if (page < 0) return;
-    const int slot = slot_of(c, p);              // of the first new row; the block's is slot - off
-    float x0[BLK][NP], x1[BLK][NP];
+    } else {
+        const int page = page_of(c, s, b, p);
+        if (page < 0) return;
+        const uint32_t at = row_at<true>(c, page, slot_of(c, p) - off, h);
+        uint8_t *xp = (is_k ? c.kx : c.vx) + at / BLK;
+        int8_t *y = (int8_t *)plane + (uint64_t)at * HD;
+        const int had = off ? *xp : 0;
+        float top = 0.f;
+        bool nan = false;
 #pragma unroll
-    for (int i = 0; i < BLK; i++)
+        for (int i = 0; i < ST; i++)
 #pragma unroll
-        for (int e = 0; e < NP; e++) {
-            x0[i][e] = i < n ? to_f32(src[i * stride + d0[e]]) : 0.f;
-            x1[i][e] = i < n ? to_f32(src[i * stride + d1[e]]) : 0.f;
-        }
-    float top = 0.f;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < BLK; i++)
-#pragma unroll
-        for (int e = 0; e < NP; e++) {
-            double a, z;
-            turned(is_k, i, e, x0[i][e], x1[i][e], a, z);
-            top = fmaxf(top, fmaxf(fabsf((float)a), fabsf((float)z)));
-            nan |= a != a || z != z;
-        }
-    top = wave_max(top);
-    const uint32_t bits = __float_as_uint(top);
-    int ex = (int)(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u);   // 127 2^ex holds top
-    ex = min(max(ex, EXP_MIN), EXP_MAX);
-    const uint32_t row = row_at<true>(c, page, slot - off, h);
-    uint8_t *xp = (is_k ? c.kx : c.vx) + row / BLK;
-    int8_t *y = (int8_t *)plane + (uint64_t)row * HD;
-    nan = __any(nan);
-    if (off) {
-        // The rows before these keep their codes, or take the greater step.
-        const int had = *xp;
-        nan |= had == EXP_NAN;
-        const int ex0 = min(max(had - EXP_BIAS, EXP_MIN), EXP_MAX);
-        if (ex > ex0) {
-            const float f = __uint_as_float((uint32_t)(127 + ex0 - ex) << 23);
-            for (int i = 0; i < off; i++)
-#pragma unroll
-                for (int e = 0; e < NP; e++) {
-                    y[i * HD + d0[e]] = (int8_t)rintf(y[i * HD + d0[e]] * f);
-                    y[i * HD + d1[e]] = (int8_t)rintf(y[i * HD + d1[e]] * f);
+            for (int e = 0; e < 4; e++) {
+                // (In 32 bits, which is as good for a maximum and holds no 64-bit values till below.)
+                const int row = i * RPS + lr, j = j0 + e;
+                float a = x0[i][e], z = x1[i][e];
+                if (turn && j < half && row < n) {
+                    const double2 w = cs[row * half + j];
+                    const float cn = (float)w.x, sn = (float)w.y, o = a;
+                    a = o * cn - z * sn;
+                    z = o * sn + z * cn;
                 }
+                if (row >= n) a = z = 0.f;
+                top = fmaxf(top, fmaxf(fabsf(a), fabsf(z)));
+                nan |= a != a || z != z;
+            }
+        top = wave_max(top);
+        const uint32_t bits = __float_as_uint(top);
+        int ex = (int)(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u);   // 127 2^ex holds top
+        ex = min(max(ex, EXP_MIN), EXP_MAX);
+        nan = __any(nan);
+        if (off) {
+            // The rows before these keep their codes, or take the greater step.
+            nan |= had == EXP_NAN;
+            const int ex0 = min(max(had - EXP_BIAS, EXP_MIN), EXP_MAX);
+            if (ex > ex0) {
+                const float f = __uint_as_float((uint32_t)(127 + ex0 - ex) << 23);
+                for (int i = lane; i < off * (HD / 4); i += 64) {
+                    i8x4 o = ((const i8x4 *)y)[i];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[e] = (int8_t)rintf(o[e] * f);
+                    ((i8x4 *)y)[i] = o;
+                }
+            }
+            ex = max(ex, ex0);
         }
-        ex = max(ex, ex0);
-    }
-    if (lane == 0) *xp = nan ? EXP_NAN : (uint8_t)(ex + EXP_BIAS);
-    const double inv = __longlong_as_double((long long)(1023 - ex) << 52);
-    auto code = [&](double x) { return (int8_t)(int)fmin(fmax(rint(x * inv), -127.0), 127.0); };
+        if (lane == 0) *xp = nan ? EXP_NAN : (uint8_t)(ex + EXP_BIAS);
+        const double inv = __longlong_as_double((long long)(1023 - ex) << 52);
+        auto code = [&](double x) { return (int8_t)(int)fmin(fmax(rint(x * inv), -127.0), 127.0); };
 #pragma unroll
-    for (int i = 0; i < BLK; i++) {
-        if (i >= n) break;
+        for (int i = 0; i < ST; i++) {
+            const int row = i * RPS + lr;
+            if (row >= n) break;
+            i8x4 a4, z4;
 #pragma unroll
-        for (int e = 0; e < NP; e++) {
-            double a, z;
-            turned(is_k, i, e, x0[i][e], x1[i][e], a, z);
-            y[(off + i) * HD + d0[e]] = code(a);
-            y[(off + i) * HD + d1[e]] = code(z);
+            for (int e = 0; e < 4; e++) {
+                double a, z;
+                turned(i, e, a, z);
+                a4[e] = code(a);
+                z4[e] = code(z);
+            }
+            put(y + (off + row) * HD, a4, z4);
         }
     }
 }
@@ -1314,9 +1391,16 @@ extern "C" int gd_kv_append_rope(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s,
     // Blocks of 16 positions that the rows can touch: rows / 16 and two ends a sequence.
     const int64_t units = std::min<int64_t>(s->n_rows, s->n_rows / BLK + 2 * std::min<int64_t>(s->n_seq, s->n_rows));
     const dim3 grid((unsigned)units, gd_blocks(H + 2 * kv->n_head_kv, 4));
+    // Fours of a row in one access: what its place, stride and rotated dims allow.
+    const int size = x_dtype == GD_F32 ? 4 : 2;
+    const bool vec = n_rot % 8 == 0 && (k_stride | v_stride | (q ? q_stride : 0)) % 4 == 0 &&
+                     ((uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_out) % (4 * size) == 0;
 #define GD_GO(HD_, I8_, T_) \
-    hipLaunchKernelGGL((k_append<HD_, I8_, T_>), grid, dim3(256), 0, ctx->stream, cache_of(kv), rows_of(kv, s), turns, \
-                       (const T_ *)q, q_stride, (T_ *)q_out, H, (const T_ *)k, k_stride, (const T_ *)v, v_stride, n_rot)
+    do { \
+        auto kernel = vec ? k_append<HD_, I8_, true, T_> : k_append<HD_, I8_, false, T_>; \
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, cache_of(kv), rows_of(kv, s), turns, (const T_ *)q, \
+                           q_stride, (T_ *)q_out, H, (const T_ *)k, k_stride, (const T_ *)v, v_stride, n_rot); \
+    } while (0)
     GD_KV_PICK(kv, x_dtype, GD_GO);
 #undef GD_GO
     GD_LAUNCHED(ctx, fn);
