@@ -467,17 +467,18 @@ struct Part {
 // transposing LDS read (no barrier in the loop).  The 16 columns of an MFMA are the
 // heads' q as f16 hi (0..7) and lo (8..15), and P likewise: both halves of a product
 // come from one instruction and are added across lanes lr, lr ^ 8.  q is brought to
-// 2^14 .. 2^15 by a power of two and weights to 2^14, so that no low half leaves f16's
+// 2^14 .. 2^15 by a power of two and weights to 2^8, so that hardly a low half leaves f16's
 // normal range; scores are in units of log2.  8-bit keys enter as whole numbers, their
 // steps scaling the scores; 8-bit values as the halves they are.  Keys that are not
 // seen have the weight 0 and zeros for values.  A block's rows are requested one
 // block ahead, its page-table entries two.
 constexpr int TW = 4;                            // waves
+constexpr float LAZY = 7.f;                      // how far (log2) weights may pass the maximum they stand at
 constexpr int MAX_SPLITS = 64;                   // what the combine weighs in one wave
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <int HD, bool I8, bool TILED, typename T>
-__global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_tokens(
+__global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && HD == 128 ? 3 : 2))) void k_attn_tokens(
         Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part, int most,
         int least, int H, float scale, Mask mask) {
     constexpr int KS = HD / 32, DT = HD / 16, VP = HD + 16;
@@ -652,7 +653,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         if (!seen) continue;
         // hi + lo of a head's score; keys 16 kt + 4 g + v of the block.  (Unscaled:
         // a weight's exponent is rounded once.)
-        float bmax = -INFINITY;
+        float top = -INFINITY;                   // of this lane's keys
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
@@ -661,24 +662,25 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
                 sc[kt][v] += gd_dpp<GD_DPP_ROR8>(sc[kt][v]);
                 if constexpr (I8) sc[kt][v] *= kstep[kt];
                 if (seen != 0xffffffffu && !(seen >> k & 1)) sc[kt][v] = none;
-                bmax = fmaxf(bmax, sc[kt][v] * sf);
+                top = fmaxf(top, sc[kt][v] * sf);
             }
-        bmax = fmaxf(bmax, __shfl_xor(bmax, 16, 64));
-        bmax = fmaxf(bmax, __shfl_xor(bmax, 32, 64));
-        const float mn = fmaxf(m, bmax);
-        if (__any(mn > m)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+        // The sums are brought to a new maximum, of all a column's lanes, only where one is
+        // over 2^LAZY of the one they stand at.
+        if (__any(top > m + LAZY)) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             l *= alpha;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) acc[dt] *= alpha;
             m = mn;
         }
-        f16x8 pf;                                // weights times 2^14, and so are l and the sums
+        f16x8 pf;                                // weights times 2^8, under 2^15, and so l and the sums
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int v = 0; v < 4; v++) {
-                float p = __builtin_amdgcn_exp2f(fmaf(sc[kt][v], sf, -m)) * 16384.f;
+                float p = __builtin_amdgcn_exp2f(fmaf(sc[kt][v], sf, -m)) * 256.f;
                 asm("" : "+v"(p));
                 l += p;
                 const f16 hi = (f16)p;
@@ -752,7 +754,6 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // mask, and where V holds a NaN or infinity its finite part and, apart, which columns see
 // the others (0 x NaN would reach them all).
 constexpr int PC = 128;                          // columns of a unit
-constexpr float LAZY = 7.f;
 template <int HD> constexpr int tile_keys() { return HD == 128 ? 64 : 32; }
 
 struct Tile {
@@ -1006,11 +1007,10 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             for (int kt = 0; kt < NT; kt++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) top = fmaxf(top, st[kt][v]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            // Sums are brought to a new maximum only where it is over 2^LAZY of the one they
-            // stand at (random scores: hardly after the first tiles).
-            const float mn = fmaxf(m, top * sf);
-            if (__any(mn > m + LAZY)) {
+            // Sums are brought to a new maximum only where a score is over 2^LAZY of the one
+            // they stand at (random scores: hardly after the first tiles).
+            if (__any(top * sf > m + LAZY)) {
+                const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * sf);
                 const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
                 l *= alpha;
 #pragma unroll
