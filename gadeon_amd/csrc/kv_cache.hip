@@ -81,11 +81,6 @@ __device__ __forceinline__ int seq_of_row(const Rows &s, int n) {
 // sequence b and place k in it, for the whole wave.  False: fewer units than that.
 template <class F>
 __device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, int &b, int &k) {
-    if (!s.row_start) {                          // a row, and a unit, each
-        b = u;
-        k = 0;
-        return u < s.n_seq && s.pos[u] >= 0;
-    }
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int c = 0; c < s.n_seq; c += 64) {
@@ -185,7 +180,13 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
     auto blocks = [](const Seq &q) {
         return q.r1 > q.r0 ? (int)(((uint32_t)q.pos % BLK + (uint32_t)(q.r1 - q.r0) + BLK - 1) / BLK) : 0;
     };
-    if (!unit_at(s, blockIdx.x, blocks, b, blk)) return;
+    if (!s.row_start) {                          // a row, and a block, each
+        b = blockIdx.x;
+        blk = 0;
+        if (s.pos[b] < 0) return;
+    } else if (!unit_at(s, blockIdx.x, blocks, b, blk)) {
+        return;
+    }
     const Seq sq = seq_at(s, b);
     // The block's new rows: n of them from row r on, the first at slot `off` of it.
     const int off = blk ? 0 : sq.pos % BLK;
@@ -459,10 +460,32 @@ struct Part {
     float2 *ml;
 };
 
+// How finely single tokens' keys are split, from the rows' own lengths (the host knows a
+// bound of them alone): the fewest blocks of a split, so that all the splits' workgroups,
+// `groups` for each, fill the `slots` that the chip holds at once; from LEAST on, what a
+// workgroup's start, end and merge cost.  Rows of much the same length are left whole.
+constexpr int LEAST = 8;
+__device__ __forceinline__ KeyBlocks<32> token_blocks(const Rows &s, const Mask &mask, int pos) {
+    return KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
+}
+__device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int groups, int slots) {
+    const int lane = threadIdx.x & 63;
+    float sum = 0.f, most = 0.f;
+    for (int b = lane; b < s.n_seq; b += 64) {
+        const int pos = s.pos[b];
+        const float n = pos < 0 ? 0.f : (float)token_blocks(s, mask, pos).n;
+        sum += n;
+        most = fmaxf(most, n);
+    }
+    sum = gd_wave_sum(sum);
+    most = wave_max(most);
+    const float least = fmaxf((float)LEAST, ceilf(sum * (float)groups / (float)slots));
+    return most <= 1.6f * least ? max(1, (int)most) : (int)least;
+}
+
 // Attention of single tokens: workgroup (row, kv head and eight of its query heads;
-// split sp) reads the split's keys once for its heads.  A row's blocks of 32 keys go to
-// as many of the `most` splits as leave each `least` of them (the other workgroups end
-// at once): ns splits, and wave w of split sp takes the blocks sp + ns (w + TW i): S = K Q^T with K straight from the cache as the A
+// split sp of ns) reads the split's keys once for its heads.  Wave w takes the blocks
+// of 32 keys sp + ns (w + TW i): S = K Q^T with K straight from the cache as the A
 // operand, and O^T += V^T P^T with V staged in the wave's own LDS rows and read by the
 // transposing LDS read (no barrier in the loop).  The 16 columns of an MFMA are the
 // heads' q as f16 hi (0..7) and lo (8..15), and P likewise: both halves of a product
@@ -480,7 +503,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 template <int HD, bool I8, bool TILED, typename T>
 __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && HD == 128 ? 3 : 2))) void k_attn_tokens(
         Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part, int most,
-        int least, int H, float scale, Mask mask) {
+        int slots, int H, float scale, Mask mask) {
     constexpr int KS = HD / 32, DT = HD / 16, VP = HD + 16;
     constexpr int KL = I8 ? KS / 2 : KS;         // 16-byte loads of a key tile, per lane
     constexpr int CPK = I8 ? HD / 16 : HD / 8;   // 16-byte chunks of a value row
@@ -491,13 +514,19 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
     __shared__ float wm[TW][8], wl[TW][8];
     static_assert(sizeof(Vs) >= (size_t)TW * 8 * HD * 4, "the merge reuses Vs");
     const int G = H / c.HKV, groups = c.HKV * ((G + 7) / 8);
-    const int n = blockIdx.x / groups, gr = blockIdx.x % groups, sp = blockIdx.y;
+    const int gr = blockIdx.x % groups;
     const int kvh = gr / ((G + 7) / 8), g8 = 8 * (gr % ((G + 7) / 8)), h0 = kvh * G + g8, nh = min(8, G - g8);
+    int n = blockIdx.x / groups, sp = 0, ns = 1;
+    if (most > 1) {
+        // The rows' splits one after the other, so that the workgroups that have none come last.
+        const int least = token_least(s, mask, groups, slots);
+        auto splits = [&](const Seq &q) { return q.r1 > q.r0 ? token_blocks(s, mask, q.pos).splits(most, least) : 0; };
+        if (!unit_at(s, n, splits, n, sp)) return;
+        ns = token_blocks(s, mask, s.pos[n]).splits(most, least);
+    }
     const int pos = s.pos[n];
     if (pos < 0) return;
-    const KeyBlocks<32> kb(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
-    const int ns = kb.splits(most, least);
-    if (sp >= ns) return;
+    const KeyBlocks<32> kb = token_blocks(s, mask, pos);
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int lr = lane & 15, g = lane >> 4, col = lr & 7;
     // Key lane % 32 of block j: its page-table entry (a load, used a block later), then its
@@ -563,39 +592,55 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
     Entry en = entry_of(j);
     Key kc = key_of(en);
     en = entry_of(j + step);
+    if (kb.n) fetch(kc);
+    // The gates of this thread's results, for the end (partials are gated by the merge).
+    float gates[8 * HD / (64 * TW)];
+#pragma unroll
+    for (int x = 0; x < 8 * HD / (64 * TW); x++) {
+        const int e = t + 64 * TW * x;
+        gates[x] = gate && ns == 1 && e < nh * HD ? to_f32(gate[n * gate_stride + (int64_t)h0 * HD + e]) : 0.f;
+    }
+    // q's operand, a share of its dims a wave.
     float sf;                                    // score factor of this lane's head
     {
+        constexpr int KW = KS / TW;
         const T *qrow = q + n * q_stride + (int64_t)(h0 + min(col, nh - 1)) * HD;
         // Dim of element e of k step ks: as the cache's 16-byte loads give them.
         auto dim = [&](int ks) { return I8 ? 64 * (ks / 2) + 16 * g + 8 * (ks % 2) : 32 * ks + 8 * g; };
-        float qv[KS][8], mx = 0.f;
+        f32x4 qv[KW][2];
+        float mx = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+        for (int i = 0; i < KW; i++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                qv[ks][e] = to_f32(qrow[dim(ks) + e]);
-                mx = fmaxf(mx, fabsf(qv[ks][e]));
+            for (int e = 0; e < 2; e++) {
+                const T *x = qrow + dim(w * KW + i) + 4 * e;
+                if constexpr (sizeof(T) == 4) qv[i][e] = *(const f32x4 *)x;
+                else qv[i][e] = __builtin_convertvector(*(const f16x4 *)x, f32x4);
+#pragma unroll
+                for (int k = 0; k < 4; k++) mx = fmaxf(mx, fabsf(qv[i][e][k]));
             }
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (lane < 8) wm[w][lane] = mx;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TW; i++) mx = fmaxf(mx, wm[i][col]);
         const int ex = min(max((int)(__float_as_uint(mx) >> 23), 40), 254) - 127;
         const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
         sf = scale * LOG2E * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
         if (fabsf(sf) < 0x1p-126f) sf = 0x1p-126f;         // weights of 1 alike; times inf not NaN
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            if (ks % TW != w) continue;
+        for (int i = 0; i < KW; i++) {
             f16x8 qf;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 f16 hi, lo;
-                gd_split_f16(col < nh ? qv[ks][e] * up : 0.f, hi, lo);
+                gd_split_f16(col < nh ? qv[i][e >> 2][e & 3] * up : 0.f, hi, lo);
                 qf[e] = lr < 8 ? hi : lo;
             }
-            Qs[ks][lane] = qf;
+            Qs[w * KW + i][lane] = qf;
         }
     }
-    if (kb.n) fetch(kc);
     const float none = sf < 0.f ? INFINITY : -INFINITY;    // the score of no key
     f32x4 acc[DT];                               // O^T rows 16 dt + 4 g + v
 #pragma unroll
@@ -640,9 +685,11 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
             } else {
                 v[0] = __builtin_bit_cast(f16x8, vreg[i]);
             }
-            if (seen != 0xffffffffu && !(seen >> k & 1))
+            if (seen != 0xffffffffu) {
+                asm volatile("");                // a branch, not selects in every block
 #pragma unroll
-                for (int x = 0; x < (I8 ? 2 : 1); x++) v[x] = f16x8{};
+                for (int x = 0; x < (I8 ? 2 : 1); x++) v[x] = seen >> k & 1 ? v[x] : f16x8{};
+            }
 #pragma unroll
             for (int x = 0; x < (I8 ? 2 : 1); x++) *(f16x8 *)(row + 8 * x) = v[x];
         }
@@ -653,17 +700,26 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
         if (!seen) continue;
         // hi + lo of a head's score; keys 16 kt + 4 g + v of the block.  (Unscaled:
         // a weight's exponent is rounded once.)
-        float top = -INFINITY;                   // of this lane's keys
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int v = 0; v < 4; v++) {
-                const int k = 16 * kt + 4 * g + v;
                 sc[kt][v] += gd_dpp<GD_DPP_ROR8>(sc[kt][v]);
                 if constexpr (I8) sc[kt][v] *= kstep[kt];
-                if (seen != 0xffffffffu && !(seen >> k & 1)) sc[kt][v] = none;
-                top = fmaxf(top, sc[kt][v] * sf);
             }
+        if (seen != 0xffffffffu) {
+            asm volatile("");
+            const uint32_t mine = seen >> (4 * g);
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) sc[kt][v] = mine & (1u << (16 * kt + v)) ? sc[kt][v] : none;
+        }
+        float top = -INFINITY;                   // of this lane's keys
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) top = fmaxf(top, sc[kt][v] * sf);
         // The sums are brought to a new maximum, of all a column's lanes, only where one is
         // over 2^LAZY of the one they stand at.
         if (__any(top > m + LAZY)) {
@@ -697,19 +753,17 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
                     f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]}, pf, acc[dt], 0, 0, 0);
         }
     }
-    // Merge the waves: each scales its sums to the common maximum.
+    // Merge the waves: each brings its sums to the common maximum.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    if (lane < 8) {
-        wm[w][lane] = m;
-        wl[w][lane] = l;
-    }
+    if (lane < 8) wm[w][lane] = m;
     __syncthreads();
     float M = -INFINITY;
 #pragma unroll
     for (int i = 0; i < TW; i++) M = fmaxf(M, wm[i][col]);
     const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
     float *red = (float *)Vs;                    // [TW][8][HD]
+    if (lane < 8) wl[w][lane] = l * f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
@@ -717,25 +771,29 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
         if (lr < 8) *(f32x4 *)&red[(w * 8 + lr) * HD + 16 * dt + 4 * g] = acc[dt] * f;
     }
     __syncthreads();
-    auto weight = [&](int i, int hh) { return wm[i][hh] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wm[i][hh] - fmaxf(fmaxf(wm[0][hh], wm[1][hh]), fmaxf(wm[2][hh], wm[3][hh]))); };
-    static_assert(TW == 4, "the waves' maxima");
-    for (int e = t; e < nh * HD; e += 64 * TW) {
-        const int hh = e / HD, d = e % HD;
+#pragma unroll
+    for (int x = 0; x < 8 * HD / (64 * TW); x++) {
+        const int e = t + 64 * TW * x, hh = e / HD, d = e % HD;
+        if (e >= nh * HD) break;
         float A = 0.f, L = 0.f;
 #pragma unroll
         for (int i = 0; i < TW; i++) {
             A += red[(i * 8 + hh) * HD + d];
-            L += wl[i][hh] * weight(i, hh);
+            L += wl[i][hh];
         }
         const int64_t row = (int64_t)n * H + h0 + hh;
         if (ns == 1) {
             float y = L == 0.f ? 0.f : A / L;
-            if (gate) y *= gd_sigmoid(to_f32(gate[n * gate_stride + (int64_t)(h0 + hh) * HD + d]));
+            if (gate) y *= gd_sigmoid(gates[x]);
             out[row * HD + d] = from_f32<T>(y);
         } else {
             part.acc[(row * most + sp) * HD + d] = A;
-            if (d == 0)
-                part.ml[row * most + sp] = make_float2(fmaxf(fmaxf(wm[0][hh], wm[1][hh]), fmaxf(wm[2][hh], wm[3][hh])), L);
+            if (d == 0) {
+                float M = wm[0][hh];
+#pragma unroll
+                for (int i = 1; i < TW; i++) M = fmaxf(M, wm[i][hh]);
+                part.ml[row * most + sp] = make_float2(M, L);
+            }
         }
     }
 }
@@ -1129,8 +1187,10 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 template <int HD>
 __device__ __forceinline__ int splits_of(const Cache &c, const Rows &s, const Mask &mask, int n, int h, int H, int most, int least) {
     if (!s.row_start) {
-        const int pos = s.pos[n];
-        return pos < 0 ? 0 : KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1)).splits(most, least);
+        // (`least` stands for the slots.)
+        const int pos = s.pos[n], groups = c.HKV * ((H / c.HKV + 7) / 8);
+        least = token_least(s, mask, groups, least);
+        return pos < 0 ? 0 : token_blocks(s, mask, pos).splits(most, least);
     }
     const int b = seq_of_row(s, n);
     if (b < 0) return 0;
@@ -1468,26 +1528,35 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const int64_t blocks = (keys + width - 1) / width;
     const int64_t wgs = tokens ? s->n_rows * kv->n_head_kv * ((G + 7) / 8)
                                : (s->n_rows * G / PC + std::min<int64_t>(s->n_seq, s->n_rows)) * kv->n_head_kv;
-    const int64_t least = tokens ? std::max<int64_t>(TW, wgs * blocks / (8 * cus)) : std::max<int64_t>(8, wgs * blocks / (4 * cus));
-    int64_t ns = std::min<int64_t>((blocks + least - 1) / least, MAX_SPLITS);
+    // Single tokens are left whole, without a merge's launch, where that is a few rounds of
+    // blocks a wave; how finely others are split, the kernel knows (token_least).
+    const int64_t slots = (kv->dtype == GD_I8 && hd == 128 ? 3 : 2) * cus;
+    const bool whole = blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus);
+    const int64_t least = tokens ? LEAST : std::max<int64_t>(8, wgs * blocks / (4 * cus));
+    int64_t ns = tokens && whole ? 1 : std::min<int64_t>((blocks + least - 1) / least, MAX_SPLITS);
     float *scratch = nullptr;
     if ((rc = split_scratch(ctx, (size_t)s->n_rows * n_head * (hd + 2) * sizeof(float), ns, &scratch))) return rc;
     const Part part{scratch, (float2 *)(scratch + s->n_rows * n_head * ns * hd)};
+    // Single tokens: a split for each `slots / groups` of all blocks at most, and one a row
+    // (token_least), with two to spare for its roundings.
+    const int64_t fine = tokens ? slots : least, groups = tokens ? wgs / s->n_rows : 1;
+    const dim3 grid = !tokens  ? dim3((unsigned)wgs, (unsigned)ns)
+                      : ns > 1 ? dim3((unsigned)(groups * std::min(s->n_rows * ns, s->n_rows + slots / groups + 2)))
+                               : dim3((unsigned)wgs);
 #define GD_GO(HD_, I8_, T_) \
     do { \
         const bool tiled = I8_ || kv->page_size % 16 == 0; \
         auto kernel = tokens ? (tiled ? k_attn_tokens<HD_, I8_, true, T_> : k_attn_tokens<HD_, I8_, I8_, T_>) \
                              : (tiled ? k_attn_rows<HD_, I8_, true, T_> : k_attn_rows<HD_, I8_, I8_, T_>); \
-        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs, (unsigned)ns), dim3(256), 0, ctx->stream, cache_of(kv), rows, \
-                           (const T_ *)q, q_stride, (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)least, \
-                           n_head, scale, mask); \
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, cache_of(kv), rows, (const T_ *)q, q_stride, \
+                           (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)fine, n_head, scale, mask); \
         if (ns > 1) { \
             GD_LAUNCHED(ctx, fn); \
             const bool many = s->n_rows * n_head >= 1024; \
             const int per = 1024 / HD_, merges = many ? (n_head + per - 1) / per : n_head; \
             auto merge = many ? k_attn_merge_many<HD_, T_> : k_attn_merge<HD_, T_>; \
             hipLaunchKernelGGL(merge, dim3((unsigned)(s->n_rows * merges)), dim3(many ? 256 : 512), 0, ctx->stream, part, \
-                               (int)ns, (int)least, cache_of(kv), rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head, \
+                               (int)ns, (int)fine, cache_of(kv), rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head, \
                                mask); \
         } \
     } while (0)
