@@ -77,6 +77,26 @@ __device__ __forceinline__ int seq_of_row(const Rows &s, int n) {
     return -1;
 }
 
+// Maximum over a wave, every lane getting it, and running sum over its lanes (by lane
+// moves within rows of 16, then rows; the whole wave active).
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, gd_dpp<GD_DPP_XOR1>(v));
+    v = fmaxf(v, gd_dpp<GD_DPP_XOR2>(v));
+    v = fmaxf(v, gd_dpp<GD_DPP_HALF_MIRROR>(v));
+    v = fmaxf(v, gd_dpp<GD_DPP_MIRROR>(v));
+    auto row = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
+    return fmaxf(fmaxf(row(0), row(16)), fmaxf(row(32), row(48)));
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // from 1, 2, 4, 8 lanes below in the row
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31);
+    const int r2 = r1 + __builtin_amdgcn_readlane(v, 47), row = (threadIdx.x & 63) >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
+}
+
 // Unit u of the sequences' units, `count` of them each (count(Seq) lane by lane): its
 // sequence b and place k in it, for the whole wave.  False: fewer units than that.
 template <class F>
@@ -85,20 +105,15 @@ __device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, int &b, i
     int base = 0;
     for (int c = 0; c < s.n_seq; c += 64) {
         const int n = c + lane < s.n_seq ? count(seq_at(s, c + lane)) : 0;
-        int sum = n;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int o = __shfl_up(sum, d, 64);
-            if (lane >= d) sum += o;
-        }
+        const int sum = wave_scan(n);
         const uint64_t past = __ballot(base + sum > u);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             b = c + l;
-            k = u - (base + __shfl(sum - n, l, 64));
+            k = u - (base + __builtin_amdgcn_readlane(sum - n, l));
             return k >= 0;
         }
-        base += __shfl(sum, 63, 64);
+        base += __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -134,12 +149,6 @@ template <typename T> __device__ __forceinline__ T from_f64(double x) {
     float f = (float)x;
     asm("" : "+v"(f));
     return from_f32<T>(f);
-}
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
 }
 
 // ---------------------------------------------------------------- append
