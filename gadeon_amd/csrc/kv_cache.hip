@@ -477,19 +477,49 @@ constexpr int LEAST = 8;
 __device__ __forceinline__ KeyBlocks<32> token_blocks(const Rows &s, const Mask &mask, int pos) {
     return KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
 }
+// From the least that an even share is, blocks(b, n, u) blocks in n a split for each of
+// sequence b's u units, to one whose splits fit the slots (or the rounds of them that whole
+// units take already).
+template <class F>
+__device__ __forceinline__ int fitting(const Rows &s, int groups, int slots, F blocks) {
+    const int lane = threadIdx.x & 63;
+    float n0 = 0.f, u0 = 0.f;                    // of this lane's first sequence
+    if (lane < s.n_seq) blocks(lane, n0, u0);
+    float share = n0 * u0, units = u0;
+    for (int b = lane + 64; b < s.n_seq; b += 64) {
+        float n, u;
+        blocks(b, n, u);
+        share += n * u;
+        units += u;
+    }
+    share = gd_wave_sum(share);
+    units = gd_wave_sum(units);
+    const float room = ceilf(fmaxf(units, 1.f) * (float)groups / (float)slots) * (float)slots / (float)groups;
+    float least = fmaxf((float)LEAST, ceilf(share / room));
+    // (Of no more than 2 units + slots / groups splits in any case: a share's worth and one a unit.)
+    for (int i = 0; i < 12; i++) {
+        float count = u0 * ceilf(n0 / least);
+        for (int b = lane + 64; b < s.n_seq; b += 64) {
+            float n, u;
+            blocks(b, n, u);
+            count += u * ceilf(n / least);
+        }
+        if (gd_wave_sum(count) <= room) break;
+        least = ceilf(least * 1.125f);
+    }
+    return (int)least;
+}
 __device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int groups, int slots) {
     const int lane = threadIdx.x & 63;
-    float sum = 0.f, most = 0.f;
-    for (int b = lane; b < s.n_seq; b += 64) {
+    float most = 0.f;
+    const int least = fitting(s, groups, slots, [&](int b, float &n, float &u) {
         const int pos = s.pos[b];
-        const float n = pos < 0 ? 0.f : (float)token_blocks(s, mask, pos).n;
-        sum += n;
+        n = pos < 0 ? 0.f : (float)token_blocks(s, mask, pos).n;
+        u = pos < 0 ? 0.f : 1.f;
         most = fmaxf(most, n);
-    }
-    sum = gd_wave_sum(sum);
+    });
     most = wave_max(most);
-    const float least = fmaxf((float)LEAST, ceilf(sum * (float)groups / (float)slots));
-    return most <= 1.6f * least ? max(1, (int)most) : (int)least;
+    return most <= 1.6f * least ? max(1, (int)most) : least;
 }
 
 // Attention of single tokens: workgroup (row, kv head and eight of its query heads;
@@ -823,17 +853,43 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
 constexpr int PC = 128;                          // columns of a unit
 template <int HD> constexpr int tile_keys() { return HD == 128 ? 64 : 32; }
 
-struct Tile {
-    int i0, i1;                                  // the unit's first and last row of its sequence
+// A sequence's units: first and last row of unit k, and its blocks of keys.
+struct Units {
+    int rows, G;
+    uint32_t pos, cap;
+    __device__ __forceinline__ Units(const Seq &q, int G_, uint32_t cap_) : rows(q.r1 - q.r0), G(G_), pos(q.pos), cap(cap_) {}
+    __device__ __forceinline__ int n() const { return (int)(((int64_t)rows * G + PC - 1) / PC); }
+    __device__ __forceinline__ int first(int k) const { return k * PC / G; }
+    __device__ __forceinline__ int last(int k) const { return min((k * PC + PC - 1) / G, rows - 1); }
+    template <int AK> __device__ __forceinline__ KeyBlocks<AK> blocks(const Mask &mask, int k) const {
+        return KeyBlocks<AK>(mask, pos + first(k), min(pos + last(k), cap - 1));
+    }
+    // Splits of each of the units: as the longest, the last, needs them.
+    template <int AK> __device__ __forceinline__ int splits(const Mask &mask, int most, int least) const {
+        const int longest = blocks<AK>(mask, n() - 1).n;
+        return longest <= 1.4f * least ? 1 : min(most, (longest + least - 1) / least);
+    }
 };
-__device__ __forceinline__ Tile tile_at(int k, int rows, int G) {
-    return Tile{k * PC / G, min((k * PC + PC - 1) / G, rows - 1)};
+// A unit's n blocks in nz splits or fewer: `per` each, `used` splits.
+struct Cut {
+    int per, used;
+    __device__ __forceinline__ Cut(int n, int nz) : per(max(1, (n + nz - 1) / nz)), used(max(1, (n + per - 1) / per)) {}
+};
+// How finely the keys are split, as token_least, each of a sequence's units taken for its
+// longest.
+template <int AK>
+__device__ __forceinline__ int unit_least(const Rows &s, const Mask &mask, int G, int HKV, int slots) {
+    return fitting(s, HKV, slots, [&](int b, float &n, float &u) {
+        const Units q(seq_at(s, b), G, s.cap);
+        u = q.rows > 0 ? (float)q.n() : 0.f;
+        n = q.rows > 0 ? (float)q.blocks<AK>(mask, q.n() - 1).n : 0.f;
+    });
 }
 
 template <int HD, bool I8, bool TILED, typename T>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 && sizeof(T) == 4 ? 1 : 2)))
 void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part,
-                 int most, int least, int H, float scale, Mask mask) {
+                 int most, int slots, int H, float scale, Mask mask) {
     constexpr bool HL = sizeof(T) == 4;          // hi + lo
     constexpr int AK = tile_keys<HD>(), NT = AK / 32, KS = HD / 16, DT = HD / 32;
     constexpr int ES = I8 ? 1 : 2, CPR = HD * ES / 16;   // 16-byte chunks of a row
@@ -846,18 +902,28 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     __shared__ uint8_t odd[2][AK][HD / 8];       // which values of V are no numbers, a bit each
     __shared__ int any_odd[2];
     const int G = H / c.HKV, kvh = blockIdx.x % c.HKV;
-    int b, k;
-    auto units = [&](const Seq &q) { return (int)(((int64_t)(q.r1 - q.r0) * G + PC - 1) / PC); };
+    int b, k, nz = 1;
+    // The sequences' units one after the other, each in its splits, so that the workgroups
+    // that have none come last; of a sequence those that see the most keys first.
+    const int least = most > 1 ? unit_least<AK>(s, mask, G, c.HKV, slots) : 0;
+    auto units = [&](const Seq &q) {
+        const Units u(q, G, s.cap);
+        return u.rows <= 0 ? 0 : u.n() * (most > 1 ? u.splits<AK>(mask, most, least) : 1);
+    };
     if (!unit_at(s, blockIdx.x / c.HKV, units, b, k)) return;
     const Seq sq = seq_at(s, b);
-    const int rows = sq.r1 - sq.r0;
-    k = units(sq) - 1 - k;                       // the units that see the most keys first
-    const Tile tl = tile_at(k, rows, G);
+    const Units un(sq, G, s.cap);
+    const int rows = un.rows;
+    if (most > 1) nz = un.splits<AK>(mask, most, least);
+    const int z = k % nz;
+    k = un.n() - 1 - k / nz;
+    const struct { int i0, i1; } tl = {un.first(k), un.last(k)};
     const uint32_t p0 = (uint32_t)sq.pos, cap1 = s.cap - 1;
-    const KeyBlocks<AK> kb(mask, p0 + tl.i0, min(p0 + tl.i1, cap1));
-    const int nz = kb.splits(most, least), z = blockIdx.y;
-    if (z >= nz) return;
-    const int per = (kb.n + nz - 1) / nz, jend = min(kb.n, (z + 1) * per);
+    const KeyBlocks<AK> kb = un.blocks<AK>(mask, k);
+    const Cut cut(kb.n, nz);
+    if (z >= cut.used) return;
+    nz = cut.used;
+    const int per = cut.per, jend = min(kb.n, (z + 1) * per);
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int lc = lane & 31, h = lane >> 5;
     // This lane's column, and the positions that the wave's columns stand at.
@@ -1194,21 +1260,20 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 
 // The splits that row n's keys were worked in for query head h (0: the row has no sequence).
 template <int HD>
-__device__ __forceinline__ int splits_of(const Cache &c, const Rows &s, const Mask &mask, int n, int h, int H, int most, int least) {
+__device__ __forceinline__ int splits_of(const Cache &c, const Rows &s, const Mask &mask, int n, int h, int H, int most, int slots) {
+    const int G = H / c.HKV;
     if (!s.row_start) {
-        // (`least` stands for the slots.)
-        const int pos = s.pos[n], groups = c.HKV * ((H / c.HKV + 7) / 8);
-        least = token_least(s, mask, groups, least);
+        const int pos = s.pos[n], least = token_least(s, mask, c.HKV * ((G + 7) / 8), slots);
         return pos < 0 ? 0 : token_blocks(s, mask, pos).splits(most, least);
     }
-    const int b = seq_of_row(s, n);
+    constexpr int AK = tile_keys<HD>();
+    const int least = unit_least<AK>(s, mask, G, c.HKV, slots), b = seq_of_row(s, n);
     if (b < 0) return 0;
     const Seq sq = seq_at(s, b);
     if (n < sq.r0 || n >= sq.r1) return 0;
-    const int G = H / c.HKV;
-    const Tile tl = tile_at(((n - sq.r0) * G + h % G) / PC, sq.r1 - sq.r0, G);
-    const uint32_t p0 = (uint32_t)sq.pos;
-    return KeyBlocks<tile_keys<HD>()>(mask, p0 + tl.i0, min(p0 + tl.i1, s.cap - 1)).splits(most, least);
+    const Units un(sq, G, s.cap);
+    const int k = ((n - sq.r0) * G + h % G) / PC;
+    return Cut(un.blocks<AK>(mask, k).n, un.splits<AK>(mask, most, least)).used;
 }
 
 template <typename T> __device__ __forceinline__ float gated(float y, const T *gate) {
@@ -1219,12 +1284,12 @@ template <typename T> __device__ __forceinline__ float gated(float y, const T *g
 // (d, r) takes the splits r, r + NR, .. of one dim, beside the splits' weights, once a
 // workgroup.
 template <int HD, typename T>
-__global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, int least, Cache c, Rows s, const T *gate,
+__global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, int slots, Cache c, Rows s, const T *gate,
                                                     int64_t gate_stride, T *out, int H, Mask mask) {
     constexpr int NR = 512 / HD;
     __shared__ float fs[MAX_SPLITS], sum[NR][HD];
     const int n = blockIdx.x / H, h = blockIdx.x % H, t = threadIdx.x, d = t % HD, r = t / HD;
-    const int ns = splits_of<HD>(c, s, mask, n, h, H, most, least);
+    const int ns = splits_of<HD>(c, s, mask, n, h, H, most, slots);
     if (ns <= 1) return;
     const float *p = part.acc + (int64_t)blockIdx.x * most * HD;
     float a[MAX_SPLITS / NR];
@@ -1256,12 +1321,12 @@ __global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, int lea
 
 // The same for many rows: HD / 4 threads a (row, head), four dims each, a split at a time.
 template <int HD, typename T>
-__global__ __launch_bounds__(256) void k_attn_merge_many(Part part, int most, int least, Cache c, Rows s, const T *gate,
+__global__ __launch_bounds__(256) void k_attn_merge_many(Part part, int most, int slots, Cache c, Rows s, const T *gate,
                                                          int64_t gate_stride, T *out, int H, Mask mask) {
     constexpr int TPR = HD / 4, RPW = 256 / TPR;
     const int groups = (H + RPW - 1) / RPW, n = blockIdx.x / groups;
     const int h = min((int)(blockIdx.x % groups) * RPW + (int)threadIdx.x / TPR, H - 1), d = 4 * (threadIdx.x % TPR);
-    const int ns = splits_of<HD>(c, s, mask, n, h, H, most, least);
+    const int ns = splits_of<HD>(c, s, mask, n, h, H, most, slots);
     if (ns <= 1) return;
     const int64_t row = (int64_t)n * H + h;
     const float2 *ml = part.ml + row * most;
@@ -1533,39 +1598,37 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const bool tokens = !s->row_start;
     const int width = tokens ? 32 : hd == 128 ? tile_keys<128>() : tile_keys<256>();
     if (window) keys = std::min(keys, (int64_t)window + (tokens ? 0 : PC / G) + width - 1 + (n_sink + width - 1) / width * width);
-    // Blocks of keys of the longest row, workgroups without a split, and splits.
+    // Blocks of keys of the longest row, workgroups of a split each, those that the chip
+    // holds at once, and the most splits.  The keys are left whole, without a merge's
+    // launch, where that is a few rounds of blocks a wave or the workgroups are many; how
+    // finely others are split, the kernels know (token_least, unit_least).
     const int64_t blocks = (keys + width - 1) / width;
-    const int64_t wgs = tokens ? s->n_rows * kv->n_head_kv * ((G + 7) / 8)
-                               : (s->n_rows * G / PC + std::min<int64_t>(s->n_seq, s->n_rows)) * kv->n_head_kv;
-    // Single tokens are left whole, without a merge's launch, where that is a few rounds of
-    // blocks a wave; how finely others are split, the kernel knows (token_least).
-    const int64_t slots = (kv->dtype == GD_I8 && hd == 128 ? 3 : 2) * cus;
-    const bool whole = blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus);
-    const int64_t least = tokens ? LEAST : std::max<int64_t>(8, wgs * blocks / (4 * cus));
-    int64_t ns = tokens && whole ? 1 : std::min<int64_t>((blocks + least - 1) / least, MAX_SPLITS);
+    const int64_t groups = tokens ? kv->n_head_kv * ((G + 7) / 8) : kv->n_head_kv;
+    const int64_t units = tokens ? s->n_rows : s->n_rows * G / PC + std::min<int64_t>(s->n_seq, s->n_rows);
+    const int64_t per_cu = tokens ? (kv->dtype == GD_I8 && hd == 128 ? 3 : 2) : 2;
+    const int64_t slots = per_cu * cus, wgs = units * groups;
+    const bool whole = tokens ? blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus) : blocks <= 12 || wgs >= 2 * slots;
+    int64_t ns = whole ? 1 : std::min<int64_t>((blocks + LEAST - 1) / LEAST, MAX_SPLITS);
     float *scratch = nullptr;
     if ((rc = split_scratch(ctx, (size_t)s->n_rows * n_head * (hd + 2) * sizeof(float), ns, &scratch))) return rc;
     const Part part{scratch, (float2 *)(scratch + s->n_rows * n_head * ns * hd)};
-    // Single tokens: a split for each `slots / groups` of all blocks at most, and one a row
-    // (token_least), with two to spare for its roundings.
-    const int64_t fine = tokens ? slots : least, groups = tokens ? wgs / s->n_rows : 1;
-    const dim3 grid = !tokens  ? dim3((unsigned)wgs, (unsigned)ns)
-                      : ns > 1 ? dim3((unsigned)(groups * std::min(s->n_rows * ns, s->n_rows + slots / groups + 2)))
-                               : dim3((unsigned)wgs);
+    // Split, the units take no more workgroups than fill the slots, or the rounds of them that
+    // whole units take (fitting), with two to spare for the kernels' roundings.
+    const dim3 grid((unsigned)(groups * (ns > 1 ? std::min(units * ns, 2 * units + slots / groups + 2) : units)));
 #define GD_GO(HD_, I8_, T_) \
     do { \
         const bool tiled = I8_ || kv->page_size % 16 == 0; \
         auto kernel = tokens ? (tiled ? k_attn_tokens<HD_, I8_, true, T_> : k_attn_tokens<HD_, I8_, I8_, T_>) \
                              : (tiled ? k_attn_rows<HD_, I8_, true, T_> : k_attn_rows<HD_, I8_, I8_, T_>); \
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, cache_of(kv), rows, (const T_ *)q, q_stride, \
-                           (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)fine, n_head, scale, mask); \
+                           (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)slots, n_head, scale, mask); \
         if (ns > 1) { \
             GD_LAUNCHED(ctx, fn); \
             const bool many = s->n_rows * n_head >= 1024; \
             const int per = 1024 / HD_, merges = many ? (n_head + per - 1) / per : n_head; \
             auto merge = many ? k_attn_merge_many<HD_, T_> : k_attn_merge<HD_, T_>; \
             hipLaunchKernelGGL(merge, dim3((unsigned)(s->n_rows * merges)), dim3(many ? 256 : 512), 0, ctx->stream, part, \
-                               (int)ns, (int)fine, cache_of(kv), rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head, \
+                               (int)ns, (int)slots, cache_of(kv), rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head, \
                                mask); \
         } \
     } while (0)
