@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -463,10 +464,12 @@ template <int W> struct KeyBlocks {
 };
 
 // Partials of the key splits: sums of head h of row n, split z, at acc [n H + h][most][HD]
-// and its (maximum, sum of weights) at ml [n H + h][most], maxima in units of log2.
+// and its (maximum, sum of weights) at ml [n H + h][most], maxima in units of log2; how
+// many splits there are at used [n H + h] (1: the row is done, and has no partials).
 struct Part {
     float *acc;
     float2 *ml;
+    int *used;
 };
 
 // How finely single tokens' keys are split, from the rows' own lengths (the host knows a
@@ -477,34 +480,28 @@ constexpr int LEAST = 8;
 __device__ __forceinline__ KeyBlocks<32> token_blocks(const Rows &s, const Mask &mask, int pos) {
     return KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
 }
-// From the least that an even share is, blocks(b, n, u) blocks in n a split for each of
-// sequence b's u units, to one whose splits fit the slots (or the rounds of them that whole
-// units take already).
+// From an even share of all blocks a slot, to what lets the splits have a slot each, those
+// of half as many blocks or fewer a part of one (they fill the gaps); blocks(b, n, u): n
+// blocks in each of sequence b's u units.
 template <class F>
 __device__ __forceinline__ int fitting(const Rows &s, int groups, int slots, F blocks) {
     const int lane = threadIdx.x & 63;
     float n0 = 0.f, u0 = 0.f;                    // of this lane's first sequence
     if (lane < s.n_seq) blocks(lane, n0, u0);
-    float share = n0 * u0, units = u0;
-    for (int b = lane + 64; b < s.n_seq; b += 64) {
-        float n, u;
-        blocks(b, n, u);
-        share += n * u;
-        units += u;
-    }
-    share = gd_wave_sum(share);
-    units = gd_wave_sum(units);
-    const float room = ceilf(fmaxf(units, 1.f) * (float)groups / (float)slots) * (float)slots / (float)groups;
-    float least = fmaxf((float)LEAST, ceilf(share / room));
-    // (Of no more than 2 units + slots / groups splits in any case: a share's worth and one a unit.)
-    for (int i = 0; i < 12; i++) {
-        float count = u0 * ceilf(n0 / least);
+    auto all = [&](auto part) {
+        float sum = part(n0, u0);
         for (int b = lane + 64; b < s.n_seq; b += 64) {
             float n, u;
             blocks(b, n, u);
-            count += u * ceilf(n / least);
+            sum += part(n, u);
         }
-        if (gd_wave_sum(count) <= room) break;
+        return gd_wave_sum(sum);
+    };
+    const float room = (float)slots / (float)groups;
+    float least = fmaxf((float)LEAST, ceilf(all([](float n, float u) { return n * u; }) / room));
+    // (At least an even share: so no more than units + slots / groups splits.)
+    for (int i = 0; i < 12; i++) {
+        if (all([&](float n, float u) { return u * (n <= 0.5f * least ? n / least : ceilf(n / least)); }) <= room) break;
         least = ceilf(least * 1.125f);
     }
     return (int)least;
@@ -825,9 +822,11 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
             float y = L == 0.f ? 0.f : A / L;
             if (gate) y *= gd_sigmoid(gates[x]);
             out[row * HD + d] = from_f32<T>(y);
+            if (most > 1 && d == 0) part.used[row] = 1;
         } else {
             part.acc[(row * most + sp) * HD + d] = A;
             if (d == 0) {
+                if (sp == 0) part.used[row] = ns;
                 float M = wm[0][hh];
 #pragma unroll
                 for (int i = 1; i < TW; i++) M = fmaxf(M, wm[i][hh]);
@@ -850,23 +849,26 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
 // result's own rounding.  A tile that some column does not see whole goes key by key: a
 // mask, and where V holds a NaN or infinity its finite part and, apart, which columns see
 // the others (0 x NaN would reach them all).
-constexpr int PC = 128;                          // columns of a unit
+// Columns of a wave, and of a unit: a wave's sums are head dim x columns, which at head
+// dim 256 leave 32 columns no registers (128 of sums, 128 of f32 rows' q).
+template <int HD> constexpr int wave_cols() { return HD == 128 ? 32 : 16; }
+template <int HD> constexpr int unit_cols() { return 4 * wave_cols<HD>(); }
 template <int HD> constexpr int tile_keys() { return HD == 128 ? 64 : 32; }
 
 // A sequence's units: first and last row of unit k, and its blocks of keys.
-struct Units {
+template <int PC, int AK> struct Units {
     int rows, G;
     uint32_t pos, cap;
     __device__ __forceinline__ Units(const Seq &q, int G_, uint32_t cap_) : rows(q.r1 - q.r0), G(G_), pos(q.pos), cap(cap_) {}
     __device__ __forceinline__ int n() const { return (int)(((int64_t)rows * G + PC - 1) / PC); }
     __device__ __forceinline__ int first(int k) const { return k * PC / G; }
     __device__ __forceinline__ int last(int k) const { return min((k * PC + PC - 1) / G, rows - 1); }
-    template <int AK> __device__ __forceinline__ KeyBlocks<AK> blocks(const Mask &mask, int k) const {
+    __device__ __forceinline__ KeyBlocks<AK> blocks(const Mask &mask, int k) const {
         return KeyBlocks<AK>(mask, pos + first(k), min(pos + last(k), cap - 1));
     }
     // Splits of each of the units: as the longest, the last, needs them.
-    template <int AK> __device__ __forceinline__ int splits(const Mask &mask, int most, int least) const {
-        const int longest = blocks<AK>(mask, n() - 1).n;
+    __device__ __forceinline__ int splits(const Mask &mask, int most, int least) const {
+        const int longest = blocks(mask, n() - 1).n;
         return longest <= 1.4f * least ? 1 : min(most, (longest + least - 1) / least);
     }
 };
@@ -877,26 +879,29 @@ struct Cut {
 };
 // How finely the keys are split, as token_least, each of a sequence's units taken for its
 // longest.
-template <int AK>
+template <int PC, int AK>
 __device__ __forceinline__ int unit_least(const Rows &s, const Mask &mask, int G, int HKV, int slots) {
     return fitting(s, HKV, slots, [&](int b, float &n, float &u) {
-        const Units q(seq_at(s, b), G, s.cap);
+        const Units<PC, AK> q(seq_at(s, b), G, s.cap);
         u = q.rows > 0 ? (float)q.n() : 0.f;
-        n = q.rows > 0 ? (float)q.blocks<AK>(mask, q.n() - 1).n : 0.f;
+        n = q.rows > 0 ? (float)q.blocks(mask, q.n() - 1).n : 0.f;
     });
 }
 
 template <int HD, bool I8, bool TILED, typename T>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 && sizeof(T) == 4 ? 1 : 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part,
                  int most, int slots, int H, float scale, Mask mask) {
     constexpr bool HL = sizeof(T) == 4;          // hi + lo
-    constexpr int AK = tile_keys<HD>(), NT = AK / 32, KS = HD / 16, DT = HD / 32;
+    constexpr int PC = unit_cols<HD>(), MF = wave_cols<HD>(), NV = MF * MF / 64;   // C values of a lane
+    using Acc = std::conditional_t<MF == 32, f32x16, f32x4>;
+    // Keys of a tile in key groups of MF; k steps of a score; dims in groups of MF.
+    constexpr int AK = tile_keys<HD>(), NT = AK / MF, KS = MF == 32 ? HD / 16 : HD / 32, DT = HD / MF;
     constexpr int ES = I8 ? 1 : 2, CPR = HD * ES / 16;   // 16-byte chunks of a row
     constexpr int CH = AK * CPR / 256, KPP = 256 / CPR;  // chunks a thread stages of K (and of V); keys of a pass
-    // V rows padded by 64 bytes: the four rows and 32 dims of a transposing read's 32 lanes
-    // then lie in 64 different banks.
-    constexpr int KP = HD + 8, VP = HD + 32, FD = 4;
+    // V rows padded so that a transposing read's 32 lanes (MF 32: four rows of 32 dims, else
+    // eight of 16) lie in 64 different banks.
+    constexpr int KP = HD + 8, VP = HD + (MF == 32 ? 32 : 16), FD = 4;
     __shared__ __attribute__((aligned(16))) f16 Ks[2][AK][KP];
     __shared__ __attribute__((aligned(16))) f16 Vs[2][AK][VP];
     __shared__ uint8_t odd[2][AK][HD / 8];       // which values of V are no numbers, a bit each
@@ -905,35 +910,35 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     int b, k, nz = 1;
     // The sequences' units one after the other, each in its splits, so that the workgroups
     // that have none come last; of a sequence those that see the most keys first.
-    const int least = most > 1 ? unit_least<AK>(s, mask, G, c.HKV, slots) : 0;
+    const int least = most > 1 ? unit_least<PC, AK>(s, mask, G, c.HKV, slots) : 0;
     auto units = [&](const Seq &q) {
-        const Units u(q, G, s.cap);
-        return u.rows <= 0 ? 0 : u.n() * (most > 1 ? u.splits<AK>(mask, most, least) : 1);
+        const Units<PC, AK> u(q, G, s.cap);
+        return u.rows <= 0 ? 0 : u.n() * (most > 1 ? u.splits(mask, most, least) : 1);
     };
     if (!unit_at(s, blockIdx.x / c.HKV, units, b, k)) return;
     const Seq sq = seq_at(s, b);
-    const Units un(sq, G, s.cap);
+    const Units<PC, AK> un(sq, G, s.cap);
     const int rows = un.rows;
-    if (most > 1) nz = un.splits<AK>(mask, most, least);
+    if (most > 1) nz = un.splits(mask, most, least);
     const int z = k % nz;
     k = un.n() - 1 - k / nz;
     const struct { int i0, i1; } tl = {un.first(k), un.last(k)};
     const uint32_t p0 = (uint32_t)sq.pos, cap1 = s.cap - 1;
-    const KeyBlocks<AK> kb = un.blocks<AK>(mask, k);
+    const KeyBlocks<AK> kb = un.blocks(mask, k);
     const Cut cut(kb.n, nz);
     if (z >= cut.used) return;
     nz = cut.used;
     const int per = cut.per, jend = min(kb.n, (z + 1) * per);
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int lc = lane & 31, h = lane >> 5;
+    const int lc = lane % MF, h = lane / MF;
     // This lane's column, and the positions that the wave's columns stand at.
-    const int col = k * PC + 32 * w + lc, i = min(col / G, rows - 1);
+    const int col = k * PC + MF * w + lc, i = min(col / G, rows - 1);
     const bool valid = col < rows * G;
     const int head = kvh * G + (valid ? col % G : G - 1);
     const int64_t n = sq.r0 + i;
     const uint32_t p = p0 + i;
-    const bool busy = k * PC + 32 * w < rows * G;
-    const uint32_t plo = p0 + min((k * PC + 32 * w) / G, rows - 1), phi = p0 + min((k * PC + 32 * w + 31) / G, rows - 1);
+    const bool busy = k * PC + MF * w < rows * G;
+    const uint32_t plo = p0 + min((k * PC + MF * w) / G, rows - 1), phi = p0 + min((k * PC + MF * w + MF - 1) / G, rows - 1);
     // Staging: key lane % AK's page-table entry a tile ahead of its row, that a tile ahead
     // of the halves in LDS, those a tile ahead of use.
     const int32_t *table = s.table + (int64_t)b * s.max_pages;
@@ -1029,9 +1034,13 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         }
         return some;
     };
+    auto mfma = [](f16x8 a, f16x8 b, Acc c) {
+        if constexpr (MF == 32) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    };
     int j = z * per;
     Entry en = entry_of(j);
-    // B operand of S^T: dims 16 ks + 8 h + e of the lane's column; the sign of the scale
+    // B operand of S^T: dims 8 (64 / MF) ks + 8 h + e of the lane's column; the sign of the scale
     // goes into it, so that the greatest product is the greatest score.
     f16x8 qh[KS], ql[HL ? KS : 1];
     float sf = fabsf(scale) * LOG2E;
@@ -1045,10 +1054,11 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
-                    x[ks][y] = *(const f32x4 *)(qrow + 16 * ks + 4 * y);
+                    x[ks][y] = *(const f32x4 *)(qrow + 512 / MF * ks + 4 * y);
 #pragma unroll
                     for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[ks][y][e]));
                 }
+            if constexpr (MF == 16) mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const int ex = min(max((int)(__float_as_uint(mx) >> 23), 40), 254) - 127;
             const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23) * (neg ? -1.f : 1.f);
@@ -1065,7 +1075,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         } else {
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                u32x4 x = *(const u32x4 *)(qrow + 16 * ks);
+                u32x4 x = *(const u32x4 *)(qrow + 512 / MF * ks);
                 if (neg) x ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
                 qh[ks] = __builtin_bit_cast(f16x8, x);
             }
@@ -1074,9 +1084,10 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     if (sf < 0x1p-126f) sf = 0x1p-126f;          // weights of 1 alike; times -inf not NaN
     if (j < jend) fetch(en);
     en = entry_of(j + 1);
-    f32x16 acc[DT];                              // O^T dims 32 dt + 8 (v / 4) + 4 h + v % 4
+    // Row 8 (v / 4) + 4 h + v % 4 of a C value v (MF 16: 4 h + v).
+    Acc acc[DT];                                 // O^T, dims MF dt + row
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) acc[dt] = f32x16{};
+    for (int dt = 0; dt < DT; dt++) acc[dt] = Acc{};
     float m = -INFINITY, l = 0.f;                // l: this lane's keys only
     bool some = j < jend && stage(j);
     uint64_t now = here & ALL;
@@ -1099,11 +1110,11 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         if (busy && k0 <= phi && !(mask.window && k0 + AK - 1 + mask.window <= plo && k0 >= (uint32_t)mask.sinks)) {
             const bool full = now == ALL && k0 + AK - 1 <= plo &&
                               (!mask.window || k0 + mask.window > phi || k0 + AK <= (uint32_t)mask.sinks);
-            f32x16 st[NT];
+            Acc st[NT];                          // S^T, keys MF kt + row
             __builtin_amdgcn_s_setprio(1);
             {
                 // A operands FD reads ahead of their products.
-                auto keys = [&](int x) { return *(const f16x8 *)&Ks[s2][x % NT * 32 + lc][x / NT * 16 + 8 * h]; };
+                auto keys = [&](int x) { return *(const f16x8 *)&Ks[s2][x % NT * MF + lc][x / NT * (512 / MF) + 8 * h]; };
                 f16x8 ka[FD];
 #pragma unroll
                 for (int x = 0; x < FD; x++) ka[x] = keys(x);
@@ -1111,8 +1122,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 #pragma unroll
                 for (int x = 0; x < NT * KS; x++) {
                     const int kt = x % NT, ks = x / NT;
-                    st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[x % FD], qh[ks], ks ? st[kt] : f32x16{}, 0, 0, 0);
-                    if constexpr (HL) st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[x % FD], ql[ks], st[kt], 0, 0, 0);
+                    st[kt] = mfma(ka[x % FD], qh[ks], ks ? st[kt] : Acc{});
+                    if constexpr (HL) st[kt] = mfma(ka[x % FD], ql[ks], st[kt]);
                     __builtin_amdgcn_sched_group_barrier(0x008, HL ? 2 : 1, 0);
                     if (x + FD < NT * KS) {
                         ka[x % FD] = keys(x + FD);
@@ -1122,16 +1133,16 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             }
             __builtin_amdgcn_s_setprio(0);
             if (!full) {
-                // Bit 8 (v / 4) + v % 4 of a 32-key half: key 4 h on, as this column sees it.
+                // A bit a key, as this column sees it.
                 auto below = [](int64_t x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; };
                 uint64_t see = below((int64_t)p - k0 + 1);
                 if (mask.window) see &= ~below((int64_t)p - mask.window + 1 - k0) | below((int64_t)mask.sinks - k0);
                 see = (see & now) >> (4 * h);
 #pragma unroll
                 for (int kt = 0; kt < NT; kt++) {
-                    const uint32_t bits = (uint32_t)(see >> (32 * kt));
+                    const uint32_t bits = (uint32_t)(see >> (MF * kt));
 #pragma unroll
-                    for (int v = 0; v < 16; v++)
+                    for (int v = 0; v < NV; v++)
                         st[kt][v] = bits & (1u << (8 * (v / 4) + v % 4)) ? st[kt][v] : -INFINITY;
                 }
             }
@@ -1139,10 +1150,11 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 #pragma unroll
             for (int kt = 0; kt < NT; kt++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) top = fmaxf(top, st[kt][v]);
+                for (int v = 0; v < NV; v++) top = fmaxf(top, st[kt][v]);
             // Sums are brought to a new maximum only where a score is over 2^LAZY of the one
             // they stand at (random scores: hardly after the first tiles).
             if (__any(top * sf > m + LAZY)) {
+                if constexpr (MF == 16) top = fmaxf(top, __shfl_xor(top, 16, 64));
                 const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * sf);
                 const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
                 l *= alpha;
@@ -1153,11 +1165,14 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             // Weights times 2^8, under 2^15 (f16 rows: in the exponent, where 32-bit rows would
             // lose bits).
             const float off = m == -INFINITY ? 0.f : HL ? -m : 8.f - m;
-            f16x8 ph[2 * NT], pl[HL ? 2 * NT : 1];
+            // P^T as B operands: keys 16 kk on (MF 32) or 32 kk, element e the row of C value e.
+            constexpr int KK = AK / (512 / MF);
+            f16x8 ph[KK], pl[HL ? KK : 1];
 #pragma unroll
             for (int kt = 0; kt < NT; kt++)
 #pragma unroll
-                for (int v = 0; v < 16; v += 2) {
+                for (int v = 0; v < NV; v += 2) {
+                    constexpr auto kk = [](int kt, int v) { return (NV * kt + v) / 8; };
                     float w0 = __builtin_amdgcn_exp2f(fmaf(st[kt][v], sf, off));
                     float w1 = __builtin_amdgcn_exp2f(fmaf(st[kt][v + 1], sf, off));
                     f16x2 hi, lo;
@@ -1165,8 +1180,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                         w0 *= 256.f;
                         w1 *= 256.f;
                         gd_split2_f16(w0, w1, hi, lo);
-                        pl[2 * kt + v / 8][v % 8] = lo[0];
-                        pl[2 * kt + v / 8][v % 8 + 1] = lo[1];
+                        pl[kk(kt, v)][(NV * kt + v) % 8] = lo[0];
+                        pl[kk(kt, v)][(NV * kt + v) % 8 + 1] = lo[1];
                     } else {
                         typedef float f32x2 __attribute__((ext_vector_type(2)));
                         hi = __builtin_convertvector((f32x2{w0, w1}), f16x2);
@@ -1177,17 +1192,17 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                     } else {
                         l = __builtin_amdgcn_fdot2(hi, f16x2{(f16)1.f, (f16)1.f}, l, false);
                     }
-                    ph[2 * kt + v / 8][v % 8] = hi[0];
-                    ph[2 * kt + v / 8][v % 8 + 1] = hi[1];
+                    ph[kk(kt, v)][(NV * kt + v) % 8] = hi[0];
+                    ph[kk(kt, v)][(NV * kt + v) % 8 + 1] = hi[1];
                 }
             {
                 typedef short s16x4 __attribute__((ext_vector_type(4)));
                 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                // V^T of keys 16 (x / DT) .., dims 32 (x % DT) + lane % 32.
+                // V^T of keys (512 / MF) (x / DT) on, dims MF (x % DT) + lane % MF.
                 auto values = [&](int x) {
-                    const f16 *v = &Vs[s2][x / DT * 16 + 4 * h + (lane >> 2 & 3)][x % DT * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
+                    const f16 *v = &Vs[s2][x / DT * (512 / MF) + 4 * h + (lane >> 2 & 3)][x % DT * MF + (MF == 32 ? 16 * (lane >> 4 & 1) : 0) + 4 * (lane & 3)];
                     const f16x4 v0 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v));
-                    const f16x4 v1 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 8 * VP)));
+                    const f16x4 v1 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 256 / MF * VP)));
                     return f16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
                 };
                 f16x8 va[FD];
@@ -1195,12 +1210,12 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                 for (int x = 0; x < FD; x++) va[x] = values(x);
                 __builtin_amdgcn_sched_group_barrier(0x100, 2 * FD, 1);
 #pragma unroll
-                for (int x = 0; x < 2 * NT * DT; x++) {
+                for (int x = 0; x < KK * DT; x++) {
                     const int kk = x / DT, dt = x % DT;
-                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[x % FD], ph[kk], acc[dt], 0, 0, 0);
-                    if constexpr (HL) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[x % FD], pl[kk], acc[dt], 0, 0, 0);
+                    acc[dt] = mfma(va[x % FD], ph[kk], acc[dt]);
+                    if constexpr (HL) acc[dt] = mfma(va[x % FD], pl[kk], acc[dt]);
                     __builtin_amdgcn_sched_group_barrier(0x008, HL ? 2 : 1, 1);
-                    if (x + FD < 2 * NT * DT) {
+                    if (x + FD < KK * DT) {
                         va[x % FD] = values(x + FD);
                         __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
                     }
@@ -1216,22 +1231,24 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-                        for (int v = 0; v < 16; v++)
-                            if (odd[s2][key][4 * dt + v / 4] >> (4 * h + v % 4) & 1) acc[dt][v] = __uint_as_float(0x7fc00000u);
+                        for (int v = 0; v < NV; v++)
+                            if (odd[s2][key][(MF * dt + 8 * (v / 4) + 4 * h) / 8] >> (4 * h % 8 + v % 4) & 1) acc[dt][v] = __uint_as_float(0x7fc00000u);
             __syncthreads();
         }
         now = next;
     }
     if (!valid) return;
+    if constexpr (MF == 16) l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     const int64_t row = n * H + head;
+    if (most > 1 && z == 0 && h == 0) part.used[row] = nz;
     if (nz > 1) {
         float *y = part.acc + (row * most + z) * HD + 4 * h;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int v = 0; v < 16; v += 4)
-                *(f32x4 *)(y + 32 * dt + 2 * v) = f32x4{acc[dt][v], acc[dt][v + 1], acc[dt][v + 2], acc[dt][v + 3]};
+            for (int v = 0; v < NV; v += 4)
+                *(f32x4 *)(y + MF * dt + 2 * v) = f32x4{acc[dt][v], acc[dt][v + 1], acc[dt][v + 2], acc[dt][v + 3]};
         if (h == 0) part.ml[row * most + z] = make_float2(m, l);
         return;
     }
@@ -1239,8 +1256,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-        for (int v = 0; v < 16; v += 4) {
-            const int d = 32 * dt + 2 * v + 4 * h;
+        for (int v = 0; v < NV; v += 4) {
+            const int d = MF * dt + 2 * v + 4 * h;
             float y[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = acc[dt][v + e] * inv;
@@ -1258,22 +1275,12 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         }
 }
 
-// The splits that row n's keys were worked in for query head h (0: the row has no sequence).
-template <int HD>
-__device__ __forceinline__ int splits_of(const Cache &c, const Rows &s, const Mask &mask, int n, int h, int H, int most, int slots) {
-    const int G = H / c.HKV;
-    if (!s.row_start) {
-        const int pos = s.pos[n], least = token_least(s, mask, c.HKV * ((G + 7) / 8), slots);
-        return pos < 0 ? 0 : token_blocks(s, mask, pos).splits(most, least);
-    }
-    constexpr int AK = tile_keys<HD>();
-    const int least = unit_least<AK>(s, mask, G, c.HKV, slots), b = seq_of_row(s, n);
-    if (b < 0) return 0;
+// Whether row n has a sequence (else nobody has written anything for it).
+__device__ __forceinline__ bool has_sequence(const Rows &s, int n) {
+    const int b = seq_of_row(s, n);
+    if (b < 0) return false;
     const Seq sq = seq_at(s, b);
-    if (n < sq.r0 || n >= sq.r1) return 0;
-    const Units un(sq, G, s.cap);
-    const int k = ((n - sq.r0) * G + h % G) / PC;
-    return Cut(un.blocks<AK>(mask, k).n, un.splits<AK>(mask, most, least)).used;
+    return n >= sq.r0 && n < sq.r1;
 }
 
 template <typename T> __device__ __forceinline__ float gated(float y, const T *gate) {
@@ -1284,13 +1291,13 @@ template <typename T> __device__ __forceinline__ float gated(float y, const T *g
 // (d, r) takes the splits r, r + NR, .. of one dim, beside the splits' weights, once a
 // workgroup.
 template <int HD, typename T>
-__global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, int slots, Cache c, Rows s, const T *gate,
-                                                    int64_t gate_stride, T *out, int H, Mask mask) {
+__global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, Rows s, const T *gate, int64_t gate_stride,
+                                                    T *out, int H) {
     constexpr int NR = 512 / HD;
     __shared__ float fs[MAX_SPLITS], sum[NR][HD];
     const int n = blockIdx.x / H, h = blockIdx.x % H, t = threadIdx.x, d = t % HD, r = t / HD;
-    const int ns = splits_of<HD>(c, s, mask, n, h, H, most, slots);
-    if (ns <= 1) return;
+    const int ns = part.used[blockIdx.x];
+    if (!has_sequence(s, n) || ns <= 1) return;
     const float *p = part.acc + (int64_t)blockIdx.x * most * HD;
     float a[MAX_SPLITS / NR];
 #pragma unroll
@@ -1321,14 +1328,14 @@ __global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, int slo
 
 // The same for many rows: HD / 4 threads a (row, head), four dims each, a split at a time.
 template <int HD, typename T>
-__global__ __launch_bounds__(256) void k_attn_merge_many(Part part, int most, int slots, Cache c, Rows s, const T *gate,
-                                                         int64_t gate_stride, T *out, int H, Mask mask) {
+__global__ __launch_bounds__(256) void k_attn_merge_many(Part part, int most, Rows s, const T *gate, int64_t gate_stride,
+                                                         T *out, int H) {
     constexpr int TPR = HD / 4, RPW = 256 / TPR;
     const int groups = (H + RPW - 1) / RPW, n = blockIdx.x / groups;
     const int h = min((int)(blockIdx.x % groups) * RPW + (int)threadIdx.x / TPR, H - 1), d = 4 * (threadIdx.x % TPR);
-    const int ns = splits_of<HD>(c, s, mask, n, h, H, most, slots);
-    if (ns <= 1) return;
     const int64_t row = (int64_t)n * H + h;
+    const int ns = part.used[row];
+    if (!has_sequence(s, n) || ns <= 1) return;
     const float2 *ml = part.ml + row * most;
     const float *p = part.acc + row * most * HD + d;
     float M = -INFINITY, L = 0.f;
@@ -1596,25 +1603,27 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const Rows rows = rows_of(kv, s);
     int64_t keys = s->max_len ? std::min<int64_t>(s->max_len, rows.cap) : rows.cap;
     const bool tokens = !s->row_start;
+    const int cols = hd == 128 ? unit_cols<128>() : unit_cols<256>();
     const int width = tokens ? 32 : hd == 128 ? tile_keys<128>() : tile_keys<256>();
-    if (window) keys = std::min(keys, (int64_t)window + (tokens ? 0 : PC / G) + width - 1 + (n_sink + width - 1) / width * width);
+    if (window) keys = std::min(keys, (int64_t)window + (tokens ? 0 : cols / G) + width - 1 + (n_sink + width - 1) / width * width);
     // Blocks of keys of the longest row, workgroups of a split each, those that the chip
     // holds at once, and the most splits.  The keys are left whole, without a merge's
     // launch, where that is a few rounds of blocks a wave or the workgroups are many; how
     // finely others are split, the kernels know (token_least, unit_least).
     const int64_t blocks = (keys + width - 1) / width;
     const int64_t groups = tokens ? kv->n_head_kv * ((G + 7) / 8) : kv->n_head_kv;
-    const int64_t units = tokens ? s->n_rows : s->n_rows * G / PC + std::min<int64_t>(s->n_seq, s->n_rows);
+    const int64_t units = tokens ? s->n_rows : s->n_rows * G / cols + std::min<int64_t>(s->n_seq, s->n_rows);
     const int64_t per_cu = tokens ? (kv->dtype == GD_I8 && hd == 128 ? 3 : 2) : 2;
     const int64_t slots = per_cu * cus, wgs = units * groups;
     const bool whole = tokens ? blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus) : blocks <= 12 || wgs >= 2 * slots;
     int64_t ns = whole ? 1 : std::min<int64_t>((blocks + LEAST - 1) / LEAST, MAX_SPLITS);
     float *scratch = nullptr;
-    if ((rc = split_scratch(ctx, (size_t)s->n_rows * n_head * (hd + 2) * sizeof(float), ns, &scratch))) return rc;
-    const Part part{scratch, (float2 *)(scratch + s->n_rows * n_head * ns * hd)};
-    // Split, the units take no more workgroups than fill the slots, or the rounds of them that
-    // whole units take (fitting), with two to spare for the kernels' roundings.
-    const dim3 grid((unsigned)(groups * (ns > 1 ? std::min(units * ns, 2 * units + slots / groups + 2) : units)));
+    if ((rc = split_scratch(ctx, (size_t)s->n_rows * n_head * (hd + 3) * sizeof(float), ns, &scratch))) return rc;
+    const int64_t sums = s->n_rows * n_head * ns;
+    const Part part{scratch, (float2 *)(scratch + sums * hd), (int *)(scratch + sums * (hd + 2))};
+    // Split, the units take no more workgroups than one each and one a slot (fitting), with
+    // two to spare for the kernels' roundings.
+    const dim3 grid((unsigned)(groups * (ns > 1 ? std::min(units * ns, units + slots / groups + 2) : units)));
 #define GD_GO(HD_, I8_, T_) \
     do { \
         const bool tiled = I8_ || kv->page_size % 16 == 0; \
@@ -1628,8 +1637,7 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
             const int per = 1024 / HD_, merges = many ? (n_head + per - 1) / per : n_head; \
             auto merge = many ? k_attn_merge_many<HD_, T_> : k_attn_merge<HD_, T_>; \
             hipLaunchKernelGGL(merge, dim3((unsigned)(s->n_rows * merges)), dim3(many ? 256 : 512), 0, ctx->stream, part, \
-                               (int)ns, (int)slots, cache_of(kv), rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head, \
-                               mask); \
+                               (int)ns, rows, (const T_ *)gate, gate_stride, (T_ *)out, n_head); \
         } \
     } while (0)
     GD_KV_PICK(kv, x_dtype, GD_GO);
