@@ -893,6 +893,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part,
                  int most, int slots, int H, float scale, Mask mask) {
     constexpr bool HL = sizeof(T) == 4;          // hi + lo
+    // A wave keeps its priority over the other of its SIMD through the softmax and the sums
+    // too where codes are made halves or rows are pairs, in us with / without it (1024 rows
+    // behind 3000, 40 heads of 128 on 8; 24 of 256 on 4): f16 rows on codes 144 / 150 and
+    // 221 / 228, f32 rows on codes 194 / 208 and 261 / 261, f32 rows on halves 188 / 194 and
+    // 214 / 229; f16 rows on halves 130 / 131 and 189 / 184, under a window of 1024 145 / 133.
+    constexpr bool HOLD = I8 || HL;
     constexpr int PC = unit_cols<HD>(), MF = wave_cols<HD>(), NV = MF * MF / 64;   // C values of a lane
     using Acc = std::conditional_t<MF == 32, f32x16, f32x4>;
     // Keys of a tile in key groups of MF; k steps of a score; dims in groups of MF.
@@ -980,11 +986,12 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     constexpr uint64_t ALL = AK == 64 ? ~0ull : 0xffffffffull;
     // The fetched tile (block j) to LDS.  Where some column does not see all of it, what is
     // no number in V goes into bits beside it, and a zero in its place.
+    bool whole = true;                           // every column sees all of the tile staged last
     auto stage = [&](int j) {
         const uint32_t k0 = kb.start(j);
         const uint64_t in = here & ALL;
-        const bool whole = in == ALL && k0 + AK - 1 <= p0 + tl.i0 &&
-                           (!mask.window || k0 + mask.window > p0 + tl.i1 || k0 + AK <= (uint32_t)mask.sinks);
+        whole = in == ALL && k0 + AK - 1 <= p0 + tl.i0 &&
+                (!mask.window || k0 + mask.window > p0 + tl.i1 || k0 + AK <= (uint32_t)mask.sinks);
         const int s2 = j & 1;
         if (t == 0) any_odd[s2] = 0;             // (set, if at all, after the barrier below)
         bool some = false;
@@ -1098,6 +1105,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         const uint32_t k0 = kb.start(j);
         const int s2 = j & 1;
         if (some) any_odd[s2] = 1;
+        const bool all_see = whole;
         // The next tile to the other half of LDS, the one after it requested.
         const uint64_t next = here & ALL;
         if (j + 1 < jend) {
@@ -1111,7 +1119,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
             const bool full = now == ALL && k0 + AK - 1 <= plo &&
                               (!mask.window || k0 + mask.window > phi || k0 + AK <= (uint32_t)mask.sinks);
             Acc st[NT];                          // S^T, keys MF kt + row
-            __builtin_amdgcn_s_setprio(1);
+            __builtin_amdgcn_s_setprio(1);       // over the SIMD's other wave, that may be staging
             {
                 // A operands FD reads ahead of their products.
                 auto keys = [&](int x) { return *(const f16x8 *)&Ks[s2][x % NT * MF + lc][x / NT * (512 / MF) + 8 * h]; };
@@ -1131,7 +1139,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                     }
                 }
             }
-            __builtin_amdgcn_s_setprio(0);
+            if constexpr (!HOLD) __builtin_amdgcn_s_setprio(0);
             if (!full) {
                 // A bit a key, as this column sees it.
                 auto below = [](int64_t x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; };
@@ -1222,8 +1230,9 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         __syncthreads();
-        if (any_odd[s2]) {
+        if (!all_see && any_odd[s2]) {
             // What is no number reaches the columns that see it.
             for (int key = 0; key < AK; key++)
                 if (kb.start(j) + key <= p && (now >> key & 1) &&
