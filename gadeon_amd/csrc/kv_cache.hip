@@ -1062,9 +1062,15 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
                     x[ks][y] = *(const f32x4 *)(qrow + 512 / MF * ks + 4 * y);
+                }
+            if (j < jend) fetch(en);             // (while the rows are on their way)
+            en = entry_of(j + 1);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int y = 0; y < 2; y++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[ks][y][e]));
-                }
             if constexpr (MF == 16) mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const int ex = min(max((int)(__float_as_uint(mx) >> 23), 40), 254) - 127;
@@ -1081,16 +1087,15 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                 }
         } else {
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                u32x4 x = *(const u32x4 *)(qrow + 512 / MF * ks);
-                if (neg) x ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-                qh[ks] = __builtin_bit_cast(f16x8, x);
-            }
+            for (int ks = 0; ks < KS; ks++) qh[ks] = *(const f16x8 *)(qrow + 512 / MF * ks);
+            if (j < jend) fetch(en);
+            en = entry_of(j + 1);
+            if (neg)
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) qh[ks] = -qh[ks];
         }
     }
     if (sf < 0x1p-126f) sf = 0x1p-126f;          // weights of 1 alike; times -inf not NaN
-    if (j < jend) fetch(en);
-    en = entry_of(j + 1);
     // Row 8 (v / 4) + 4 h + v % 4 of a C value v (MF 16: 4 h + v).
     Acc acc[DT];                                 // O^T, dims MF dt + row
 #pragma unroll
@@ -1624,7 +1629,17 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const int64_t units = tokens ? s->n_rows : s->n_rows * G / cols + std::min<int64_t>(s->n_seq, s->n_rows);
     const int64_t per_cu = tokens ? (kv->dtype == GD_I8 && hd == 128 ? 3 : 2) : 2;
     const int64_t slots = per_cu * cus, wgs = units * groups;
-    const bool whole = tokens ? blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus) : blocks <= 12 || wgs >= 2 * slots;
+    // Rows' partials cost a full chip some 15 us, and a split saves what lets the workgroups
+    // fill it; but the longest row may be one of a few, which split share the chip.  f16 rows on
+    // codes, us whole / split: 10 blocks 28 / 31; 12 on a fifth of the slots 38 / 35, on 0.6 of
+    // them 44 / 46; 24 on 0.7 56 / 57, on all 57 / 64; 64 on 0.7 123 / 89, on 1.2 127 / 90, on
+    // 1.8 183 / 196.
+    bool whole;
+    if (tokens)
+        whole = blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus);
+    else
+        whole = blocks <= 10 || (blocks <= 24 && blocks * (slots - wgs) <= 8 * slots) ||
+                (blocks <= 128 && 2 * wgs >= 3 * slots) || wgs >= 4 * slots;
     int64_t ns = whole ? 1 : std::min<int64_t>((blocks + LEAST - 1) / LEAST, MAX_SPLITS);
     float *scratch = nullptr;
     if ((rc = split_scratch(ctx, (size_t)s->n_rows * n_head * (hd + 3) * sizeof(float), ns, &scratch))) return rc;
