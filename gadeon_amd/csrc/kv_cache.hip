@@ -112,7 +112,7 @@ __device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, int &b, i
             const int l = __ffsll((unsigned long long)past) - 1;
             b = c + l;
             k = u - (base + __builtin_amdgcn_readlane(sum - n, l));
-            return k >= 0;
+            return k >= 0 && k < __builtin_amdgcn_readlane(n, l);    // (sums past 2^31: no row_start)
         }
         base += __builtin_amdgcn_readlane(sum, 63);
     }
@@ -482,28 +482,29 @@ __device__ __forceinline__ KeyBlocks<32> token_blocks(const Rows &s, const Mask 
 }
 // From an even share of all blocks a slot, to what lets the splits have a slot each, those
 // of half as many blocks or fewer a part of one (they fill the gaps); blocks(b, n, u): n
-// blocks in each of sequence b's u units.
+// blocks in each of sequence b's u units.  Over 64 sequences fill the chip as they are, and
+// the even share is left (200 tokens of up to 6000 positions, 40 heads of 128 on 8: 92 us,
+// fitted 107).
 template <class F>
 __device__ __forceinline__ int fitting(const Rows &s, int groups, int slots, F blocks) {
     const int lane = threadIdx.x & 63;
-    float n0 = 0.f, u0 = 0.f;                    // of this lane's first sequence
-    if (lane < s.n_seq) blocks(lane, n0, u0);
-    auto all = [&](auto part) {
-        float sum = part(n0, u0);
-        for (int b = lane + 64; b < s.n_seq; b += 64) {
-            float n, u;
-            blocks(b, n, u);
-            sum += part(n, u);
-        }
-        return gd_wave_sum(sum);
-    };
-    const float room = (float)slots / (float)groups;
-    float least = fmaxf((float)LEAST, ceilf(all([](float n, float u) { return n * u; }) / room));
-    // (At least an even share: so no more than units + slots / groups splits.)
-    for (int i = 0; i < 12; i++) {
-        if (all([&](float n, float u) { return u * (n <= 0.5f * least ? n / least : ceilf(n / least)); }) <= room) break;
-        least = ceilf(least * 1.125f);
+    float n = 0.f, u = 0.f;                      // of this lane's sequence
+    if (lane < s.n_seq) blocks(lane, n, u);
+    float sum = n * u;
+#pragma unroll 4
+    for (int b = lane + 64; b < s.n_seq; b += 64) {
+        float nb, ub;
+        blocks(b, nb, ub);
+        sum += nb * ub;
     }
+    const float room = (float)slots / (float)groups;
+    float least = fmaxf((float)LEAST, ceilf(gd_wave_sum(sum) / room));
+    // (At least an even share: so no more than units + slots / groups splits.)
+    if (s.n_seq <= 64)
+        for (int i = 0; i < 12; i++) {
+            if (gd_wave_sum(u * (n <= 0.5f * least ? n / least : ceilf(n / least))) <= room) break;
+            least = ceilf(least * 1.125f);
+        }
     return (int)least;
 }
 __device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int groups, int slots) {
@@ -944,7 +945,9 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     const int64_t n = sq.r0 + i;
     const uint32_t p = p0 + i;
     const bool busy = k * PC + MF * w < rows * G;
-    const uint32_t plo = p0 + min((k * PC + MF * w) / G, rows - 1), phi = p0 + min((k * PC + MF * w + MF - 1) / G, rows - 1);
+    const uint32_t plo = p0 + min((k * PC + MF * w) / G, rows - 1);
+    const uint32_t seen_from = mask.window && plo >= (uint32_t)mask.window ? plo - mask.window + 1 : 0;
+    const uint32_t phi = p0 + min((k * PC + MF * w + MF - 1) / G, rows - 1);
     // Staging: key lane % AK's page-table entry a tile ahead of its row, that a tile ahead
     // of the halves in LDS, those a tile ahead of use.
     const int32_t *table = s.table + (int64_t)b * s.max_pages;
@@ -1120,7 +1123,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         }
         __builtin_amdgcn_sched_barrier(0);
         // The wave's own view of the tile.
-        if (busy && k0 <= phi && !(mask.window && k0 + AK - 1 + mask.window <= plo && k0 >= (uint32_t)mask.sinks)) {
+        if (busy && k0 <= phi && !(seen_from > k0 + AK - 1 && k0 >= (uint32_t)mask.sinks)) {
             const bool full = now == ALL && k0 + AK - 1 <= plo &&
                               (!mask.window || k0 + mask.window > phi || k0 + AK <= (uint32_t)mask.sinks);
             Acc st[NT];                          // S^T, keys MF kt + row
@@ -1310,7 +1313,7 @@ __global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, Rows s,
     constexpr int NR = 512 / HD;
     __shared__ float fs[MAX_SPLITS], sum[NR][HD];
     const int n = blockIdx.x / H, h = blockIdx.x % H, t = threadIdx.x, d = t % HD, r = t / HD;
-    const int ns = part.used[blockIdx.x];
+    const int ns = min(part.used[blockIdx.x], most);
     if (!has_sequence(s, n) || ns <= 1) return;
     const float *p = part.acc + (int64_t)blockIdx.x * most * HD;
     float a[MAX_SPLITS / NR];
@@ -1348,7 +1351,7 @@ __global__ __launch_bounds__(256) void k_attn_merge_many(Part part, int most, Ro
     const int groups = (H + RPW - 1) / RPW, n = blockIdx.x / groups;
     const int h = min((int)(blockIdx.x % groups) * RPW + (int)threadIdx.x / TPR, H - 1), d = 4 * (threadIdx.x % TPR);
     const int64_t row = (int64_t)n * H + h;
-    const int ns = part.used[row];
+    const int ns = min(part.used[row], most);
     if (!has_sequence(s, n) || ns <= 1) return;
     const float2 *ml = part.ml + row * most;
     const float *p = part.acc + row * most * HD + d;
@@ -1394,10 +1397,11 @@ int check_kv(gd_ctx *ctx, const char *fn, const gd_kv *kv, bool planes) {
     return GD_OK;
 }
 
+constexpr int64_t MAX_WGS = 1 << 24;             // workgroups of a launch: their threads are counted in 32 bits
 int check_seqs(gd_ctx *ctx, const char *fn, const gd_seqs *s) {
     GD_REQUIRE(ctx, s, "%s: null sequences", fn);
-    GD_REQUIRE(ctx, s->n_seq >= 0 && s->n_rows >= 0 && s->n_rows < (1LL << 31), "%s: %d sequences, %lld rows", fn,
-               s->n_seq, (long long)s->n_rows);
+    GD_REQUIRE(ctx, s->n_seq >= 0 && s->n_rows >= 0 && s->n_rows < MAX_WGS, "%s: %d sequences, %lld rows", fn, s->n_seq,
+               (long long)s->n_rows);
     GD_REQUIRE(ctx, s->row_start || s->n_rows == s->n_seq,
                "%s: %lld rows of %d sequences need row_start (one row each without)", fn, (long long)s->n_rows, s->n_seq);
     GD_REQUIRE(ctx, s->n_rows == 0 || s->n_seq == 0 || (s->pos && s->page_table), "%s: null positions or page table", fn);
@@ -1518,19 +1522,24 @@ extern "C" int gd_kv_append_rope(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s,
     GD_REQUIRE(ctx, n_rot >= 0 && n_rot % 2 == 0 && n_rot <= hd, "%s: n_rot %d must be even and at most head_dim %d", fn,
                n_rot, hd);
     GD_REQUIRE(ctx, n_rot == 0 || (base > 0.f && std::isfinite(base)), "%s: rotation base %g", fn, (double)base);
+    const int64_t widest = std::max({q ? q_stride : 0, k_stride, v_stride});
+    GD_REQUIRE(ctx, widest < (1LL << 31), "%s: row stride %lld", fn, (long long)widest);
     if (q) {
         GD_REQUIRE(ctx, q_out && n_head > 0 && n_head <= 65536, "%s: q of %d heads without q_out", fn, n_head);
         GD_REQUIRE(ctx, q_stride >= (int64_t)n_head * hd, "%s: q rows of %d heads overlap at stride %lld", fn, n_head,
                    (long long)q_stride);
         const int64_t size = x_dtype == GD_F32 ? 4 : 2, row = (int64_t)n_head * hd;
-        const uintptr_t a = (uintptr_t)q, o = (uintptr_t)q_out;
-        GD_REQUIRE(ctx, (a == o && q_stride == row) || !s->n_rows || a + ((s->n_rows - 1) * q_stride + row) * size <= o ||
-                            o + s->n_rows * row * size <= a,
+        const uintptr_t o = (uintptr_t)q_out, o_end = o + s->n_rows * row * size;
+        auto apart = [&](const void *x, int64_t stride, int64_t elems) {
+            const uintptr_t a = (uintptr_t)x;
+            return !s->n_rows || a + ((s->n_rows - 1) * stride + elems) * size <= o || o_end <= a;
+        };
+        GD_REQUIRE(ctx, (q == q_out && q_stride == row) || apart(q, q_stride, row),
                    "%s: q turned in place needs q_out = q and rows of n_head * head_dim (stride %lld)", fn,
                    (long long)q_stride);
+        const int64_t kv_row = (int64_t)kv->n_head_kv * hd;
+        GD_REQUIRE(ctx, apart(k, k_stride, kv_row) && apart(v, v_stride, kv_row), "%s: q_out in the place of k or v", fn);
     }
-    const int64_t widest = std::max({q ? q_stride : 0, k_stride, v_stride});
-    GD_REQUIRE(ctx, widest < (1LL << 31), "%s: row stride %lld", fn, (long long)widest);
     GD_CHECK_CTX(ctx);
     if (!s->n_rows || !s->n_seq) return GD_OK;
     GD_HIP(ctx, hipSetDevice(ctx->device));
@@ -1636,10 +1645,15 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     // 1.8 183 / 196.
     bool whole;
     if (tokens)
-        whole = blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus);
+        // Tokens of up to 6000 positions whole / split: 200 of 8 kv heads (twice the slots) 118 /
+        // 99, 500 213 / 250, 1500 456 / 653; 500 of 4 (3.9 times) 248 / 244.  Past 1024 blocks a
+        // long one of them would be the call's time.
+        whole = blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus) || (blocks <= 256 * TW && wgs >= 4 * slots) ||
+                wgs >= 16 * slots;
     else
         whole = blocks <= 10 || (blocks <= 24 && blocks * (slots - wgs) <= 8 * slots) ||
                 (blocks <= 128 && 2 * wgs >= 3 * slots) || wgs >= 4 * slots;
+    GD_REQUIRE(ctx, wgs + slots + 2 * groups < MAX_WGS, "%s: %lld rows of %d heads", fn, (long long)s->n_rows, n_head);
     int64_t ns = whole ? 1 : std::min<int64_t>((blocks + LEAST - 1) / LEAST, MAX_SPLITS);
     float *scratch = nullptr;
     if ((rc = split_scratch(ctx, (size_t)s->n_rows * n_head * (hd + 3) * sizeof(float), ns, &scratch))) return rc;

@@ -24,7 +24,7 @@
  *     out: K = reduction length (GGUF ne0), R = output rows (reference "M",
  *     GGUF ne1), T = tokens (reference "N").  out[T][R] = X[T][K] . W[R][K]^T.
  *   - Activation dtype codes: GD_F32 (IEEE binary32) and GD_F16 (binary16,
- *     passed as uint16_t bit patterns).
+ *     passed as uint16_t bit patterns); GD_I8 is a cache's (gd_kv).
  */
 #ifndef GADEON_HIP_H
 #define GADEON_HIP_H
@@ -105,10 +105,10 @@ int gd_timer_stop(gd_ctx *ctx, float *ms);
  * recording).  A failing entry inside a recording leaves the capture open;
  * gd_graph_end then fails and discards it.  A graph holds the workspace its
  * calls use, shared with the context's other calls, and attention partials of
- * its own (8 MiB, where it records gd_attn_paged or gd_attn_batch), until it is
- * destroyed: it may outlive its context, and be launched on another one as
- * long as the workspace of the first is not in use at the same time (which GEMMs
- * of f32 rows or split K and gd_gdn_prefill do). */
+ * its own (8 MiB, where it records gd_attn_paged, gd_attn_batch or gd_kv_attn),
+ * until it is destroyed: it may outlive its context, and be launched on another one
+ * as long as the workspace of the first is not in use at the same time (which GEMMs
+ * of f32 rows or split K, gd_gdn_prefill and gd_kv_attn of split keys do). */
 typedef struct gd_graph gd_graph;
 int gd_graph_begin(gd_ctx *ctx);
 int gd_graph_end(gd_ctx *ctx, gd_graph **out);
@@ -400,8 +400,10 @@ int gd_attn_batch(gd_ctx *ctx, const float *q, const uint16_t *k_cache,
  * row_start[0], from row_start[n_seq] on).  A table entry outside [0, n_pages),
  * and a position past max_pages * page_size, is a page that is not there: rows for
  * it are not kept and its keys are not seen (so a program with a window may drop
- * pages that left it).  No two rows of a call may name the same slot, and of an
- * 8-bit cache no two sequences the same block. */
+ * pages that left it).  Sequences may share pages that are only read; no two rows of
+ * an append may name the same slot, and of an 8-bit cache no two sequences the same
+ * block.  Arguments are checked before the context: gd_last_error(NULL) tells what is
+ * wrong with them where that is null. */
 #define GD_KV_BLOCK 16
 
 typedef struct gd_kv {
@@ -414,15 +416,15 @@ typedef struct gd_kv {
 } gd_kv;
 
 typedef struct gd_seqs {
-    int64_t n_rows;              /* rows of q, k, v and out */
+    int64_t n_rows;              /* rows of q, k, v and out, under 2^24 */
     const int32_t *row_start;    /* [n_seq + 1] or null */
     const int32_t *pos;          /* [n_seq] */
     const int32_t *rope_shift;   /* [n_seq] or null: rows are rotated at position + shift */
     const int32_t *page_table;   /* [n_seq][max_pages] */
     int n_seq, max_pages;
     int max_len;                 /* most positions of a sequence with this call's rows, as far as the
-                                    caller knows (0: max_pages * page_size): how finely the keys
-                                    are split goes by it, no result depends on it */
+                                    caller knows (0: max_pages * page_size): whether the keys are
+                                    split goes by it, what is seen does not */
 } gd_seqs;
 
 /* Allocate a cache's planes, zeroed (free with gd_kv_free). */
@@ -434,8 +436,8 @@ int gd_kv_free(gd_ctx *ctx, gd_kv *kv);
  * strides in elements) to the cache at their positions, k turned as gd_rope turns it
  * (n_rot even, 0 for none; here the angle's phase is exact at any position and its
  * cos and sin are formed in 64 bits).  With q not null, q [n_rows][n_head]
- * [head_dim] is turned likewise into q_out (contiguous rows, x_dtype; q_out may be
- * q where q_stride is n_head * head_dim).  One launch; the result of gd_rope twice
+ * [head_dim] is turned likewise into q_out (contiguous rows, x_dtype; apart from k and
+ * v; q_out may be q where q_stride is n_head * head_dim).  One launch; the result of gd_rope twice
  * and gd_kv_append for each sequence (MetalEnc.ropeBatch, kvAppendBatch,
  * MetalEnc.swift:817-847).
  *   GD_F16: rounded to nearest; values past f16's range are held as its largest.
@@ -466,7 +468,11 @@ int gd_kv_read(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, void *k_out, v
  * are worked as f16 hi + lo pairs (about 22 bits), f16 ones in f16 products with f32
  * sums.  A NaN or infinity in the cache reaches only the rows that see it, which
  * are then not to be relied on.  Two launches where the keys are split; partials go to
- * the context's or the recording's scratch as gd_attn_paged's.  MetalEnc.attnPaged and
+ * the context's or the recording's scratch as gd_attn_paged's, or, where that would
+ * bound the splits, to the context workspace, which the call may grow to 256 MiB (a
+ * recording takes it as it is, with fewer splits).  Sums are formed in a fixed order for
+ * the same lengths of all the call's sequences and the same max_len; others may split a
+ * row's keys elsewhere and round its last bits otherwise.  MetalEnc.attnPaged and
  * attnBatch (MetalEnc.swift:679-706, 966-1025), the latter's window included. */
 int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const void *q, int64_t q_stride,
                const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,

@@ -406,7 +406,7 @@ MASKS = [(0, 0), (1, 0), (40, 0), (100, 5), (64, 130), (1000, 1), (1 << 30, 3)]
 
 
 def check_attention(ctx, seqs, dtype, x16, hd, H, hkv, page, window, sinks, gated, seed=0, row_start=True, max_len=0,
-                    scale=None, tell=""):
+                    scale=None):
     with Batch(ctx, seqs, dtype, hkv, hd, page, seed=seed, row_start=row_start, lead=2 if row_start else 0,
                trail=3 if row_start else 0) as bt:
         KV = bt.fill()
@@ -466,6 +466,54 @@ def test_many_sequences(ctx, dtype):
     chunks = [(int(rng.integers(0, 60)), int(rng.integers(0, 5))) for _ in range(130)]
     for seqs, start in ((tokens, False), (tokens, True), (chunks, True)):
         check_attention(ctx, seqs, dtype, True, 128, 10, 2, 16, 0, 0, False, row_start=start)
+
+
+@pytest.mark.parametrize("dtype", [ga.I8, ga.F16], ids=["i8", "f16"])
+@pytest.mark.parametrize("n", [130, 70])
+def test_many_sequences_of_split_keys(ctx, dtype, n):
+    """More sequences than a wave has lanes, a few of them long, idle ones among them."""
+    rng = np.random.default_rng(n)
+    long = [(3000, 1), (1800, 40), (2500, 7)]
+    tokens = [(int(p), 1) for p in rng.integers(-5, 60, n)]
+    chunks = [(int(rng.integers(-5, 60)), int(rng.integers(0, 3))) for _ in range(n)]
+    for b, (p, r) in zip((0, n // 2, n - 1), long):
+        tokens[b], chunks[b] = (p, 1), (p, r)
+    for seqs, start in ((tokens, False), (tokens, True), (chunks, True)):
+        check_attention(ctx, seqs, dtype, False, 128, 6, 2, 16, 0, 0, False, row_start=start)
+
+
+@pytest.mark.parametrize("which", ["tokens", "ragged"])
+def test_the_largest_window_is_none(ctx, which):
+    outs = []
+    for window in (0, 2**31 - 1):
+        with Batch(ctx, ATTN[which], ga.I8, 2, 128, 16, row_start=which == "ragged") as bt:
+            bt.fill()
+            bt.desc.max_len = 4005
+            q = rows_of(bt.rng, (bt.n, 4, 128), False)
+            dq, do = bt.put(q), bt.put(np.zeros_like(q))
+            ctx.gd_kv_attn(*bt.ref, dq, 512, None, 0, do, ga.F32, 4, 0.1, window, 0)
+            outs.append(ctx.get(do, q.shape, np.float32))
+    assert outs[0].any() and np.array_equal(*outs)
+
+
+def test_row_starts_out_of_bounds(ctx):
+    """Row starts before the first row and past the last one are taken for those; rows that no
+    sequence has stay."""
+    with Batch(ctx, [(0, 9), (40, 5), (7, 20)], ga.F16, 2, 128, 16) as bt:
+        KV = bt.fill()
+        q = rows_of(bt.rng, (bt.n, 4, 128), False)
+        dq, do = bt.put(q), bt.put(np.full_like(q, -77))
+        ctx.set(bt.desc.row_start, np.array([-2**31, 9, 14, 2**31 - 1], np.int32))
+        ctx.gd_kv_attn(*bt.ref, dq, 512, None, 0, do, ga.F32, 4, 0.1, 0, 0)
+        got = ctx.get(do, q.shape, np.float32)
+        for b, rows in enumerate((slice(0, 9), slice(9, 14), slice(14, 34))):
+            want = attend(q[rows], *KV[b], (0, 40, 7)[b], np.float32(0.1), 0, 0, None)
+            assert np.abs(got[rows] - want).max() <= bound(q[rows], *KV[b], 0.1, False)
+        ctx.set(bt.desc.row_start, np.array([9, 3, 14, 5], np.int32))        # no rows, 3 .. 13, no rows
+        ctx.set(do, np.full_like(q, -77))
+        ctx.gd_kv_attn(*bt.ref, dq, 512, None, 0, do, ga.F32, 4, 0.1, 0, 0)
+        got = ctx.get(do, q.shape, np.float32)
+        assert (got[:3] == -77).all() and (got[14:] == -77).all() and (got[3:14] != -77).all()
 
 
 @pytest.mark.parametrize("dtype", [ga.I8, ga.F16], ids=["i8", "f16"])
@@ -633,6 +681,49 @@ def test_a_conversation_and_its_replays(ctx, dtype):
 
     for a, b in zip(program(False), program(True)):
         assert np.array_equal(a, b)
+
+
+def test_recordings_that_share_a_workspace(ctx):
+    """Partials past the attention scratch: two recordings replayed in turn with eager calls
+    between them, the workspace grown by one after they were made."""
+    def batch(seqs, H, seed):
+        bt = Batch(ctx, seqs, ga.I8, 2, 128, 16, seed=seed)
+        bt.fill()
+        q = rows_of(bt.rng, (bt.n, H, 128), False)
+        dq, do = bt.put(q), bt.put(np.zeros_like(q))
+
+        def run(graph=None):
+            ctx.set(do, np.zeros_like(q))
+            if graph:
+                ctx.gd_graph_launch(graph)
+            else:
+                call()
+            return ctx.get(do, q.shape, np.float32)
+
+        def call():
+            ctx.gd_kv_attn(*bt.ref, dq, H * 128, None, 0, do, ga.F32, H, 0.1, 0, 0)
+        return bt, call, run
+
+    small, large = [batch([(3000, 60), (10, 4), (900, 90)], 8, 1), batch([(1500, 130)], 16, 2)], batch([(2000, 700)], 16, 3)
+    try:
+        want, graphs = [], []
+        for _, call, run in small:
+            want.append(run())
+            g = C.c_void_p()
+            ctx.gd_graph_begin()
+            call()
+            ctx.gd_graph_end(C.byref(g))
+            graphs.append(g)
+        big = large[2]()
+        for _ in range(3):
+            for (_, _, run), w, g in zip(small, want, graphs):
+                assert w.any() and np.array_equal(run(g), w)
+                assert np.array_equal(large[2](), big) and np.array_equal(run(), w)
+        for g in graphs:
+            ctx.lib.gd_graph_destroy(g)
+    finally:
+        for bt, _, _ in (*small, large):
+            bt.close()
 
 
 def test_f16_cache_is_the_other_entries_cache(ctx):

@@ -53,7 +53,7 @@ CACHES = [(dict(k=None), "null cache plane"), (dict(v_exp=None), "null cache pla
           (dict(page_size=24), "page size 24"), (dict(page_size=0), "page size 0"), (dict(n_pages=0), "0 pages"),
           (dict(n_pages=1 << 31), "pages"), (dict(n_pages=-1), "-1 pages"), (dict(v=P + 8), "16-byte aligned"),
           (dict(page_size=1 << 24, n_head_kv=4096, n_pages=1 << 30), "pages")]
-BATCHES = [(dict(n_seq=-1), "-1 sequences"), (dict(n_rows=-1), "-1 rows"), (dict(n_rows=1 << 31), "rows"),
+BATCHES = [(dict(n_seq=-1), "-1 sequences"), (dict(n_rows=-1), "-1 rows"), (dict(n_rows=1 << 24), "16777216 rows"),
            (dict(row_start=None), "need row_start"), (dict(pos=None), "null positions"),
            (dict(page_table=None), "page table"), (dict(max_pages=0), "max_pages 0"), (dict(max_len=-1), "max_len -1")]
 
@@ -82,7 +82,9 @@ def test_null_structs(entry):
     (dict(n_rot=130), "n_rot 130"), (dict(n_rot=-2), "n_rot -2"), (dict(base=0.0), "base"),
     (dict(base=float("nan")), "base"), (dict(base=float("inf")), "base"), (dict(q_out=None), "without q_out"),
     (dict(n_head=0), "0 heads"), (dict(q_stride=511), "overlap"), (dict(q_out=P, q_stride=1024), "in place"),
-    (dict(x=ga.I8), "row dtype 2"), (dict(k_stride=1 << 31), "row stride")])
+    (dict(x=ga.I8), "row dtype 2"), (dict(k_stride=1 << 31), "row stride"),
+    (dict(k=3 * P, q_out=3 * P), "place of k or v"), (dict(v=2 * P + 512 * 4 * 6 - 16), "place of k or v"),
+    (dict(v=2 * P - 16), "place of k or v")])
 def test_refused_appends(kw, words):
     refused(append(**kw), words)
 
@@ -105,7 +107,9 @@ def test_refused_attention(kw, words):
 
 
 def test_rows_by_heads_past_31_bits():
-    refused(attn(s=seqs(n_rows=1 << 30, max_pages=1)), "rows of 4 heads")
+    n = (1 << 24) - 1
+    refused(attn(c=kv(n_head_kv=256), s=seqs(n_rows=n, max_pages=1), n_head=256, q=P << 8, q_stride=1 << 15, gate=None,
+                 out=P << 30), "16777215 rows of 256 heads")
 
 
 @pytest.mark.parametrize("kw,words", [(dict(dtype=ga.F32), "cache dtype"), (dict(head_dim=96), "head_dim 96"),
