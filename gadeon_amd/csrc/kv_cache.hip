@@ -472,21 +472,26 @@ struct Part {
     int *used;
 };
 
-// How finely single tokens' keys are split, from the rows' own lengths (the host knows a
-// bound of them alone): the fewest blocks of a split, so that all the splits' workgroups,
-// `groups` for each, fill the `slots` that the chip holds at once; from LEAST on, what a
-// workgroup's start, end and merge cost.  Rows of much the same length are left whole.
-constexpr int LEAST = 8;
+// How finely keys are split, from the sequences' own lengths (the host knows a bound of
+// them alone): the fewest blocks of a split, so that all the splits' workgroups, `groups`
+// for each, fill the `slots` that the chip holds at once; and no fewer than what a
+// workgroup's start, end and merge cost: for tokens 8 blocks of head dim 128 and 4 of 256
+// (one token of 600 positions, us at 4 / 8 / 16 blocks: 40 heads of 128 11.5 / 12.3 / 14.8,
+// 24 of 256 on codes 14.3 / 16.5 / 21, on halves 16.3 / 18.9 / 26; 32 of up to 3000 behind an
+// append, heads of 128, 28.3 / 25.8 / 27.6), for rows 8 (4 to 16 alike within 2%).
+constexpr int token_fewest(int hd) { return 1024 / hd; }
+constexpr int ROWS_FEWEST = 8;
 __device__ __forceinline__ KeyBlocks<32> token_blocks(const Rows &s, const Mask &mask, int pos) {
     return KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
 }
 // From an even share of all blocks a slot, to what lets the splits have a slot each, those
-// of half as many blocks or fewer a part of one (they fill the gaps); blocks(b, n, u): n
-// blocks in each of sequence b's u units.  Over 64 sequences fill the chip as they are, and
-// the even share is left (200 tokens of up to 6000 positions, 40 heads of 128 on 8: 92 us,
-// fitted 107).
+// of half as many blocks or fewer a part of one, as they fill the gaps (64 tokens of up to
+// 8192 positions 41 us, a slot for each 59; a mixed batch of prompt chunks 115 and 197);
+// blocks(b, n, u): n blocks in each of sequence b's u units.  Over 64 sequences fill the chip
+// as they are, and the even share is left (200 tokens of up to 6000 positions, 40 heads of
+// 128 on 8: 92 us, fitted 107).
 template <class F>
-__device__ __forceinline__ int fitting(const Rows &s, int groups, int slots, F blocks) {
+__device__ __forceinline__ int fitting(const Rows &s, int groups, int slots, int fewest, F blocks) {
     const int lane = threadIdx.x & 63;
     float n = 0.f, u = 0.f;                      // of this lane's sequence
     if (lane < s.n_seq) blocks(lane, n, u);
@@ -498,7 +503,7 @@ __device__ __forceinline__ int fitting(const Rows &s, int groups, int slots, F b
         sum += nb * ub;
     }
     const float room = (float)slots / (float)groups;
-    float least = fmaxf((float)LEAST, ceilf(gd_wave_sum(sum) / room));
+    float least = fmaxf((float)fewest, ceilf(gd_wave_sum(sum) / room));
     // (At least an even share: so no more than units + slots / groups splits.)
     if (s.n_seq <= 64)
         for (int i = 0; i < 12; i++) {
@@ -507,17 +512,12 @@ __device__ __forceinline__ int fitting(const Rows &s, int groups, int slots, F b
         }
     return (int)least;
 }
-__device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int groups, int slots) {
-    const int lane = threadIdx.x & 63;
-    float most = 0.f;
-    const int least = fitting(s, groups, slots, [&](int b, float &n, float &u) {
+__device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int groups, int slots, int fewest) {
+    return fitting(s, groups, slots, fewest, [&](int b, float &n, float &u) {
         const int pos = s.pos[b];
         n = pos < 0 ? 0.f : (float)token_blocks(s, mask, pos).n;
         u = pos < 0 ? 0.f : 1.f;
-        most = fmaxf(most, n);
     });
-    most = wave_max(most);
-    return most <= 1.6f * least ? max(1, (int)most) : least;
 }
 
 // Attention of single tokens: workgroup (row, kv head and eight of its query heads;
@@ -534,11 +534,12 @@ __device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int 
 // block ahead, its page-table entries two.
 constexpr int TW = 4;                            // waves
 constexpr float LAZY = 7.f;                      // how far (log2) weights may pass the maximum they stand at
+                                                 // (0, as ever: 1 to 6% more time)
 constexpr int MAX_SPLITS = 64;                   // what the combine weighs in one wave
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <int HD, bool I8, bool TILED, typename T>
-__global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && HD == 128 ? 3 : 2))) void k_attn_tokens(
+__global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || HD == 128 ? 2 : 3))) void k_attn_tokens(
         Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part, int most,
         int slots, int H, float scale, Mask mask) {
     constexpr int KS = HD / 32, DT = HD / 16, VP = HD + 16;
@@ -556,7 +557,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 && H
     int n = blockIdx.x / groups, sp = 0, ns = 1;
     if (most > 1) {
         // The rows' splits one after the other, so that the workgroups that have none come last.
-        const int least = token_least(s, mask, groups, slots);
+        const int least = token_least(s, mask, groups, slots, token_fewest(HD));
         auto splits = [&](const Seq &q) { return q.r1 > q.r0 ? token_blocks(s, mask, q.pos).splits(most, least) : 0; };
         if (!unit_at(s, n, splits, n, sp)) return;
         ns = token_blocks(s, mask, s.pos[n]).splits(most, least);
@@ -882,7 +883,7 @@ struct Cut {
 // longest.
 template <int PC, int AK>
 __device__ __forceinline__ int unit_least(const Rows &s, const Mask &mask, int G, int HKV, int slots) {
-    return fitting(s, HKV, slots, [&](int b, float &n, float &u) {
+    return fitting(s, HKV, slots, ROWS_FEWEST, [&](int b, float &n, float &u) {
         const Units<PC, AK> q(seq_at(s, b), G, s.cap);
         u = q.rows > 0 ? (float)q.n() : 0.f;
         n = q.rows > 0 ? (float)q.blocks(mask, q.n() - 1).n : 0.f;
@@ -1628,7 +1629,8 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const bool tokens = !s->row_start;
     const int cols = hd == 128 ? unit_cols<128>() : unit_cols<256>();
     const int width = tokens ? 32 : hd == 128 ? tile_keys<128>() : tile_keys<256>();
-    if (window) keys = std::min(keys, (int64_t)window + (tokens ? 0 : cols / G) + width - 1 + (n_sink + width - 1) / width * width);
+    if (window)
+        keys = std::min(keys, (int64_t)window + (tokens ? 0 : cols / G) + width - 1 + ((int64_t)n_sink + width - 1) / width * width);
     // Blocks of keys of the longest row, workgroups of a split each, those that the chip
     // holds at once, and the most splits.  The keys are left whole, without a merge's
     // launch, where that is a few rounds of blocks a wave or the workgroups are many; how
@@ -1636,8 +1638,7 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const int64_t blocks = (keys + width - 1) / width;
     const int64_t groups = tokens ? kv->n_head_kv * ((G + 7) / 8) : kv->n_head_kv;
     const int64_t units = tokens ? s->n_rows : s->n_rows * G / cols + std::min<int64_t>(s->n_seq, s->n_rows);
-    const int64_t per_cu = tokens ? (kv->dtype == GD_I8 && hd == 128 ? 3 : 2) : 2;
-    const int64_t slots = per_cu * cus, wgs = units * groups;
+    const int64_t slots = 2 * cus, wgs = units * groups;
     // Rows' partials cost a full chip some 15 us, and a split saves what lets the workgroups
     // fill it; but the longest row may be one of a few, which split share the chip.  f16 rows on
     // codes, us whole / split: 10 blocks 28 / 31; 12 on a fifth of the slots 38 / 35, on 0.6 of
@@ -1645,16 +1646,19 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     // 1.8 183 / 196.
     bool whole;
     if (tokens)
-        // Tokens of up to 6000 positions whole / split: 200 of 8 kv heads (twice the slots) 118 /
+        // f16 tokens on codes, us whole / split: one of 20 blocks 11.7 / 12.1 (heads of 256 18 /
+        // 14), 32 of up to 20 blocks 12.2 / 15.2, of 34 under a window 17.6 / 26.5, of up to 47
+        // 20.5 / 15.0.  Tokens of up to 6000 positions: 200 of 8 kv heads (3.1 times the slots) 118 /
         // 99, 500 213 / 250, 1500 456 / 653; 500 of 4 (3.9 times) 248 / 244.  Past 1024 blocks a
         // long one of them would be the call's time.
-        whole = blocks <= 4 * TW || (blocks <= 12 * TW && wgs >= cus) || (blocks <= 256 * TW && wgs >= 4 * slots) ||
+        whole = blocks <= 4 * TW || (blocks <= 9 * TW && wgs >= cus) || (blocks <= 256 * TW && wgs >= 4 * slots) ||
                 wgs >= 16 * slots;
     else
         whole = blocks <= 10 || (blocks <= 24 && blocks * (slots - wgs) <= 8 * slots) ||
                 (blocks <= 128 && 2 * wgs >= 3 * slots) || wgs >= 4 * slots;
     GD_REQUIRE(ctx, wgs + slots + 2 * groups < MAX_WGS, "%s: %lld rows of %d heads", fn, (long long)s->n_rows, n_head);
-    int64_t ns = whole ? 1 : std::min<int64_t>((blocks + LEAST - 1) / LEAST, MAX_SPLITS);
+    const int least = tokens ? token_fewest(hd) : ROWS_FEWEST;
+    int64_t ns = whole ? 1 : std::min<int64_t>((blocks + least - 1) / least, MAX_SPLITS);
     float *scratch = nullptr;
     if ((rc = split_scratch(ctx, (size_t)s->n_rows * n_head * (hd + 3) * sizeof(float), ns, &scratch))) return rc;
     const int64_t sums = s->n_rows * n_head * ns;
@@ -1671,6 +1675,8 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
                            (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)slots, n_head, scale, mask); \
         if (ns > 1) { \
             GD_LAUNCHED(ctx, fn); \
+            /* (a workgroup a row and head: one token of 24 heads, 64 splits, 24 us, by the other \
+               31.8; 2560 rows and heads 114.8 and 75.2) */ \
             const bool many = s->n_rows * n_head >= 1024; \
             const int per = 1024 / HD_, merges = many ? (n_head + per - 1) / per : n_head; \
             auto merge = many ? k_attn_merge_many<HD_, T_> : k_attn_merge<HD_, T_>; \

@@ -485,15 +485,19 @@ def test_many_sequences_of_split_keys(ctx, dtype, n):
 @pytest.mark.parametrize("which", ["tokens", "ragged"])
 def test_the_largest_window_is_none(ctx, which):
     outs = []
-    for window in (0, 2**31 - 1):
+    for window, sinks in ((0, 0), (2**31 - 1, 0), (2**31 - 1, 2**31 - 1), (1, 2**31 - 1)):
         with Batch(ctx, ATTN[which], ga.I8, 2, 128, 16, row_start=which == "ragged") as bt:
-            bt.fill()
+            KV, start = bt.fill(), bt.start
             bt.desc.max_len = 4005
             q = rows_of(bt.rng, (bt.n, 4, 128), False)
             dq, do = bt.put(q), bt.put(np.zeros_like(q))
-            ctx.gd_kv_attn(*bt.ref, dq, 512, None, 0, do, ga.F32, 4, 0.1, window, 0)
+            ctx.gd_kv_attn(*bt.ref, dq, 512, None, 0, do, ga.F32, 4, 0.1, window, sinks)
             outs.append(ctx.get(do, q.shape, np.float32))
-    assert outs[0].any() and np.array_equal(*outs)
+    assert outs[0].any() and all(np.array_equal(outs[0], o) for o in outs[1:3])
+    for b, (p, r) in enumerate(ATTN[which]):                 # (maybe split elsewhere)
+        rows = slice(start[b], start[b] + r) if which == "ragged" else slice(b, b + 1)
+        if p >= 0 and r:
+            assert np.abs(outs[3][rows] - outs[0][rows]).max() <= 2 * bound(q[rows], *KV[b], 0.1, False)
 
 
 def test_row_starts_out_of_bounds(ctx):
