@@ -160,31 +160,29 @@ struct Turns {
     uint64_t t[128];
 };
 
-// Four elements at x as floats, and back.
-template <typename T, bool VEC> __device__ __forceinline__ f32x4 load4(const T *x) {
-    if constexpr (!VEC) return f32x4{to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3])};
-    else if constexpr (sizeof(T) == 4) return *(const f32x4 *)x;
-    else return __builtin_convertvector(*(const f16x4 *)x, f32x4);
-}
-
 // Rotates and appends the rows that fall into one block of 16 positions of a
 // sequence (unit blockIdx.x), and turns its query rows: wave w of workgroup y takes
-// the heads 4 y + w of H query heads, then the kv heads' keys, then their values.
+// the heads 4 y + w of the kv heads' keys, then their values, then the query heads (the
+// longest work first).
 //   A lane holds eight elements of a row as two fours, whose elements make four of the
 // rotated pairs (j and j + n_rot / 2, n_rot a multiple of 8) or eight of the dims behind
 // them: 64 lanes are four rows of head dim 128 or two of 256, the block's 16 rows that
-// many steps, all requested at once (a row at a time 46 us for 2175 rows of 24 / 4 x
-// 256, its loads one after the other).
+// many steps, all requested at once (a row at a time 46 us for 2119 rows of 24 / 4 x
+// 256, its loads one after the other) and beside them the rows' pages.
 //   The cos and sin of the block's positions are formed once a workgroup, and rows turned,
 // in 64 bits: from turns in 32 one code in 40 000 came out on the other side of a
 // border, and one half in 700 a step off.
+//   Bytes bound it, every row read and written once, as far as there are rows enough to
+// hide a chain of some 8 us (the unit, its rows, the turns, the block's maximum, codes):
+// 2119 f16 rows of 24 / 4 heads of 256 into codes move 65 MB in 19 us, 3.4 TB/s; 1000 f32
+// rows of 16 / 8 heads of 128 into halves 29 MB in 11.
 template <int HD, bool I8, bool VEC, typename T>
 __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, const T *q, int64_t q_stride, T *q_out,
                                                 int H, const T *kx, int64_t k_stride, const T *vx, int64_t v_stride,
                                                 int n_rot) {
     // Lanes of a row, rows of a step, steps; pairs of a lane are VEC ? 4 : 1 wide.
     constexpr int LPR = HD / 8, RPS = 64 / LPR, ST = BLK / RPS;
-    __shared__ double2 cs[BLK * (HD / 2)];
+    extern __shared__ double2 cs[];              // [BLK][n_rot / 2]
     const int t = threadIdx.x, lane = t & 63, half = n_rot / 2;
     int b, blk;
     auto blocks = [](const Seq &q) {
@@ -204,8 +202,8 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
     const int r = sq.r0 + skip, n = min(BLK - off, sq.r1 - r);
     const uint32_t p = (uint32_t)sq.pos + (uint32_t)skip;
     const int hs = blockIdx.y * 4 + (t >> 6), H2 = H + 2 * c.HKV;
-    const bool is_q = hs < H, is_k = !is_q && hs < H + c.HKV;
-    const int h = is_q ? hs : hs - H - (is_k ? 0 : c.HKV);
+    const bool is_k = hs < c.HKV, is_q = hs >= 2 * c.HKV;
+    const int h = is_q ? hs - 2 * c.HKV : is_k ? hs : hs - c.HKV;
     // This lane's place: row `lr` of a step's, elements d0 .. and d1 .. of it.  Without VEC
     // (any n_rot, any alignment) element e of both is a pair of its own.
     const int lr = lane / LPR, j0 = 4 * (lane % LPR);
@@ -218,7 +216,8 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
             d1 = d0 + 4;
         }
     };
-    f32x4 x0[ST], x1[ST];
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 x0[ST], x1[ST];
     if (hs < H2) {
         const T *src = (is_q ? q + r * q_stride : is_k ? kx + r * k_stride : vx + r * v_stride) + (int64_t)h * HD;
         const int64_t stride = is_q ? q_stride : is_k ? k_stride : v_stride;
@@ -228,18 +227,26 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
             if constexpr (VEC) {
                 int d0, d1;
                 dims(0, d0, d1);
-                x0[i] = load4<T, true>(row + d0);
-                x1[i] = load4<T, true>(row + d1);
+                x0[i] = *(const T4 *)(row + d0);
+                x1[i] = *(const T4 *)(row + d1);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     int d0, d1;
                     dims(e, d0, d1);
-                    x0[i][e] = to_f32(row[d0]);
-                    x1[i][e] = to_f32(row[d1]);
+                    x0[i][e] = row[d0];
+                    x1[i][e] = row[d1];
                 }
             }
         }
+    }
+    // The rows' pages, and the exponent of a block that has rows before these.
+    int page[I8 ? 1 : ST], had = 0;
+    if (hs < H2 && !is_q) {
+#pragma unroll
+        for (int i = 0; i < (I8 ? 1 : ST); i++) page[i] = page_of(c, s, b, I8 ? p : p + i * RPS + lr);
+        if constexpr (I8)
+            if (off && page[0] >= 0) had = (is_k ? c.kx : c.vx)[row_at<true>(c, page[0], slot_of(c, p) - off, h) / BLK];
     }
     const int64_t rp = (int64_t)p + (s.shift ? s.shift[b] : 0);
     for (int i = t; i < n * half; i += 256) {
@@ -253,7 +260,7 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
     const bool turn = is_q || is_k;
     // Element e of step i, turned where it is one of the rotated.
     auto turned = [&](int i, int e, double &a, double &z) {
-        a = x0[i][e], z = x1[i][e];
+        a = to_f32<T>(x0[i][e]), z = to_f32<T>(x1[i][e]);
         const int row = i * RPS + lr, j = j0 + e;
         if (turn && j < half && row < n) {
             const double2 w = cs[row * half + j];
@@ -279,7 +286,6 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
             }
         }
     };
-    typedef T T4 __attribute__((ext_vector_type(4)));
     typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
     typedef int8_t i8x4 __attribute__((ext_vector_type(4)));
     if (is_q) {
@@ -304,9 +310,6 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
         // A page may end inside the block.  Values past f16's range are held as its
         // largest.
         auto f16_of = [](double x) { return from_f64<uint16_t>(x > 65504. ? 65504. : x < -65504. ? -65504. : x); };
-        int page[ST];
-#pragma unroll
-        for (int i = 0; i < ST; i++) page[i] = page_of(c, s, b, p + i * RPS + lr);
 #pragma unroll
         for (int i = 0; i < ST; i++) {
             const int row = i * RPS + lr;
@@ -324,12 +327,10 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
         }
         return;
     } else {
-        const int page = page_of(c, s, b, p);
-        if (page < 0) return;
-        const uint32_t at = row_at<true>(c, page, slot_of(c, p) - off, h);
+        if (page[0] < 0) return;
+        const uint32_t at = row_at<true>(c, page[0], slot_of(c, p) - off, h);
         uint8_t *xp = (is_k ? c.kx : c.vx) + at / BLK;
         int8_t *y = (int8_t *)plane + (uint64_t)at * HD;
-        const int had = off ? *xp : 0;
         float top = 0.f;
         bool nan = false;
 #pragma unroll
@@ -338,7 +339,7 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
             for (int e = 0; e < 4; e++) {
                 // (In 32 bits, which is as good for a maximum and holds no 64-bit values till below.)
                 const int row = i * RPS + lr, j = j0 + e;
-                float a = x0[i][e], z = x1[i][e];
+                float a = to_f32<T>(x0[i][e]), z = to_f32<T>(x1[i][e]);
                 if (turn && j < half && row < n) {
                     const double2 w = cs[row * half + j];
                     const float cn = (float)w.x, sn = (float)w.y, o = a;
@@ -1556,6 +1557,7 @@ extern "C" int gd_kv_append_rope(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s,
     // Blocks of 16 positions that the rows can touch: rows / 16 and two ends a sequence.
     const int64_t units = std::min<int64_t>(s->n_rows, s->n_rows / BLK + 2 * std::min<int64_t>(s->n_seq, s->n_rows));
     const dim3 grid((unsigned)units, gd_blocks(H + 2 * kv->n_head_kv, 4));
+    const unsigned lds = BLK * (n_rot / 2) * sizeof(double2);
     // Fours of a row in one access: what its place, stride and rotated dims allow.
     const int size = x_dtype == GD_F32 ? 4 : 2;
     const bool vec = n_rot % 8 == 0 && (k_stride | v_stride | (q ? q_stride : 0)) % 4 == 0 &&
@@ -1563,7 +1565,7 @@ extern "C" int gd_kv_append_rope(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s,
 #define GD_GO(HD_, I8_, T_) \
     do { \
         auto kernel = vec ? k_append<HD_, I8_, true, T_> : k_append<HD_, I8_, false, T_>; \
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, cache_of(kv), rows_of(kv, s), turns, (const T_ *)q, \
+        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, ctx->stream, cache_of(kv), rows_of(kv, s), turns, (const T_ *)q, \
                            q_stride, (T_ *)q_out, H, (const T_ *)k, k_stride, (const T_ *)v, v_stride, n_rot); \
     } while (0)
     GD_KV_PICK(kv, x_dtype, GD_GO);
