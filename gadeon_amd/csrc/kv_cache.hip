@@ -393,7 +393,8 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
 // ---------------------------------------------------------------- read
 
 // Rows of the cache as values, eight dims a thread: thread i over [row][K then V]
-// [head][HD / 8].  Rows of pages that are not there come out as zeros.
+// [head][HD / 8].  Rows of pages that are not there come out as zeros.  Its launch bounds it
+// up to some hundred rows (3 us), bytes beyond (2300 rows of 4 heads of 256, 14 MB, 5.4 us).
 template <int HD, bool I8, typename T>
 __global__ __launch_bounds__(256) void k_read(Cache c, Rows s, T *k_out, T *v_out) {
     const int per = 2 * c.HKV * (HD / 8), n = blockIdx.x;
@@ -533,6 +534,13 @@ __device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int 
 // steps scaling the scores; 8-bit values as the halves they are.  Keys that are not
 // seen have the weight 0 and zeros for values.  A block's rows are requested one
 // block ahead, its page-table entries two.
+//   Memory bounds long rows: 64 tokens of 4096 positions, 40 heads of 128 on 8, 101 us in
+// codes (5.3 TB/s), 192 in halves (5.6).  Short ones are a chain of loads (position, page,
+// keys: 2.5 us) and the merge of the waves (1.7): one token of 331 positions 8.7 us.  64 of
+// up to 8192 (125 MB) take 33: two long ones' splits beside many of a few keys.
+//   Two waves a SIMD, three for halves of head dim 256 (us at 2 / 3 waves: codes of 128, 64
+// tokens of up to 8192 positions, 41 / 46; of 256, up to 4096, 37 / 51; halves of 256, one
+// token of 600 positions, 21 / 19; the register budget sets the compiler's schedule).
 constexpr int TW = 4;                            // waves
 constexpr float LAZY = 7.f;                      // how far (log2) weights may pass the maximum they stand at
                                                  // (0, as ever: 1 to 6% more time)
@@ -852,6 +860,15 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
 // result's own rounding.  A tile that some column does not see whole goes key by key: a
 // mask, and where V holds a NaN or infinity its finite part and, apart, which columns see
 // the others (0 x NaN would reach them all).
+//   512 f16 rows behind 3584 positions of codes, 40 heads of 128 on 8: 67 us, 600 TFLOP/s;
+// 4096 under a window of 1024 133 us, 570; f32 rows (twice the products) of 24 heads of 256
+// on 4 530.  No unit of the CU is full (matrix cores 30% busy, vector ALUs 47%, LDS 30%):
+// with the registers of two waves a SIMD a wave's chain of staging, scores, weights and sums
+// is what lasts, 2.0 to 2.5 us for two waves' tiles, a lone one 1.7.  Measured and left out:
+// units of twice the columns, eight waves to a tile (codes of 256 219 -> 207 us, but f32 rows
+// of chunks 115 -> 122, under a window 133 -> 145); scores formed a tile ahead, beside the
+// weights of the last (143 -> 154, of 256 219 -> 261); tiles of 32 keys and three waves a
+// SIMD (1024 rows 143 -> 127, 512 75 -> 84).
 // Columns of a wave, and of a unit: a wave's sums are head dim x columns, which at head
 // dim 256 leave 32 columns no registers (128 of sums, 128 of f32 rows' q).
 template <int HD> constexpr int wave_cols() { return HD == 128 ? 32 : 16; }
@@ -1308,7 +1325,7 @@ template <typename T> __device__ __forceinline__ float gated(float y, const T *g
 
 // Merges the partials (up to `most` <= MAX_SPLITS) of head h of row n, few rows: thread
 // (d, r) takes the splits r, r + NR, .. of one dim, beside the splits' weights, once a
-// workgroup.
+// workgroup.  A chain of loads: 4.6 us for 64 splits of 24 heads of 256.
 template <int HD, typename T>
 __global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, Rows s, const T *gate, int64_t gate_stride,
                                                     T *out, int H) {
@@ -1346,6 +1363,7 @@ __global__ __launch_bounds__(512) void k_attn_merge(Part part, int most, Rows s,
 }
 
 // The same for many rows: HD / 4 threads a (row, head), four dims each, a split at a time.
+// Bytes bound it: 20480 rows and heads of 128 in 3 splits, 37 MB, 11 us.
 template <int HD, typename T>
 __global__ __launch_bounds__(256) void k_attn_merge_many(Part part, int most, Rows s, const T *gate, int64_t gate_stride,
                                                          T *out, int H) {
