@@ -480,9 +480,10 @@ struct Part {
 // workgroup's start, end and merge cost: for tokens 8 blocks of head dim 128 and 4 of 256
 // (one token of 600 positions, us at 4 / 8 / 16 blocks: 40 heads of 128 11.5 / 12.3 / 14.8,
 // 24 of 256 on codes 14.3 / 16.5 / 21, on halves 16.3 / 18.9 / 26; 32 of up to 3000 behind an
-// append, heads of 128, 28.3 / 25.8 / 27.6), for rows 8 (4 to 16 alike within 2%).
+// append, heads of 128, 28.3 / 25.8 / 27.6), for rows 4 (2 rows behind 8191 of codes, at 2 / 4 /
+// 8: 17.3 / 17.3 / 24.1, 16 of 8 sequences 29.2 / 30.7 / 35.0; full chips alike).
 constexpr int token_fewest(int hd) { return 1024 / hd; }
-constexpr int ROWS_FEWEST = 8;
+constexpr int ROWS_FEWEST = 4;
 __device__ __forceinline__ KeyBlocks<32> token_blocks(const Rows &s, const Mask &mask, int pos) {
     return KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
 }
@@ -538,9 +539,10 @@ __device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int 
 // codes (5.3 TB/s), 192 in halves (5.6).  Short ones are a chain of loads (position, page,
 // keys: 2.5 us) and the merge of the waves (1.7): one token of 331 positions 8.7 us.  64 of
 // up to 8192 (125 MB) take 33: two long ones' splits beside many of a few keys.
-//   Two waves a SIMD, three for halves of head dim 256 (us at 2 / 3 waves: codes of 128, 64
-// tokens of up to 8192 positions, 41 / 46; of 256, up to 4096, 37 / 51; halves of 256, one
-// token of 600 positions, 21 / 19; the register budget sets the compiler's schedule).
+//   Two waves a SIMD or more, where halves of head dim 256 (32 KiB of them in flight a wave)
+// take 380 registers and one: us of two with spills / one, 24 heads on 4: one token of 600
+// positions 16.8 / 15.9, 64 of up to 8192 88 / 81, eight 27 / 33.  Codes of 128 at two / three,
+// 64 tokens of up to 8192, 40 heads on 8: 41 / 46; codes of 256, up to 4096, 37 / 51.
 constexpr int TW = 4;                            // waves
 constexpr float LAZY = 7.f;                      // how far (log2) weights may pass the maximum they stand at
                                                  // (0, as ever: 1 to 6% more time)
@@ -548,7 +550,7 @@ constexpr int MAX_SPLITS = 64;                   // what the combine weighs in o
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <int HD, bool I8, bool TILED, typename T>
-__global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || HD == 128 ? 2 : 3))) void k_attn_tokens(
+__global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || HD == 128 ? 2 : 1))) void k_attn_tokens(
         Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part, int most,
         int slots, int H, float scale, Mask mask) {
     constexpr int KS = HD / 32, DT = HD / 16, VP = HD + 16;
@@ -618,7 +620,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
                 for (int i = 0; i < KL; i++) kreg[kt][i] = *(const u32x4 *)(kp + kplace + 64 * i);
 #pragma unroll
                 for (int i = kt * VCH / 2; i < (kt + 1) * VCH / 2; i++)
-                    vreg[i] = *(const u32x4 *)(vp + (uint32_t)(vplace + i * KPV % 16 * pitch));
+                    vreg[i] = *(const u32x4 *)(vp + (uint64_t)(i * KPV % 16 * pitch) + vplace);
             }
         } else {
 #pragma unroll
@@ -1658,7 +1660,7 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const int64_t blocks = (keys + width - 1) / width;
     const int64_t groups = tokens ? kv->n_head_kv * ((G + 7) / 8) : kv->n_head_kv;
     const int64_t units = tokens ? s->n_rows : s->n_rows * G / cols + std::min<int64_t>(s->n_seq, s->n_rows);
-    const int64_t slots = 2 * cus, wgs = units * groups;
+    const int64_t slots = (tokens && hd == 256 && kv->dtype == GD_F16 ? 1 : 2) * cus, wgs = units * groups;    // (k_attn_tokens' registers)
     // Rows' partials cost a full chip some 15 us, and a split saves what lets the workgroups
     // fill it; but the longest row may be one of a few, which split share the chip.  f16 rows on
     // codes, us whole / split: 10 blocks 28 / 31; 12 on a fifth of the slots 38 / 35, on 0.6 of
