@@ -99,19 +99,23 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // Unit u of the sequences' units, `count` of them each (count(Seq) lane by lane): its
-// sequence b and place k in it, for the whole wave.  False: fewer units than that.
+// sequence b, which is sq, and place k in it, for the whole wave.  False: fewer units than
+// that.
 template <class F>
-__device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, int &b, int &k) {
+__device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, int &b, int &k, Seq &sq) {
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int c = 0; c < s.n_seq; c += 64) {
-        const int n = c + lane < s.n_seq ? count(seq_at(s, c + lane)) : 0;
+        Seq q = {0, 0, 0};
+        if (c + lane < s.n_seq) q = seq_at(s, c + lane);
+        const int n = c + lane < s.n_seq ? count(q) : 0;
         const int sum = wave_scan(n);
         const uint64_t past = __ballot(base + sum > u);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             b = c + l;
             k = u - (base + __builtin_amdgcn_readlane(sum - n, l));
+            sq = {__builtin_amdgcn_readlane(q.r0, l), __builtin_amdgcn_readlane(q.r1, l), __builtin_amdgcn_readlane(q.pos, l)};
             return k >= 0 && k < __builtin_amdgcn_readlane(n, l);    // (sums past 2^31: no row_start)
         }
         base += __builtin_amdgcn_readlane(sum, 63);
@@ -185,17 +189,18 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
     extern __shared__ double2 cs[];              // [BLK][n_rot / 2]
     const int t = threadIdx.x, lane = t & 63, half = n_rot / 2;
     int b, blk;
+    Seq sq;
     auto blocks = [](const Seq &q) {
         return q.r1 > q.r0 ? (int)(((uint32_t)q.pos % BLK + (uint32_t)(q.r1 - q.r0) + BLK - 1) / BLK) : 0;
     };
     if (!s.row_start) {                          // a row, and a block, each
         b = blockIdx.x;
         blk = 0;
-        if (s.pos[b] < 0) return;
-    } else if (!unit_at(s, blockIdx.x, blocks, b, blk)) {
+        sq = seq_at(s, b);
+        if (sq.pos < 0) return;
+    } else if (!unit_at(s, blockIdx.x, blocks, b, blk, sq)) {
         return;
     }
-    const Seq sq = seq_at(s, b);
     // The block's new rows: n of them from row r on, the first at slot `off` of it.
     const int off = blk ? 0 : sq.pos % BLK;
     const int skip = blk ? blk * BLK - sq.pos % BLK : 0;
@@ -565,16 +570,19 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
     const int G = H / c.HKV, groups = c.HKV * ((G + 7) / 8);
     const int gr = blockIdx.x % groups;
     const int kvh = gr / ((G + 7) / 8), g8 = 8 * (gr % ((G + 7) / 8)), h0 = kvh * G + g8, nh = min(8, G - g8);
-    int n = blockIdx.x / groups, sp = 0, ns = 1;
+    int n = blockIdx.x / groups, sp = 0, ns = 1, pos;
     if (most > 1) {
         // The rows' splits one after the other, so that the workgroups that have none come last.
         const int least = token_least(s, mask, groups, slots, token_fewest(HD));
         auto splits = [&](const Seq &q) { return q.r1 > q.r0 ? token_blocks(s, mask, q.pos).splits(most, least) : 0; };
-        if (!unit_at(s, n, splits, n, sp)) return;
-        ns = token_blocks(s, mask, s.pos[n]).splits(most, least);
+        Seq sq;
+        if (!unit_at(s, n, splits, n, sp, sq)) return;
+        pos = sq.pos;
+        ns = token_blocks(s, mask, pos).splits(most, least);
+    } else {
+        pos = s.pos[n];
+        if (pos < 0) return;
     }
-    const int pos = s.pos[n];
-    if (pos < 0) return;
     const KeyBlocks<32> kb = token_blocks(s, mask, pos);
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int lr = lane & 15, g = lane >> 4, col = lr & 7;
@@ -943,8 +951,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         const Units<PC, AK> u(q, G, s.cap);
         return u.rows <= 0 ? 0 : u.n() * (most > 1 ? u.splits(mask, most, least) : 1);
     };
-    if (!unit_at(s, blockIdx.x / c.HKV, units, b, k)) return;
-    const Seq sq = seq_at(s, b);
+    Seq sq;
+    if (!unit_at(s, blockIdx.x / c.HKV, units, b, k, sq)) return;
     const Units<PC, AK> un(sq, G, s.cap);
     const int rows = un.rows;
     if (most > 1) nz = un.splits(mask, most, least);
