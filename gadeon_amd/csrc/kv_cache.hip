@@ -98,27 +98,30 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
 }
 
-// Unit u of the sequences' units, `count` of them each (count(Seq) lane by lane): its
-// sequence b, which is sq, and place k in it, for the whole wave.  False: fewer units than
-// that.
-template <class F>
-__device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, int &b, int &k, Seq &sq) {
+// Unit u of the sequences' units, `count` of them each (count(Seq) lane by lane), class by
+// class (class_of(Seq): 0 .. classes - 1; all in one of more than 64 sequences): its sequence
+// b, which is sq, and place k in it, for the whole wave.  False: fewer units than that.
+template <int classes, class F, class G>
+__device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, G class_of, int &b, int &k, Seq &sq) {
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int c = 0; c < s.n_seq; c += 64) {
         Seq q = {0, 0, 0};
         if (c + lane < s.n_seq) q = seq_at(s, c + lane);
         const int n = c + lane < s.n_seq ? count(q) : 0;
-        const int sum = wave_scan(n);
-        const uint64_t past = __ballot(base + sum > u);
-        if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            b = c + l;
-            k = u - (base + __builtin_amdgcn_readlane(sum - n, l));
-            sq = {__builtin_amdgcn_readlane(q.r0, l), __builtin_amdgcn_readlane(q.r1, l), __builtin_amdgcn_readlane(q.pos, l)};
-            return k >= 0 && k < __builtin_amdgcn_readlane(n, l);    // (sums past 2^31: no row_start)
+        const int mine = classes > 1 && s.n_seq <= 64 ? class_of(q) : 0;
+#pragma unroll
+        for (int x = 0; x < classes; x++) {
+            const int nx = mine == x ? n : 0, sum = wave_scan(nx), all = __builtin_amdgcn_readlane(sum, 63);
+            if (u - base < all) {
+                const int l = __ffsll((unsigned long long)__ballot(base + sum > u)) - 1;
+                b = c + l;
+                k = u - (base + __builtin_amdgcn_readlane(sum - nx, l));
+                sq = {__builtin_amdgcn_readlane(q.r0, l), __builtin_amdgcn_readlane(q.r1, l), __builtin_amdgcn_readlane(q.pos, l)};
+                return k >= 0 && k < __builtin_amdgcn_readlane(nx, l);   // (sums past 2^31: no row_start)
+            }
+            base += all;
         }
-        base += __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -198,7 +201,7 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
         blk = 0;
         sq = seq_at(s, b);
         if (sq.pos < 0) return;
-    } else if (!unit_at(s, blockIdx.x, blocks, b, blk, sq)) {
+    } else if (!unit_at<1>(s, blockIdx.x, blocks, [](const Seq &) { return 0; }, b, blk, sq)) {
         return;
     }
     // The block's new rows: n of them from row r on, the first at slot `off` of it.
@@ -493,8 +496,10 @@ __device__ __forceinline__ KeyBlocks<32> token_blocks(const Rows &s, const Mask 
     return KeyBlocks<32>(mask, (uint32_t)pos, min((uint32_t)pos, s.cap - 1));
 }
 // From an even share of all blocks a slot, to what lets the splits have a slot each, those
-// of half as many blocks or fewer a part of one, as they fill the gaps (64 tokens of up to
-// 8192 positions 41 us, a slot for each 59; a mixed batch of prompt chunks 115 and 197);
+// of half as many blocks or fewer a part of one, their start counted as two blocks, as they
+// come last and fill the gaps (unit_at; 64 tokens of up to 8192 positions 41 us, a slot for
+// each 59; a mixed batch of prompt chunks 115 and 197; the long ones first 38 and 117, 32
+// chunks of up to 200 behind 2500, 24 heads of 256 on 4, 107 -> 94, 16 of them 64 -> 71);
 // blocks(b, n, u): n blocks in each of sequence b's u units.  Over 64 sequences fill the chip
 // as they are, and the even share is left (200 tokens of up to 6000 positions, 40 heads of
 // 128 on 8: 92 us, fitted 107).
@@ -515,7 +520,7 @@ __device__ __forceinline__ int fitting(const Rows &s, int groups, int slots, int
     // (At least an even share: so no more than units + slots / groups splits.)
     if (s.n_seq <= 64)
         for (int i = 0; i < 12; i++) {
-            if (gd_wave_sum(u * (n <= 0.5f * least ? n / least : ceilf(n / least))) <= room) break;
+            if (gd_wave_sum(u * (n <= 0.5f * least ? fminf(n + 2.f, least) / least : ceilf(n / least))) <= room) break;
             least = ceilf(least * 1.125f);
         }
     return (int)least;
@@ -572,11 +577,13 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
     const int kvh = gr / ((G + 7) / 8), g8 = 8 * (gr % ((G + 7) / 8)), h0 = kvh * G + g8, nh = min(8, G - g8);
     int n = blockIdx.x / groups, sp = 0, ns = 1, pos;
     if (most > 1) {
-        // The rows' splits one after the other, so that the workgroups that have none come last.
+        // The rows' splits one after the other, long rows' first, so that the workgroups that
+        // have none come last.
         const int least = token_least(s, mask, groups, slots, token_fewest(HD));
         auto splits = [&](const Seq &q) { return q.r1 > q.r0 ? token_blocks(s, mask, q.pos).splits(most, least) : 0; };
         Seq sq;
-        if (!unit_at(s, n, splits, n, sp, sq)) return;
+        auto order = [&](const Seq &q) { return q.r1 > q.r0 && token_blocks(s, mask, q.pos).n > 0.5f * least ? 0 : 1; };
+        if (!unit_at<2>(s, n, splits, order, n, sp, sq)) return;
         pos = sq.pos;
         ns = token_blocks(s, mask, pos).splits(most, least);
     } else {
@@ -945,14 +952,20 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     const int G = H / c.HKV, kvh = blockIdx.x % c.HKV;
     int b, k, nz = 1;
     // The sequences' units one after the other, each in its splits, so that the workgroups
-    // that have none come last; of a sequence those that see the most keys first.
+    // that have none come last; the long sequences first, and of each the units that see the
+    // most keys.
     const int least = most > 1 ? unit_least<PC, AK>(s, mask, G, c.HKV, slots) : 0;
     auto units = [&](const Seq &q) {
         const Units<PC, AK> u(q, G, s.cap);
         return u.rows <= 0 ? 0 : u.n() * (most > 1 ? u.splits(mask, most, least) : 1);
     };
     Seq sq;
-    if (!unit_at(s, blockIdx.x / c.HKV, units, b, k, sq)) return;
+    auto order = [&](const Seq &q) {
+        const Units<PC, AK> u(q, G, s.cap);
+        const int n = u.rows > 0 ? u.blocks(mask, u.n() - 1).n : 0;
+        return n > 0.5f * least ? 0 : n > 0.2f * least ? 1 : 2;
+    };
+    if (!unit_at<3>(s, blockIdx.x / c.HKV, units, order, b, k, sq)) return;
     const Units<PC, AK> un(sq, G, s.cap);
     const int rows = un.rows;
     if (most > 1) nz = un.splits(mask, most, least);
