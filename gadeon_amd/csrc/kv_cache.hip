@@ -548,7 +548,7 @@ __device__ __forceinline__ int token_least(const Rows &s, const Mask &mask, int 
 //   Memory bounds long rows: 64 tokens of 4096 positions, 40 heads of 128 on 8, 101 us in
 // codes (5.3 TB/s), 192 in halves (5.6).  Short ones are a chain of loads (position, page,
 // keys: 2.5 us) and the merge of the waves (1.7): one token of 331 positions 8.7 us.  64 of
-// up to 8192 (125 MB) take 33: two long ones' splits beside many of a few keys.
+// up to 8192 (125 MB) take 29: long rows' splits beside many of a few keys.
 //   Two waves a SIMD or more, where halves of head dim 256 (32 KiB of them in flight a wave)
 // take 380 registers and one: us of two with spills / one, 24 heads on 4: one token of 600
 // positions 16.8 / 15.9, 64 of up to 8192 88 / 81, eight 27 / 33.  Codes of 128 at two / three,
@@ -1480,6 +1480,14 @@ int check_x(gd_ctx *ctx, const char *fn, int dtype) {
     return GD_OK;
 }
 
+// A positive number modulo 1 as a fraction of 2^64, from its 64 bits and exponent (floorl and
+// a conversion a pair took 3 us of a call's 8.3 at 128 rotated dims).
+uint64_t fraction(long double x) {
+    int up;
+    const uint64_t bits = (uint64_t)(frexpl(x, &up) * 0x1p64L);          // x = bits 2^(up - 64)
+    return up > 63 || up < -63 ? 0 : up >= 0 ? bits << up : bits >> -up;
+}
+
 Cache cache_of(const gd_kv *kv) {
     return Cache{kv->k, kv->v, kv->k_exp, kv->v_exp, (uint32_t)kv->n_pages, kv->n_head_kv, kv->page_size,
                  FastDiv((uint32_t)kv->page_size)};
@@ -1590,10 +1598,7 @@ extern "C" int gd_kv_append_rope(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s,
     // under 2^-57 of itself, which even position 2^31 turns into less than 2^-28 of a turn.
     Turns turns;
     long double turn = 0.159154943091895335768883763372514362L, by = n_rot ? powl(base, -2.0L / n_rot) : 0.0L;
-    for (int j = 0; j < n_rot / 2; j++, turn *= by) {
-        long double f = turn - floorl(turn);
-        turns.t[j] = f >= 1.0L - 0x1p-64L ? 0 : (uint64_t)(f * 0x1p64L);
-    }
+    for (int j = 0; j < n_rot / 2; j++, turn *= by) turns.t[j] = fraction(turn);
     const int H = q ? n_head : 0;
     // Blocks of 16 positions that the rows can touch: rows / 16 and two ends a sequence.
     const int64_t units = std::min<int64_t>(s->n_rows, s->n_rows / BLK + 2 * std::min<int64_t>(s->n_seq, s->n_rows));
