@@ -114,9 +114,9 @@ __device__ __forceinline__ bool unit_at(const Rows &s, int u, F count, G class_o
         for (int x = 0; x < classes; x++) {
             const int nx = mine == x ? n : 0, sum = wave_scan(nx), all = __builtin_amdgcn_readlane(sum, 63);
             if (u - base < all) {
-                const int l = __ffsll((unsigned long long)__ballot(base + sum > u)) - 1;
+                const int l = __ffsll((unsigned long long)__ballot(sum > u - base)) - 1;
                 b = c + l;
-                k = u - (base + __builtin_amdgcn_readlane(sum - nx, l));
+                k = u - base - __builtin_amdgcn_readlane(sum - nx, l);
                 sq = {__builtin_amdgcn_readlane(q.r0, l), __builtin_amdgcn_readlane(q.r1, l), __builtin_amdgcn_readlane(q.pos, l)};
                 return k >= 0 && k < __builtin_amdgcn_readlane(nx, l);   // (sums past 2^31: no row_start)
             }
