@@ -1695,7 +1695,7 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     bool whole;
     if (tokens)
         // f16 tokens on codes, us whole / split: one of 20 blocks 11.7 / 12.1 (heads of 256 18 /
-        // 14), 32 of up to 20 blocks 12.2 / 15.2, of 34 under a window 17.6 / 26.5, of up to 47
+        // 14), 32 of up to 20 blocks 12.2 / 15.2, of 34 under a window 17.9 / 21.7, of up to 47
         // 20.5 / 15.0.  Tokens of up to 6000 positions: 200 of 8 kv heads (3.1 times the slots) 118 /
         // 99, 500 213 / 250, 1500 456 / 653; 500 of 4 (3.9 times) 248 / 244.  Past 1024 blocks a
         // long one of them would be the call's time.
