@@ -1659,6 +1659,12 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     GD_REQUIRE(ctx, window >= 0 && n_sink >= 0, "%s: window %d, n_sink %d", fn, window, n_sink);
     GD_REQUIRE(ctx, std::isfinite(scale), "%s: scale %g", fn, (double)scale);
     GD_REQUIRE(ctx, s->n_rows * n_head < (1LL << 31) - 256, "%s: %lld rows of %d heads", fn, (long long)s->n_rows, n_head);
+    const bool tokens = !s->row_start;
+    const int G = n_head / kv->n_head_kv, cols = hd == 128 ? unit_cols<128>() : unit_cols<256>();
+    const int64_t groups = tokens ? kv->n_head_kv * ((G + 7) / 8) : kv->n_head_kv;
+    const int64_t units = tokens ? s->n_rows : s->n_rows * G / cols + std::min<int64_t>(s->n_seq, s->n_rows);
+    // (Splits add no more than the chip's slots and two units.)
+    GD_REQUIRE(ctx, units * groups < MAX_WGS - (1 << 16), "%s: %lld rows of %d heads", fn, (long long)s->n_rows, n_head);
     // Workgroups read their q and gate before they write: in place only row on row.
     const size_t span = (size_t)s->n_rows * row * size;
     auto apart = [&](const void *x, int64_t stride) {
@@ -1671,11 +1677,9 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     if (!s->n_rows || !s->n_seq) return GD_OK;
     GD_HIP(ctx, hipSetDevice(ctx->device));
     const Mask mask{window, window ? n_sink : 0};
-    const int G = n_head / kv->n_head_kv, cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
+    const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
     const Rows rows = rows_of(kv, s);
     int64_t keys = s->max_len ? std::min<int64_t>(s->max_len, rows.cap) : rows.cap;
-    const bool tokens = !s->row_start;
-    const int cols = hd == 128 ? unit_cols<128>() : unit_cols<256>();
     const int width = tokens ? 32 : hd == 128 ? tile_keys<128>() : tile_keys<256>();
     if (window)
         keys = std::min(keys, (int64_t)window + (tokens ? 0 : cols / G) + width - 1 + ((int64_t)n_sink + width - 1) / width * width);
@@ -1684,8 +1688,6 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     // launch, where that is a few rounds of blocks a wave or the workgroups are many; how
     // finely others are split, the kernels know (token_least, unit_least).
     const int64_t blocks = (keys + width - 1) / width;
-    const int64_t groups = tokens ? kv->n_head_kv * ((G + 7) / 8) : kv->n_head_kv;
-    const int64_t units = tokens ? s->n_rows : s->n_rows * G / cols + std::min<int64_t>(s->n_seq, s->n_rows);
     const int64_t slots = (tokens && hd == 256 && kv->dtype == GD_F16 ? 1 : 2) * cus, wgs = units * groups;    // (k_attn_tokens' registers)
     // Rows' partials cost a full chip some 15 us, and a split saves what lets the workgroups
     // fill it; but the longest row may be one of a few, which split share the chip.  f16 rows on
@@ -1704,7 +1706,6 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     else
         whole = blocks <= 10 || (blocks <= 24 && blocks * (slots - wgs) <= 8 * slots) ||
                 (blocks <= 128 && 2 * wgs >= 3 * slots) || wgs >= 4 * slots;
-    GD_REQUIRE(ctx, wgs + slots + 2 * groups < MAX_WGS, "%s: %lld rows of %d heads", fn, (long long)s->n_rows, n_head);
     const int least = tokens ? token_fewest(hd) : ROWS_FEWEST;
     int64_t ns = whole ? 1 : std::min<int64_t>((blocks + least - 1) / least, MAX_SPLITS);
     float *scratch = nullptr;

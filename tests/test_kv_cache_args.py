@@ -112,6 +112,12 @@ def test_rows_by_heads_past_31_bits():
                  out=P << 30), "16777215 rows of 256 heads")
 
 
+def test_more_workgroups_than_a_launch_has():
+    refused(attn(s=seqs(n_rows=1 << 23, n_seq=1 << 23, row_start=None)), "8388608 rows of 4 heads")
+    refused(attn(c=kv(n_head_kv=4096), s=seqs(n_rows=1 << 13, n_seq=1 << 13), n_head=4096, q=P << 8, q_stride=1 << 19,
+                 gate=None, out=P << 30), "8192 rows of 4096 heads")
+
+
 @pytest.mark.parametrize("kw,words", [(dict(dtype=ga.F32), "cache dtype"), (dict(head_dim=96), "head_dim 96"),
                                       (dict(page_size=8), "page size 8"), (dict(n_pages=0), "0 pages"),
                                       (dict(out=None), "null out pointer")])
