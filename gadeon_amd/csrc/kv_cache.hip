@@ -1392,10 +1392,13 @@ __global__ __launch_bounds__(256) void k_attn_merge_many(Part part, int most, Ro
                                                          T *out, int H) {
     constexpr int TPR = HD / 4, RPW = 256 / TPR;
     const int groups = (H + RPW - 1) / RPW, n = blockIdx.x / groups;
-    const int h = min((int)(blockIdx.x % groups) * RPW + (int)threadIdx.x / TPR, H - 1), d = 4 * (threadIdx.x % TPR);
+    const int h = (int)(blockIdx.x % groups) * RPW + (int)threadIdx.x / TPR, d = 4 * (threadIdx.x % TPR);
+    // (has_sequence takes whole waves.  Threads past the last head leave it alone: out may be
+    // gate, which is read where out is written.)
+    if (!has_sequence(s, n) || h >= H) return;
     const int64_t row = (int64_t)n * H + h;
     const int ns = min(part.used[row], most);
-    if (!has_sequence(s, n) || ns <= 1) return;
+    if (ns <= 1) return;
     const float2 *ml = part.ml + row * most;
     const float *p = part.acc + row * most * HD + d;
     float M = -INFINITY, L = 0.f;

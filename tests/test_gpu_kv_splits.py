@@ -1,0 +1,50 @@
+"""gd_kv_attn where keys are split and merged: results in the place of q or of the
+gate, bit for bit those of a buffer of their own (which test_gpu_kv_cache.py's 64-bit
+statement holds), for each merge: few rows and many, tokens and chunks, head counts
+that fill its groups of heads and ones that do not."""
+import numpy as np
+import pytest
+
+import gadeon_amd as ga
+from test_gpu_kv_cache import Batch, attend, bound, raw, rows_of
+
+pytestmark = pytest.mark.gpu
+
+# (sequences, whether they are tokens): 1 to 4 rows, then over 1024 rows and heads.
+FEW = {"token": [(3000, 1)], "tokens": [(2000, 1), (-1, 1), (3100, 1), (70, 1)], "chunk": [(2900, 3)]}
+
+
+def many(which, H):
+    rows = 1024 // H + 9
+    if which == "tokens":
+        return [(1400 + i if i % 8 == 5 else i, 1) for i in range(rows)]
+    return [(2100, rows - 40), (5, 3), (-1, 2), (1700, 35)]
+
+
+@pytest.mark.parametrize("dtype", [ga.I8, ga.F16], ids=["i8", "f16"])
+@pytest.mark.parametrize("x16", [False, True], ids=["f32rows", "f16rows"])
+@pytest.mark.parametrize("hd,H,hkv", [(128, 10, 2), (128, 8, 2), (128, 3, 3), (256, 6, 1), (256, 18, 2)])
+@pytest.mark.parametrize("which", [*FEW, "many tokens", "many rows"])
+def test_in_place_of_split_keys(ctx, dtype, x16, hd, H, hkv, which):
+    seqs = FEW[which] if which in FEW else many(which.split()[1], H)
+    with Batch(ctx, seqs, dtype, hkv, hd, 16, row_start="tok" not in which) as bt:
+        KV, x = bt.fill(), ga.F16 if x16 else ga.F32
+        q, g = (rows_of(bt.rng, (bt.n, H, hd), x16) for _ in "qg")
+        dq, dg, do = (bt.put(raw(a)) for a in (q, g, np.zeros_like(q)))
+        row, scale = H * hd, hd ** -0.5
+        ctx.gd_kv_attn(*bt.ref, dq, row, dg, row, do, x, H, scale, 0, 0)
+        out = ctx.get(do, q.shape, q.dtype)
+        done = np.repeat([p >= 0 for p, _ in seqs], [r for _, r in seqs])
+        for b, (p, r) in enumerate(seqs):                   # (some rows of each: the rest bit for bit below)
+            at = slice(bt.start[b] + max(0, r - 3), bt.start[b] + r)
+            want = attend(q[at], *KV[b], p + max(0, r - 3), np.float32(scale), 0, 0, g[at]) if p >= 0 else out[at]
+            assert np.abs(out[at] - want).max() <= bound(q[at], *KV[b], scale, x16), (b, p, r)
+        for again in range(3):                              # out over the gate, then over q
+            ctx.set(dg, raw(g))
+            ctx.gd_kv_attn(*bt.ref, dq, row, dg, row, dg, x, H, scale, 0, 0)
+            got = ctx.get(dg, q.shape, q.dtype)
+            assert np.array_equal(got[done], out[done]) and np.array_equal(got[~done], g[~done])
+        ctx.set(dg, raw(g))
+        ctx.gd_kv_attn(*bt.ref, dq, row, dg, row, dq, x, H, scale, 0, 0)
+        got = ctx.get(dq, q.shape, q.dtype)
+        assert np.array_equal(got[done], out[done]) and np.array_equal(got[~done], q[~done])
