@@ -183,10 +183,12 @@ struct Turns {
 // hide a chain of some 8 us (the unit, its rows, the turns, the block's maximum, codes):
 // 2119 f16 rows of 24 / 4 heads of 256 into codes move 65 MB in 19 us, 3.4 TB/s; 1000 f32
 // rows of 16 / 8 heads of 128 into halves 29 MB in 11.
+//   f32 rows of 128 into codes are held to six waves a SIMD (two registers: 2000 rows of 40 / 8
+// heads 31.4 us at five, 30.2 at six).
 template <int HD, bool I8, bool VEC, typename T>
-__global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, const T *q, int64_t q_stride, T *q_out,
-                                                int H, const T *kx, int64_t k_stride, const T *vx, int64_t v_stride,
-                                                int n_rot) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 && I8 && VEC && sizeof(T) == 4 ? 6 : 1)))
+void k_append(Cache c, Rows s, Turns turns, const T *q, int64_t q_stride, T *q_out, int H, const T *kx, int64_t k_stride,
+              const T *vx, int64_t v_stride, int n_rot) {
     // Lanes of a row, rows of a step, steps; pairs of a lane are VEC ? 4 : 1 wide.
     constexpr int LPR = HD / 8, RPS = 64 / LPR, ST = BLK / RPS;
     extern __shared__ double2 cs[];              // [BLK][n_rot / 2]
@@ -345,7 +347,7 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
         for (int i = 0; i < ST; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                // (In 32 bits, which is as good for a maximum and holds no 64-bit values till below.)
+                // (In 32 bits, which holds no 64-bit values till below.)
                 const int row = i * RPS + lr, j = j0 + e;
                 float a = to_f32<T>(x0[i][e]), z = to_f32<T>(x1[i][e]);
                 if (turn && j < half && row < n) {
@@ -358,16 +360,25 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
                 top = fmaxf(top, fmaxf(fabsf(a), fabsf(z)));
                 nan |= a != a || z != z;
             }
+        const float mine = top;
         top = wave_max(top);
-        const uint32_t bits = __float_as_uint(top);
-        int ex = (int)(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u);   // 127 2^ex holds top
+        // 127 2^ex holds top.  A turned key's is off by three roundings of its pair's larger
+        // element, 1.5 times top at most: 5 steps of 32 bits.  So with one of them near the
+        // border the lesser exponent is taken here, and looked at again in 64 bits behind the codes.
+        const uint32_t bits = __float_as_uint(top), frac = bits & 0x7fffffu;
+        const bool near = is_k && frac - (0x7e0000u - 32) <= 64u && __any(j0 < half && __float_as_uint(mine) >= bits - 64);
+        int ex = (int)(bits >> 23) - 127 - 6 + (frac > 0x7e0000u && !near);
         ex = min(max(ex, EXP_MIN), EXP_MAX);
         nan = __any(nan);
+        int ex0 = EXP_MIN;
         if (off) {
-            // The rows before these keep their codes, or take the greater step.
             nan |= had == EXP_NAN;
-            const int ex0 = min(max(had - EXP_BIAS, EXP_MIN), EXP_MAX);
-            if (ex > ex0) {
+            ex0 = min(max(had - EXP_BIAS, EXP_MIN), EXP_MAX);
+            ex = max(ex, ex0);
+        }
+        // The exponent, and the rows before these: they keep their codes, or take the greater step.
+        auto settle = [&] {
+            if (off && ex > ex0) {
                 const float f = __uint_as_float((uint32_t)(127 + ex0 - ex) << 23);
                 for (int i = lane; i < off * (HD / 4); i += 64) {
                     i8x4 o = ((const i8x4 *)y)[i];
@@ -376,11 +387,13 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
                     ((i8x4 *)y)[i] = o;
                 }
             }
-            ex = max(ex, ex0);
-        }
-        if (lane == 0) *xp = nan ? EXP_NAN : (uint8_t)(ex + EXP_BIAS);
-        const double inv = __longlong_as_double((long long)(1023 - ex) << 52);
-        auto code = [&](double x) { return (int8_t)(int)fmin(fmax(rint(x * inv), -127.0), 127.0); };
+            if (lane == 0) *xp = nan ? EXP_NAN : (uint8_t)(ex + EXP_BIAS);
+        };
+        if (!near) settle();
+        auto code = [](double x, int ex) {
+            const double inv = __longlong_as_double((long long)(1023 - ex) << 52);
+            return (int8_t)(int)fmin(fmax(rint(x * inv), -127.0), 127.0);
+        };
 #pragma unroll
         for (int i = 0; i < ST; i++) {
             const int row = i * RPS + lr;
@@ -390,11 +403,35 @@ __global__ __launch_bounds__(256) void k_append(Cache c, Rows s, Turns turns, co
             for (int e = 0; e < 4; e++) {
                 double a, z;
                 turned(i, e, a, z);
-                a4[e] = code(a);
-                z4[e] = code(z);
+                a4[e] = code(a, ex);
+                z4[e] = code(z, ex);
             }
             put(y + (off + row) * HD, a4, z4);
         }
+        if (!near) return;
+        // (The rows read once more: rare, and done without the registers that hold them.)
+        auto pairs = [&](auto f) {
+#pragma unroll 1
+            for (int row = lr; row < n; row += RPS)
+#pragma unroll 2
+                for (int e = 0; e < 4; e++) {
+                    const T *x = kx + (r + row) * k_stride + (int64_t)h * HD;
+                    int d0, d1;
+                    dims(e, d0, d1);
+                    const double o = to_f32<T>(x[d0]), u = to_f32<T>(x[d1]);
+                    const double2 w = j0 + e < half ? cs[row * half + j0 + e] : double2{1., 0.};
+                    f((off + row) * HD + d0, o * w.x - u * w.y);
+                    f((off + row) * HD + d1, o * w.y + u * w.x);
+                }
+        };
+        bool more = false;
+        const double most = 127. * __longlong_as_double((long long)(1023 + ex) << 52);
+        pairs([&](int, double x) { more |= fabs(x) > most; });
+        if (__any(more) && ex < EXP_MAX) {
+            ex++;
+            pairs([&](int at, double x) { y[at] = code(x, ex); });
+        }
+        settle();
     }
 }
 
