@@ -58,6 +58,9 @@ int gd_prefill_scratch_attach(gd_ctx *ctx);
 int gd_fail(gd_ctx *ctx, int code, const char *fmt, ...);
 // Grow-only context workspace of at least `bytes`; valid until the next call.
 int gd_ctx_workspace(gd_ctx *ctx, size_t bytes, void **out);
+// Grows it to `bytes` if it can be, for a call that can do with less: without the memory, or
+// inside a recording, it stays as it is, and that is no failure.
+void gd_ctx_workspace_grow(gd_ctx *ctx, size_t bytes);
 // Map a HIP error to a GD code with a message naming `what`.
 int gd_hip_fail(gd_ctx *ctx, hipError_t e, const char *what);
 // Matrix-core GEMV (checked by the caller); ksplit > 1 writes K-split partial

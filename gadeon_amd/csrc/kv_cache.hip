@@ -1493,16 +1493,20 @@ int check_seqs(gd_ctx *ctx, const char *fn, const gd_seqs *s) {
 }
 
 // Memory for the partials of ns key splits, `bytes` each: the attention scratch where it
-// holds them, else the context's workspace, up to WS_BYTES; ns becomes what there is memory
-// for (1: none needed).  A recording takes the workspace as it is.
+// holds them, else the context's workspace, which may grow to WS_BYTES, by powers of two so
+// that batches that grow seldom do it; ns becomes what there is memory for (1: none needed).
+// A recording takes the workspace as it is.
 constexpr size_t WS_BYTES = 256u << 20;
 int split_scratch(gd_ctx *ctx, size_t bytes, int64_t &ns, float **scratch) {
     size_t most = GD_ATTN_SCRATCH_BYTES;
     void *p = nullptr;
-    if (ns > 1 && ns * bytes > most) {
-        const size_t want = std::min<size_t>(ns * bytes, std::max(bytes, WS_BYTES / bytes * bytes));
-        const size_t have = ctx->recording ? std::min(want, ctx->ws_bytes) : want;
-        if (have / bytes > most / bytes && have / bytes > 1) {
+    if (ns > 1 && ns * bytes > most && 2 * bytes <= WS_BYTES) {
+        const size_t want = std::min<size_t>(ns * bytes, WS_BYTES / bytes * bytes);
+        size_t room = 2 * most;
+        while (room < want) room *= 2;
+        if (ctx->ws_bytes < want) gd_ctx_workspace_grow(ctx, room);
+        const size_t have = std::min(want, ctx->ws_bytes);
+        if (have / bytes > std::max<size_t>(1, most / bytes)) {
             const int rc = gd_ctx_workspace(ctx, have, &p);
             if (rc) return rc;
             most = have;

@@ -142,6 +142,17 @@ int gd_ctx_workspace(gd_ctx *ctx, size_t bytes, void **out) {
     return GD_OK;
 }
 
+void gd_ctx_workspace_grow(gd_ctx *ctx, size_t bytes) {
+    if (ctx->recording || ctx->ws_bytes >= bytes) return;
+    gd_buf *b = gd_buf_new(bytes);
+    if (!b) return;
+    // Work enqueued on the stream may still use the one before.
+    if (ctx->ws) (void)hipStreamSynchronize(ctx->stream);
+    gd_buf_drop(ctx->ws);
+    ctx->ws = b;
+    ctx->ws_bytes = bytes;
+}
+
 float *gd_attn_scratch(gd_ctx *ctx) {
     if (!ctx->recording) return ctx->attn ? (float *)ctx->attn->p : nullptr;
     if (!ctx->rec_attn) ctx->rec_attn = gd_buf_new(GD_ATTN_SCRATCH_BYTES);

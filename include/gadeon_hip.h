@@ -469,8 +469,9 @@ int gd_kv_read(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, void *k_out, v
  * sums.  A NaN or infinity in the cache reaches only the rows that see it, which
  * are then not to be relied on.  Two launches where the keys are split; partials go to
  * the context's or the recording's scratch as gd_attn_paged's, or, where that would
- * bound the splits, to the context workspace, which the call may grow to 256 MiB (a
- * recording takes it as it is, with fewer splits).  Sums are formed in a fixed order for
+ * bound the splits, to the context workspace, which the call may grow to 256 MiB (where
+ * there is no memory for that, and in a recording, it is taken as it is, with fewer
+ * splits).  Sums are formed in a fixed order for
  * the same lengths of all the call's sequences and the same max_len; others may split a
  * row's keys elsewhere and round its last bits otherwise.  MetalEnc.attnPaged and
  * attnBatch (MetalEnc.swift:679-706, 966-1025), the latter's window included. */
