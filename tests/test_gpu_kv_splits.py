@@ -1,12 +1,13 @@
-"""gd_kv_attn where keys are split and merged: results in the place of q or of the
-gate, bit for bit those of a buffer of their own (which test_gpu_kv_cache.py's 64-bit
-statement holds), for each merge: few rows and many, tokens and chunks, head counts
-that fill its groups of heads and ones that do not."""
+"""gd_kv_attn where keys are split and merged, against the statement in 64 bits of
+test_gpu_kv_cache.py: results in the place of q or of the gate, bit for bit those of a
+buffer of their own, for each merge (few rows and many, tokens and chunks, head
+counts that fill its groups of heads and ones that do not); up to the most splits and
+past them; and a cache of halves in pages of whole tiles, at every length."""
 import numpy as np
 import pytest
 
 import gadeon_amd as ga
-from test_gpu_kv_cache import Batch, attend, bound, raw, rows_of
+from test_gpu_kv_cache import ATTN, Batch, attend, bound, check_attention, raw, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +49,39 @@ def test_in_place_of_split_keys(ctx, dtype, x16, hd, H, hkv, which):
         ctx.gd_kv_attn(*bt.ref, dq, row, dg, row, dq, x, H, scale, 0, 0)
         got = ctx.get(dq, q.shape, q.dtype)
         assert np.array_equal(got[done], out[done]) and np.array_equal(got[~done], q[~done])
+
+
+# Blocks of 32 keys (chunks of head dim 128: 64) of a long sequence, at least 8 (4 of head dim 256,
+# 4 of chunks) a split, 64 splits at most: 24 to 47 splits at 6000 positions, 32 to 64 at 10000,
+# 64 of more blocks each at 20000.
+@pytest.mark.parametrize("cache,page", [(ga.I8, 16), (ga.F16, 16), (ga.F16, 20)], ids=["i8", "f16", "f16odd"])
+@pytest.mark.parametrize("hd,H,hkv", [(128, 5, 1), (128, 8, 2), (256, 6, 1), (256, 12, 2)])
+@pytest.mark.parametrize("T", [6000, 10000, 20000])
+@pytest.mark.parametrize("rows", [0, 3], ids=["token", "chunk"])
+def test_most_splits(ctx, cache, page, hd, H, hkv, T, rows):
+    check_attention(ctx, [(T, max(rows, 1))], cache, hd == 256, hd, H, hkv, page, 0, 0, True, seed=T, row_start=rows > 0)
+
+
+@pytest.mark.parametrize("cache", [ga.I8, ga.F16], ids=["i8", "f16"])
+@pytest.mark.parametrize("x16,hd,H", [(False, 128, 8), (True, 256, 6)])
+def test_most_splits_of_many_rows(ctx, cache, x16, hd, H):
+    """Over 1024 rows and heads in 50 splits or more of a long sequence, a short one beside it."""
+    check_attention(ctx, [(17000, 1024 // H + 1), (3, 40)], cache, x16, hd, H, 1, 16, 0, 0, True)
+
+
+@pytest.mark.parametrize("x16", [False, True], ids=["f32rows", "f16rows"])
+@pytest.mark.parametrize("hd,H,hkv", [(128, 40, 8), (128, 3, 3), (256, 24, 4), (256, 18, 1)])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("which", list(ATTN))
+def test_pages_of_whole_tiles_of_halves(ctx, x16, hd, H, hkv, page, which):
+    check_attention(ctx, ATTN[which], ga.F16, x16, hd, H, hkv, page, 0, 0, H != 3, seed=hd + H,
+                    row_start=not which.startswith("tok"))
+
+
+@pytest.mark.parametrize("x16", [False, True], ids=["f32rows", "f16rows"])
+@pytest.mark.parametrize("which", list(ATTN))
+@pytest.mark.parametrize("window,sinks", [(1, 0), (40, 0), (100, 5), (64, 130), (1000, 1), (1 << 30, 3)])
+def test_windows_over_pages_of_whole_tiles_of_halves(ctx, x16, which, window, sinks):
+    for hd, H, hkv in ((128, 10, 2), (256, 6, 1)):
+        check_attention(ctx, ATTN[which], ga.F16, x16, hd, H, hkv, 32, window, sinks, x16, seed=window,
+                        row_start=not which.startswith("tok"))
