@@ -535,8 +535,8 @@ __device__ __forceinline__ KeyBlocks<32> token_blocks(const Rows &s, const Mask 
 // From an even share of all blocks a slot, to what lets the splits have a slot each, those
 // of half as many blocks or fewer a part of one, their start counted as two blocks, as they
 // come last and fill the gaps (unit_at; 64 tokens of up to 8192 positions 41 us, a slot for
-// each 59; a mixed batch of prompt chunks 115 and 197; the long ones first 38 and 117, 32
-// chunks of up to 200 behind 2500, 24 heads of 256 on 4, 107 -> 94, 16 of them 64 -> 71);
+// each 59; a mixed batch of prompt chunks 115 and 197; the long ones' workgroups first: 37 and
+// 115, k_attn_tokens, k_attn_rows);
 // blocks(b, n, u): n blocks in each of sequence b's u units.  Over 64 sequences fill the chip
 // as they are, and the even share is left (200 tokens of up to 6000 positions, 40 heads of
 // 128 on 8: 92 us, fitted 107).
@@ -615,7 +615,9 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
     int n = blockIdx.x / groups, sp = 0, ns = 1, pos;
     if (most > 1) {
         // The rows' splits one after the other, long rows' first, so that the workgroups that
-        // have none come last.
+        // have none come last.  (us in any order / border at 0.25 / 0.5 / 0.75: 64 of up to 8192,
+        // codes, 40 heads of 128 on 8, 41 / 37 / 37 / 39, halves 62 / 56 / 57 / 56, 24 of 256 on 4
+        // 71 / 64 / 64 / 73; 32 of up to 3000, halves, 19.7 / 19.9 / 18.6 / 18.5.)
         const int least = token_least(s, mask, groups, slots, token_fewest(HD));
         auto splits = [&](const Seq &q) { return q.r1 > q.r0 ? token_blocks(s, mask, q.pos).splits(most, least) : 0; };
         Seq sq;
@@ -990,7 +992,11 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     int b, k, nz = 1;
     // The sequences' units one after the other, each in its splits, so that the workgroups
     // that have none come last; the long sequences first, and of each the units that see the
-    // most keys.
+    // most keys.  Borders of the three classes in blocks of a split, us of one class / 0.7 and
+    // 0.3 / 0.5 and 0.2 / 0.35 and 0.1: chunks of up to 200 f16 rows, codes of 24 heads of 256
+    // on 4, 16 behind 1500 65 / 57 / 54 / 54, behind 2500 64 / 61 / 70 / 62, behind 5000 91 / 82 /
+    // 82 / 82; 32 of them 81 / 76 / 78 / 79, 109 / 95 / 94 / 95, 145 / 124 / 124 / 124; 20 of f32
+    // rows behind 5000 115 / 119 / 118 / 115, 32 on halves 156 / 136 / 128 / 126.
     const int least = most > 1 ? unit_least<PC, AK>(s, mask, G, c.HKV, slots) : 0;
     auto units = [&](const Seq &q) {
         const Units<PC, AK> u(q, G, s.cap);
@@ -1000,7 +1006,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     auto order = [&](const Seq &q) {
         const Units<PC, AK> u(q, G, s.cap);
         const int n = u.rows > 0 ? u.blocks(mask, u.n() - 1).n : 0;
-        return n > 0.5f * least ? 0 : n > 0.2f * least ? 1 : 2;
+        return n > 0.35f * least ? 0 : n > 0.1f * least ? 1 : 2;
     };
     if (!unit_at<3>(s, blockIdx.x / c.HKV, units, order, b, k, sq)) return;
     const Units<PC, AK> un(sq, G, s.cap);
