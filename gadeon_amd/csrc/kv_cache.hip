@@ -1746,13 +1746,18 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     // 1.8 183 / 196.
     bool whole;
     if (tokens)
-        // f16 tokens on codes, us whole / split: one of 20 blocks 11.7 / 12.1 (heads of 256 18 /
-        // 14), 32 of up to 20 blocks 12.2 / 15.2, of 34 under a window 17.9 / 21.7, of up to 47
-        // 20.5 / 15.0.  Tokens of up to 6000 positions: 200 of 8 kv heads (3.1 times the slots) 118 /
-        // 99, 500 213 / 250, 1500 456 / 653; 500 of 4 (3.9 times) 248 / 244.  Past 1024 blocks a
-        // long one of them would be the call's time.
-        whole = blocks <= 4 * TW || (blocks <= 9 * TW && wgs >= cus) || (blocks <= 256 * TW && wgs >= 4 * slots) ||
-                wgs >= 16 * slots;
+        // f16 tokens on codes, us whole / split, 40 heads of 128 on 8 (24 of 256 on 4): one of 13
+        // blocks 10.2 / 12.0 (15.8 / 14.0), of 18 11.5 / 12.0 (17.8 / 14.0), of 25 14.0 / 11.9.
+        // Of 34 blocks under a window, lengths alike / up to 16000, by workgroups: 128 17.7 / 18.3
+        // and 17.5 / 15.0; 192 18.3 / 22.6 and 17.7 / 16.8; 248 19.0 / 22.7 and 17.9 / 19.4; 256 19.3 /
+        // 22.9 and 17.9 / 18.5; f32 rows on halves of 192 23.4 / 30.9 and 16.5 / 18.1 (heads of 256,
+        // codes: 192 31.2 / 35.0 and 28.3 / 25.8; 252 35.9 / 38.7 and 28.5 / 31.3; halves of 192 45.7 /
+        // 48.8 and 37.8 / 39.2).  Of 38 and 256 workgroups 19.6 / 23.1 and 18.5 / 15.1.
+        //   Tokens of up to 6000 positions: 200 of 8 kv heads (3.1 times the slots) 118 / 99, 500 213 /
+        // 250, 1500 456 / 653; 500 of 4 (3.9 times) 248 / 244.  Past 1024 blocks a long one of them
+        // would be the call's time.
+        whole = blocks <= (hd == 128 ? 5 : 4) * TW || (blocks <= 9 * TW && 8 * wgs >= (hd == 128 ? 6 : 7) * cus) ||
+                (blocks <= 256 * TW && wgs >= 4 * slots) || wgs >= 16 * slots;
     else
         whole = blocks <= 10 || (blocks <= 24 && blocks * (slots - wgs) <= 8 * slots) ||
                 (blocks <= 128 && 2 * wgs >= 3 * slots) || wgs >= 4 * slots;

@@ -1,0 +1,34 @@
+"""Where gd_kv_attn splits its rows' keys and where it leaves them whole, next to the borders, on
+the CPU: the number of splits that it launches with, through the stand-in for the HIP runtime."""
+import pytest
+
+from test_kv_cache_memory import run
+
+BODY = r"""
+def splits(rows, positions, tokens, hd=128, hkv=8, window=0, n_seq=None, dtype=ga.I8, heads=2):
+    kv = ga.KV(k=P, v=P, k_exp=P, v_exp=P, n_pages=10, dtype=dtype, n_head_kv=hkv, head_dim=hd, page_size=16)
+    s = ga.Seqs(n_rows=rows, row_start=None if tokens else P, pos=P, rope_shift=None, page_table=P,
+                n_seq=rows if tokens else n_seq, max_pages=2000, max_len=positions)
+    i("launches").value = 0
+    H = heads * hkv
+    ctx.gd_kv_attn(kv, s, P, H * hd, None, 0, P + (1 << 32), ga.F32, H, 0.1, window, 4)
+    n = i("splits").value
+    assert i("launches").value == (2 if n > 1 else 1)
+    return n
+ctx = ga.Context(0)
+"""
+
+
+def test_tokens(tmp_path):
+    """(256 CUs: the stand-in tells none, and that is what is taken.)"""
+    run(tmp_path, BODY + r"""
+# few blocks of 32 keys are left whole: 20 at head dim 128, 16 at 256
+assert splits(1, 640, True) == 1 < splits(1, 641, True)
+assert splits(1, 512, True, hd=256) == 1 < splits(1, 513, True, hd=256)
+# up to 36 where the workgroups fill three quarters of the CUs, or seven eighths
+assert splits(24, 1152, True) == 1 < splits(23, 1152, True) and splits(24, 1153, True) > 1
+assert splits(31, 16000, True, window=1024) == 1 < splits(16, 16000, True, window=1024)
+assert splits(56, 1152, True, hd=256, hkv=4) == 1 < splits(55, 1152, True, hd=256, hkv=4)
+# any of a full chip's, times over
+assert splits(256, 30000, True) == 1 < splits(255, 30000, True)
+""")
