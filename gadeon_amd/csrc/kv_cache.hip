@@ -1741,9 +1741,14 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
     const int64_t slots = (tokens && hd == 256 && kv->dtype == GD_F16 ? 1 : 2) * cus, wgs = units * groups;    // (k_attn_tokens' registers)
     // Rows' partials cost a full chip some 15 us, and a split saves what lets the workgroups
     // fill it; but the longest row may be one of a few, which split share the chip.  f16 rows on
-    // codes, us whole / split: 10 blocks 28 / 31; 12 on a fifth of the slots 38 / 35, on 0.6 of
-    // them 44 / 46; 24 on 0.7 56 / 57, on all 57 / 64; 64 on 0.7 123 / 89, on 1.2 127 / 90, on
-    // 1.8 183 / 196.
+    // codes, us whole / split, 40 heads of 128 on 8 (24 of 256 on 4): 10 blocks 28 / 31; 12 of 96
+    // workgroups, lengths alike 33 / 32 (29 / 30) and mixed 32 / 22 (28 / 20), of 240 34 / 39 (30 / 38)
+    // and 33 / 29 (29 / 25); 19 of 240 47 / 46 (41 / 44) and 45 / 25 (39 / 25), of 288 55 / 61 (48 / 54)
+    // and 45 / 27 (39 / 24), of 480 58 / 64 (51 / 59) and 46 / 29 (40 / 27); 24 of 384 67 / 73 (58 / 65)
+    // and 54 / 30 (47 / 28); 64 of 360 123 / 89, of 620 127 / 90, of 930 183 / 196.  Under a window
+    // lengths count alike: 15 blocks of 156 to 208 workgroups, f32 rows on halves, 39 / 38 to 43,
+    // codes 36 / 33 to 39, of 224 and more 39 / 44 to 46 and 36 / 40; 13 of 184 35.5 / 35.2, 17 of 216
+    // 41 / 38, of 232 41 / 45.
     bool whole;
     if (tokens)
         // f16 tokens on codes, us whole / split, 40 heads of 128 on 8 (24 of 256 on 4): one of 13
@@ -1759,7 +1764,7 @@ extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const 
         whole = blocks <= (hd == 128 ? 5 : 4) * TW || (blocks <= 9 * TW && 8 * wgs >= (hd == 128 ? 6 : 7) * cus) ||
                 (blocks <= 256 * TW && wgs >= 4 * slots) || wgs >= 16 * slots;
     else
-        whole = blocks <= 10 || (blocks <= 24 && blocks * (slots - wgs) <= 8 * slots) ||
+        whole = blocks <= 10 || (blocks <= 24 && blocks * (slots - wgs) <= (window ? 9 : 8) * slots) ||
                 (blocks <= 128 && 2 * wgs >= 3 * slots) || wgs >= 4 * slots;
     const int least = tokens ? token_fewest(hd) : ROWS_FEWEST;
     int64_t ns = whole ? 1 : std::min<int64_t>((blocks + least - 1) / least, MAX_SPLITS);

@@ -32,3 +32,18 @@ assert splits(56, 1152, True, hd=256, hkv=4) == 1 < splits(55, 1152, True, hd=25
 # any of a full chip's, times over
 assert splits(256, 30000, True) == 1 < splits(255, 30000, True)
 """)
+
+
+def test_rows(tmp_path):
+    """A unit is 128 columns (64 at head dim 256), a workgroup one of a kv head, a block 64 keys (32)."""
+    run(tmp_path, BODY + r"""
+chunks = lambda n, positions, window=0, hd=256: splits(16 * n, positions, False, hd=hd, hkv=4, window=window, n_seq=n, heads=4)
+# 16 rows of 4 heads: a unit each, and one a sequence besides
+assert chunks(60, 320) == 1 < chunks(4, 321)               # 10 blocks
+assert chunks(30, 480) == 1 < chunks(29, 480)              # 15 blocks from 240 workgroups on
+assert chunks(26, 16000, 400) == 1 < chunks(25, 16000, 400)               # .. under a window from 208
+assert chunks(24, 0, 0) > 1                                # no bound known: the tables' 32000 positions
+assert chunks(42, 768) > 1 and chunks(43, 768) == 1        # 24 blocks: 344
+assert chunks(95, 769) > 1 and chunks(96, 769) == 1        # up to 128: 768
+assert chunks(96, 4097) > 1 and chunks(256, 4097) == 1     # 2048
+""")
