@@ -391,9 +391,10 @@ int gd_attn_batch(gd_ctx *ctx, const float *q, const uint16_t *k_cache,
  * Planes are 16-byte aligned device memory, from gd_kv_alloc or the caller's own.
  *
  * gd_seqs: the rows of a call and where they belong.  Sequence b has the rows
- * row_start[b] .. row_start[b+1]-1 (row_start ascending, [n_seq + 1]; null: one
- * row each, n_rows == n_seq), at the positions pos[b], pos[b]+1, ..; position p is
- * at slot p % page_size of page page_table[b][p / page_size].  All four arrays are
+ * row_start[b] .. row_start[b+1]-1 (row_start ascending, [n_seq + 1], n_seq at most
+ * 65536, which the kernels walk: some hundreds are what it is meant for; null: one row
+ * each, n_rows == n_seq), at the positions pos[b], pos[b]+1, ..; position p is at slot
+ * p % page_size of page page_table[b][p / page_size].  All four arrays are
  * device memory read by the kernels, so a recorded graph may be replayed on
  * changed positions, rows and tables.  A sequence with a negative pos is idle: its
  * rows are not touched, and neither are rows that no sequence has (before

@@ -47,3 +47,15 @@ assert chunks(42, 768) > 1 and chunks(43, 768) == 1        # 24 blocks: 344
 assert chunks(95, 769) > 1 and chunks(96, 769) == 1        # up to 128: 768
 assert chunks(96, 4097) > 1 and chunks(256, 4097) == 1     # 2048
 """)
+
+
+@pytest.mark.parametrize("entry", ["append", "read", "attn"])
+def test_more_ragged_sequences_than_are_walked(entry):
+    import test_kv_cache_args as args
+    call = getattr(args, entry)
+    args.refused(call(s=args.seqs(n_rows=70000, n_seq=65537)), "65537 sequences with row_start (65536 at most)")
+    args.refused(call(s=args.seqs(n_rows=6, n_seq=2**31 - 1)), "65536 at most")
+    before = args.ga.load().gd_last_error(None)
+    kw = {"append": dict(q=None, q_out=None), "read": {}, "attn": dict(q=args.P, out=args.P, gate=None)}[entry]
+    for s in (args.seqs(n_rows=70000, n_seq=65536), args.seqs(n_rows=70000, n_seq=70000, row_start=None)):
+        assert call(s=s, **kw) == args.ga.GD_EINVAL and args.ga.load().gd_last_error(None) == before   # the context alone
