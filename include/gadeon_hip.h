@@ -466,8 +466,10 @@ int gd_kv_read(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, void *k_out, v
  * n_head_kv), times sigmoid(gate[h]) where gate is not null; zeros where it sees no
  * position.  q, gate and out have x_dtype (GD_F32 or GD_F16), out contiguous rows, all
  * 16-byte aligned, row strides (in elements) too; out may be q or gate.  f32 rows
- * are worked as f16 hi + lo pairs (about 22 bits), f16 ones in f16 products with f32
- * sums.  A NaN or infinity in the cache reaches only the rows that see it, which
+ * and their weights are worked as f16 hi + lo pairs (about 22 bits), with f32 sums; f16
+ * rows as they are, their weights as pairs in single tokens (row_start null) and rounded
+ * to f16 (11 bits) in chunks, so that one row's result may differ by about its own
+ * rounding between the two.  A NaN or infinity in the cache reaches only the rows that see it, which
  * are then not to be relied on.  Two launches where the keys are split; partials go to
  * the context's or the recording's scratch as gd_attn_paged's, or, where that would
  * bound the splits, to the context workspace, which the call may grow to 256 MiB (where
