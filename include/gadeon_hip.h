@@ -399,7 +399,7 @@ int gd_attn_batch(gd_ctx *ctx, const float *q, const uint16_t *k_cache,
  * changed positions, rows and tables.  A sequence with a negative pos is idle: its
  * rows are not touched, and neither are rows that no sequence has (before
  * row_start[0], from row_start[n_seq] on).  A table entry outside [0, n_pages),
- * and a position past max_pages * page_size, is a page that is not there: rows for
+ * and a position past max_pages * page_size or 2^31 - 2, is a page that is not there: rows for
  * it are not kept and its keys are not seen (so a program with a window may drop
  * pages that left it).  Sequences may share pages that are only read; no two rows of
  * an append may name the same slot, and of an 8-bit cache no two sequences the same
