@@ -919,11 +919,11 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
 // 2^8), f16 rows as they are, with weights rounded to f16 and summed as rounded: 2^-11 of a
 // weight at most, as the result's own rounding, and less of a sum of many (errors against 64 bits
 // 2.6e-4 of the result's norm, with weights as pairs 2.1e-4, the result's rounding alone; in us
-// without / with pairs: the first two below 73 / 87 and 134 / 157, 1024 rows after 3000 of codes 144 / 163 and of
-// heads of 256 221 / 243).  k_attn_tokens, which memory bounds, takes them as pairs.  The gate of
-// f16 rows is a hardware reciprocal of 1 + 2^x: two roundings of 32 bits.  A tile that some column does not see whole goes key by key: a
-// mask, and where V holds a NaN or infinity its finite part and, apart, which columns see
-// the others (0 x NaN would reach them all).
+// without / with pairs: the first two below 73 / 87 and 134 / 157, 1024 rows after 3000 of codes
+// 144 / 163 and of heads of 256 221 / 243).  k_attn_tokens, which memory bounds, takes them as
+// pairs.  The gate of f16 rows is a hardware reciprocal of 1 + 2^x: two roundings of 32 bits.  A
+// tile that some column does not see whole goes key by key: a mask, and where V holds a NaN or
+// infinity its finite part and, apart, which columns see the others (0 x NaN would reach them all).
 //   512 f16 rows behind 3584 positions of codes, 40 heads of 128 on 8: 67 us, 600 TFLOP/s;
 // 4096 under a window of 1024 133 us, 570; f32 rows (twice the products) of 24 heads of 256
 // on 4 530.  No unit of the CU is full (matrix cores 31% busy, vector ALUs 50%, LDS 31%):

@@ -398,9 +398,9 @@ int gd_attn_batch(gd_ctx *ctx, const float *q, const uint16_t *k_cache,
  * device memory read by the kernels, so a recorded graph may be replayed on
  * changed positions, rows and tables.  A sequence with a negative pos is idle: its
  * rows are not touched, and neither are rows that no sequence has (before
- * row_start[0], from row_start[n_seq] on).  A table entry outside [0, n_pages),
- * and a position past max_pages * page_size or 2^31 - 2, is a page that is not there: rows for
- * it are not kept and its keys are not seen (so a program with a window may drop
+ * row_start[0], from row_start[n_seq] on).  A table entry outside [0, n_pages), and a
+ * position past max_pages * page_size or 2^31 - 2, is a page that is not there: rows
+ * for it are not kept and its keys are not seen (so a program with a window may drop
  * pages that left it).  Sequences may share pages that are only read; no two rows of
  * an append may name the same slot, and of an 8-bit cache no two sequences the same
  * block.  Arguments are checked before the context: gd_last_error(NULL) tells what is
@@ -469,14 +469,14 @@ int gd_kv_read(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, void *k_out, v
  * and their weights are worked as f16 hi + lo pairs (about 22 bits), with f32 sums; f16
  * rows as they are, their weights as pairs in single tokens (row_start null) and rounded
  * to f16 (11 bits) in chunks, so that one row's result may differ by about its own
- * rounding between the two.  A NaN or infinity in the cache reaches only the rows that see it, which
- * are then not to be relied on.  Two launches where the keys are split; partials go to
- * the context's or the recording's scratch as gd_attn_paged's, or, where that would
- * bound the splits, to the context workspace, which the call may grow to 256 MiB (where
- * there is no memory for that, and in a recording, it is taken as it is, with fewer
- * splits).  Sums are formed in a fixed order for
- * the same lengths of all the call's sequences and the same max_len; others may split a
- * row's keys elsewhere and round its last bits otherwise.  MetalEnc.attnPaged and
+ * rounding between the two.  A NaN or infinity in the cache reaches only the rows that
+ * see it, which are then not to be relied on.  Two launches where the keys are split;
+ * partials go to the context's or the recording's scratch as gd_attn_paged's, or, where
+ * that would bound the splits, to the context workspace, which the call may grow to 256
+ * MiB (where there is no memory for that, and in a recording, it is taken as it is, with
+ * fewer splits).  Sums are formed in a fixed order for the same lengths of all the call's
+ * sequences, the same max_len and the same memory for partials; others may split a row's
+ * keys elsewhere and round its last bits otherwise.  MetalEnc.attnPaged and
  * attnBatch (MetalEnc.swift:679-706, 966-1025), the latter's window included. */
 int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const void *q, int64_t q_stride,
                const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
