@@ -41,6 +41,11 @@ class Seqs(C.Structure):
                 ("page_table", _vp), ("n_seq", _i), ("max_pages", _i), ("max_len", _i)]
 
 
+class Scores(C.Structure):
+    """How attention scores are made and masked, arrays in device memory (gd_scores)."""
+    _fields_ = [("cap", _f), ("window", _i), ("n_sink", _i), ("slope", _vp), ("first", _vp), ("prefix", _vp)]
+
+
 class StackConfig(C.Structure):
     _fields_ = [(n, _i) for n in ("n_layer", "n_embd", "n_ff", "n_head", "n_head_kv", "head_dim",
                                   "n_rot")] + [("rope_base", _f), ("eps", _f)] + \
@@ -49,7 +54,7 @@ class StackConfig(C.Structure):
 
 
 _Q2WP = C.POINTER(Q2W)
-_KVP, _SEQSP = C.POINTER(KV), C.POINTER(Seqs)
+_KVP, _SEQSP, _SCORESP = C.POINTER(KV), C.POINTER(Seqs), C.POINTER(Scores)
 
 # name -> (restype, argtypes)
 _PROTOS = {
@@ -103,6 +108,7 @@ _PROTOS = {
                                _f]),
     "gd_kv_read": (_i, [_vp, _KVP, _SEQSP, _vp, _vp, _i]),
     "gd_kv_attn": (_i, [_vp, _KVP, _SEQSP, _vp, _i64, _vp, _i64, _vp, _i, _i, _f, _i, _i]),
+    "gd_kv_attn_scored": (_i, [_vp, _KVP, _SEQSP, _vp, _i64, _vp, _i64, _vp, _i, _i, _f, _SCORESP]),
     "gd_gdn_gate": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64]),
     "gd_gdn_conv": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i64]),
     "gd_l2norm_rows": (_i, [_vp, _vp, _i, _i, _i64, _i64, _f]),

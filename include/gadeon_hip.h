@@ -482,6 +482,29 @@ int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const void *q,
                const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
                int window, int n_sink);
 
+/* How gd_kv_attn_scored makes scores and masks them; arrays in device memory, so that a
+ * recorded graph may be replayed on changed ones. */
+typedef struct gd_scores {
+    float cap;                   /* > 0 (1e-30 .. 1e30): a score s becomes cap tanh(s / cap); 0: stays */
+    int window, n_sink;          /* as gd_kv_attn's */
+    const float *slope;          /* [n_head] or null: slope[h] |p - t| is taken off the (capped) score of
+                                    the query at position p and the key at t */
+    const int32_t *first;        /* [n_rows] or null: a row sees no position before first[row] (where its
+                                    document starts; one past its own position, as INT32_MAX: it sees none) */
+    const int32_t *prefix;       /* [n_seq] or null: every row of sequence b sees the positions t <
+                                    prefix[b], those behind its own too, as far as the sequence has them with
+                                    this call's rows, and whatever the window */
+} gd_scores;
+
+/* gd_kv_attn with the scores and masks of `scores`: the row at position p of sequence b sees
+ * t >= first[row] where t <= p and (window == 0, t > p - window or t < n_sink), or t <
+ * prefix[b]; out[h] = softmax(score) . v, gated, zeros where it sees nothing.  In all else as
+ * gd_kv_attn (and its very results where cap is 0 and the arrays are null): rows, types,
+ * alignment, workspace, recording.  A cap's tanh is formed to some 2^-22 of itself for f32 rows. */
+int gd_kv_attn_scored(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const void *q, int64_t q_stride,
+                      const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
+                      const gd_scores *scores);
+
 /* ---- GDN recurrence -----------------------------------------------------------
  * State S[nV][dS][dS] f32, key-major: S[h][i*dS + j], i = key, j = value
  * (GDN.swift:9-16, Kernels.metal:1225).  Head map hk = hv % nK
