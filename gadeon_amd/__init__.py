@@ -46,6 +46,11 @@ class Scores(C.Structure):
     _fields_ = [("cap", _f), ("window", _i), ("n_sink", _i), ("slope", _vp), ("first", _vp), ("prefix", _vp)]
 
 
+class KVPages(C.Structure):
+    """Who holds which page of the caches, arrays in device memory (gd_kv_pages)."""
+    _fields_ = [("refs", _vp), ("table", _vp), ("n_pages", _i64), ("n_seq", _i), ("max_pages", _i), ("page_size", _i)]
+
+
 class StackConfig(C.Structure):
     _fields_ = [(n, _i) for n in ("n_layer", "n_embd", "n_ff", "n_head", "n_head_kv", "head_dim",
                                   "n_rot")] + [("rope_base", _f), ("eps", _f)] + \
@@ -55,6 +60,7 @@ class StackConfig(C.Structure):
 
 _Q2WP = C.POINTER(Q2W)
 _KVP, _SEQSP, _SCORESP = C.POINTER(KV), C.POINTER(Seqs), C.POINTER(Scores)
+_PAGESP = C.POINTER(KVPages)
 
 # name -> (restype, argtypes)
 _PROTOS = {
@@ -109,6 +115,11 @@ _PROTOS = {
     "gd_kv_read": (_i, [_vp, _KVP, _SEQSP, _vp, _vp, _i]),
     "gd_kv_attn": (_i, [_vp, _KVP, _SEQSP, _vp, _i64, _vp, _i64, _vp, _i, _i, _f, _i, _i]),
     "gd_kv_attn_scored": (_i, [_vp, _KVP, _SEQSP, _vp, _i64, _vp, _i64, _vp, _i, _i, _f, _SCORESP]),
+    "gd_kv_fork": (_i, [_vp, _PAGESP, _vp, _vp, _vp, _i]),
+    "gd_kv_release": (_i, [_vp, _PAGESP, _vp, _vp, _vp, _i]),
+    "gd_kv_reserve": (_i, [_vp, _PAGESP, _SEQSP, _vp, _vp, _vp]),
+    "gd_kv_compact": (_i, [_vp, _PAGESP, _vp, _vp]),
+    "gd_kv_copy_pages": (_i, [_vp, _KVP, _i, _vp, _vp, _i64]),
     "gd_gdn_gate": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64]),
     "gd_gdn_conv": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i64]),
     "gd_l2norm_rows": (_i, [_vp, _vp, _i, _i, _i64, _i64, _f]),

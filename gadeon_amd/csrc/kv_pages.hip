@@ -1,0 +1,493 @@
+// The pages of the paged KV cache: which sequence holds which, on the device, so that a
+// serving loop that forks, extends, ends and packs conversations needs no host round trip.
+// One table and one count of references serve all layers' caches; copies of pages that a
+// call decides on go into a list, which gd_kv_copy_pages carries out for every layer.
+//
+// The reference keeps one conversation's pages in a pool of the host (MetalKVPool.swift:
+// pages allocated one by one, a snapshot shares full ones and copies the last).
+#include "kv_core.h"
+
+namespace {
+
+// What the kernels need of a gd_kv_pages.  Its arrays are device data: no entry of them is
+// trusted with an address.
+struct Pages {
+    int32_t *refs, *table;
+    uint32_t n_pages;
+    int n_seq, max_pages, P;
+    __device__ __forceinline__ bool there(int page) const { return (uint32_t)page < n_pages; }
+    __device__ __forceinline__ int32_t *row(int b) const { return table + (int64_t)b * max_pages; }
+};
+
+__device__ __forceinline__ void count(const Pages &pg, int page, int by) {
+    if (pg.there(page)) (void)__hip_atomic_fetch_add(&pg.refs[page], by, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---------------------------------------------------------------- fork, release
+
+constexpr int EW = 1024;                         // entries of a workgroup
+
+// Workgroup (order i, EW entries): row dst[i] takes over src[i]'s entries of the first len[i]
+// positions.  No source is the place of another order, so that rows are only read or only
+// written; counts are whole numbers, whose order of addition shows nowhere.
+__global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, const int32_t *dst, const int32_t *len, int n) {
+    const int i = blockIdx.x, s = src[i], d = dst[i], most = len[i];
+    bool bad = (uint32_t)s >= (uint32_t)pg.n_seq || (uint32_t)d >= (uint32_t)pg.n_seq;
+    for (int j = threadIdx.x; j < n; j += 256) bad |= src[j] == d || (j > i && dst[j] == d);
+    if (__syncthreads_or(bad)) return;
+    const int32_t *from = pg.row(s);
+    int32_t *to = pg.row(d);
+    const int end = min(pg.max_pages, (int)(blockIdx.y + 1) * EW);
+    for (int e = blockIdx.y * EW + threadIdx.x; e < end; e += 256) {
+        const int old = to[e], page = (int64_t)e * pg.P < most ? from[e] : -1, now = pg.there(page) ? page : -1;
+        if (old == now) continue;
+        count(pg, old, -1);
+        count(pg, now, 1);
+        to[e] = now;
+    }
+}
+
+// Workgroup (order i, EW entries): sequence seq[i] drops the pages that hold no position of
+// from[i] .. to[i] - 1.  An entry is exchanged, so that one named twice is dropped once.
+__global__ __launch_bounds__(256) void k_release(Pages pg, const int32_t *seq, const int32_t *from, const int32_t *to) {
+    const int i = blockIdx.x, b = seq[i];
+    if ((uint32_t)b >= (uint32_t)pg.n_seq) return;
+    const int64_t lo = from ? from[i] : 0, hi = to[i];
+    int32_t *row = pg.row(b);
+    const int end = min(pg.max_pages, (int)(blockIdx.y + 1) * EW);
+    for (int e = blockIdx.y * EW + threadIdx.x; e < end; e += 256) {
+        const int64_t p = (int64_t)e * pg.P;
+        if ((p + pg.P > lo && p < hi) || !pg.there(row[e])) continue;
+        count(pg, __hip_atomic_exchange(&row[e], -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), -1);
+    }
+}
+
+// ---------------------------------------------------------------- reserve
+
+constexpr int RT = 1024;                         // threads of the one workgroup
+
+// Sum over the threads up to this one; `all` gets the whole sum.  LDS `sums` of two times RT / 64
+// ints, halves in turn (a barrier a call).  (Held at 2^29, which is over all entries that there
+// may be: sequences that share rows could pass 2^31.)
+__device__ __forceinline__ int block_scan(int v, int *sums, int &turn, int &all) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int sum = wave_scan(v);
+    int *s = sums + (turn ^= 1) * (RT / 64);
+    if (lane == 63) s[w] = sum;
+    __syncthreads();
+    int before = 0;
+    all = 0;
+    for (int i = 0; i < RT / 64; i++) {
+        before = min(before + (i < w ? s[i] : 0), 1 << 29);
+        all = min(all + s[i], 1 << 29);
+    }
+    return before + sum;
+}
+
+// Per sequence where its entries start among all; per page the entries that share it and the
+// last of them; per entry (of the rows of the call, sequence by sequence) what is known of it.
+struct Work {
+    int32_t *start, *uses, *last, *seq, *entry, *page, *flags, *rank, *fresh;
+    int most;                                    // entries that there is room for
+    static size_t ints(int64_t n_seq, int64_t n_pages, int64_t most) { return n_seq + 1 + 2 * n_pages + 6 * most; }
+};
+enum { NEED = 1, KEEP = 2, SHARED = 4, TAIL = 8 };
+
+// One workgroup: the entries of the new rows in order, which of them need a page (none there,
+// or one shared with others, of which the last keeps it if no other than these name it), the
+// first free pages in order, the k-th need the k-th page.  A sequence gets all or nothing:
+// what it needs, if all up to it fits.
+//   The chain of its steps bounds it, some 0.7 us each.
+__global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_page, Work wk, int32_t *copies, int32_t *n_copies,
+                                                int32_t *pos_out) {
+    __shared__ int sums[2 * RT / 64];
+    const int t = threadIdx.x;
+    int turn = 0, all;
+    // Entries of each sequence.
+    int entries = 0;
+    for (int b0 = 0; b0 < s.n_seq; b0 += RT) {
+        const int b = b0 + t;
+        int n = 0, pos = -1;
+        if (b < s.n_seq) {
+            pos = s.pos[b];
+            const Seq q = seq_at(s, b);
+            if (q.r1 > q.r0 && (uint32_t)q.pos < s.cap) {
+                const uint32_t last = min((uint32_t)q.pos + (uint32_t)(q.r1 - q.r0 - 1), s.cap - 1);
+                n = (int)(by_page(last) - by_page(q.pos)) + 1;
+            }
+        }
+        const int upto = block_scan(n, sums, turn, all);
+        if (b < s.n_seq) {
+            wk.start[b] = min(entries + upto - n, wk.most);
+            pos_out[b] = pos;
+            // (More than there is room for only of rows that sequences share.)
+            for (int i = 0, c = entries + upto - n; i < n && c < wk.most; i++, c++) {
+                const int e = (int)by_page(pos) + i;
+                wk.seq[c] = b;
+                wk.entry[c] = e;
+                wk.flags[c] = (int64_t)e * pg.P < pos ? TAIL : 0;
+            }
+        }
+        entries = min(entries + all, wk.most);
+    }
+    if (t == 0) wk.start[s.n_seq] = entries;
+    __syncthreads();
+    // The pages that they name; those shared are counted.
+    bool some = false;
+    for (int c = t; c < entries; c += RT) {
+        const int page = pg.row(wk.seq[c])[wk.entry[c]];
+        const bool there = pg.there(page), shared = there && pg.refs[page] > 1;
+        wk.page[c] = there ? page : -1;
+        if (shared) {
+            wk.flags[c] |= SHARED;
+            wk.uses[page] = 0;
+            wk.last[page] = -1;
+            some = true;
+        }
+    }
+    __threadfence();
+    some = __syncthreads_or(some);
+    if (some) {
+        for (int c = t; c < entries; c += RT)
+            if (wk.flags[c] & SHARED) {
+                atomicAdd(&wk.uses[wk.page[c]], 1);
+                atomicMax(&wk.last[wk.page[c]], c);
+            }
+        __threadfence();
+        __syncthreads();
+    }
+    auto now = [](const int32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    int needs = 0;
+    for (int c0 = 0; c0 < entries; c0 += RT) {
+        const int c = c0 + t;
+        int f = 0;
+        if (c < entries) {
+            const int page = wk.page[c];
+            f = wk.flags[c];
+            if (page < 0) f |= NEED;
+            else if (f & SHARED) f |= now(&wk.uses[page]) == pg.refs[page] && now(&wk.last[page]) == c ? KEEP : NEED;
+            wk.flags[c] = f;
+        }
+        const int upto = block_scan(f & NEED ? 1 : 0, sums, turn, all);
+        if (c < entries) wk.rank[c] = needs + upto;
+        needs += all;
+    }
+    // Free pages, as many as are needed, the lowest first.
+    int found = 0;
+    for (uint32_t p0 = 0; p0 < pg.n_pages && found < needs; p0 += 4 * RT) {
+        const uint32_t p = p0 + 4 * t;
+        int free[4], n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) n += free[i] = p + i < pg.n_pages && pg.refs[p + i] <= 0;
+        int at = found + block_scan(n, sums, turn, all) - n;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (free[i] && at < needs) wk.fresh[at++] = (int32_t)(p + i);
+        found += all;
+    }
+    __syncthreads();
+    int copied = 0;
+    for (int c0 = 0; c0 < entries; c0 += RT) {
+        const int c = c0 + t;
+        bool copy = false;
+        int old = -1, page = -1;
+        if (c < entries) {
+            const int f = wk.flags[c], b = wk.seq[c];
+            if (f & (NEED | KEEP)) {
+                const int whole = wk.rank[min(wk.start[b + 1], entries) - 1];    // needs up to the sequence's end
+                if (whole > found) {
+                    pos_out[b] = -1;
+                } else if (f & NEED) {
+                    old = wk.page[c];
+                    page = wk.fresh[wk.rank[c] - 1];
+                    pg.row(b)[wk.entry[c]] = page;
+                    pg.refs[page] = 1;
+                    count(pg, old, -1);
+                    copy = (f & (SHARED | TAIL)) == (SHARED | TAIL);
+                }
+            }
+        }
+        const int upto = block_scan(copy, sums, turn, all);
+        if (copy) {
+            copies[2 * (copied + upto - 1)] = old;
+            copies[2 * (copied + upto - 1) + 1] = page;
+        }
+        copied += all;
+    }
+    if (t == 0) *n_copies = copied;
+}
+
+// ---------------------------------------------------------------- compact
+
+constexpr int CP = 4096, CT = 256;               // pages and threads of a workgroup
+
+__device__ __forceinline__ int workgroup_sum(int v, int *red) {
+    const int sum = __builtin_amdgcn_readlane(wave_scan(v), 63);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
+// Pages in use of each CP.
+__global__ __launch_bounds__(CT) void k_used(Pages pg, int32_t *counts) {
+    __shared__ int red[CT / 64];
+    int n = 0;
+    for (uint32_t p = blockIdx.x * (uint32_t)CP + threadIdx.x, i = 0; i < CP / CT; i++, p += CT)
+        n += p < pg.n_pages && pg.refs[p] > 0;
+    n = workgroup_sum(n, red);
+    if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
+// With n pages in use: the k-th lowest free page goes into low[k] if it lies below n, the k-th
+// highest one in use into high[k] if it does not, which are as many, k into to[page]; to[page] of
+// a free one is -1.
+__global__ __launch_bounds__(CT) void k_rank(Pages pg, const int32_t *counts, int chunks, int32_t *low, int32_t *high, int32_t *to,
+                                             int32_t *n_moves) {
+    __shared__ int red[CT / 64], waves[CT / 64];
+    int before = 0, n = 0;
+    for (int i = threadIdx.x; i < chunks; i += CT) {
+        n += counts[i];
+        before += i < (int)blockIdx.x ? counts[i] : 0;
+    }
+    n = workgroup_sum(n, red);
+    before = workgroup_sum(before, red);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        n_moves[1] = n;
+        if (n == 0) n_moves[0] = 0;
+    }
+    for (uint32_t p0 = blockIdx.x * (uint32_t)CP; p0 < min(pg.n_pages, (blockIdx.x + 1) * (uint32_t)CP); p0 += CT) {
+        const uint32_t p = p0 + threadIdx.x;
+        const bool in = p < pg.n_pages, used = in && pg.refs[p] > 0;
+        const int sum = wave_scan(used);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        int at = before + sum - used;            // pages in use before this one
+#pragma unroll
+        for (int i = 0; i < CT / 64; i++) {
+            at += i < (int)(threadIdx.x >> 6) ? waves[i] : 0;
+            before += waves[i];
+        }
+        if (!in) continue;
+        if (p < (uint32_t)n) {
+            if (!used) low[p - at] = (int32_t)p;
+            if (p == (uint32_t)n - 1) n_moves[0] = (int)p - at + !used;
+        } else {
+            if (used) high[n - 1 - at] = (int32_t)p;
+            to[p] = used ? n - 1 - at : -1;
+        }
+    }
+}
+
+// The moves, their counts of references, and the table's entries that name moved pages.
+__global__ __launch_bounds__(CT) void k_move(Pages pg, const int32_t *low, const int32_t *high, const int32_t *to, const int32_t *n_moves,
+                                             int32_t *moves) {
+    const int64_t i0 = blockIdx.x * (int64_t)CT + threadIdx.x, step = (int64_t)gridDim.x * CT;
+    const int n = n_moves[1], k = n_moves[0];
+    for (int64_t i = i0; i < k; i += step) {
+        const int src = high[i], dst = low[i];
+        moves[2 * i] = src;
+        moves[2 * i + 1] = dst;
+        pg.refs[dst] = pg.refs[src];
+        pg.refs[src] = 0;
+    }
+    if (k == 0) return;
+    for (int64_t i = i0; i < (int64_t)pg.n_seq * pg.max_pages; i += step) {
+        const int page = pg.table[i];
+        if (page >= n && pg.there(page) && to[page] >= 0) pg.table[i] = low[to[page]];
+    }
+}
+
+// ---------------------------------------------------------------- copy
+
+constexpr int LAYERS = 64;                       // of a launch
+struct Layer {
+    void *k, *v;
+    uint8_t *kx, *vx;
+    uint32_t bytes, exps;                        // of a page of a plane, and its exponents
+};
+struct Layers {
+    Layer l[LAYERS];
+};
+
+// Workgroup (pairs from x on, plane y of the layers, slice z): SLICE bytes of a page, four
+// 16-byte loads a thread in flight.  Bytes bound it.
+constexpr uint32_t SLICE = 16384;
+__global__ __launch_bounds__(256) void k_copy(Layers layers, uint32_t n_pages, const int32_t *pairs, const int32_t *n_pairs, int most) {
+    const Layer l = layers.l[blockIdx.y >> 1];
+    const bool is_k = !(blockIdx.y & 1);
+    char *plane = (char *)(is_k ? l.k : l.v);
+    uint8_t *exps = is_k ? l.kx : l.vx;
+    const int n = n_pairs ? min(max(*n_pairs, 0), most) : most;
+    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+        const int src = pairs[2 * i], dst = pairs[2 * i + 1];
+        if ((uint32_t)src >= n_pages || (uint32_t)dst >= n_pages || src == dst) continue;
+        const char *x = plane + (uint64_t)src * l.bytes;
+        char *y = plane + (uint64_t)dst * l.bytes;
+        for (uint64_t at = (uint64_t)blockIdx.z * SLICE; at < l.bytes; at += (uint64_t)gridDim.z * SLICE) {
+            u32x4 r[SLICE / 4096];
+#pragma unroll
+            for (uint32_t j = 0; j < SLICE / 4096; j++) {
+                const uint64_t a = at + j * 4096 + threadIdx.x * 16;
+                if (a < l.bytes) r[j] = *(const u32x4 *)(x + a);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < SLICE / 4096; j++) {
+                const uint64_t a = at + j * 4096 + threadIdx.x * 16;
+                if (a < l.bytes) *(u32x4 *)(y + a) = r[j];
+            }
+        }
+        if (blockIdx.z == 0)
+            for (uint32_t j = threadIdx.x; j < l.exps; j += 256)
+                exps[(uint64_t)dst * l.exps + j] = exps[(uint64_t)src * l.exps + j];
+    }
+}
+
+// ---------------------------------------------------------------- checks
+
+int check_pages(gd_ctx *ctx, const char *fn, const gd_kv_pages *pg) {
+    GD_REQUIRE(ctx, pg, "%s: null pages", fn);
+    GD_REQUIRE(ctx, pg->n_pages > 0 && pg->n_pages < (1LL << 31) - 2 * CP, "%s: %lld pages", fn, (long long)pg->n_pages);
+    GD_REQUIRE(ctx, pg->n_seq >= 0 && pg->n_seq < MAX_WGS && pg->max_pages > 0, "%s: %d sequences of %d pages", fn, pg->n_seq,
+               pg->max_pages);
+    GD_REQUIRE(ctx, pg->page_size > 0 && pg->page_size <= (1 << 24), "%s: page size %d", fn, pg->page_size);
+    GD_REQUIRE(ctx, pg->refs && (pg->table || !pg->n_seq), "%s: null refs or table", fn);
+    GD_REQUIRE(ctx, ((uintptr_t)pg->refs | (uintptr_t)pg->table) % 4 == 0, "%s: refs and table must be 4-byte aligned", fn);
+    return GD_OK;
+}
+Pages pages_of(const gd_kv_pages *pg) {
+    return Pages{pg->refs, pg->table, (uint32_t)pg->n_pages, pg->n_seq, pg->max_pages, pg->page_size};
+}
+
+// Orders of a call: workgroups walk them all, and are counted as a launch's.
+constexpr int MAX_ORDERS = 1 << 16;
+int check_orders(gd_ctx *ctx, const char *fn, const gd_kv_pages *pg, int n, const void *a, const void *b, const void *c) {
+    GD_REQUIRE(ctx, n >= 0 && n <= MAX_ORDERS, "%s: %d orders (%d at most)", fn, n, MAX_ORDERS);
+    GD_REQUIRE(ctx, n == 0 || (a && b), "%s: null orders", fn);
+    GD_REQUIRE(ctx, ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) % 4 == 0, "%s: orders must be 4-byte aligned", fn);
+    const int64_t chunks = ((int64_t)pg->max_pages + EW - 1) / EW;
+    GD_REQUIRE(ctx, chunks < 65536 && n * chunks < MAX_WGS, "%s: %d orders over %d pages each", fn, n, pg->max_pages);
+    return GD_OK;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------- C ABI
+// Arguments are checked before the context is looked at (as the other entries of the cache).
+
+extern "C" int gd_kv_fork(gd_ctx *ctx, const gd_kv_pages *pg, const int32_t *src, const int32_t *dst, const int32_t *len, int n) {
+    const char *fn = "gd_kv_fork";
+    int rc;
+    if ((rc = check_pages(ctx, fn, pg)) || (rc = check_orders(ctx, fn, pg, n, src, dst, len))) return rc;
+    GD_REQUIRE(ctx, n == 0 || len, "%s: null orders", fn);
+    GD_CHECK_CTX(ctx);
+    if (!n || !pg->n_seq) return GD_OK;
+    GD_HIP(ctx, hipSetDevice(ctx->device));
+    hipLaunchKernelGGL(k_fork, dim3(n, gd_blocks(pg->max_pages, EW)), dim3(256), 0, ctx->stream, pages_of(pg), src, dst, len, n);
+    GD_LAUNCHED(ctx, fn);
+    return GD_OK;
+}
+
+extern "C" int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pg, const int32_t *seq, const int32_t *from, const int32_t *to, int n) {
+    const char *fn = "gd_kv_release";
+    int rc;
+    if ((rc = check_pages(ctx, fn, pg)) || (rc = check_orders(ctx, fn, pg, n, seq, to, from))) return rc;
+    GD_CHECK_CTX(ctx);
+    if (!n || !pg->n_seq) return GD_OK;
+    GD_HIP(ctx, hipSetDevice(ctx->device));
+    hipLaunchKernelGGL(k_release, dim3(n, gd_blocks(pg->max_pages, EW)), dim3(256), 0, ctx->stream, pages_of(pg), seq, from, to);
+    GD_LAUNCHED(ctx, fn);
+    return GD_OK;
+}
+
+extern "C" int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pg, const gd_seqs *s, int32_t *copies, int32_t *n_copies, int32_t *pos_out) {
+    const char *fn = "gd_kv_reserve";
+    int rc;
+    if ((rc = check_pages(ctx, fn, pg)) || (rc = check_seqs(ctx, fn, s))) return rc;
+    GD_REQUIRE(ctx, s->n_seq == pg->n_seq && s->max_pages == pg->max_pages && (s->page_table == pg->table || !s->n_rows),
+               "%s: the sequences' table is not the pages' (%d x %d and %d x %d)", fn, s->n_seq, s->max_pages, pg->n_seq, pg->max_pages);
+    GD_REQUIRE(ctx, n_copies && (!s->n_seq || (copies && pos_out)), "%s: null copies or positions", fn);
+    GD_REQUIRE(ctx, ((uintptr_t)copies | (uintptr_t)n_copies | (uintptr_t)pos_out) % 4 == 0, "%s: outputs must be 4-byte aligned", fn);
+    GD_REQUIRE(ctx, !s->n_seq || s->pos, "%s: null positions or page table", fn);
+    GD_CHECK_CTX(ctx);
+    GD_HIP(ctx, hipSetDevice(ctx->device));
+    const int64_t cap = std::min<int64_t>((int64_t)pg->max_pages * pg->page_size, 0x7fffffff);
+    const Rows rows{s->row_start, s->pos, nullptr, s->page_table, (int)s->n_rows, s->n_seq, s->max_pages, (uint32_t)cap};
+    // Entries of the rows: a page for each page_size of them, and two ends a sequence.
+    Work wk;
+    wk.most = (int)(s->n_rows / pg->page_size + 2 * std::min<int64_t>(s->n_seq, s->n_rows));
+    void *ws;
+    if ((rc = gd_ctx_workspace(ctx, Work::ints(s->n_seq, pg->n_pages, wk.most) * 4, &ws))) return rc;
+    int32_t *at = (int32_t *)ws;
+    auto take = [&](int64_t n) { int32_t *p = at; at += n; return p; };
+    wk.start = take(s->n_seq + 1);
+    wk.uses = take(pg->n_pages);
+    wk.last = take(pg->n_pages);
+    for (int32_t **p : {&wk.seq, &wk.entry, &wk.page, &wk.flags, &wk.rank, &wk.fresh}) *p = take(wk.most);
+    hipLaunchKernelGGL(k_reserve, dim3(1), dim3(RT), 0, ctx->stream, pages_of(pg), rows, FastDiv((uint32_t)pg->page_size), wk, copies,
+                       n_copies, pos_out);
+    GD_LAUNCHED(ctx, fn);
+    return GD_OK;
+}
+
+extern "C" int gd_kv_compact(gd_ctx *ctx, const gd_kv_pages *pg, int32_t *moves, int32_t *n_moves) {
+    const char *fn = "gd_kv_compact";
+    int rc;
+    if ((rc = check_pages(ctx, fn, pg))) return rc;
+    GD_REQUIRE(ctx, moves && n_moves, "%s: null moves", fn);
+    GD_REQUIRE(ctx, ((uintptr_t)moves | (uintptr_t)n_moves) % 4 == 0, "%s: moves must be 4-byte aligned", fn);
+    GD_CHECK_CTX(ctx);
+    GD_HIP(ctx, hipSetDevice(ctx->device));
+    const int chunks = (int)gd_blocks(pg->n_pages, CP);
+    void *ws;
+    if ((rc = gd_ctx_workspace(ctx, ((size_t)chunks + 3 * pg->n_pages) * 4, &ws))) return rc;
+    int32_t *counts = (int32_t *)ws, *low = counts + chunks, *high = low + pg->n_pages, *to = high + pg->n_pages;
+    const Pages p = pages_of(pg);
+    hipLaunchKernelGGL(k_used, dim3(chunks), dim3(CT), 0, ctx->stream, p, counts);
+    GD_LAUNCHED(ctx, fn);
+    hipLaunchKernelGGL(k_rank, dim3(chunks), dim3(CT), 0, ctx->stream, p, counts, chunks, low, high, to, n_moves);
+    GD_LAUNCHED(ctx, fn);
+    const int64_t entries = std::max<int64_t>((int64_t)pg->n_seq * pg->max_pages, pg->n_pages);
+    hipLaunchKernelGGL(k_move, dim3(std::min<int64_t>((entries + CT - 1) / CT, 2048)), dim3(CT), 0, ctx->stream, p, low, high, to, n_moves,
+                       moves);
+    GD_LAUNCHED(ctx, fn);
+    return GD_OK;
+}
+
+extern "C" int gd_kv_copy_pages(gd_ctx *ctx, const gd_kv *kv, int n_kv, const int32_t *pairs, const int32_t *n_pairs, int64_t max_pairs) {
+    const char *fn = "gd_kv_copy_pages";
+    int rc;
+    GD_REQUIRE(ctx, n_kv >= 0 && (kv || !n_kv), "%s: %d caches", fn, n_kv);
+    for (int i = 0; i < n_kv; i++) {
+        if ((rc = check_kv(ctx, fn, kv + i, true))) return rc;
+        GD_REQUIRE(ctx, kv[i].n_pages == kv[0].n_pages, "%s: caches of %lld and %lld pages", fn, (long long)kv[0].n_pages,
+                   (long long)kv[i].n_pages);
+        const int64_t bytes = (int64_t)kv[i].page_size * kv[i].n_head_kv * kv[i].head_dim * (kv[i].dtype == GD_F16 ? 2 : 1);
+        GD_REQUIRE(ctx, bytes < (1LL << 32), "%s: pages of %lld bytes", fn, (long long)bytes);
+    }
+    GD_REQUIRE(ctx, max_pairs >= 0 && max_pairs < (1LL << 30), "%s: %lld pairs", fn, (long long)max_pairs);
+    GD_REQUIRE(ctx, max_pairs == 0 || pairs, "%s: null pairs", fn);
+    GD_REQUIRE(ctx, ((uintptr_t)pairs | (uintptr_t)n_pairs) % 4 == 0, "%s: pairs must be 4-byte aligned", fn);
+    GD_CHECK_CTX(ctx);
+    if (!max_pairs) return GD_OK;
+    GD_HIP(ctx, hipSetDevice(ctx->device));
+    for (int i0 = 0; i0 < n_kv; i0 += LAYERS) {
+        const int n = std::min(LAYERS, n_kv - i0);
+        Layers layers = {};
+        uint32_t widest = 0;
+        for (int i = 0; i < n; i++) {
+            const gd_kv &c = kv[i0 + i];
+            const bool i8 = c.dtype == GD_I8;
+            const uint32_t rows = (uint32_t)c.page_size * c.n_head_kv;
+            layers.l[i] = Layer{c.k, c.v, c.k_exp, c.v_exp, rows * c.head_dim * (i8 ? 1 : 2), i8 ? rows / BLK : 0};
+            widest = std::max(widest, layers.l[i].bytes);
+        }
+        const int64_t slices = std::min<int64_t>(((int64_t)widest + SLICE - 1) / SLICE, 1024);
+        const int64_t x = std::min<int64_t>(max_pairs, std::max<int64_t>(1, 4096 / (2 * n * slices)));
+        hipLaunchKernelGGL(k_copy, dim3((unsigned)x, 2 * n, (unsigned)slices), dim3(256), 0, ctx->stream, layers, (uint32_t)kv[0].n_pages,
+                           pairs, n_pairs, (int)max_pairs);
+        GD_LAUNCHED(ctx, fn);
+    }
+    return GD_OK;
+}

@@ -505,6 +505,63 @@ int gd_kv_attn_scored(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const v
                       const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
                       const gd_scores *scores);
 
+/* ---- the pages of a cache -------------------------------------------------------
+ * Who holds which page, kept on the device by the same table that gd_seqs.page_table is, for
+ * all layers' caches alike (their gd_kv have the same n_pages and page_size): a page number
+ * stands for that page of every layer.  refs[page] counts the table's entries that name
+ * it, 0 for a free page; a program may hold pages by counts of its own (a prompt kept for
+ * later), and starts with refs all 0 and the table all -1.  An entry outside [0, n_pages) names
+ * no page.  The entries below enqueue kernels alone, so that a serving step is recorded whole:
+ * gd_kv_reserve, gd_kv_copy_pages, then gd_kv_append_rope and gd_kv_attn on the positions
+ * that gd_kv_reserve gave.  (MetalKVPool.swift keeps one conversation's pages on the host.) */
+typedef struct gd_kv_pages {
+    int32_t *refs;               /* [n_pages] */
+    int32_t *table;              /* [n_seq][max_pages] */
+    int64_t n_pages;
+    int n_seq, max_pages, page_size;
+} gd_kv_pages;
+
+/* For i < n (65536 at most; src, dst, len device memory): sequence dst[i] becomes a branch of
+ * src[i]: its entries those of the pages that hold src's first len[i] positions, the others -1,
+ * what it held before released.  No page is copied: gd_kv_reserve does that for the one that
+ * either goes on in.  Left out is an order of a sequence outside [0, n_seq), one whose dst is a
+ * src of the call (its own too), and one whose dst a later order names. */
+int gd_kv_fork(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *src, const int32_t *dst, const int32_t *len, int n);
+
+/* For i < n (65536 at most): sequence seq[i] keeps the pages that hold one of its positions
+ * from[i] .. to[i]-1 (from null: 0 ..), and its other entries become -1, their pages' counts one
+ * less: to = 0 ends it, to = its position takes back pages reserved behind, from = position - window
+ * lets go what a window has passed.  A sequence may be named more than once; one outside [0, n_seq)
+ * is left out. */
+int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *seq, const int32_t *from, const int32_t *to, int n);
+
+/* Pages for the rows of a call (seqs' table is pages', with as many sequences): every entry of a
+ * sequence's positions pos .. pos + rows - 1 (as far as the table goes) that names no page, or one
+ * that others name too, gets a free page, counted once; a shared one's count falls by one, but
+ * the last of the entries that share it, in the sequences' order, keeps it if no other than these
+ * name it.  The k-th entry, sequence by sequence, gets the k-th lowest page free before the call.  A page replaced that holds
+ * positions before pos goes into copies as (from, to): copies[2 n_seq] at most, *n_copies of them
+ * (device memory both; the rest of copies stays), for gd_kv_copy_pages before rows are appended.
+ *   pos_out[n_seq] (may be pos) is pos, or -1 where the free pages do not suffice for all
+ * needs up to this sequence's last: it keeps what it had, and the calls that take pos_out leave
+ * it alone (also where it needs none but keeps a page that a sequence before it shares).
+ * Uses the context workspace (8 bytes a page and 24 an entry of the rows). */
+int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pages, const gd_seqs *seqs, int32_t *copies, int32_t *n_copies,
+                  int32_t *pos_out);
+
+/* Closes the cache up: with n pages in use (counted at least once), the highest of them goes to
+ * the lowest free page, and so on while that is lower, so that those in use are 0 .. n-1 and the
+ * planes behind them may go.  Entries and counts follow; moves[2 n_pages] at most gets the
+ * (from, to) pairs in that order, n_moves[2] their number and n (device memory both), for
+ * gd_kv_copy_pages before the cache is used again.  Uses the context workspace (12 bytes a page). */
+int gd_kv_compact(gd_ctx *ctx, const gd_kv_pages *pages, int32_t *moves, int32_t *n_moves);
+
+/* Copies whole pages, codes with their exponents, in each of the n_kv caches (which have the same
+ * n_pages): for i < *n_pairs (device memory; null: max_pairs; at most max_pairs either way) page
+ * pairs[2 i] to page pairs[2 i + 1].  A page written to must not be named by another pair.  Pairs outside
+ * [0, n_pages) are left out.  A launch for 64 caches. */
+int gd_kv_copy_pages(gd_ctx *ctx, const gd_kv *kv, int n_kv, const int32_t *pairs, const int32_t *n_pairs, int64_t max_pairs);
+
 /* ---- GDN recurrence -----------------------------------------------------------
  * State S[nV][dS][dS] f32, key-major: S[h][i*dS + j], i = key, j = value
  * (GDN.swift:9-16, Kernels.metal:1225).  Head map hk = hv % nK
