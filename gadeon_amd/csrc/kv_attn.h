@@ -6,6 +6,8 @@
 
 namespace {
 
+constexpr float LOG2E = 1.4426950408889634f;
+
 // How scores are made and which keys are seen.  Plain: every key up to the query's own, or
 // those of a window and the first `sinks`.
 struct Mask {
@@ -16,7 +18,7 @@ struct Mask {
 // in units of log2; no key before first[row], and every key before prefix[b].
 struct Scores {
     int window, sinks;
-    float cap;                                   // 0: none
+    float cap, p[5];                             // 0: none; cap P (cap_scores)
     const float *slope;
     const int32_t *first, *prefix;
     static constexpr bool SCORED = true;
@@ -93,15 +95,40 @@ template <class How> __device__ __forceinline__ uint32_t doc_of(const How &m, in
     else return 0;
 }
 
-// y = cap tanh(y / cap) of a score in units of log2.  Below half the cap by tanh(x) = x P(x^2),
-// P the polynomial of least relative error with P(0) = 1 (2^-26): (1 - e) / (1 + e), e =
-// exp(-2 |x|), would lose there what scores far below the cap have left.
-__device__ __forceinline__ float capped(float y, float cap, float inv) {
-    const float x = y * inv, u = x * x;
-    const float p = fmaf(u, fmaf(u, fmaf(u, fmaf(u, 0.01724149100482464f, -0.05304549261927605f), 0.13325878977775574f), -0.333331435918808f), 1.0f);
-    const float e = __builtin_amdgcn_exp2f(-2.885390081777927f * fabsf(x));
-    const float big = copysignf(cap * (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), y);
-    return fabsf(x) < 0.5f ? y * p : big;
+// cap tanh(x), x = v[i] to_x: scores over their cap, all of a wave's in one of two ways.  Where
+// every |x| is under 1/2, as cap x P(x^2), P the polynomial of least relative error (2^-26; of
+// one degree less 2^-20, which f16 rows take); else as cap - 2 cap / (1 + e^2x), whose error of
+// some 2^-24 of the cap is then one of the greatest score's own.  (Seven or six instructions a
+// score, and three with two of a quarter's rate; both and a choice of either cost 22.)
+template <bool FINE, int N, int V, class Vec>
+__device__ __forceinline__ void cap_scores(const Scores &how, float to_x, Vec (&s)[N]) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int v = 0; v < V; v++) most = fmaxf(most, fabsf(s[i][v]));
+    if (__any(!(most * fabsf(to_x) < 0.5f))) {
+        const float to_e = to_x * (2.f * LOG2E);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const float e = __builtin_amdgcn_exp2f(s[i][v] * to_e);
+                s[i][v] = fmaf(-2.f * how.cap, __builtin_amdgcn_rcpf(1.f + e), how.cap);
+                if (v % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const float x = s[i][v] * to_x, u = x * x;
+                float p = FINE ? fmaf(u, how.p[4], how.p[3]) : how.p[3];
+                p = fmaf(u, fmaf(u, fmaf(u, p, how.p[2]), how.p[1]), how.p[0]);
+                s[i][v] = x * p;
+                if (v % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+            }
+    }
 }
 
 // Partials of the key splits: sums of head h of row n, split z, at acc [n H + h][most][HD]
@@ -188,7 +215,6 @@ constexpr int TW = 4;                            // waves
 constexpr float LAZY = 7.f;                      // how far (log2) weights may pass the maximum they stand at
                                                  // (0, as ever: 1 to 6% more time)
 constexpr int MAX_SPLITS = 64;                   // what the combine weighs in one wave
-constexpr float LOG2E = 1.4426950408889634f;
 
 template <int HD, bool I8, bool TILED, typename T, class How>
 __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || HD == 128 ? 2 : 1))) void k_attn_tokens(
@@ -343,6 +369,8 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
     float slope = 0.f;                           // of this lane's head
     if constexpr (How::SCORED)
         if (mask.slope) slope = mask.slope[h0 + min(col, nh - 1)] * LOG2E;
+    float to_x = 0.f;                            // a score over its cap
+    if constexpr (How::SCORED) to_x = sf / mask.cap;
     f32x4 acc[DT];                               // O^T rows 16 dt + 4 g + v
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -409,15 +437,22 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
                 sc[kt][v] += gd_dpp<GD_DPP_ROR8>(sc[kt][v]);
                 if constexpr (I8) sc[kt][v] *= kstep[kt];
             }
+        const uint32_t mine = seen >> (4 * g);
+        auto unseen = [&](float x) {
+            if (seen == 0xffffffffu) return;
+            asm volatile("");
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) sc[kt][v] = mine & (1u << (16 * kt + v)) ? sc[kt][v] : x;
+        };
         if constexpr (How::SCORED) {
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++) sc[kt] *= sf;
             if (mask.cap > 0.f) {
-                const float inv = 1.0f / mask.cap;
+                unseen(0.f);                     // (what is not seen has no part in how the others are capped)
+                cap_scores<true, 2, 4>(mask, to_x, sc);
+            } else {
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++) sc[kt][v] = capped(sc[kt][v], mask.cap, inv);
+                for (int kt = 0; kt < 2; kt++) sc[kt] *= sf;
             }
             if (mask.slope) {
                 // (All seen keys lie before the token.)
@@ -428,14 +463,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
                     for (int v = 0; v < 4; v++) sc[kt][v] = fmaf(-slope, d - (float)(16 * kt + v), sc[kt][v]);
             }
         }
-        if (seen != 0xffffffffu) {
-            asm volatile("");
-            const uint32_t mine = seen >> (4 * g);
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int v = 0; v < 4; v++) sc[kt][v] = mine & (1u << (16 * kt + v)) ? sc[kt][v] : none;
-        }
+        unseen(none);
         float top = -INFINITY;                   // of this lane's keys
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
@@ -842,6 +870,13 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         }
     }
     if (sf < 0x1p-126f) sf = 0x1p-126f;          // weights of 1 alike; times -inf not NaN
+    // A score over its cap; the units of scores once they are capped, and once they are biased.
+    float to_x = 0.f, capped = sf, unit = sf;
+    if constexpr (How::SCORED) {
+        to_x = sf / mask.cap;
+        if (mask.cap > 0.f) capped = unit = 1.f;
+        if (mask.slope) unit = 1.f;
+    }
     // Row 8 (v / 4) + 4 h + v % 4 of a C value v (MF 16: 4 h + v).
     Acc acc[DT];                                 // O^T, dims MF dt + row
 #pragma unroll
@@ -891,15 +926,27 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                 }
             }
             if constexpr (!HOLD) __builtin_amdgcn_s_setprio(0);
+            uint64_t see = 0;                    // a bit a key, as this column sees it
+            if (!full) {
+                auto below = [](int64_t x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; };
+                see = below((int64_t)p - k0 + 1);
+                if (mask.window) see &= ~below((int64_t)p - mask.window + 1 - k0) | below((int64_t)mask.sinks - k0);
+                if constexpr (How::SCORED) see = (see | below((int64_t)un.prefix - k0)) & ~below((int64_t)doc - k0);
+                see = (see & now) >> (4 * h);
+            }
+            auto unseen = [&](float x) {
+                if (full) return;
+#pragma unroll
+                for (int kt = 0; kt < NT; kt++) {
+                    const uint32_t bits = (uint32_t)(see >> (MF * kt));
+#pragma unroll
+                    for (int v = 0; v < NV; v++) st[kt][v] = bits & (1u << (8 * (v / 4) + v % 4)) ? st[kt][v] : x;
+                }
+            };
             if constexpr (How::SCORED) {
-#pragma unroll
-                for (int kt = 0; kt < NT; kt++) st[kt] *= sf;
                 if (mask.cap > 0.f) {
-                    const float inv = 1.0f / mask.cap;
-#pragma unroll
-                    for (int kt = 0; kt < NT; kt++)
-#pragma unroll
-                        for (int v = 0; v < NV; v++) st[kt][v] = capped(st[kt][v], mask.cap, inv);
+                    unseen(0.f);                 // (what nobody sees has no part in how the others are capped)
+                    cap_scores<HL, NT, NV>(mask, to_x, st);
                 }
                 if (mask.slope) {
                     const float d = (float)(int)(p - k0 - 4 * h);
@@ -907,24 +954,10 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                     for (int kt = 0; kt < NT; kt++)
 #pragma unroll
                         for (int v = 0; v < NV; v++)
-                            st[kt][v] = fmaf(-slope, fabsf(d - (float)(MF * kt + 8 * (v / 4) + v % 4)), st[kt][v]);
+                            st[kt][v] = fmaf(-slope, fabsf(d - (float)(MF * kt + 8 * (v / 4) + v % 4)), st[kt][v] * capped);
                 }
             }
-            if (!full) {
-                // A bit a key, as this column sees it.
-                auto below = [](int64_t x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; };
-                uint64_t see = below((int64_t)p - k0 + 1);
-                if (mask.window) see &= ~below((int64_t)p - mask.window + 1 - k0) | below((int64_t)mask.sinks - k0);
-                if constexpr (How::SCORED) see = (see | below((int64_t)un.prefix - k0)) & ~below((int64_t)doc - k0);
-                see = (see & now) >> (4 * h);
-#pragma unroll
-                for (int kt = 0; kt < NT; kt++) {
-                    const uint32_t bits = (uint32_t)(see >> (MF * kt));
-#pragma unroll
-                    for (int v = 0; v < NV; v++)
-                        st[kt][v] = bits & (1u << (8 * (v / 4) + v % 4)) ? st[kt][v] : -INFINITY;
-                }
-            }
+            unseen(-INFINITY);
             float top = -INFINITY;
 #pragma unroll
             for (int kt = 0; kt < NT; kt++)
@@ -932,7 +965,6 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                 for (int v = 0; v < NV; v++) top = fmaxf(top, st[kt][v]);
             // Sums are brought to a new maximum only where a score is over 2^LAZY of the one
             // they stand at (random scores: hardly after the first tiles).
-            const float unit = How::SCORED ? 1.0f : sf;    // of st
             if (__any(top * unit > m + LAZY)) {
                 if constexpr (MF == 16) top = fmaxf(top, __shfl_xor(top, 16, 64));
                 const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * unit);
@@ -953,8 +985,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 #pragma unroll
                 for (int v = 0; v < NV; v += 2) {
                     constexpr auto kk = [](int kt, int v) { return (NV * kt + v) / 8; };
-                    float w0 = __builtin_amdgcn_exp2f(How::SCORED ? st[kt][v] + off : fmaf(st[kt][v], sf, off));
-                    float w1 = __builtin_amdgcn_exp2f(How::SCORED ? st[kt][v + 1] + off : fmaf(st[kt][v + 1], sf, off));
+                    float w0 = __builtin_amdgcn_exp2f(fmaf(st[kt][v], unit, off));
+                    float w1 = __builtin_amdgcn_exp2f(fmaf(st[kt][v + 1], unit, off));
                     f16x2 hi, lo;
                     if constexpr (HL) {
                         w0 *= 256.f;
