@@ -37,13 +37,21 @@ __global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, cons
     if (__syncthreads_or(bad)) return;
     const int32_t *from = pg.row(s);
     int32_t *to = pg.row(d);
-    const int end = min(pg.max_pages, (int)(blockIdx.y + 1) * EW);
-    for (int e = blockIdx.y * EW + threadIdx.x; e < end; e += 256) {
-        const int old = to[e], page = (int64_t)e * pg.P < most ? from[e] : -1, now = pg.there(page) ? page : -1;
-        if (old == now) continue;
-        count(pg, old, -1);
-        count(pg, now, 1);
-        to[e] = now;
+    const int e0 = blockIdx.y * EW + threadIdx.x;
+    int old[EW / 256], now[EW / 256];
+#pragma unroll
+    for (int x = 0; x < EW / 256; x++) {
+        const int e = e0 + 256 * x;
+        old[x] = e < pg.max_pages ? to[e] : -1;
+        now[x] = e < pg.max_pages && (int64_t)e * pg.P < most ? from[e] : -1;
+    }
+#pragma unroll
+    for (int x = 0; x < EW / 256; x++) {
+        if (!pg.there(now[x])) now[x] = -1;
+        if (old[x] == now[x]) continue;
+        count(pg, old[x], -1);
+        count(pg, now[x], 1);
+        to[e0 + 256 * x] = now[x];
     }
 }
 
@@ -54,12 +62,19 @@ __global__ __launch_bounds__(256) void k_release(Pages pg, const int32_t *seq, c
     if ((uint32_t)b >= (uint32_t)pg.n_seq) return;
     const int64_t lo = from ? from[i] : 0, hi = to[i];
     int32_t *row = pg.row(b);
-    const int end = min(pg.max_pages, (int)(blockIdx.y + 1) * EW);
-    for (int e = blockIdx.y * EW + threadIdx.x; e < end; e += 256) {
+    const int e0 = blockIdx.y * EW + threadIdx.x;
+    int old[EW / 256];
+#pragma unroll
+    for (int x = 0; x < EW / 256; x++) {
+        const int e = e0 + 256 * x;
         const int64_t p = (int64_t)e * pg.P;
-        if ((p + pg.P > lo && p < hi) || !pg.there(row[e])) continue;
-        count(pg, __hip_atomic_exchange(&row[e], -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), -1);
+        old[x] = e < pg.max_pages && !(p + pg.P > lo && p < hi) ? row[e] : -1;
     }
+#pragma unroll
+    for (int x = 0; x < EW / 256; x++)
+        if (pg.there(old[x])) old[x] = __hip_atomic_exchange(&row[e0 + 256 * x], -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int x = 0; x < EW / 256; x++) count(pg, old[x], -1);
 }
 
 // ---------------------------------------------------------------- reserve
@@ -217,9 +232,180 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
     if (t == 0) *n_copies = copied;
 }
 
+// The same for FEW sequences and entries at most, in registers and LDS: a thread's four
+// sequences, four entries, four pages of a round.  Shared pages are counted in a table by a
+// hash of theirs, whose places depend on who comes first, but not what stands there.
+//   A chain of three loads (row, entry, count) bounds it.
+constexpr int FEW = 4 * RT, SLOTS = 2 * FEW;
+struct FewLds {
+    int pos[FEW], entry[FEW], start[FEW + 1];    // of a sequence: its position (-1: denied), first entry, and that one's place
+    union {                                      // (one after the other)
+        int owner[FEW];                          // the sequence that starts at an entry, from 1 on
+        struct { int page[SLOTS], uses[SLOTS], last[SLOTS]; };
+        struct { int rank[FEW], fresh[FEW]; };   // an entry's needs up to it; free pages
+    };
+    int sums[2 * RT / 64];
+};
+
+__global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by_page, int most, int32_t *copies, int32_t *n_copies,
+                                                    int32_t *pos_out) {
+    __shared__ FewLds l;
+    const int t = threadIdx.x;
+    int turn = 0, all;
+    int refs[4];                                 // the first round's, on their way
+#pragma unroll
+    for (int j = 0; j < 4; j++) refs[j] = 4u * t + j < pg.n_pages ? pg.refs[4 * t + j] : 1;
+    int n[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int b = 4 * t + j;
+        n[j] = 0;
+        l.owner[b] = 0;
+        if (b >= s.n_seq) continue;
+        const Seq q = seq_at(s, b);
+        l.pos[b] = q.pos;
+        if (q.r1 > q.r0 && (uint32_t)q.pos < s.cap) {
+            const uint32_t last = min((uint32_t)q.pos + (uint32_t)(q.r1 - q.r0 - 1), s.cap - 1);
+            l.entry[b] = (int)by_page(q.pos);
+            n[j] = min((int)by_page(last) - l.entry[b] + 1, FEW);
+        }
+        sum += n[j];
+    }
+    int at = block_scan(sum, l.sums, turn, all) - sum;
+    const int entries = min(all, most);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int b = 4 * t + j;
+        if (b < s.n_seq) l.start[b] = min(at, most);
+        if (n[j] && at < most) l.owner[at] = b + 1;
+        at += n[j];
+    }
+    if (t == 0) l.start[s.n_seq] = entries;
+    __syncthreads();
+    // Entries 4 t ..: the last sequence that starts at or before each.
+    int seq[4], page[4], e[4], f[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) seq[j] = max(l.owner[4 * t + j], j ? seq[j - 1] : 0);
+    int top = seq[3];
+    for (int i = 1; i < 64; i *= 2) {
+        const int o = __shfl_up(top, i, 64);
+        if ((t & 63) >= i) top = max(top, o);
+    }
+    int before = __shfl_up(top, 1, 64);
+    if ((t & 63) == 0) before = 0;
+    int *w = l.sums + (turn ^= 1) * (RT / 64);
+    if ((t & 63) == 63) w[t >> 6] = top;
+    __syncthreads();
+    for (int i = 0; i < (t >> 6); i++) before = max(before, w[i]);
+    bool some = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int c = 4 * t + j;
+        page[j] = -1;
+        f[j] = 0;
+        if (c >= entries) continue;
+        seq[j] = max(seq[j], before) - 1;
+        e[j] = l.entry[seq[j]] + c - l.start[seq[j]];
+        page[j] = pg.row(seq[j])[e[j]];
+    }
+    int held[4];                                 // counts of the entries' pages
+#pragma unroll
+    for (int j = 0; j < 4; j++) held[j] = pg.there(page[j]) ? pg.refs[page[j]] : 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (4 * t + j >= entries) continue;
+        if (!pg.there(page[j])) f[j] = NEED;
+        else if (held[j] > 1) f[j] = SHARED;
+        some |= f[j] == SHARED;
+    }
+    if (__syncthreads_or(some)) {
+        for (int i = t; i < SLOTS; i += RT) {
+            l.page[i] = -1;
+            l.uses[i] = 0;
+            l.last[i] = -1;
+        }
+        __syncthreads();
+        auto slot = [&](int page) {              // its place; every probe ends, as half of them are free
+            int i = (int)((uint32_t)page * 2654435761u >> 19) % SLOTS;
+            for (;; i = (i + 1) % SLOTS) {
+                const int there = atomicCAS(&l.page[i], -1, page);
+                if (there == -1 || there == page) return i;
+            }
+        };
+        int at[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (f[j] & SHARED) {
+                at[j] = slot(page[j]);
+                atomicAdd(&l.uses[at[j]], 1);
+                atomicMax(&l.last[at[j]], 4 * t + j);
+            }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (f[j] & SHARED) f[j] |= l.uses[at[j]] == held[j] && l.last[at[j]] == 4 * t + j ? KEEP : NEED;
+    }
+    sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) sum += f[j] & NEED;
+    int rank = block_scan(sum, l.sums, turn, all) - sum;
+    const int needs = all;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        rank += f[j] & NEED;
+        if (4 * t + j < entries) l.rank[4 * t + j] = rank;
+    }
+    int found = 0;
+    for (uint32_t p0 = 0; p0 < pg.n_pages && found < needs; p0 += 4 * RT) {
+        const uint32_t p = p0 + 4 * t;
+        if (p0)
+#pragma unroll
+            for (int j = 0; j < 4; j++) refs[j] = p + j < pg.n_pages ? pg.refs[p + j] : 1;
+        sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum += refs[j] <= 0;
+        int at = found + block_scan(sum, l.sums, turn, all) - sum;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (refs[j] <= 0 && at < needs) l.fresh[at++] = (int)(p + j);
+        found += all;
+    }
+    __syncthreads();
+    // (Nobody reads a count or an entry of the table any more.)
+    int fresh[4];
+    sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        fresh[j] = -1;
+        if (!(f[j] & (NEED | KEEP))) continue;
+        const int b = seq[j];
+        const int p = l.pos[b];                  // (another thread may set it to -1: then this entry is denied too)
+        if (l.rank[l.start[b + 1] - 1] > found) {
+            l.pos[b] = -1;
+        } else if (f[j] & NEED) {
+            fresh[j] = l.fresh[l.rank[4 * t + j] - 1];
+            pg.row(b)[e[j]] = fresh[j];
+            pg.refs[fresh[j]] = 1;
+            count(pg, page[j], -1);
+            if (f[j] & SHARED && (int64_t)e[j] * pg.P < p) sum++;
+            else fresh[j] = -1;
+        }
+    }
+    at = block_scan(sum, l.sums, turn, all) - sum;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (fresh[j] >= 0) {
+            copies[2 * at] = page[j];
+            copies[2 * at++ + 1] = fresh[j];
+        }
+        if (4 * t + j < s.n_seq) pos_out[4 * t + j] = l.pos[4 * t + j];
+    }
+    if (t == 0) *n_copies = all;
+}
+
 // ---------------------------------------------------------------- compact
 
-constexpr int CP = 4096, CT = 256;               // pages and threads of a workgroup
+constexpr int CT = 256, CP = 4 * CT;             // threads and pages of a workgroup
 
 __device__ __forceinline__ int workgroup_sum(int v, int *red) {
     const int sum = __builtin_amdgcn_readlane(wave_scan(v), 63);
@@ -232,51 +418,64 @@ __device__ __forceinline__ int workgroup_sum(int v, int *red) {
 // Pages in use of each CP.
 __global__ __launch_bounds__(CT) void k_used(Pages pg, int32_t *counts) {
     __shared__ int red[CT / 64];
+    const uint32_t p = blockIdx.x * (uint32_t)CP + threadIdx.x;
     int n = 0;
-    for (uint32_t p = blockIdx.x * (uint32_t)CP + threadIdx.x, i = 0; i < CP / CT; i++, p += CT)
-        n += p < pg.n_pages && pg.refs[p] > 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) n += p + j * CT < pg.n_pages && pg.refs[p + j * CT] > 0;
     n = workgroup_sum(n, red);
     if (threadIdx.x == 0) counts[blockIdx.x] = n;
 }
 
 // With n pages in use: the k-th lowest free page goes into low[k] if it lies below n, the k-th
 // highest one in use into high[k] if it does not, which are as many, k into to[page]; to[page] of
-// a free one is -1.
-__global__ __launch_bounds__(CT) void k_rank(Pages pg, const int32_t *counts, int chunks, int32_t *low, int32_t *high, int32_t *to,
-                                             int32_t *n_moves) {
-    __shared__ int red[CT / 64], waves[CT / 64];
+// a free one is -1.  Without `counts` every workgroup counts all pages itself.
+__global__ __launch_bounds__(CT) void k_rank(Pages pg, const int32_t *counts, int32_t *low, int32_t *high, int32_t *to, int32_t *n_moves) {
+    __shared__ int red[CT / 64];
+    const uint32_t first = blockIdx.x * (uint32_t)CP;
+    int used[4], own = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t p = first + 4 * threadIdx.x + j;
+        own += used[j] = p < pg.n_pages && pg.refs[p] > 0;
+    }
     int before = 0, n = 0;
-    for (int i = threadIdx.x; i < chunks; i += CT) {
-        n += counts[i];
-        before += i < (int)blockIdx.x ? counts[i] : 0;
+    if (counts) {
+        for (int i = threadIdx.x; i < (int)gridDim.x; i += CT) {
+            n += counts[i];
+            before += i < (int)blockIdx.x ? counts[i] : 0;
+        }
+    } else {
+#pragma unroll 8
+        for (uint32_t p = threadIdx.x; p < pg.n_pages; p += CT) {
+            const int u = pg.refs[p] > 0;
+            n += u;
+            before += p < first ? u : 0;
+        }
     }
     n = workgroup_sum(n, red);
     before = workgroup_sum(before, red);
+    const int upto = wave_scan(own);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = upto;
+    __syncthreads();
+    int at = before + upto - own;                // pages in use before this thread's
+    for (int i = 0; i < (int)(threadIdx.x >> 6); i++) at += red[i];
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         n_moves[1] = n;
         if (n == 0) n_moves[0] = 0;
     }
-    for (uint32_t p0 = blockIdx.x * (uint32_t)CP; p0 < min(pg.n_pages, (blockIdx.x + 1) * (uint32_t)CP); p0 += CT) {
-        const uint32_t p = p0 + threadIdx.x;
-        const bool in = p < pg.n_pages, used = in && pg.refs[p] > 0;
-        const int sum = wave_scan(used);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = sum;
-        __syncthreads();
-        int at = before + sum - used;            // pages in use before this one
 #pragma unroll
-        for (int i = 0; i < CT / 64; i++) {
-            at += i < (int)(threadIdx.x >> 6) ? waves[i] : 0;
-            before += waves[i];
-        }
-        if (!in) continue;
+    for (int j = 0; j < 4; j++) {
+        const uint32_t p = first + 4 * threadIdx.x + j;
+        if (p >= pg.n_pages) break;
         if (p < (uint32_t)n) {
-            if (!used) low[p - at] = (int32_t)p;
-            if (p == (uint32_t)n - 1) n_moves[0] = (int)p - at + !used;
+            if (!used[j]) low[p - at] = (int32_t)p;
+            if (p == (uint32_t)n - 1) n_moves[0] = (int)p - at + !used[j];
         } else {
-            if (used) high[n - 1 - at] = (int32_t)p;
-            to[p] = used ? n - 1 - at : -1;
+            if (used[j]) high[n - 1 - at] = (int32_t)p;
+            to[p] = used[j] ? n - 1 - at : -1;
         }
+        at += used[j];
     }
 }
 
@@ -417,6 +616,12 @@ extern "C" int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pg, const gd_seqs *
     // Entries of the rows: a page for each page_size of them, and two ends a sequence.
     Work wk;
     wk.most = (int)(s->n_rows / pg->page_size + 2 * std::min<int64_t>(s->n_seq, s->n_rows));
+    if (s->n_seq <= FEW && wk.most <= FEW) {
+        hipLaunchKernelGGL(k_reserve_few, dim3(1), dim3(RT), 0, ctx->stream, pages_of(pg), rows, FastDiv((uint32_t)pg->page_size), wk.most,
+                           copies, n_copies, pos_out);
+        GD_LAUNCHED(ctx, fn);
+        return GD_OK;
+    }
     void *ws;
     if ((rc = gd_ctx_workspace(ctx, Work::ints(s->n_seq, pg->n_pages, wk.most) * 4, &ws))) return rc;
     int32_t *at = (int32_t *)ws;
@@ -440,13 +645,16 @@ extern "C" int gd_kv_compact(gd_ctx *ctx, const gd_kv_pages *pg, int32_t *moves,
     GD_CHECK_CTX(ctx);
     GD_HIP(ctx, hipSetDevice(ctx->device));
     const int chunks = (int)gd_blocks(pg->n_pages, CP);
+    const bool alone = pg->n_pages <= 16 * CP;   // pages that each workgroup of k_rank counts itself
     void *ws;
     if ((rc = gd_ctx_workspace(ctx, ((size_t)chunks + 3 * pg->n_pages) * 4, &ws))) return rc;
     int32_t *counts = (int32_t *)ws, *low = counts + chunks, *high = low + pg->n_pages, *to = high + pg->n_pages;
     const Pages p = pages_of(pg);
-    hipLaunchKernelGGL(k_used, dim3(chunks), dim3(CT), 0, ctx->stream, p, counts);
-    GD_LAUNCHED(ctx, fn);
-    hipLaunchKernelGGL(k_rank, dim3(chunks), dim3(CT), 0, ctx->stream, p, counts, chunks, low, high, to, n_moves);
+    if (!alone) {
+        hipLaunchKernelGGL(k_used, dim3(chunks), dim3(CT), 0, ctx->stream, p, counts);
+        GD_LAUNCHED(ctx, fn);
+    }
+    hipLaunchKernelGGL(k_rank, dim3(chunks), dim3(CT), 0, ctx->stream, p, alone ? nullptr : counts, low, high, to, n_moves);
     GD_LAUNCHED(ctx, fn);
     const int64_t entries = std::max<int64_t>((int64_t)pg->n_seq * pg->max_pages, pg->n_pages);
     hipLaunchKernelGGL(k_move, dim3(std::min<int64_t>((entries + CT - 1) / CT, 2048)), dim3(CT), 0, ctx->stream, p, low, high, to, n_moves,

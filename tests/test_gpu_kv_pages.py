@@ -214,7 +214,8 @@ def test_entries_that_name_no_page(ctx):
         d.compact()
 
 
-@pytest.mark.parametrize("size", SIZES, ids=str)
+# (The last ones pass 4096 sequences or entries of their rows.)
+@pytest.mark.parametrize("size", SIZES + [(4000, 2, 16, 9000), (4500, 3, 16, 15000), (3, 6000, 1, 20000)], ids=str)
 @pytest.mark.parametrize("tokens", [True, False], ids=["tokens", "chunks"])
 @pytest.mark.parametrize("seed", [0, 1, 2])
 def test_reserve(ctx, size, tokens, seed):
@@ -233,6 +234,18 @@ def test_reserve(ctx, size, tokens, seed):
             if not tokens and step == 4:
                 rows[-1] = width * P + 5                        # past the table
             d.reserve(pos.tolist(), rows.tolist(), tokens, in_place=step == 3)
+
+
+@pytest.mark.parametrize("n", [1000, 4096, 4097, 9000])
+@pytest.mark.parametrize("groups", [1, 7, 499])
+def test_reserve_many_that_share(ctx, n, groups):
+    """All sequences go on in a page that they share in groups: of each the last keeps it."""
+    with Device(ctx, n, 2, 16, n + 3 * groups) as d:
+        d.m.table[:, 0] = (np.arange(n) % groups) * 3
+        d.m.refs[:] = np.bincount(d.m.table[:, 0], minlength=len(d.m.refs))
+        d.set()
+        out, copies = d.reserve((np.arange(n) % 15 + 1).tolist(), [1] * n, True)
+        assert (out >= 0).all() and len(copies) == n - groups
 
 
 def test_reserve_shares_out(ctx):
@@ -263,11 +276,15 @@ def test_reserve_when_full_keeps_on(ctx):
 
 def test_rows_that_overlap_stay_in_bounds(ctx):
     """Row starts that do not ascend (which they must): something is reserved, nothing else touched."""
-    n = 1500
-    with Device(ctx, n, 40, 1, 70000) as d:
+    for n, width in ((1500, 40), (1200, 3), (5000, 40)):
+        overlap(ctx, n, width)
+
+
+def overlap(ctx, n, width):
+    with Device(ctx, n, width, 1, 70000) as d:
         s = d.seqs([0] * n, [1] * n, False)
         start = np.zeros(n + 1, I32)
-        start[1::2] = n                                         # 750 times all rows
+        start[1::2] = n                                         # every other one has all rows
         d.ctx.set(s.row_start, start)
         ctx.gd_kv_reserve(d.ref, C.byref(s), d.copies, d.n, d.pos_out)
         table, refs = ctx.get(d.table, d.m.table.shape, I32), ctx.get(d.refs, 70000, I32)
