@@ -32,9 +32,7 @@ constexpr int EW = 1024;                         // entries of a workgroup
 // written; counts are whole numbers, whose order of addition shows nowhere.
 __global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, const int32_t *dst, const int32_t *len, int n) {
     const int i = blockIdx.x, s = src[i], d = dst[i], most = len[i];
-    bool bad = (uint32_t)s >= (uint32_t)pg.n_seq || (uint32_t)d >= (uint32_t)pg.n_seq;
-    for (int j = threadIdx.x; j < n; j += 256) bad |= src[j] == d || (j > i && dst[j] == d);
-    if (__syncthreads_or(bad)) return;
+    if ((uint32_t)s >= (uint32_t)pg.n_seq || (uint32_t)d >= (uint32_t)pg.n_seq) return;
     const int32_t *from = pg.row(s);
     int32_t *to = pg.row(d);
     const int e0 = blockIdx.y * EW + threadIdx.x;
@@ -45,6 +43,9 @@ __global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, cons
         old[x] = e < pg.max_pages ? to[e] : -1;
         now[x] = e < pg.max_pages && (int64_t)e * pg.P < most ? from[e] : -1;
     }
+    bool bad = false;                            // (seen while the rows are on their way)
+    for (int j = threadIdx.x; j < n; j += 256) bad |= src[j] == d || (j > i && dst[j] == d);
+    if (__syncthreads_or(bad)) return;
 #pragma unroll
     for (int x = 0; x < EW / 256; x++) {
         if (!pg.there(now[x])) now[x] = -1;
@@ -56,43 +57,54 @@ __global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, cons
 }
 
 // Workgroup (order i, EW entries): sequence seq[i] drops the pages that hold no position of
-// from[i] .. to[i] - 1.  An entry is exchanged, so that one named twice is dropped once.
+// from[i] .. to[i] - 1, but for those that an order before it drops from the same sequence.
+// (By an exchange of each entry instead, 1 to 2 us more.)
 __global__ __launch_bounds__(256) void k_release(Pages pg, const int32_t *seq, const int32_t *from, const int32_t *to) {
     const int i = blockIdx.x, b = seq[i];
     if ((uint32_t)b >= (uint32_t)pg.n_seq) return;
-    const int64_t lo = from ? from[i] : 0, hi = to[i];
+    auto drops = [&](int i, int e) {
+        const int64_t p = (int64_t)e * pg.P;
+        return !(p + pg.P > (from ? from[i] : 0) && p < to[i]);
+    };
     int32_t *row = pg.row(b);
     const int e0 = blockIdx.y * EW + threadIdx.x;
     int old[EW / 256];
 #pragma unroll
     for (int x = 0; x < EW / 256; x++) {
         const int e = e0 + 256 * x;
-        const int64_t p = (int64_t)e * pg.P;
-        old[x] = e < pg.max_pages && !(p + pg.P > lo && p < hi) ? row[e] : -1;
+        old[x] = e < pg.max_pages && drops(i, e) ? row[e] : -1;
     }
+    bool before = false;
+    for (int j = threadIdx.x; j < i; j += 256) before |= seq[j] == b;
+    if (__syncthreads_or(before))
+        for (int j = 0; j < i; j++)
+            if (seq[j] == b)
+#pragma unroll
+                for (int x = 0; x < EW / 256; x++)
+                    if (drops(j, e0 + 256 * x)) old[x] = -1;
 #pragma unroll
     for (int x = 0; x < EW / 256; x++)
-        if (pg.there(old[x])) old[x] = __hip_atomic_exchange(&row[e0 + 256 * x], -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-    for (int x = 0; x < EW / 256; x++) count(pg, old[x], -1);
+        if (pg.there(old[x])) {
+            row[e0 + 256 * x] = -1;
+            count(pg, old[x], -1);
+        }
 }
 
 // ---------------------------------------------------------------- reserve
 
-constexpr int RT = 1024;                         // threads of the one workgroup
 
-// Sum over the threads up to this one; `all` gets the whole sum.  LDS `sums` of two times RT / 64
+// Sum over the threads up to this one; `all` gets the whole sum.  LDS `sums` of two times T / 64
 // ints, halves in turn (a barrier a call).  (Held at 2^29, which is over all entries that there
 // may be: sequences that share rows could pass 2^31.)
-__device__ __forceinline__ int block_scan(int v, int *sums, int &turn, int &all) {
+template <int T> __device__ __forceinline__ int block_scan(int v, int *sums, int &turn, int &all) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int sum = wave_scan(v);
-    int *s = sums + (turn ^= 1) * (RT / 64);
+    int *s = sums + (turn ^= 1) * (T / 64);
     if (lane == 63) s[w] = sum;
     __syncthreads();
     int before = 0;
     all = 0;
-    for (int i = 0; i < RT / 64; i++) {
+    for (int i = 0; i < T / 64; i++) {
         before = min(before + (i < w ? s[i] : 0), 1 << 29);
         all = min(all + s[i], 1 << 29);
     }
@@ -113,6 +125,7 @@ enum { NEED = 1, KEEP = 2, SHARED = 4, TAIL = 8 };
 // first free pages in order, the k-th need the k-th page.  A sequence gets all or nothing:
 // what it needs, if all up to it fits.
 //   The chain of its steps bounds it, some 0.7 us each.
+constexpr int RT = 1024;                         // threads
 __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_page, Work wk, int32_t *copies, int32_t *n_copies,
                                                 int32_t *pos_out) {
     __shared__ int sums[2 * RT / 64];
@@ -131,7 +144,7 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
                 n = (int)(by_page(last) - by_page(q.pos)) + 1;
             }
         }
-        const int upto = block_scan(n, sums, turn, all);
+        const int upto = block_scan<RT>(n, sums, turn, all);
         if (b < s.n_seq) {
             wk.start[b] = min(entries + upto - n, wk.most);
             pos_out[b] = pos;
@@ -183,7 +196,7 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
             else if (f & SHARED) f |= now(&wk.uses[page]) == pg.refs[page] && now(&wk.last[page]) == c ? KEEP : NEED;
             wk.flags[c] = f;
         }
-        const int upto = block_scan(f & NEED ? 1 : 0, sums, turn, all);
+        const int upto = block_scan<RT>(f & NEED ? 1 : 0, sums, turn, all);
         if (c < entries) wk.rank[c] = needs + upto;
         needs += all;
     }
@@ -194,7 +207,7 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
         int free[4], n = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) n += free[i] = p + i < pg.n_pages && pg.refs[p + i] <= 0;
-        int at = found + block_scan(n, sums, turn, all) - n;
+        int at = found + block_scan<RT>(n, sums, turn, all) - n;
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (free[i] && at < needs) wk.fresh[at++] = (int32_t)(p + i);
@@ -222,7 +235,7 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
                 }
             }
         }
-        const int upto = block_scan(copy, sums, turn, all);
+        const int upto = block_scan<RT>(copy, sums, turn, all);
         if (copy) {
             copies[2 * (copied + upto - 1)] = old;
             copies[2 * (copied + upto - 1) + 1] = page;
@@ -232,24 +245,26 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
     if (t == 0) *n_copies = copied;
 }
 
-// The same for FEW sequences and entries at most, in registers and LDS: a thread's four
+// The same for 4 T sequences and entries at most, in registers and LDS: a thread's four
 // sequences, four entries, four pages of a round.  Shared pages are counted in a table by a
 // hash of theirs, whose places depend on who comes first, but not what stands there.
 //   A chain of three loads (row, entry, count) bounds it.
-constexpr int FEW = 4 * RT, SLOTS = 2 * FEW;
-struct FewLds {
+template <int T> struct FewLds {
+    static constexpr int FEW = 4 * T, SLOTS = 2 * FEW;
     int pos[FEW], entry[FEW], start[FEW + 1];    // of a sequence: its position (-1: denied), first entry, and that one's place
     union {                                      // (one after the other)
         int owner[FEW];                          // the sequence that starts at an entry, from 1 on
         struct { int page[SLOTS], uses[SLOTS], last[SLOTS]; };
         struct { int rank[FEW], fresh[FEW]; };   // an entry's needs up to it; free pages
     };
-    int sums[2 * RT / 64];
+    int sums[2 * T / 64];
 };
 
-__global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by_page, int most, int32_t *copies, int32_t *n_copies,
+template <int T>
+__global__ __launch_bounds__(T) void k_reserve_few(Pages pg, Rows s, FastDiv by_page, int most, int32_t *copies, int32_t *n_copies,
                                                     int32_t *pos_out) {
-    __shared__ FewLds l;
+    __shared__ FewLds<T> l;
+    constexpr int FEW = l.FEW, SLOTS = l.SLOTS;
     const int t = threadIdx.x;
     int turn = 0, all;
     int refs[4];                                 // the first round's, on their way
@@ -271,7 +286,7 @@ __global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by
         }
         sum += n[j];
     }
-    int at = block_scan(sum, l.sums, turn, all) - sum;
+    int at = block_scan<T>(sum, l.sums, turn, all) - sum;
     const int entries = min(all, most);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -293,7 +308,7 @@ __global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by
     }
     int before = __shfl_up(top, 1, 64);
     if ((t & 63) == 0) before = 0;
-    int *w = l.sums + (turn ^= 1) * (RT / 64);
+    int *w = l.sums + (turn ^= 1) * (T / 64);
     if ((t & 63) == 63) w[t >> 6] = top;
     __syncthreads();
     for (int i = 0; i < (t >> 6); i++) before = max(before, w[i]);
@@ -319,14 +334,14 @@ __global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by
         some |= f[j] == SHARED;
     }
     if (__syncthreads_or(some)) {
-        for (int i = t; i < SLOTS; i += RT) {
+        for (int i = t; i < SLOTS; i += T) {
             l.page[i] = -1;
             l.uses[i] = 0;
             l.last[i] = -1;
         }
         __syncthreads();
         auto slot = [&](int page) {              // its place; every probe ends, as half of them are free
-            int i = (int)((uint32_t)page * 2654435761u >> 19) % SLOTS;
+            int i = (int)((uint32_t)page * 2654435761u >> 16) % SLOTS;
             for (;; i = (i + 1) % SLOTS) {
                 const int there = atomicCAS(&l.page[i], -1, page);
                 if (there == -1 || there == page) return i;
@@ -348,7 +363,7 @@ __global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by
     sum = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) sum += f[j] & NEED;
-    int rank = block_scan(sum, l.sums, turn, all) - sum;
+    int rank = block_scan<T>(sum, l.sums, turn, all) - sum;
     const int needs = all;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -356,7 +371,7 @@ __global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by
         if (4 * t + j < entries) l.rank[4 * t + j] = rank;
     }
     int found = 0;
-    for (uint32_t p0 = 0; p0 < pg.n_pages && found < needs; p0 += 4 * RT) {
+    for (uint32_t p0 = 0; p0 < pg.n_pages && found < needs; p0 += 4 * T) {
         const uint32_t p = p0 + 4 * t;
         if (p0)
 #pragma unroll
@@ -364,7 +379,7 @@ __global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by
         sum = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) sum += refs[j] <= 0;
-        int at = found + block_scan(sum, l.sums, turn, all) - sum;
+        int at = found + block_scan<T>(sum, l.sums, turn, all) - sum;
 #pragma unroll
         for (int j = 0; j < 4; j++)
             if (refs[j] <= 0 && at < needs) l.fresh[at++] = (int)(p + j);
@@ -391,7 +406,7 @@ __global__ __launch_bounds__(RT) void k_reserve_few(Pages pg, Rows s, FastDiv by
             else fresh[j] = -1;
         }
     }
-    at = block_scan(sum, l.sums, turn, all) - sum;
+    at = block_scan<T>(sum, l.sums, turn, all) - sum;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         if (fresh[j] >= 0) {
@@ -432,13 +447,20 @@ __global__ __launch_bounds__(CT) void k_used(Pages pg, int32_t *counts) {
 __global__ __launch_bounds__(CT) void k_rank(Pages pg, const int32_t *counts, int32_t *low, int32_t *high, int32_t *to, int32_t *n_moves) {
     __shared__ int red[CT / 64];
     const uint32_t first = blockIdx.x * (uint32_t)CP;
-    int used[4], own = 0;
+    // Which of pages p .. p + 3 are in use.
+    auto used_at = [&](uint32_t p, int (&used)[4]) {
+        typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+        i32x4 r = {0, 0, 0, 0};
+        if (p + 4 <= pg.n_pages) r = *(const i32x4 *)(pg.refs + p);
+        else
+            for (int j = 0; j < 4; j++) r[j] = p + j < pg.n_pages ? pg.refs[p + j] : 0;
+        int n = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t p = first + 4 * threadIdx.x + j;
-        own += used[j] = p < pg.n_pages && pg.refs[p] > 0;
-    }
-    int before = 0, n = 0;
+        for (int j = 0; j < 4; j++) n += used[j] = r[j] > 0;
+        return n;
+    };
+    int used[4], before = 0, n = 0;
+    const int own = used_at(first + 4 * threadIdx.x, used);
     if (counts) {
         for (int i = threadIdx.x; i < (int)gridDim.x; i += CT) {
             n += counts[i];
@@ -446,10 +468,11 @@ __global__ __launch_bounds__(CT) void k_rank(Pages pg, const int32_t *counts, in
         }
     } else {
 #pragma unroll 8
-        for (uint32_t p = threadIdx.x; p < pg.n_pages; p += CT) {
-            const int u = pg.refs[p] > 0;
+        for (uint32_t c = 0; c < gridDim.x; c++) {
+            int any[4];
+            const int u = used_at(c * CP + 4 * threadIdx.x, any);
             n += u;
-            before += p < first ? u : 0;
+            before += c < blockIdx.x ? u : 0;
         }
     }
     n = workgroup_sum(n, red);
@@ -483,6 +506,8 @@ __global__ __launch_bounds__(CT) void k_rank(Pages pg, const int32_t *counts, in
 __global__ __launch_bounds__(CT) void k_move(Pages pg, const int32_t *low, const int32_t *high, const int32_t *to, const int32_t *n_moves,
                                              int32_t *moves) {
     const int64_t i0 = blockIdx.x * (int64_t)CT + threadIdx.x, step = (int64_t)gridDim.x * CT;
+    const int64_t entries = (int64_t)pg.n_seq * pg.max_pages;
+    int page = i0 < entries ? pg.table[i0] : -1;     // (on its way beside the counts)
     const int n = n_moves[1], k = n_moves[0];
     for (int64_t i = i0; i < k; i += step) {
         const int src = high[i], dst = low[i];
@@ -492,9 +517,11 @@ __global__ __launch_bounds__(CT) void k_move(Pages pg, const int32_t *low, const
         pg.refs[src] = 0;
     }
     if (k == 0) return;
-    for (int64_t i = i0; i < (int64_t)pg.n_seq * pg.max_pages; i += step) {
-        const int page = pg.table[i];
-        if (page >= n && pg.there(page) && to[page] >= 0) pg.table[i] = low[to[page]];
+    for (int64_t i = i0; i < entries; i += step) {
+        if (i != i0) page = pg.table[i];
+        if (page < n || !pg.there(page)) continue;
+        const int at = to[page];
+        if (at >= 0) pg.table[i] = low[at];
     }
 }
 
@@ -616,9 +643,11 @@ extern "C" int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pg, const gd_seqs *
     // Entries of the rows: a page for each page_size of them, and two ends a sequence.
     Work wk;
     wk.most = (int)(s->n_rows / pg->page_size + 2 * std::min<int64_t>(s->n_seq, s->n_rows));
-    if (s->n_seq <= FEW && wk.most <= FEW) {
-        hipLaunchKernelGGL(k_reserve_few, dim3(1), dim3(RT), 0, ctx->stream, pages_of(pg), rows, FastDiv((uint32_t)pg->page_size), wk.most,
-                           copies, n_copies, pos_out);
+    const int few = std::max(s->n_seq, wk.most) <= 4 * 256 ? 256 : 1024;
+    if (std::max(s->n_seq, wk.most) <= 4 * few) {
+        auto kernel = few == 256 ? k_reserve_few<256> : k_reserve_few<1024>;
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(few), 0, ctx->stream, pages_of(pg), rows, FastDiv((uint32_t)pg->page_size), wk.most, copies,
+                           n_copies, pos_out);
         GD_LAUNCHED(ctx, fn);
         return GD_OK;
     }
