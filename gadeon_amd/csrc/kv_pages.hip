@@ -538,32 +538,43 @@ struct Layers {
 };
 
 // Workgroup (pairs from x on, plane y of the layers, slice z): SLICE bytes of a page, four
-// 16-byte loads a thread in flight.  Bytes bound it.
+// 16-byte loads a thread in flight.  Bytes bound it: 1750 pages of 32 KiB in 16 planes, 1 GB read
+// and written, 176 us, 5.7 TB/s.  What is written goes past the caches (copies of a step in 16
+// layers 17.2 -> 16.4 us, large ones 207 -> 202), and so does what is read where it is more than
+// they hold for long (-> 196; few pages, which later calls copy again, 16.4 -> 20.5): LARGE.
 constexpr uint32_t SLICE = 16384;
+constexpr uint64_t LARGE = 96u << 20;            // bytes: 80 MB copied 38 us so, 42 past the caches, 120 MB 60 and 58
 __global__ __launch_bounds__(256) void k_copy(Layers layers, uint32_t n_pages, const int32_t *pairs, const int32_t *n_pairs, int most) {
     const Layer l = layers.l[blockIdx.y >> 1];
     const bool is_k = !(blockIdx.y & 1);
     char *plane = (char *)(is_k ? l.k : l.v);
     uint8_t *exps = is_k ? l.kx : l.vx;
     const int n = n_pairs ? min(max(*n_pairs, 0), most) : most;
+    const bool large = (uint64_t)n * l.bytes * gridDim.y > LARGE;
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
         const int src = pairs[2 * i], dst = pairs[2 * i + 1];
         if ((uint32_t)src >= n_pages || (uint32_t)dst >= n_pages || src == dst) continue;
         const char *x = plane + (uint64_t)src * l.bytes;
         char *y = plane + (uint64_t)dst * l.bytes;
-        for (uint64_t at = (uint64_t)blockIdx.z * SLICE; at < l.bytes; at += (uint64_t)gridDim.z * SLICE) {
-            u32x4 r[SLICE / 4096];
+        auto slices = [&](auto past) {
+            for (uint64_t at = (uint64_t)blockIdx.z * SLICE; at < l.bytes; at += (uint64_t)gridDim.z * SLICE) {
+                u32x4 r[SLICE / 4096];
 #pragma unroll
-            for (uint32_t j = 0; j < SLICE / 4096; j++) {
-                const uint64_t a = at + j * 4096 + threadIdx.x * 16;
-                if (a < l.bytes) r[j] = *(const u32x4 *)(x + a);
-            }
+                for (uint32_t j = 0; j < SLICE / 4096; j++) {
+                    const uint64_t a = at + j * 4096 + threadIdx.x * 16;
+                    if (a >= l.bytes) continue;
+                    if constexpr (past) r[j] = __builtin_nontemporal_load((const u32x4 *)(x + a));
+                    else r[j] = *(const u32x4 *)(x + a);
+                }
 #pragma unroll
-            for (uint32_t j = 0; j < SLICE / 4096; j++) {
-                const uint64_t a = at + j * 4096 + threadIdx.x * 16;
-                if (a < l.bytes) *(u32x4 *)(y + a) = r[j];
+                for (uint32_t j = 0; j < SLICE / 4096; j++) {
+                    const uint64_t a = at + j * 4096 + threadIdx.x * 16;
+                    if (a < l.bytes) __builtin_nontemporal_store(r[j], (u32x4 *)(y + a));
+                }
             }
-        }
+        };
+        if (large) slices(std::true_type());
+        else slices(std::false_type());
         if (blockIdx.z == 0)
             for (uint32_t j = threadIdx.x; j < l.exps; j += 256)
                 exps[(uint64_t)dst * l.exps + j] = exps[(uint64_t)src * l.exps + j];
@@ -721,7 +732,7 @@ extern "C" int gd_kv_copy_pages(gd_ctx *ctx, const gd_kv *kv, int n_kv, const in
             widest = std::max(widest, layers.l[i].bytes);
         }
         const int64_t slices = std::min<int64_t>(((int64_t)widest + SLICE - 1) / SLICE, 1024);
-        const int64_t x = std::min<int64_t>(max_pairs, std::max<int64_t>(1, 4096 / (2 * n * slices)));
+        const int64_t x = std::min<int64_t>(max_pairs, std::max<int64_t>(1, 16384 / (2 * n * slices)));
         hipLaunchKernelGGL(k_copy, dim3((unsigned)x, 2 * n, (unsigned)slices), dim3(256), 0, ctx->stream, layers, (uint32_t)kv[0].n_pages,
                            pairs, n_pairs, (int)max_pairs);
         GD_LAUNCHED(ctx, fn);
