@@ -246,7 +246,7 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
 }
 
 // The same for 4 T sequences and entries at most, in registers and LDS: a thread's four
-// sequences, four entries, four pages of a round.  Shared pages are counted in a table by a
+// sequences, four entries, sixteen pages of a round.  Shared pages are counted in a table by a
 // hash of theirs, whose places depend on who comes first, but not what stands there.
 //   A chain of three loads (row, entry, count) bounds it.
 template <int T> struct FewLds {
@@ -267,9 +267,23 @@ __global__ __launch_bounds__(T) void k_reserve_few(Pages pg, Rows s, FastDiv by_
     constexpr int FEW = l.FEW, SLOTS = l.SLOTS;
     const int t = threadIdx.x;
     int turn = 0, all;
-    int refs[4];                                 // the first round's, on their way
+    // Which of the pages p .. p + 15 are free, a bit each; the first round's on their way.
+    auto free_of = [&](uint32_t p) {
+        typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+        i32x4 r[4];
+        uint32_t free = 0;
+        if (p + 16 <= pg.n_pages) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) refs[j] = 4u * t + j < pg.n_pages ? pg.refs[4 * t + j] : 1;
+            for (int j = 0; j < 4; j++) r[j] = *(const i32x4 *)(pg.refs + p + 4 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) r[j / 4][j % 4] = p + j < pg.n_pages ? pg.refs[p + j] : 1;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) free |= (r[j / 4][j % 4] <= 0) << j;
+        return free;
+    };
+    uint32_t free = free_of(16 * t);
     int n[4], sum = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -371,18 +385,12 @@ __global__ __launch_bounds__(T) void k_reserve_few(Pages pg, Rows s, FastDiv by_
         if (4 * t + j < entries) l.rank[4 * t + j] = rank;
     }
     int found = 0;
-    for (uint32_t p0 = 0; p0 < pg.n_pages && found < needs; p0 += 4 * T) {
-        const uint32_t p = p0 + 4 * t;
-        if (p0)
-#pragma unroll
-            for (int j = 0; j < 4; j++) refs[j] = p + j < pg.n_pages ? pg.refs[p + j] : 1;
-        sum = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) sum += refs[j] <= 0;
+    for (uint32_t p0 = 0; p0 < pg.n_pages && found < needs; p0 += 16 * T) {
+        const uint32_t p = p0 + 16 * t;
+        if (p0) free = free_of(p);
+        sum = __popc(free);
         int at = found + block_scan<T>(sum, l.sums, turn, all) - sum;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (refs[j] <= 0 && at < needs) l.fresh[at++] = (int)(p + j);
+        for (; free && at < needs; free &= free - 1) l.fresh[at++] = (int)p + __ffs(free) - 1;
         found += all;
     }
     __syncthreads();
@@ -549,10 +557,14 @@ __global__ __launch_bounds__(256) void k_copy(Layers layers, uint32_t n_pages, c
     const bool is_k = !(blockIdx.y & 1);
     char *plane = (char *)(is_k ? l.k : l.v);
     uint8_t *exps = is_k ? l.kx : l.vx;
+    int i = blockIdx.x, src = pairs[2 * i], dst = pairs[2 * i + 1];    // (on their way beside the count)
     const int n = n_pairs ? min(max(*n_pairs, 0), most) : most;
     const bool large = (uint64_t)n * l.bytes * gridDim.y > LARGE;
-    for (int i = blockIdx.x; i < n; i += gridDim.x) {
-        const int src = pairs[2 * i], dst = pairs[2 * i + 1];
+    for (; i < n; i += gridDim.x) {
+        if (i != (int)blockIdx.x) {
+            src = pairs[2 * i];
+            dst = pairs[2 * i + 1];
+        }
         if ((uint32_t)src >= n_pages || (uint32_t)dst >= n_pages || src == dst) continue;
         const char *x = plane + (uint64_t)src * l.bytes;
         char *y = plane + (uint64_t)dst * l.bytes;
