@@ -13,15 +13,23 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct Mask {
     int window, sinks;                           // window 0: every key up to the query's own
     static constexpr bool SCORED = false;
+    using Tokens = Mask;                         // what k_attn_tokens is compiled for
 };
 // Beside that (gd_scores): scores capped at `cap` and -slope[h] times the distance added, both
 // in units of log2; no key before first[row], and every key before prefix[b].
-struct Scores {
+struct ScoreArgs {
     int window, sinks;
-    float cap, p[5];                             // 0: none; cap P (cap_scores)
+    float cap;                                   // 0: none
     const float *slope;
     const int32_t *first, *prefix;
-    static constexpr bool SCORED = true;
+};
+// BY_EXP: there is a cap, and an exponential makes it (cap_score); prompt chunks are compiled for
+// that apart, as a branch to the other ways in their loop costs registers (1021 f32 rows after 3003 of 16
+// heads, capped and biased, 97 us; 106 with the branch).
+template <bool BY_EXP_> struct Scores : ScoreArgs {
+    static constexpr bool SCORED = true, BY_EXP = BY_EXP_;
+    using Tokens = Scores<false>;
+    operator Tokens() const { return {*this}; }
 };
 
 // Four codes as two pairs of halves: byte c ^ 0x80 below 0x64 is the half 1152 + c.
@@ -61,7 +69,7 @@ template <int W> struct KeyBlocks {
 template <int W> struct ScoredBlocks {
     uint32_t lo, sinks, doc;
     int ns, n, from;                             // blocks of sinks, in all; the first of them
-    __device__ __forceinline__ ScoredBlocks(const Scores &m, uint32_t first, uint32_t last, uint32_t prefix, uint32_t doc_) : doc(doc_) {
+    __device__ __forceinline__ ScoredBlocks(const ScoreArgs &m, uint32_t first, uint32_t last, uint32_t prefix, uint32_t doc_) : doc(doc_) {
         lo = m.window && first >= (uint32_t)m.window ? first - m.window + 1 : 0;
         sinks = min(max((uint32_t)m.sinks, prefix), lo);
         from = (int)(doc / W);
@@ -82,7 +90,7 @@ template <int W> __device__ __forceinline__ KeyBlocks<W> blocks_of(const Mask &m
     return KeyBlocks<W>(m, first, last);
 }
 template <int W>
-__device__ __forceinline__ ScoredBlocks<W> blocks_of(const Scores &m, uint32_t first, uint32_t last, uint32_t prefix, uint32_t doc) {
+__device__ __forceinline__ ScoredBlocks<W> blocks_of(const ScoreArgs &m, uint32_t first, uint32_t last, uint32_t prefix, uint32_t doc) {
     return ScoredBlocks<W>(m, first, last, prefix, doc);
 }
 // A sequence's prefix and a row's document's first position (0: none).
@@ -95,40 +103,30 @@ template <class How> __device__ __forceinline__ uint32_t doc_of(const How &m, in
     else return 0;
 }
 
-// cap tanh(x), x = v[i] to_x: scores over their cap, all of a wave's in one of two ways.  Where
-// every |x| is under 1/2, as cap x P(x^2), P the polynomial of least relative error (2^-26; of
-// one degree less 2^-20, which f16 rows take); else as cap - 2 cap / (1 + e^2x), whose error of
-// some 2^-24 of the cap is then one of the greatest score's own.  (Seven or six instructions a
-// score, and three with two of a quarter's rate; both and a choice of either cost 22.)
-template <bool FINE, int N, int V, class Vec>
-__device__ __forceinline__ void cap_scores(const Scores &how, float to_x, Vec (&s)[N]) {
-    float most = 0.f;
+// Scores s capped: cap tanh(x), x = s to_x.  BY_EXP as cap - 2 cap / (1 + e^2x), off by some
+// 2^-23 of the cap: for caps that this is little of, up to EXP_CAP (what the scores' sums of
+// products lose; of f16 rows, whose weights are rounded to 2^-11, EXP_CAP_F16).  Else as cap x P(x^2) /
+// Q(x^2), off by 2^-25.5 of itself at most over |x| <= TANH_END, from where on tanh is 1 to 2^-25:
+// degrees and coefficients by least squares reweighted to the least relative error, all of them
+// positive.  In slots of an instruction at full rate 11 and 17 a score.
+//   (Measured and left out: where all scores of a wave are under half the cap, the polynomial of
+// tanh alone, 6 or 7: 107 us where one way alone takes 97; and what a row sees made its neighbours' last bits.)
+constexpr float TANH_END = 9.02f, EXP_CAP = 64.f, EXP_CAP_F16 = 1024.f;
+template <bool BY_EXP> __device__ __forceinline__ float cap_score(const ScoreArgs &how, float s, float to_x) {
+    if constexpr (!BY_EXP) {
+        const float x = __builtin_amdgcn_fmed3f(s * to_x, -TANH_END, TANH_END), u = x * x;
+        const float p = fmaf(fmaf(fmaf(fmaf(u, 1.33190953e-08f, 2.05835024e-05f), u, 3.49403605e-03f), u, 1.33797193e-01f), u, 9.99999979e-01f);
+        const float q = fmaf(fmaf(fmaf(fmaf(u, 7.76203024e-07f, 3.28309512e-04f), u, 2.58710791e-02f), u, 4.67130345e-01f), u, 1.f);
+        return how.cap * x * (p * __builtin_amdgcn_rcpf(q));
+    } else {
+        return fmaf(-2.f * how.cap, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * (to_x * (2.f * LOG2E)))), how.cap);
+    }
+}
+template <bool BY_EXP, int N, int V, class Vec> __device__ __forceinline__ void cap_scores(const ScoreArgs &how, float to_x, Vec (&s)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
-        for (int v = 0; v < V; v++) most = fmaxf(most, fabsf(s[i][v]));
-    if (__any(!(most * fabsf(to_x) < 0.5f))) {
-        const float to_e = to_x * (2.f * LOG2E);
-#pragma unroll
-        for (int i = 0; i < N; i++)
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                const float e = __builtin_amdgcn_exp2f(s[i][v] * to_e);
-                s[i][v] = fmaf(-2.f * how.cap, __builtin_amdgcn_rcpf(1.f + e), how.cap);
-                if (v % 8 == 7) __builtin_amdgcn_sched_barrier(0);
-            }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++)
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                const float x = s[i][v] * to_x, u = x * x;
-                float p = FINE ? fmaf(u, how.p[4], how.p[3]) : how.p[3];
-                p = fmaf(u, fmaf(u, fmaf(u, p, how.p[2]), how.p[1]), how.p[0]);
-                s[i][v] = x * p;
-                if (v % 8 == 7) __builtin_amdgcn_sched_barrier(0);
-            }
-    }
+        for (int v = 0; v < V; v++) s[i][v] = cap_score<BY_EXP>(how, s[i][v], to_x);
 }
 
 // Partials of the key splits: sums of head h of row n, split z, at acc [n H + h][most][HD]
@@ -448,8 +446,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
         };
         if constexpr (How::SCORED) {
             if (mask.cap > 0.f) {
-                unseen(0.f);                     // (what is not seen has no part in how the others are capped)
-                cap_scores<true, 2, 4>(mask, to_x, sc);
+                cap_scores<false, 2, 4>(mask, to_x, sc);
             } else {
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++) sc[kt] *= sf;
@@ -874,7 +871,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     float to_x = 0.f, capped = sf, unit = sf;
     if constexpr (How::SCORED) {
         to_x = sf / mask.cap;
-        if (mask.cap > 0.f) capped = unit = 1.f;
+        if (How::BY_EXP || mask.cap > 0.f) capped = unit = 1.f;
         if (mask.slope) unit = 1.f;
     }
     // Row 8 (v / 4) + 4 h + v % 4 of a C value v (MF 16: 4 h + v).
@@ -944,10 +941,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
                 }
             };
             if constexpr (How::SCORED) {
-                if (mask.cap > 0.f) {
-                    unseen(0.f);                 // (what nobody sees has no part in how the others are capped)
-                    cap_scores<HL, NT, NV>(mask, to_x, st);
-                }
+                if constexpr (How::BY_EXP) cap_scores<true, NT, NV>(mask, to_x, st);
+                else if (mask.cap > 0.f) cap_scores<false, NT, NV>(mask, to_x, st);
                 if (mask.slope) {
                     const float d = (float)(int)(p - k0 - 4 * h);
 #pragma unroll
@@ -1279,10 +1274,16 @@ int attn(gd_ctx *ctx, const char *fn, const AttnArgs &a, int window, int n_sink,
 #define GD_GO(HD_, I8_, T_) \
     do { \
         const bool tiled = I8_ || kv->page_size % 16 == 0; \
-        auto kernel = tokens ? (tiled ? k_attn_tokens<HD_, I8_, true, T_, How> : k_attn_tokens<HD_, I8_, I8_, T_, How>) \
-                             : (tiled ? k_attn_rows<HD_, I8_, true, T_, How> : k_attn_rows<HD_, I8_, I8_, T_, How>); \
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, cache_of(kv), rows, (const T_ *)q, q_stride, \
-                           (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)slots, n_head, scale, mask); \
+        if (tokens) { \
+            auto kernel = tiled ? k_attn_tokens<HD_, I8_, true, T_, typename How::Tokens> : k_attn_tokens<HD_, I8_, I8_, T_, typename How::Tokens>; \
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, cache_of(kv), rows, (const T_ *)q, q_stride, \
+                               (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)slots, n_head, scale, \
+                               (typename How::Tokens)mask); \
+        } else { \
+            auto kernel = tiled ? k_attn_rows<HD_, I8_, true, T_, How> : k_attn_rows<HD_, I8_, I8_, T_, How>; \
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, cache_of(kv), rows, (const T_ *)q, q_stride, \
+                               (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)slots, n_head, scale, mask); \
+        } \
         if (ns > 1) { \
             GD_LAUNCHED(ctx, fn); \
             /* (a workgroup a row and head: one token of 24 heads, 64 splits, 24 us, by the other \

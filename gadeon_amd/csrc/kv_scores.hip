@@ -17,11 +17,8 @@ extern "C" int gd_kv_attn_scored(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s,
     const int window = how->window, sinks = window ? how->n_sink : 0;
     if (how->cap == 0.f && !how->slope && !how->first && !how->prefix)
         return gd_kv_attn(ctx, kv, s, q, q_stride, gate, gate_stride, out, x_dtype, n_head, scale, window, how->n_sink);
-    // tanh(x) / x over x^2 < 1/4: of degree 4 to 2^-26 of itself, and of degree 3 to 2^-20.
-    static const float fine[] = {1.f, -0.333331435918808f, 0.13325878977775574f, -0.05304549261927605f, 0.01724149100482464f};
-    static const float f16[] = {1.f, -0.33328160643577576f, 0.13205359876155853f, -0.0447506420314312f, 0.f};
-    const float cap = how->cap * LOG2E;
-    Scores mask{window, sinks, cap, {}, how->slope, how->first, how->prefix};
-    for (int i = 0; i < 5; i++) mask.p[i] = cap * (x_dtype == GD_F32 || !s || !s->row_start ? fine : f16)[i];
-    return attn(ctx, fn, a, window, how->n_sink, mask, !how->prefix);
+    const ScoreArgs args{window, sinks, how->cap * LOG2E, how->slope, how->first, how->prefix};
+    if (how->cap > 0.f && how->cap <= (x_dtype == GD_F32 ? EXP_CAP : EXP_CAP_F16))
+        return attn(ctx, fn, a, window, how->n_sink, Scores<true>{args}, !how->prefix);
+    return attn(ctx, fn, a, window, how->n_sink, Scores<false>{args}, !how->prefix);
 }
