@@ -637,8 +637,16 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     // V rows padded so that a transposing read's 32 lanes (MF 32: four rows of 32 dims, else
     // eight of 16) lie in 64 different banks.
     constexpr int KP = HD + 8, VP = HD + (MF == 32 ? 32 : 16), FD = 4;
-    __shared__ __attribute__((aligned(16))) f16 Ks[2][AK][KP];
-    __shared__ __attribute__((aligned(16))) f16 Vs[2][AK][VP];
+    constexpr int OP = HD + 4;
+    __shared__ union __attribute__((aligned(16))) {
+        struct {
+            f16 K[2][AK][KP], V[2][AK][VP];
+        };
+        float O[PC][OP];                         // at the end, the columns' results
+    } lds;
+    auto &Ks = lds.K;
+    auto &Vs = lds.V;
+    __shared__ int2 out_row[PC];                 // of a column: its row, and that times H + its head (-1 past the last one)
     __shared__ uint8_t odd[2][AK][HD / 8];       // which values of V are no numbers, a bit each
     __shared__ int any_odd[2];
     const int G = H / c.HKV, kvh = blockIdx.x % c.HKV;
@@ -695,6 +703,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     const int head = kvh * G + (valid ? col % G : G - 1);
     const int64_t n = sq.r0 + i;
     const uint32_t p = p0 + i;
+    if (h == 0) out_row[MF * w + lc] = make_int2((int)n, valid ? (int)n * H + head : -1);
     const bool busy = k * PC + MF * w < rows * G;
     const uint32_t plo = p0 + min((k * PC + MF * w) / G, rows - 1);
     const uint32_t seen_from = mask.window && plo >= (uint32_t)mask.window ? plo - mask.window + 1 : 0;
@@ -1044,42 +1053,55 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         }
         now = next;
     }
-    if (!valid) return;
+    // Through LDS, so that a row is written, and its gate read, in whole lines.
+    constexpr int TPR = HD / 8, RPP = 256 / TPR, PASS = PC / RPP;    // threads of a row, eight dims each; rows of a pass
+    const int d = 8 * (t % TPR);
+    typedef T T8 __attribute__((ext_vector_type(8), aligned(16)));
+    T8 gates[PASS];
+    if (gate && nz == 1)
+#pragma unroll
+        for (int x = 0; x < PASS; x++) {
+            const int2 row = out_row[x * RPP + t / TPR];
+            if (row.y >= 0) gates[x] = *(const T8 *)(gate + row.x * gate_stride + (row.y - (int64_t)row.x * H) * HD + d);
+        }
     if constexpr (MF == 16) l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    const int64_t row = n * H + head;
-    if (most > 1 && z == 0 && h == 0) part.used[row] = nz;
-    if (nz > 1) {
-        float *y = part.acc + (row * most + z) * HD + 4 * h;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-            for (int v = 0; v < NV; v += 4)
-                *(f32x4 *)(y + MF * dt + 2 * v) = f32x4{acc[dt][v], acc[dt][v + 1], acc[dt][v + 2], acc[dt][v + 3]};
-        if (h == 0) part.ml[row * most + z] = make_float2(m, l);
-        return;
+    if (valid && h == 0) {
+        const int64_t row = n * H + head;
+        if (most > 1 && z == 0) part.used[row] = nz;
+        if (nz > 1) part.ml[row * most + z] = make_float2(m, l);
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = nz > 1 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-        for (int v = 0; v < NV; v += 4) {
-            const int d = MF * dt + 2 * v + 4 * h;
-            float y[4];
+        for (int v = 0; v < NV; v += 4)
+            *(f32x4 *)&lds.O[MF * w + lc][MF * dt + 2 * v + 4 * h] =
+                    f32x4{acc[dt][v] * inv, acc[dt][v + 1] * inv, acc[dt][v + 2] * inv, acc[dt][v + 3] * inv};
+    __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = acc[dt][v + e] * inv;
-            if (gate) {
-                const T *gr = gate + n * gate_stride + (int64_t)head * HD + d;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    y[e] *= HL ? gd_sigmoid(to_f32(gr[e])) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * to_f32(gr[e])));
-            }
-            if constexpr (HL)
-                *(f32x4 *)(out + row * HD + d) = f32x4{y[0], y[1], y[2], y[3]};
-            else
-                *(uint64_t *)(out + row * HD + d) = (uint64_t)gd_f2h(y[0]) | ((uint64_t)gd_f2h(y[1]) << 16) |
-                                                    ((uint64_t)gd_f2h(y[2]) << 32) | ((uint64_t)gd_f2h(y[3]) << 48);
+    for (int x = 0; x < PASS; x++) {
+        const int r = x * RPP + t / TPR;
+        const int64_t row = out_row[r].y;
+        if (row < 0) continue;
+        f32x4 y[2] = {*(const f32x4 *)&lds.O[r][d], *(const f32x4 *)&lds.O[r][d + 4]};
+        if (nz > 1) {
+            float *p = part.acc + (row * most + z) * HD + d;
+            *(f32x4 *)p = y[0];
+            *(f32x4 *)(p + 4) = y[1];
+            continue;
         }
+        if (gate)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float g = to_f32<T>(gates[x][e]);
+                y[e / 4][e % 4] *= HL ? gd_sigmoid(g) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * g));
+            }
+        T8 o;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = from_f32<T>(y[e / 4][e % 4]);
+        *(T8 *)(out + row * HD + d) = o;
+    }
 }
 
 // Whether row n has a sequence (else nobody has written anything for it).

@@ -78,9 +78,12 @@ __device__ __forceinline__ float wave_max(float v) {
     return fmaxf(fmaxf(row(0), row(16)), fmaxf(row(32), row(48)));
 }
 __device__ __forceinline__ uint32_t wave_least(uint32_t v) {
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) v = min(v, (uint32_t)__shfl_xor((int)v, i, 64));
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+    v = min(v, __float_as_uint(gd_dpp<GD_DPP_XOR1>(__uint_as_float(v))));
+    v = min(v, __float_as_uint(gd_dpp<GD_DPP_XOR2>(__uint_as_float(v))));
+    v = min(v, __float_as_uint(gd_dpp<GD_DPP_HALF_MIRROR>(__uint_as_float(v))));
+    v = min(v, __float_as_uint(gd_dpp<GD_DPP_MIRROR>(__uint_as_float(v))));
+    auto row = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    return min(min(row(0), row(16)), min(row(32), row(48)));
 }
 __device__ __forceinline__ int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // from 1, 2, 4, 8 lanes below in the row
