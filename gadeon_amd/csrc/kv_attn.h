@@ -363,12 +363,15 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
             Qs[w * KW + i][lane] = qf;
         }
     }
-    const float none = sf < 0.f && !How::SCORED ? INFINITY : -INFINITY;    // the score of no key
-    float slope = 0.f;                           // of this lane's head
-    if constexpr (How::SCORED)
+    // A score over its cap; the units of scores once they are capped, and once they are biased.
+    float slope = 0.f, to_x = 0.f, capped = sf, unit = sf;
+    if constexpr (How::SCORED) {
         if (mask.slope) slope = mask.slope[h0 + min(col, nh - 1)] * LOG2E;
-    float to_x = 0.f;                            // a score over its cap
-    if constexpr (How::SCORED) to_x = sf / mask.cap;
+        to_x = sf / mask.cap;
+        if (mask.cap > 0.f) capped = unit = 1.f;
+        if (mask.slope) unit = 1.f;
+    }
+    const float none = unit < 0.f ? INFINITY : -INFINITY;    // the score of no key
     f32x4 acc[DT];                               // O^T rows 16 dt + 4 g + v
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -445,19 +448,14 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
                 for (int v = 0; v < 4; v++) sc[kt][v] = mine & (1u << (16 * kt + v)) ? sc[kt][v] : x;
         };
         if constexpr (How::SCORED) {
-            if (mask.cap > 0.f) {
-                cap_scores<false, 2, 4>(mask, to_x, sc);
-            } else {
-#pragma unroll
-                for (int kt = 0; kt < 2; kt++) sc[kt] *= sf;
-            }
+            if (mask.cap > 0.f) cap_scores<false, 2, 4>(mask, to_x, sc);
             if (mask.slope) {
                 // (All seen keys lie before the token.)
-                const float d = (float)(int)((uint32_t)pos - kb.start(now) - 4 * g);
+                const float b = -slope * (float)(int)((uint32_t)pos - kb.start(now) - 4 * g);
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-                    for (int v = 0; v < 4; v++) sc[kt][v] = fmaf(-slope, d - (float)(16 * kt + v), sc[kt][v]);
+                    for (int v = 0; v < 4; v++) sc[kt][v] = fmaf(sc[kt][v], capped, fmaf(slope, (float)(16 * kt + v), b));
             }
         }
         unseen(none);
@@ -465,7 +463,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-            for (int v = 0; v < 4; v++) top = fmaxf(top, How::SCORED ? sc[kt][v] : sc[kt][v] * sf);
+            for (int v = 0; v < 4; v++) top = fmaxf(top, sc[kt][v] * unit);
         // The sums are brought to a new maximum, of all a column's lanes, only where one is
         // over 2^LAZY of the one they stand at.
         if (__any(top > m + LAZY)) {
@@ -482,7 +480,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int v = 0; v < 4; v++) {
-                float p = __builtin_amdgcn_exp2f(How::SCORED ? sc[kt][v] - m : fmaf(sc[kt][v], sf, -m)) * 256.f;
+                float p = __builtin_amdgcn_exp2f(fmaf(sc[kt][v], unit, -m)) * 256.f;
                 asm("" : "+v"(p));
                 l += p;
                 const f16 hi = (f16)p;

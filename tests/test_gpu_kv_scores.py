@@ -162,6 +162,29 @@ def test_split_keys(ctx, dtype, what):
             check(ctx, seqs, dtype, n == 40, 256 if n == 3 else 128, 6, 2, 16, what, gated=n == 3, row_start=start, seed=n)
 
 
+@pytest.mark.parametrize("H,hkv,rows", [(40, 8, 1700), (24, 1, 2800)])
+def test_documents_of_many_units(ctx, H, hkv, rows):
+    """More workgroups than the chip holds, which go by their documents' lengths; over 512 units of a
+    sequence, where they do not."""
+    seqs = [(0, rows), (50, 130), (700, 1)]
+    with Batch(ctx, seqs, ga.F16, hkv, 128, 16) as bt:
+        KV, rng = bt.fill(), bt.rng
+        q = (rows_of(rng, (bt.n, H, 128), True) * 3).astype(np.float16)
+        first, _ = masks(rng, seqs, "odd", False)
+        first[:rows] = np.minimum(np.sort(rng.choice(rows, 9))[rng.integers(0, 9, rows // 100 + 1)].repeat(100)[:rows], np.arange(rows))
+        got, again = run(ctx, bt, q, q, dict(first=first, cap=20.0))
+        for b, (p, r) in enumerate(seqs):
+            at = slice(bt.start[b], bt.start[b] + r)
+            pick = [0, H // 2, H - 1]                       # (heads of the first and the last kv head)
+            for h in pick:
+                one = lambda x: x[at][:, h:h + 1]           # noqa: E731
+                K, V = (c[:, h // (H // hkv)][:, None] for c in KV[b])
+                want = attend(one(q), K, V, p, np.float32(0.1), 0, 0, one(q), 20.0, None, first[at])
+                err, most = np.abs(one(got) - want).max(), most_off(one(q), K, V, p, 0.1, True, 20.0, None)
+                assert err <= most, (b, h, err, most)
+        assert np.array_equal(again(), got)
+
+
 @pytest.mark.parametrize("x16", [False, True], ids=["f32rows", "f16rows"])
 def test_plain_scores_are_the_other_entrys(ctx, x16):
     """No cap and no arrays: gd_kv_attn's results; arrays that change nothing: within its bound."""
