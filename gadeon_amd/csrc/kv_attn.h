@@ -239,8 +239,17 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
         const int least = token_least(s, mask, groups, slots, token_fewest(HD));
         auto splits = [&](const Seq &q, int b) { return q.r1 > q.r0 ? token_blocks(s, mask, b, q.pos).splits(most, least) : 0; };
         Seq sq;
-        auto order = [&](const Seq &q, int b) { return q.r1 > q.r0 && token_blocks(s, mask, b, q.pos).n > 0.5f * least ? 0 : 1; };
-        if (!unit_at<2>(s, n, splits, order, n, sp, sq)) return;
+        //   A workgroup a CU (ONE): by the splits' lengths in quarters, as a slot's last one is not
+        // hidden behind another: 64 of up to 12000, halves, 24 of 256 on 4, 111 us in two classes, 102
+        // in four, under a window of 4096 83 and 75.5; codes of 128, two a CU, 34.8 and 35.2.
+        constexpr bool ONE = !I8 && HD == 256;
+        auto order = [&](const Seq &q, int b) {
+            const Blocks<32, How> kb = token_blocks(s, mask, b, q.pos);
+            if (!ONE) return q.r1 > q.r0 && kb.n > 0.5f * least ? 0 : 1;
+            const float part = q.r1 > q.r0 ? (float)kb.n / (float)(kb.splits(most, least) * least) : 0.f;
+            return part > 0.75f ? 0 : part > 0.5f ? 1 : part > 0.25f ? 2 : 3;
+        };
+        if (!unit_at<ONE ? 4 : 2>(s, n, splits, order, n, sp, sq)) return;
         pos = sq.pos;
         ns = token_blocks(s, mask, n, pos).splits(most, least);
     } else {
