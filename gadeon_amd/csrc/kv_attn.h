@@ -1094,15 +1094,15 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         }
         now = next;
     }
-    // Through LDS, so that a row is written, and its gate read, in whole lines.
-    constexpr int TPR = HD / 8, RPP = 256 / TPR, PASS = PC / RPP;    // threads of a row, eight dims each; rows of a pass
-    const int d = 8 * (t % TPR);
+    // Through LDS, each wave its own columns, so that a row is written, and its gate read, in whole lines.
+    constexpr int TPR = HD / 8, RPP = 64 / TPR, PASS = MF / RPP;     // lanes of a row, eight dims each; rows of a pass
+    const int d = 8 * (lane % TPR), r0 = MF * w + lane / TPR;
     typedef T T8 __attribute__((ext_vector_type(8), aligned(16)));
     T8 gates[PASS];
     if (gate && nz == 1)
 #pragma unroll
         for (int x = 0; x < PASS; x++) {
-            const int2 row = out_row[x * RPP + t / TPR];
+            const int2 row = out_row[r0 + x * RPP];
             if (row.y >= 0) gates[x] = *(const T8 *)(gate + row.x * gate_stride + (row.y - (int64_t)row.x * H) * HD + d);
         }
     if constexpr (MF == 16) l += __shfl_xor(l, 16, 64);
@@ -1119,10 +1119,10 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         for (int v = 0; v < NV; v += 4)
             *(f32x4 *)&lds.O[MF * w + lc][MF * dt + 2 * v + 4 * h] =
                     f32x4{acc[dt][v] * inv, acc[dt][v + 1] * inv, acc[dt][v + 2] * inv, acc[dt][v + 3] * inv};
-    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int x = 0; x < PASS; x++) {
-        const int r = x * RPP + t / TPR;
+        const int r = r0 + x * RPP;
         const int64_t row = out_row[r].y;
         if (row < 0) continue;
         f32x4 y[2] = {*(const f32x4 *)&lds.O[r][d], *(const f32x4 *)&lds.O[r][d + 4]};
