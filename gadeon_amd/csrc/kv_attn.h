@@ -718,24 +718,6 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         if (mask.first && (int)gridDim.x > slots) k = un.by_document(mask, k, sq.r0);
     const struct { int i0, i1; } tl = {un.first(k), un.last(k)};
     const uint32_t p0 = (uint32_t)sq.pos, cap1 = s.cap - 1;
-    // The documents of the unit's rows: the first start of them, and the last.
-    uint32_t doc0 = 0, doc1 = 0;
-    if constexpr (How::SCORED)
-        if (mask.first) {
-            uint32_t a = ~0u, z = 0;
-            for (int r = tl.i0 + (int)(threadIdx.x & 63); r <= tl.i1; r += 64) {
-                const uint32_t d = doc_of(mask, sq.r0 + r);
-                a = min(a, d);
-                z = max(z, d);
-            }
-            doc0 = wave_least(a);
-            doc1 = ~wave_least(~z);
-        }
-    const Blocks<AK, How> kb = un.blocks(mask, k, doc0);
-    const Cut cut(kb.n, nz);
-    if (z >= cut.used) return;
-    nz = cut.used;
-    const int per = cut.per, jend = min(kb.n, (z + 1) * per);
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int lc = lane % MF, h = lane / MF;
     // This lane's column, and the positions that the wave's columns stand at.
@@ -745,22 +727,51 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     const int64_t n = sq.r0 + i;
     const uint32_t p = p0 + i;
     if (h == 0) out_row[MF * w + lc] = make_int2((int)n, valid ? (int)n * H + head : -1);
+    // The column's row of q, and scored rows' documents and slope: all requested at once (what they
+    // wait for one after the other is a microsecond each).
+    typedef T T8 __attribute__((ext_vector_type(8), aligned(16)));
+    T8 qraw[KS];
+    {
+        const T *qrow = q + n * q_stride + (int64_t)head * HD + 8 * h;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) qraw[ks] = *(const T8 *)(qrow + 512 / MF * ks);
+    }
+    uint32_t doc = 0, doc0 = 0, doc1 = 0, docs0 = 0, docs1 = 0;      // the column's; the unit's and the wave's first and last
+    float slope = 0.f;
+    if constexpr (How::SCORED) {
+        if (mask.slope) slope = mask.slope[head] * LOG2E;
+        if (mask.first) {
+            doc = doc_of(mask, n);
+            uint32_t a = doc, z = doc;           // (a wave's columns, then all rows of the unit, of which it has some)
+            constexpr int RL = PC / 64 + 1;
+            uint32_t d[RL];
+#pragma unroll
+            for (int x = 0; x < RL; x++) d[x] = tl.i0 + lane + 64 * x <= tl.i1 ? doc_of(mask, sq.r0 + tl.i0 + lane + 64 * x) : doc;
+#pragma unroll
+            for (int x = 0; x < RL; x++) {
+                a = min(a, d[x]);
+                z = max(z, d[x]);
+            }
+            doc0 = wave_least(a);
+            doc1 = ~wave_least(~z);
+        }
+    }
+    const Blocks<AK, How> kb = un.blocks(mask, k, doc0);
+    const Cut cut(kb.n, nz);
+    if (z >= cut.used) return;
+    nz = cut.used;
+    const int per = cut.per, jend = min(kb.n, (z + 1) * per);
     const bool busy = k * PC + MF * w < rows * G;
     const uint32_t plo = p0 + min((k * PC + MF * w) / G, rows - 1);
     const uint32_t seen_from = mask.window && plo >= (uint32_t)mask.window ? plo - mask.window + 1 : 0;
     const uint32_t phi = p0 + min((k * PC + MF * w + MF - 1) / G, rows - 1);
     // Scored: positions that every row sees whole, before the window too, and this column's document.
     const uint32_t sinks = How::SCORED ? max((uint32_t)mask.sinks, un.prefix) : (uint32_t)mask.sinks;
-    uint32_t doc = 0, docs0 = 0, docs1 = 0;      // (docs: the wave's first and last)
-    float slope = 0.f;
-    if constexpr (How::SCORED) {
+    if constexpr (How::SCORED)
         if (mask.first) {
-            doc = doc_of(mask, n);
             docs0 = wave_least(doc);
             docs1 = ~wave_least(~doc);
         }
-        if (mask.slope) slope = mask.slope[head] * LOG2E;
-    }
     auto sees = [&](uint32_t t) {                // whether this column sees position t, if its page is there
         const bool near = t <= p && (!mask.window || t + mask.window > p || t < (uint32_t)mask.sinks);
         if constexpr (How::SCORED) return (near || t < un.prefix) && t >= doc;
@@ -873,25 +884,15 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     f16x8 qh[KS], ql[HL ? KS : 1];
     float sf = fabsf(scale) * LOG2E;
     {
-        const T *qrow = q + n * q_stride + (int64_t)head * HD + 8 * h;
         const bool neg = scale < 0.f;
+        if (j < jend) fetch(en);                 // (while the rows are on their way)
+        en = entry_of(j + 1);
         if constexpr (HL) {
-            f32x4 x[KS][2];
             float mx = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    x[ks][y] = *(const f32x4 *)(qrow + 512 / MF * ks + 4 * y);
-                }
-            if (j < jend) fetch(en);             // (while the rows are on their way)
-            en = entry_of(j + 1);
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int y = 0; y < 2; y++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[ks][y][e]));
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qraw[ks][e]));
             if constexpr (MF == 16) mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const int ex = min(max((int)(__float_as_uint(mx) >> 23), 40), 254) - 127;
@@ -902,15 +903,13 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     f16 hi, lo;
-                    gd_split_f16(x[ks][e >> 2][e & 3] * up, hi, lo);
+                    gd_split_f16(qraw[ks][e] * up, hi, lo);
                     qh[ks][e] = hi;
                     ql[ks][e] = lo;
                 }
         } else {
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) qh[ks] = *(const f16x8 *)(qrow + 512 / MF * ks);
-            if (j < jend) fetch(en);
-            en = entry_of(j + 1);
+            for (int ks = 0; ks < KS; ks++) qh[ks] = __builtin_bit_cast(f16x8, qraw[ks]);
             if (neg)
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) qh[ks] = -qh[ks];
@@ -1097,7 +1096,6 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     // Through LDS, each wave its own columns, so that a row is written, and its gate read, in whole lines.
     constexpr int TPR = HD / 8, RPP = 64 / TPR, PASS = MF / RPP;     // lanes of a row, eight dims each; rows of a pass
     const int d = 8 * (lane % TPR), r0 = MF * w + lane / TPR;
-    typedef T T8 __attribute__((ext_vector_type(8), aligned(16)));
     T8 gates[PASS];
     if (gate && nz == 1)
 #pragma unroll

@@ -291,7 +291,8 @@ def overlap(ctx, n, width):
         assert np.array_equal(refs, np.bincount(table[table >= 0], minlength=70000)) and refs.max() == 1
 
 
-@pytest.mark.parametrize("size,seed", [(s, i) for s in SIZES for i in range(3)] + [((40, 600, 16, 30000), 0), ((2, 3, 16, 300001), 1)], ids=str)
+@pytest.mark.parametrize("size,seed", [(s, i) for s in SIZES for i in range(3)] + [((40, 600, 16, 30000), 0), ((2, 3, 16, 300001), 1), ((200, 400, 16, 16000), 0),
+                                       ((100, 300, 16, 16384), 1), ((100, 100, 16, 16385), 0), ((1, 65537, 16, 900), 1)], ids=str)
 def test_compact(ctx, size, seed):
     rng = np.random.default_rng(seed)
     with Device(ctx, *size) as d:
