@@ -571,11 +571,12 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
 // tile that some column does not see whole goes key by key: a mask, and where V holds a NaN or
 // infinity its finite part and, apart, which columns see the others (0 x NaN would reach them all).
 //   512 f16 rows behind 3584 positions of codes, 40 heads of 128 on 8: 67 us, 600 TFLOP/s;
-// 4096 under a window of 1024 133 us, 570; f32 rows (twice the products) of 24 heads of 256
+// 4096 under a window of 1024 127 us, 600; f32 rows (twice the products) of 24 heads of 256
 // on 4 530.  No unit of the CU is full (matrix cores 31% busy, vector ALUs 50%, LDS 31%):
 // with the registers of two waves a SIMD a wave's chain of staging, scores, weights and sums
 // is what lasts, 2.0 to 2.5 us for two waves' tiles, a lone one 1.7.  (f32 rows of 128 take all
-// 256 registers, and 4 of them memory on codes, 2 on halves of odd pages.)  Measured and left out:
+// 256 registers.)  Results leave through LDS, which takes the 16 bytes a lane and line that the
+// products' layout gives (20 mixed f32 chunks 115 -> 107 us, the window's 133 -> 127).  Measured and left out:
 // units of twice the columns, eight waves to a tile (codes of 256 219 -> 207 us, but f32 rows
 // of chunks 115 -> 122, under a window 133 -> 145); scores formed a tile ahead, beside the
 // weights of the last (143 -> 154, of 256 219 -> 261); tiles of 32 keys and three waves a
@@ -609,7 +610,8 @@ template <int PC, int AK, class How> struct Units {
     }
     // Unit k from the last one back, with those first that a document gives over half the most
     // keys, then a quarter (a workgroup of 20 tiles that starts last is the call's time; 4096 rows of 14
-    // documents, two and a half rounds of workgroups, 116 us in the rows' order, 106 so).
+    // documents, two and a half rounds of workgroups, 116 us in the rows' order, 108 so; of many short ones
+    // 50 and 53).
     __device__ __forceinline__ int by_document(const How &mask, int k, int r0) const {
         constexpr int MOST = 8;                  // units a lane
         const int lane = threadIdx.x & 63, last_unit = n() - 1;

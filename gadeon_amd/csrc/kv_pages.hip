@@ -30,6 +30,8 @@ constexpr int EW = 1024;                         // entries of a workgroup
 // Workgroup (order i, EW entries): row dst[i] takes over src[i]'s entries of the first len[i]
 // positions.  No source is the place of another order, so that rows are only read or only
 // written; counts are whole numbers, whose order of addition shows nowhere.
+//   The counts bound many orders: 400 of 2048 entries add 138 000 of them in random lines in 11 us (with
+// the ends of 300 others 22 a pass, without any count 12); few are a launch and three loads, 2.4.
 __global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, const int32_t *dst, const int32_t *len, int n) {
     const int i = blockIdx.x, s = src[i], d = dst[i], most = len[i];
     if ((uint32_t)s >= (uint32_t)pg.n_seq || (uint32_t)d >= (uint32_t)pg.n_seq) return;
@@ -58,7 +60,6 @@ __global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, cons
 
 // Workgroup (order i, EW entries): sequence seq[i] drops the pages that hold no position of
 // from[i] .. to[i] - 1, but for those that an order before it drops from the same sequence.
-// (By an exchange of each entry instead, 1 to 2 us more.)
 __global__ __launch_bounds__(256) void k_release(Pages pg, const int32_t *seq, const int32_t *from, const int32_t *to) {
     const int i = blockIdx.x, b = seq[i];
     if ((uint32_t)b >= (uint32_t)pg.n_seq) return;
@@ -124,7 +125,7 @@ enum { NEED = 1, KEEP = 2, SHARED = 4, TAIL = 8 };
 // or one shared with others, of which the last keeps it if no other than these name it), the
 // first free pages in order, the k-th need the k-th page.  A sequence gets all or nothing:
 // what it needs, if all up to it fits.
-//   The chain of its steps bounds it, some 0.7 us each.
+//   The chain of its steps bounds it, a dozen of some 0.7 us each.
 constexpr int RT = 1024;                         // threads
 __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_page, Work wk, int32_t *copies, int32_t *n_copies,
                                                 int32_t *pos_out) {
@@ -248,7 +249,9 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
 // The same for 4 T sequences and entries at most, in registers and LDS: a thread's four
 // sequences, four entries, sixteen pages of a round.  Shared pages are counted in a table by a
 // hash of theirs, whose places depend on who comes first, but not what stands there.
-//   A chain of three loads (row, entry, count) bounds it.
+//   A chain of three loads (row, entry, count) and a dozen short steps bounds it: 8.5 us for 200 prompts
+// of 700 rows at most, pages of 64, 7 for 64 tokens (k_reserve took 17 and 15).  256 threads where
+// they do: 1024 take a microsecond or two more; one wave the same.
 template <int T> struct FewLds {
     static constexpr int FEW = 4 * T, SLOTS = 2 * FEW;
     int pos[FEW], entry[FEW], start[FEW + 1];    // of a sequence: its position (-1: denied), first entry, and that one's place
@@ -546,8 +549,8 @@ struct Layers {
 };
 
 // Workgroup (pairs from x on, plane y of the layers, slice z): SLICE bytes of a page, four
-// 16-byte loads a thread in flight.  Bytes bound it: 1750 pages of 32 KiB in 16 planes, 1 GB read
-// and written, 176 us, 5.7 TB/s.  What is written goes past the caches (copies of a step in 16
+// 16-byte loads a thread in flight.  Bytes bound it: some 950 pages of 32 KiB in 16 planes, 1 GB
+// read and written, 180 us, 5.6 TB/s.  What is written goes past the caches (copies of a step in 16
 // layers 17.2 -> 16.4 us, large ones 207 -> 202), and so does what is read where it is more than
 // they hold for long (-> 196; few pages, which later calls copy again, 16.4 -> 20.5): LARGE.
 constexpr uint32_t SLICE = 16384;

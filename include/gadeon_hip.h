@@ -105,10 +105,11 @@ int gd_timer_stop(gd_ctx *ctx, float *ms);
  * recording).  A failing entry inside a recording leaves the capture open;
  * gd_graph_end then fails and discards it.  A graph holds the workspace its
  * calls use, shared with the context's other calls, and attention partials of
- * its own (8 MiB, where it records gd_attn_paged, gd_attn_batch or gd_kv_attn),
+ * its own (8 MiB, where it records gd_attn_paged, gd_attn_batch, gd_kv_attn or gd_kv_attn_scored),
  * until it is destroyed: it may outlive its context, and be launched on another one
  * as long as the workspace of the first is not in use at the same time (which GEMMs
- * of f32 rows or split K, gd_gdn_prefill and gd_kv_attn of split keys do). */
+ * of f32 rows or split K, gd_gdn_prefill, gd_kv_attn and gd_kv_attn_scored of split keys,
+ * gd_kv_reserve of many entries and gd_kv_compact do). */
 typedef struct gd_graph gd_graph;
 int gd_graph_begin(gd_ctx *ctx);
 int gd_graph_end(gd_ctx *ctx, gd_graph **out);
@@ -500,7 +501,8 @@ typedef struct gd_scores {
  * t >= first[row] where t <= p and (window == 0, t > p - window or t < n_sink), or t <
  * prefix[b]; out[h] = softmax(score) . v, gated, zeros where it sees nothing.  In all else as
  * gd_kv_attn (and its very results where cap is 0 and the arrays are null): rows, types,
- * alignment, workspace, recording.  A cap's tanh is formed to some 2^-22 of itself for f32 rows. */
+ * alignment, workspace, recording.  Capped scores are off by some 2^-22 of the cap at caps up to
+ * 64 (f16 rows of chunks: 1024), and of themselves beyond. */
 int gd_kv_attn_scored(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const void *q, int64_t q_stride,
                       const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
                       const gd_scores *scores);
@@ -545,7 +547,8 @@ int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *seq, con
  *   pos_out[n_seq] (may be pos) is pos, or -1 where the free pages do not suffice for all
  * needs up to this sequence's last: it keeps what it had, and the calls that take pos_out leave
  * it alone (also where it needs none but keeps a page that a sequence before it shares).
- * Uses the context workspace (8 bytes a page and 24 an entry of the rows). */
+ * Past 4096 sequences or entries of the rows (a bound of them: n_rows / page_size + 2 n_seq) it uses the
+ * context workspace, 8 bytes a page and 24 an entry. */
 int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pages, const gd_seqs *seqs, int32_t *copies, int32_t *n_copies,
                   int32_t *pos_out);
 
