@@ -112,6 +112,8 @@ template <class How> __device__ __forceinline__ uint32_t doc_of(const How &m, in
 //   (Measured and left out: where all scores of a wave are under half the cap, the polynomial of
 // tanh alone, 6 or 7: 107 us where one way alone takes 97; and what a row sees made its neighbours' last bits.)
 constexpr float TANH_END = 9.02f, EXP_CAP = 64.f, EXP_CAP_F16 = 1024.f;
+// to_x of scores in units of sf (bounded: a score of 0 times infinity is not 0).
+__device__ __forceinline__ float over_cap(float sf, const ScoreArgs &how) { return __builtin_amdgcn_fmed3f(sf / how.cap, -0x1p120f, 0x1p120f); }
 template <bool BY_EXP> __device__ __forceinline__ float cap_score(const ScoreArgs &how, float s, float to_x) {
     if constexpr (!BY_EXP) {
         const float x = __builtin_amdgcn_fmed3f(s * to_x, -TANH_END, TANH_END), u = x * x;
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
     float slope = 0.f, to_x = 0.f, capped = sf, unit = sf;
     if constexpr (How::SCORED) {
         if (mask.slope) slope = mask.slope[h0 + min(col, nh - 1)] * LOG2E;
-        to_x = sf / mask.cap;
+        to_x = over_cap(sf, mask);
         if (mask.cap > 0.f) capped = unit = 1.f;
         if (mask.slope) unit = 1.f;
     }
@@ -921,7 +923,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     // A score over its cap; the units of scores once they are capped, and once they are biased.
     float to_x = 0.f, capped = sf, unit = sf;
     if constexpr (How::SCORED) {
-        to_x = sf / mask.cap;
+        to_x = over_cap(sf, mask);
         if (How::BY_EXP || mask.cap > 0.f) capped = unit = 1.f;
         if (mask.slope) unit = 1.f;
     }

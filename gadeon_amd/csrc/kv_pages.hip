@@ -112,6 +112,63 @@ template <int T> __device__ __forceinline__ int block_scan(int v, int *sums, int
     return before + sum;
 }
 
+// The counts of pages p .. p + 15 (1 behind the last one), and which are free, a bit each.
+struct Counts {
+    typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+    i32x4 r[4];
+    __device__ __forceinline__ Counts() {}
+    __device__ __forceinline__ Counts(const Pages &pg, uint32_t p) {
+        if (p + 16 <= pg.n_pages) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) r[j] = *(const i32x4 *)(pg.refs + p + 4 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) r[j / 4][j % 4] = p + j < pg.n_pages ? pg.refs[p + j] : 1;
+        }
+    }
+    __device__ __forceinline__ int least() const {
+        int m = 1;
+#pragma unroll
+        for (int j = 0; j < 16; j++) m = min(m, r[j / 4][j % 4]);
+        return m;
+    }
+    __device__ __forceinline__ uint32_t free() const {
+        uint32_t f = 0;
+#pragma unroll
+        for (int j = 0; j < 16; j++) f |= (r[j / 4][j % 4] <= 0) << j;
+        return f;
+    }
+};
+
+// The lowest `needs` free pages, in order, into fresh; how many there are.  `first`: the counts of
+// pages 16 t .., on their way since before.  As the lowest free pages are taken first, those before
+// them are in use: they are passed 64 a thread (32 of 1024 threads), by a look at the least count. (64 tokens
+// behind 131072 pages in use 23 us, of which 9 without them; by 16 a thread, all ranked, 37.)
+template <int T>
+__device__ __forceinline__ int take_free(const Pages &pg, const Counts &first, int needs, int32_t *fresh, int *sums, int &turn) {
+    int found = 0, all;
+    auto take = [&](uint32_t free, uint32_t p) {
+        const int n = __popc(free);
+        int at = found + block_scan<T>(n, sums, turn, all) - n;
+        for (; free && at < needs; free &= free - 1) fresh[at++] = (int32_t)p + __ffs(free) - 1;
+        found += all;
+    };
+    if (needs) take(first.free(), 16 * threadIdx.x);
+    constexpr int PARTS = T > 256 ? 2 : 4;       // (registers)
+    for (uint32_t p0 = 16 * T; p0 < pg.n_pages && found < needs; p0 += 16 * PARTS * T) {
+        Counts c[PARTS];
+        int least = 1;
+#pragma unroll
+        for (int i = 0; i < PARTS; i++) c[i] = Counts(pg, p0 + 16 * (i * T + threadIdx.x));
+#pragma unroll
+        for (int i = 0; i < PARTS; i++) least = min(least, c[i].least());
+        if (!__syncthreads_or(least <= 0)) continue;
+#pragma unroll
+        for (int i = 0; i < PARTS; i++) take(c[i].free(), p0 + 16 * (i * T + threadIdx.x));
+    }
+    return found;
+}
+
 // Per sequence where its entries start among all; per page the entries that share it and the
 // last of them; per entry (of the rows of the call, sequence by sequence) what is known of it.
 struct Work {
@@ -201,19 +258,7 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
         if (c < entries) wk.rank[c] = needs + upto;
         needs += all;
     }
-    // Free pages, as many as are needed, the lowest first.
-    int found = 0;
-    for (uint32_t p0 = 0; p0 < pg.n_pages && found < needs; p0 += 4 * RT) {
-        const uint32_t p = p0 + 4 * t;
-        int free[4], n = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) n += free[i] = p + i < pg.n_pages && pg.refs[p + i] <= 0;
-        int at = found + block_scan<RT>(n, sums, turn, all) - n;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (free[i] && at < needs) wk.fresh[at++] = (int32_t)(p + i);
-        found += all;
-    }
+    const int found = take_free<RT>(pg, Counts(pg, 16 * t), needs, wk.fresh, sums, turn);
     __syncthreads();
     int copied = 0;
     for (int c0 = 0; c0 < entries; c0 += RT) {
@@ -247,7 +292,7 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
 }
 
 // The same for 4 T sequences and entries at most, in registers and LDS: a thread's four
-// sequences, four entries, sixteen pages of a round.  Shared pages are counted in a table by a
+// sequences and four entries.  Shared pages are counted in a table by a
 // hash of theirs, whose places depend on who comes first, but not what stands there.
 //   A chain of three loads (row, entry, count) and a dozen short steps bounds it: 8.5 us for 200 prompts
 // of 700 rows at most, pages of 64, 7 for 64 tokens (k_reserve took 17 and 15).  256 threads where
@@ -270,23 +315,7 @@ __global__ __launch_bounds__(T) void k_reserve_few(Pages pg, Rows s, FastDiv by_
     constexpr int FEW = l.FEW, SLOTS = l.SLOTS;
     const int t = threadIdx.x;
     int turn = 0, all;
-    // Which of the pages p .. p + 15 are free, a bit each; the first round's on their way.
-    auto free_of = [&](uint32_t p) {
-        typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
-        i32x4 r[4];
-        uint32_t free = 0;
-        if (p + 16 <= pg.n_pages) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) r[j] = *(const i32x4 *)(pg.refs + p + 4 * j);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; j++) r[j / 4][j % 4] = p + j < pg.n_pages ? pg.refs[p + j] : 1;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; j++) free |= (r[j / 4][j % 4] <= 0) << j;
-        return free;
-    };
-    uint32_t free = free_of(16 * t);
+    const Counts first(pg, 16 * t);              // on its way
     int n[4], sum = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -387,15 +416,7 @@ __global__ __launch_bounds__(T) void k_reserve_few(Pages pg, Rows s, FastDiv by_
         rank += f[j] & NEED;
         if (4 * t + j < entries) l.rank[4 * t + j] = rank;
     }
-    int found = 0;
-    for (uint32_t p0 = 0; p0 < pg.n_pages && found < needs; p0 += 16 * T) {
-        const uint32_t p = p0 + 16 * t;
-        if (p0) free = free_of(p);
-        sum = __popc(free);
-        int at = found + block_scan<T>(sum, l.sums, turn, all) - sum;
-        for (; free && at < needs; free &= free - 1) l.fresh[at++] = (int)p + __ffs(free) - 1;
-        found += all;
-    }
+    const int found = take_free<T>(pg, first, needs, l.fresh, l.sums, turn);
     __syncthreads();
     // (Nobody reads a count or an entry of the table any more.)
     int fresh[4];
@@ -666,9 +687,9 @@ extern "C" int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pg, const gd_seqs *
     GD_HIP(ctx, hipSetDevice(ctx->device));
     const int64_t cap = std::min<int64_t>((int64_t)pg->max_pages * pg->page_size, 0x7fffffff);
     const Rows rows{s->row_start, s->pos, nullptr, s->page_table, (int)s->n_rows, s->n_seq, s->max_pages, (uint32_t)cap};
-    // Entries of the rows: a page for each page_size of them, and two ends a sequence.
+    // Entries of the rows: a page for each page_size of them, and two ends a sequence; one of a single row.
     Work wk;
-    wk.most = (int)(s->n_rows / pg->page_size + 2 * std::min<int64_t>(s->n_seq, s->n_rows));
+    wk.most = (int)(s->row_start ? s->n_rows / pg->page_size + 2 * std::min<int64_t>(s->n_seq, s->n_rows) : s->n_rows);
     const int few = std::max(s->n_seq, wk.most) <= 4 * 256 ? 256 : 1024;
     if (std::max(s->n_seq, wk.most) <= 4 * few) {
         auto kernel = few == 256 ? k_reserve_few<256> : k_reserve_few<1024>;

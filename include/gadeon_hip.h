@@ -547,7 +547,7 @@ int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *seq, con
  *   pos_out[n_seq] (may be pos) is pos, or -1 where the free pages do not suffice for all
  * needs up to this sequence's last: it keeps what it had, and the calls that take pos_out leave
  * it alone (also where it needs none but keeps a page that a sequence before it shares).
- * Past 4096 sequences or entries of the rows (a bound of them: n_rows / page_size + 2 n_seq) it uses the
+ * Past 4096 sequences or entries of the rows (a bound of them: n_seq of single rows, else n_rows / page_size + 2 n_seq) it uses the
  * context workspace, 8 bytes a page and 24 an entry. */
 int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pages, const gd_seqs *seqs, int32_t *copies, int32_t *n_copies,
                   int32_t *pos_out);

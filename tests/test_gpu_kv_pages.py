@@ -236,6 +236,19 @@ def test_reserve(ctx, size, tokens, seed):
             d.reserve(pos.tolist(), rows.tolist(), tokens, in_place=step == 3)
 
 
+@pytest.mark.parametrize("n", [5, 300, 1500, 4200])
+@pytest.mark.parametrize("n_pages", [16383, 16384, 20479, 20481, 37000, 70001])
+def test_reserve_behind_pages_in_use(ctx, n, n_pages):
+    """Free pages behind many in use: at the end, one here and there, one too few."""
+    for free in ([*range(n_pages - n, n_pages)], [1, 4095, 4096, 16383] + [*range(n_pages - n + 1, n_pages)],
+                 [*range(n_pages - n + 1, n_pages)], [*range(0, n_pages, max(1, n_pages // n))]):
+        with Device(ctx, n, 1, 16, n_pages) as d:
+            d.m.refs[:] = 1
+            d.m.refs[[f for f in free if f < n_pages]] = 0
+            d.set()
+            d.reserve([0] * n, [1] * n, True)
+
+
 @pytest.mark.parametrize("n", [1000, 4096, 4097, 9000])
 @pytest.mark.parametrize("groups", [1, 7, 499])
 def test_reserve_many_that_share(ctx, n, groups):

@@ -147,6 +147,25 @@ def test_scales(ctx, scale):
             check(ctx, ATTN[which], ga.I8, x16, 128, 4, 2, 16, "cap bias", row_start=which == "later", scale=scale)
 
 
+@pytest.mark.parametrize("cap,scale", [(1e-30, 1e30), (1e-30, -1e30), (64.0, 1e30), (1e-30, 1e-30), (1e30, 1e30)])
+def test_caps_and_scales_far_apart(ctx, cap, scale):
+    """Rows of zeros have scores of 0 whatever they are scaled by; a cap of next to nothing leaves
+    next to nothing of the others' scores: all keys weigh the same."""
+    for seqs, start in (([(700, 1), (31, 1)], False), ([(700, 90), (31, 3)], True)):
+        for x16 in (False, True):
+            with Batch(ctx, seqs, ga.F16, 2, 128, 16, row_start=start) as bt:
+                KV = bt.fill()
+                q = rows_of(bt.rng, (bt.n, 4, 128), x16)
+                if cap > 1:
+                    q[:] = 0
+                q[::2] = 0
+                got, _ = run(ctx, bt, q, None, dict(cap=cap), scale=scale)
+                for b, (p, r) in enumerate(seqs):
+                    rows = slice(bt.start[b], bt.start[b] + r)
+                    want = attend(q[rows] * 0, *KV[b], p, 1.0, 0, 0, None)
+                    assert np.abs(got[rows] - want).max() <= bound(q[rows] * 0, *KV[b], 1.0, x16) + 2.0 ** -24, (b, x16)
+
+
 @pytest.mark.parametrize("dtype", [ga.I8, ga.F16], ids=["i8", "f16"])
 @pytest.mark.parametrize("what", ["cap bias", "doc prefix", "odd doc"])
 def test_split_keys(ctx, dtype, what):
