@@ -592,13 +592,14 @@ template <int HD> constexpr int tile_keys() { return HD == 128 ? 64 : 32; }
 // A sequence's units: first and last row of unit k, and its blocks of keys.
 template <int PC, int AK, class How> struct Units {
     int rows, G;
+    FastDiv by_g;                                // (a division by G is some 30 instructions, and there are many)
     uint32_t pos, cap;
     uint32_t prefix;                             // of the sequence's positions
-    __device__ __forceinline__ Units(const Seq &q, int G_, uint32_t cap_, const How &mask, int b)
-        : rows(q.r1 - q.r0), G(G_), pos(q.pos), cap(cap_), prefix(min(prefix_of(mask, b), pos + rows)) {}
+    __device__ __forceinline__ Units(const Seq &q, int G_, const FastDiv &by_g_, uint32_t cap_, const How &mask, int b)
+        : rows(q.r1 - q.r0), G(G_), by_g(by_g_), pos(q.pos), cap(cap_), prefix(min(prefix_of(mask, b), pos + rows)) {}
     __device__ __forceinline__ int n() const { return (int)(((int64_t)rows * G + PC - 1) / PC); }
-    __device__ __forceinline__ int first(int k) const { return k * PC / G; }
-    __device__ __forceinline__ int last(int k) const { return min((k * PC + PC - 1) / G, rows - 1); }
+    __device__ __forceinline__ int first(int k) const { return (int)by_g(k * PC); }
+    __device__ __forceinline__ int last(int k) const { return min((int)by_g(k * PC + PC - 1), rows - 1); }
     // Position of the last key that some row up to i sees.
     __device__ __forceinline__ uint32_t last_key(int i) const { return How::SCORED ? max(pos + i, prefix - (prefix > 0)) : pos + i; }
     __device__ __forceinline__ Blocks<AK, How> blocks(const How &mask, int k, uint32_t doc = 0) const {
@@ -652,9 +653,9 @@ struct Cut {
 // How finely the keys are split, as token_least, each of a sequence's units taken for its
 // longest.
 template <int PC, int AK, class How>
-__device__ __forceinline__ int unit_least(const Rows &s, const How &mask, int G, int HKV, int slots) {
+__device__ __forceinline__ int unit_least(const Rows &s, const How &mask, int G, const FastDiv &by_g, int HKV, int slots) {
     return fitting(s, HKV, slots, ROWS_FEWEST, [&](int b, float &n, float &u) {
-        const Units<PC, AK, How> q(seq_at(s, b), G, s.cap, mask, b);
+        const Units<PC, AK, How> q(seq_at(s, b), G, by_g, s.cap, mask, b);
         u = q.rows > 0 ? (float)q.n() : 0.f;
         n = q.rows > 0 ? (float)q.blocks(mask, q.n() - 1).n : 0.f;
     });
@@ -663,7 +664,7 @@ __device__ __forceinline__ int unit_least(const Rows &s, const How &mask, int G,
 template <int HD, bool I8, bool TILED, typename T, class How>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, int64_t gate_stride, T *out, Part part,
-                 int most, int slots, int H, float scale, How mask) {
+                 int most, int slots, int H, float scale, How mask, FastDiv by_g) {
     constexpr bool HL = sizeof(T) == 4;          // hi + lo
     // A wave keeps its priority over the other of its SIMD through the softmax and the sums
     // too where codes are made halves or rows are pairs, in us with / without it (1024 rows
@@ -702,19 +703,19 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     // on 4, 16 behind 1500 65 / 57 / 54 / 54, behind 2500 64 / 61 / 70 / 62, behind 5000 91 / 82 /
     // 82 / 82; 32 of them 81 / 76 / 78 / 79, 109 / 95 / 94 / 95, 145 / 124 / 124 / 124; 20 of f32
     // rows behind 5000 115 / 119 / 118 / 115, 32 on halves 156 / 136 / 128 / 126.
-    const int least = most > 1 ? unit_least<PC, AK, How>(s, mask, G, c.HKV, slots) : 0;
+    const int least = most > 1 ? unit_least<PC, AK, How>(s, mask, G, by_g, c.HKV, slots) : 0;
     auto units = [&](const Seq &q, int b) {
-        const Units<PC, AK, How> u(q, G, s.cap, mask, b);
+        const Units<PC, AK, How> u(q, G, by_g, s.cap, mask, b);
         return u.rows <= 0 ? 0 : u.n() * (most > 1 ? u.splits(mask, most, least) : 1);
     };
     Seq sq;
     auto order = [&](const Seq &q, int b) {
-        const Units<PC, AK, How> u(q, G, s.cap, mask, b);
+        const Units<PC, AK, How> u(q, G, by_g, s.cap, mask, b);
         const int n = u.rows > 0 ? u.blocks(mask, u.n() - 1).n : 0;
         return n > 0.35f * least ? 0 : n > 0.1f * least ? 1 : 2;
     };
     if (!unit_at<3>(s, blockIdx.x / c.HKV, units, order, b, k, sq)) return;
-    const Units<PC, AK, How> un(sq, G, s.cap, mask, b);
+    const Units<PC, AK, How> un(sq, G, by_g, s.cap, mask, b);
     const int rows = un.rows;
     if (most > 1) nz = un.splits(mask, most, least);
     const int z = k % nz;
@@ -726,9 +727,9 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int lc = lane % MF, h = lane / MF;
     // This lane's column, and the positions that the wave's columns stand at.
-    const int col = k * PC + MF * w + lc, i = min(col / G, rows - 1);
+    const int col = k * PC + MF * w + lc, i = min((int)by_g(col), rows - 1);
     const bool valid = col < rows * G;
-    const int head = kvh * G + (valid ? col % G : G - 1);
+    const int head = kvh * G + (valid ? col - i * G : G - 1);
     const int64_t n = sq.r0 + i;
     const uint32_t p = p0 + i;
     if (h == 0) out_row[MF * w + lc] = make_int2((int)n, valid ? (int)n * H + head : -1);
@@ -767,9 +768,9 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     nz = cut.used;
     const int per = cut.per, jend = min(kb.n, (z + 1) * per);
     const bool busy = k * PC + MF * w < rows * G;
-    const uint32_t plo = p0 + min((k * PC + MF * w) / G, rows - 1);
+    const uint32_t plo = p0 + min((int)by_g(k * PC + MF * w), rows - 1);
     const uint32_t seen_from = mask.window && plo >= (uint32_t)mask.window ? plo - mask.window + 1 : 0;
-    const uint32_t phi = p0 + min((k * PC + MF * w + MF - 1) / G, rows - 1);
+    const uint32_t phi = p0 + min((int)by_g(k * PC + MF * w + MF - 1), rows - 1);
     // Scored: positions that every row sees whole, before the window too, and this column's document.
     const uint32_t sinks = How::SCORED ? max((uint32_t)mask.sinks, un.prefix) : (uint32_t)mask.sinks;
     if constexpr (How::SCORED)
@@ -1354,7 +1355,8 @@ int attn(gd_ctx *ctx, const char *fn, const AttnArgs &a, int window, int n_sink,
         } else { \
             auto kernel = tiled ? k_attn_rows<HD_, I8_, true, T_, How> : k_attn_rows<HD_, I8_, I8_, T_, How>; \
             hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, cache_of(kv), rows, (const T_ *)q, q_stride, \
-                               (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)slots, n_head, scale, mask); \
+                               (const T_ *)gate, gate_stride, (T_ *)out, part, (int)ns, (int)slots, n_head, scale, mask, \
+                               FastDiv((uint32_t)G)); \
         } \
         if (ns > 1) { \
             GD_LAUNCHED(ctx, fn); \
