@@ -557,6 +557,54 @@ __global__ __launch_bounds__(CT) void k_move(Pages pg, const int32_t *low, const
     }
 }
 
+// All of it in one workgroup, for 4 T pages at most: four pages a thread, what they become in LDS.
+template <int T>
+__global__ __launch_bounds__(T) void k_compact_few(Pages pg, int entries, int32_t *moves, int32_t *n_moves) {
+    __shared__ int low[4 * T], to[4 * T], sums[2 * T / 64];
+    const int t = threadIdx.x;
+    int turn = 0, n, refs[4], own = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) own += (refs[j] = 4u * t + j < pg.n_pages ? pg.refs[4 * t + j] : 0) > 0;
+    int page = t < entries ? pg.table[t] : -1;   // (on its way beside the counts)
+    const int before = block_scan<T>(own, sums, turn, n) - own;
+    int at = before;                             // pages in use before
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int p = 4 * t + j;
+        if (p < n && refs[j] <= 0) low[p - at] = p;
+        if (p == n - 1) n_moves[0] = p - at + (refs[j] <= 0);
+        at += refs[j] > 0;
+    }
+    if (t == 0) {
+        n_moves[1] = n;
+        if (n == 0) n_moves[0] = 0;
+    }
+    __syncthreads();                             // (all counts are read)
+    at = before;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int p = 4 * t + j;
+        if (p < n) {
+            at += refs[j] > 0;
+            continue;
+        }
+        to[p] = -1;
+        if (refs[j] <= 0) continue;
+        const int k = n - 1 - at++, dst = low[k];
+        to[p] = dst;
+        moves[2 * k] = p;
+        moves[2 * k + 1] = dst;
+        pg.refs[dst] = refs[j];
+        pg.refs[p] = 0;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = t; i < entries; i += T) {
+        if (i != t) page = pg.table[i];
+        if (page >= n && pg.there(page) && to[page] >= 0) pg.table[i] = to[page];
+    }
+}
+
 // ---------------------------------------------------------------- copy
 
 constexpr int LAYERS = 64;                       // of a launch
@@ -720,8 +768,18 @@ extern "C" int gd_kv_compact(gd_ctx *ctx, const gd_kv_pages *pg, int32_t *moves,
     GD_REQUIRE(ctx, ((uintptr_t)moves | (uintptr_t)n_moves) % 4 == 0, "%s: moves must be 4-byte aligned", fn);
     GD_CHECK_CTX(ctx);
     GD_HIP(ctx, hipSetDevice(ctx->device));
+    // One launch or two, us by pages and entries of the table: 100, 150 6.1 / 8.2; 1000, 1000 6.1 / 8.4 (256
+    // threads); 2000, 4000 7.2 / 8.8; 4000, 6000 8.2 / 9.1; 4000, 24000 13.6 / 8.8 (1024).
+    const int64_t all = (int64_t)pg->n_seq * pg->max_pages;
+    if (pg->n_pages <= 4 * 1024 && all <= 6 * 1024) {
+        const bool least = pg->n_pages <= 4 * 256 && all <= 8 * 256;
+        auto kernel = least ? k_compact_few<256> : k_compact_few<1024>;
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(least ? 256 : 1024), 0, ctx->stream, pages_of(pg), (int)all, moves, n_moves);
+        GD_LAUNCHED(ctx, fn);
+        return GD_OK;
+    }
     const int chunks = (int)gd_blocks(pg->n_pages, CP);
-    const bool alone = pg->n_pages <= 16 * CP;   // pages that each workgroup of k_rank counts itself
+    const bool alone = pg->n_pages <= 16 * CP;   // pages that each workgroup of k_rank counts itself (a launch less, 3 us)
     void *ws;
     if ((rc = gd_ctx_workspace(ctx, ((size_t)chunks + 3 * pg->n_pages) * 4, &ws))) return rc;
     int32_t *counts = (int32_t *)ws, *low = counts + chunks, *high = low + pg->n_pages, *to = high + pg->n_pages;

@@ -556,7 +556,8 @@ int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pages, const gd_seqs *seqs, in
  * the lowest free page, and so on while that is lower, so that those in use are 0 .. n-1 and the
  * planes behind them may go.  Entries and counts follow; moves[2 n_pages] at most gets the
  * (from, to) pairs in that order, n_moves[2] their number and n (device memory both), for
- * gd_kv_copy_pages before the cache is used again.  Uses the context workspace (12 bytes a page). */
+ * gd_kv_copy_pages before the cache is used again.  Past 4096 pages or 6144 entries of the table
+ * it uses the context workspace, 12 bytes a page. */
 int gd_kv_compact(gd_ctx *ctx, const gd_kv_pages *pages, int32_t *moves, int32_t *n_moves);
 
 /* Copies whole pages, codes with their exponents, in each of the n_kv caches (which have the same

@@ -304,8 +304,13 @@ def overlap(ctx, n, width):
         assert np.array_equal(refs, np.bincount(table[table >= 0], minlength=70000)) and refs.max() == 1
 
 
-@pytest.mark.parametrize("size,seed", [(s, i) for s in SIZES for i in range(3)] + [((40, 600, 16, 30000), 0), ((2, 3, 16, 300001), 1), ((200, 400, 16, 16000), 0),
-                                       ((100, 300, 16, 16384), 1), ((100, 100, 16, 16385), 0), ((1, 65537, 16, 900), 1)], ids=str)
+# (Around 1024, 4096 and 16384 pages, 2048 and 6144 entries of the table, where other kernels take over.)
+EDGES = [((40, 600, 16, 30000), 0), ((2, 3, 16, 300001), 1), ((200, 400, 16, 16000), 0), ((100, 300, 16, 16384), 1),
+         ((100, 100, 16, 16385), 0), ((1, 65537, 16, 900), 1), ((20, 300, 16, 4096), 0), ((20, 308, 16, 4096), 1),
+         ((20, 300, 16, 4097), 0), ((20, 102, 16, 1024), 0), ((20, 103, 16, 1024), 1), ((9, 50, 16, 1025), 0)]
+
+
+@pytest.mark.parametrize("size,seed", [(s, i) for s in SIZES for i in range(3)] + EDGES, ids=str)
 def test_compact(ctx, size, seed):
     rng = np.random.default_rng(seed)
     with Device(ctx, *size) as d:
@@ -319,6 +324,49 @@ def test_compact(ctx, size, seed):
         d.compact()
         d.compact()
         assert not len(d.m.compact()[0])
+
+
+@pytest.mark.parametrize("n,n_pages", [(40, 900), (5000, 20000)])
+def test_recordings(ctx, n, n_pages):
+    """Reserving, releasing and closing up as recorded graphs, replayed in turn with calls between that
+    grow the workspace and use it, every time as the model has it."""
+    rng = np.random.default_rng(n)
+    with Device(ctx, n, 3, 16, n_pages) as d:
+        s = d.seqs([0] * n, [1] * n, True)
+        gone, to = d.put(np.zeros(n // 3, I32)), d.put(np.zeros(n // 3, I32))
+        calls = [lambda: ctx.gd_kv_reserve(d.ref, C.byref(s), d.copies, d.n, d.pos_out),
+                 lambda: ctx.gd_kv_release(d.ref, gone, None, to, n // 3), lambda: ctx.gd_kv_compact(d.ref, d.moves, d.n)]
+        graphs = []
+        for call in calls:
+            call()
+            graphs.append(C.c_void_p())
+            ctx.gd_graph_begin()
+            call()
+            ctx.gd_graph_end(C.byref(graphs[-1]))
+        d.set()                                                 # (as it was)
+        big = Device(ctx, 4, 4, 16, 200000)
+        for i in range(4):
+            pos = rng.integers(-1, 40, n)
+            ctx.set(s.pos, pos.astype(I32))
+            out, copies = d.m.reserve(pos.tolist(), [1] * n)
+            ctx.gd_graph_launch(graphs[0])
+            assert np.array_equal(ctx.get(d.pos_out, n, I32), out) and ctx.get(d.n, 1, I32)[0] == len(copies)
+            d.same()
+            filled(big, rng)
+            big.compact()
+            which = rng.integers(0, n, n // 3)
+            ctx.set(gone, which.astype(I32))
+            d.m.release(which, None, [0] * len(which))
+            ctx.gd_graph_launch(graphs[1])
+            d.same()
+            big.reserve([0, 5, -1, 63], [1] * 4, True)
+            moves, used = d.m.compact()
+            ctx.gd_graph_launch(graphs[2])
+            assert list(ctx.get(d.n, 2, I32)) == [len(moves), used]
+            d.same()
+        big.__exit__()
+        for g in graphs:
+            ctx.lib.gd_graph_destroy(g)
 
 
 # ------------------------------------------------------------------ copies
