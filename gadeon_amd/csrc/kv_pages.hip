@@ -291,12 +291,13 @@ __global__ __launch_bounds__(RT) void k_reserve(Pages pg, Rows s, FastDiv by_pag
     if (t == 0) *n_copies = copied;
 }
 
-// The same for 4 T sequences and entries at most, in registers and LDS: a thread's four
-// sequences and four entries.  Shared pages are counted in a table by a
-// hash of theirs, whose places depend on who comes first, but not what stands there.
-//   A chain of three loads (row, entry, count) and a dozen short steps bounds it: 8.5 us for 200 prompts
-// of 700 rows at most, pages of 64, 7 for 64 tokens (k_reserve took 17 and 15).  256 threads where
-// they do: 1024 take a microsecond or two more; one wave the same.
+// The same for 4 T sequences and entries at most, in registers and LDS, T of them a round.  Single
+// rows' entries are the sequences; others' are found by the sequence that starts last at or before
+// each.  Shared pages are counted in a table by a hash of theirs, whose places depend on who comes
+// first, but not what stands there.
+//   A chain of three loads (row, entry, count) and a dozen short steps bounds it: 6.7 us for 64
+// tokens, 8.6 for 200 prompts (k_reserve some 15 and 17; four entries of a thread beside each other
+// instead of T apart 9.0 and 9.2).
 template <int T> struct FewLds {
     static constexpr int FEW = 4 * T, SLOTS = 2 * FEW;
     int pos[FEW], entry[FEW], start[FEW + 1];    // of a sequence: its position (-1: denied), first entry, and that one's place
@@ -312,71 +313,76 @@ template <int T>
 __global__ __launch_bounds__(T) void k_reserve_few(Pages pg, Rows s, FastDiv by_page, int most, int32_t *copies, int32_t *n_copies,
                                                     int32_t *pos_out) {
     __shared__ FewLds<T> l;
-    constexpr int FEW = l.FEW, SLOTS = l.SLOTS;
+    constexpr int SLOTS = l.SLOTS, R = 4;
     const int t = threadIdx.x;
+    const bool single = !s.row_start;
     int turn = 0, all;
     const Counts first(pg, 16 * t);              // on its way
-    int n[4], sum = 0;
+    if (!single)
+        for (int i = t; i < most; i += T) l.owner[i] = 0;
+    int n[R], entries = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int b = 4 * t + j;
+    for (int j = 0; j < R; j++) {
+        const int b = j * T + t;
         n[j] = 0;
-        l.owner[b] = 0;
-        if (b >= s.n_seq) continue;
-        const Seq q = seq_at(s, b);
-        l.pos[b] = q.pos;
-        if (q.r1 > q.r0 && (uint32_t)q.pos < s.cap) {
-            const uint32_t last = min((uint32_t)q.pos + (uint32_t)(q.r1 - q.r0 - 1), s.cap - 1);
-            l.entry[b] = (int)by_page(q.pos);
-            n[j] = min((int)by_page(last) - l.entry[b] + 1, FEW);
+        if (j * T >= s.n_seq) continue;
+        if (b < s.n_seq) {
+            const Seq q = seq_at(s, b);
+            l.pos[b] = q.pos;
+            if (q.r1 > q.r0 && (uint32_t)q.pos < s.cap) {
+                const uint32_t last = min((uint32_t)q.pos + (uint32_t)(q.r1 - q.r0 - 1), s.cap - 1);
+                l.entry[b] = (int)by_page(q.pos);
+                n[j] = min((int)by_page(last) - l.entry[b] + 1, (int)l.FEW);
+            }
         }
-        sum += n[j];
-    }
-    int at = block_scan<T>(sum, l.sums, turn, all) - sum;
-    const int entries = min(all, most);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int b = 4 * t + j;
+        if (single) continue;
+        const int at = entries + block_scan<T>(n[j], l.sums, turn, all) - n[j];
         if (b < s.n_seq) l.start[b] = min(at, most);
         if (n[j] && at < most) l.owner[at] = b + 1;
-        at += n[j];
+        entries += all;
     }
+    entries = single ? s.n_seq : min(entries, most);
     if (t == 0) l.start[s.n_seq] = entries;
-    __syncthreads();
-    // Entries 4 t ..: the last sequence that starts at or before each.
-    int seq[4], page[4], e[4], f[4];
+    if (!single) __syncthreads();
+    int seq[R], page[R], e[R], f[R], owner = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) seq[j] = max(l.owner[4 * t + j], j ? seq[j - 1] : 0);
-    int top = seq[3];
-    for (int i = 1; i < 64; i *= 2) {
-        const int o = __shfl_up(top, i, 64);
-        if ((t & 63) >= i) top = max(top, o);
-    }
-    int before = __shfl_up(top, 1, 64);
-    if ((t & 63) == 0) before = 0;
-    int *w = l.sums + (turn ^= 1) * (T / 64);
-    if ((t & 63) == 63) w[t >> 6] = top;
-    __syncthreads();
-    for (int i = 0; i < (t >> 6); i++) before = max(before, w[i]);
-    bool some = false;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int c = 4 * t + j;
+    for (int j = 0; j < R; j++) {
+        const int c = j * T + t;
         page[j] = -1;
         f[j] = 0;
-        if (c >= entries) continue;
-        seq[j] = max(seq[j], before) - 1;
-        e[j] = l.entry[seq[j]] + c - l.start[seq[j]];
+        if (j * T >= entries) continue;
+        if (single) {
+            seq[j] = c;
+            if (!n[j]) continue;
+            e[j] = l.entry[c];                   // (its own)
+        } else {
+            int top = c < entries ? l.owner[c] : 0;
+            for (int i = 1; i < 64; i *= 2) {
+                const int o = __shfl_up(top, i, 64);
+                if ((t & 63) >= i) top = max(top, o);
+            }
+            int *w = l.sums + (turn ^= 1) * (T / 64);
+            if ((t & 63) == 63) w[t >> 6] = top;
+            __syncthreads();
+            int before = owner;                  // of the waves before this one
+            for (int i = 0; i < T / 64; i++) {
+                before = max(before, i < (t >> 6) ? w[i] : 0);
+                owner = max(owner, w[i]);
+            }
+            if (c >= entries) continue;
+            seq[j] = max(top, before) - 1;
+            e[j] = l.entry[seq[j]] + c - l.start[seq[j]];
+        }
+        f[j] = NEED;
         page[j] = pg.row(seq[j])[e[j]];
     }
-    int held[4];                                 // counts of the entries' pages
+    int held[R];                                 // counts of the entries' pages
 #pragma unroll
-    for (int j = 0; j < 4; j++) held[j] = pg.there(page[j]) ? pg.refs[page[j]] : 0;
+    for (int j = 0; j < R; j++) held[j] = f[j] && pg.there(page[j]) ? pg.refs[page[j]] : 0;
+    bool some = false;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (4 * t + j >= entries) continue;
-        if (!pg.there(page[j])) f[j] = NEED;
-        else if (held[j] > 1) f[j] = SHARED;
+    for (int j = 0; j < R; j++) {
+        if (f[j] && pg.there(page[j])) f[j] = held[j] > 1 ? SHARED : 0;
         some |= f[j] == SHARED;
     }
     if (__syncthreads_or(some)) {
@@ -393,61 +399,59 @@ __global__ __launch_bounds__(T) void k_reserve_few(Pages pg, Rows s, FastDiv by_
                 if (there == -1 || there == page) return i;
             }
         };
-        int at[4];
+        int at[R];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int j = 0; j < R; j++)
             if (f[j] & SHARED) {
                 at[j] = slot(page[j]);
                 atomicAdd(&l.uses[at[j]], 1);
-                atomicMax(&l.last[at[j]], 4 * t + j);
+                atomicMax(&l.last[at[j]], j * T + t);
             }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (f[j] & SHARED) f[j] |= l.uses[at[j]] == held[j] && l.last[at[j]] == 4 * t + j ? KEEP : NEED;
+        for (int j = 0; j < R; j++)
+            if (f[j] & SHARED) f[j] |= l.uses[at[j]] == held[j] && l.last[at[j]] == j * T + t ? KEEP : NEED;
+        __syncthreads();                         // (the ranks take their place)
     }
-    sum = 0;
+    int rank[R], needs = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) sum += f[j] & NEED;
-    int rank = block_scan<T>(sum, l.sums, turn, all) - sum;
-    const int needs = all;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        rank += f[j] & NEED;
-        if (4 * t + j < entries) l.rank[4 * t + j] = rank;
+    for (int j = 0; j < R; j++) {
+        if (j * T >= entries) continue;
+        rank[j] = needs + block_scan<T>(f[j] & NEED, l.sums, turn, all);
+        if (!single && j * T + t < entries) l.rank[j * T + t] = rank[j];
+        needs += all;
     }
     const int found = take_free<T>(pg, first, needs, l.fresh, l.sums, turn);
     __syncthreads();
     // (Nobody reads a count or an entry of the table any more.)
-    int fresh[4];
-    sum = 0;
+    int copied = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        fresh[j] = -1;
-        if (!(f[j] & (NEED | KEEP))) continue;
-        const int b = seq[j];
-        const int p = l.pos[b];                  // (another thread may set it to -1: then this entry is denied too)
-        if (l.rank[l.start[b + 1] - 1] > found) {
-            l.pos[b] = -1;
-        } else if (f[j] & NEED) {
-            fresh[j] = l.fresh[l.rank[4 * t + j] - 1];
-            pg.row(b)[e[j]] = fresh[j];
-            pg.refs[fresh[j]] = 1;
-            count(pg, page[j], -1);
-            if (f[j] & SHARED && (int64_t)e[j] * pg.P < p) sum++;
-            else fresh[j] = -1;
+    for (int j = 0; j < R; j++) {
+        if (j * T >= entries) continue;
+        int fresh = -1;
+        if (f[j] & (NEED | KEEP)) {
+            const int b = seq[j], p = l.pos[b];  // (another thread may set it to -1: then this entry is denied too)
+            if ((single ? rank[j] : l.rank[l.start[b + 1] - 1]) > found) {
+                l.pos[b] = -1;
+            } else if (f[j] & NEED) {
+                const int now = l.fresh[rank[j] - 1];
+                pg.row(b)[e[j]] = now;
+                pg.refs[now] = 1;
+                count(pg, page[j], -1);
+                if (f[j] & SHARED && (int64_t)e[j] * pg.P < p) fresh = now;
+            }
         }
-    }
-    at = block_scan<T>(sum, l.sums, turn, all) - sum;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (fresh[j] >= 0) {
+        const int at = copied + block_scan<T>(fresh >= 0, l.sums, turn, all) - 1;
+        if (fresh >= 0) {
             copies[2 * at] = page[j];
-            copies[2 * at++ + 1] = fresh[j];
+            copies[2 * at + 1] = fresh;
         }
-        if (4 * t + j < s.n_seq) pos_out[4 * t + j] = l.pos[4 * t + j];
+        copied += all;
     }
-    if (t == 0) *n_copies = all;
+#pragma unroll
+    for (int j = 0; j < R; j++)
+        if (j * T + t < s.n_seq) pos_out[j * T + t] = l.pos[j * T + t];
+    if (t == 0) *n_copies = copied;
 }
 
 // ---------------------------------------------------------------- compact
@@ -738,9 +742,11 @@ extern "C" int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pg, const gd_seqs *
     // Entries of the rows: a page for each page_size of them, and two ends a sequence; one of a single row.
     Work wk;
     wk.most = (int)(s->row_start ? s->n_rows / pg->page_size + 2 * std::min<int64_t>(s->n_seq, s->n_rows) : s->n_rows);
-    const int few = std::max(s->n_seq, wk.most) <= 4 * 256 ? 256 : 1024;
-    if (std::max(s->n_seq, wk.most) <= 4 * few) {
-        auto kernel = few == 256 ? k_reserve_few<256> : k_reserve_few<1024>;
+    // us of 256 / 512 / 1024 threads: 200 tokens 6.9 / 7.4 / 9, 400 7.9 / 7.6 / 8.5, 1000 14.6 / 10.0 / 9.7; 200
+    // prompts of up to 600 entries 9.2 / 8.6 / 10.1.
+    const int widest = std::max(s->n_seq, wk.most), few = widest <= 512 ? 256 : widest <= 2048 ? 512 : 1024;
+    if (widest <= 4 * few) {
+        auto kernel = few == 256 ? k_reserve_few<256> : few == 512 ? k_reserve_few<512> : k_reserve_few<1024>;
         hipLaunchKernelGGL(kernel, dim3(1), dim3(few), 0, ctx->stream, pages_of(pg), rows, FastDiv((uint32_t)pg->page_size), wk.most, copies,
                            n_copies, pos_out);
         GD_LAUNCHED(ctx, fn);

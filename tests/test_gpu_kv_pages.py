@@ -215,7 +215,8 @@ def test_entries_that_name_no_page(ctx):
 
 
 # (The last ones pass 4096 sequences or entries of their rows.)
-@pytest.mark.parametrize("size", SIZES + [(4000, 2, 16, 9000), (4500, 3, 16, 15000), (3, 6000, 1, 20000)], ids=str)
+@pytest.mark.parametrize("size", SIZES + [(512, 5, 16, 3000), (513, 2, 16, 1500), (2049, 2, 16, 6000), (4000, 2, 16, 9000), (4500, 3, 16, 15000),
+                                         (3, 6000, 1, 20000)], ids=str)
 @pytest.mark.parametrize("tokens", [True, False], ids=["tokens", "chunks"])
 @pytest.mark.parametrize("seed", [0, 1, 2])
 def test_reserve(ctx, size, tokens, seed):
@@ -249,7 +250,7 @@ def test_reserve_behind_pages_in_use(ctx, n, n_pages):
             d.reserve([0] * n, [1] * n, True)
 
 
-@pytest.mark.parametrize("n", [1000, 4096, 4097, 9000])
+@pytest.mark.parametrize("n", [500, 1000, 4096, 4097, 9000])
 @pytest.mark.parametrize("groups", [1, 7, 499])
 def test_reserve_many_that_share(ctx, n, groups):
     """All sequences go on in a page that they share in groups: of each the last keeps it."""
