@@ -108,7 +108,7 @@ template <class How> __device__ __forceinline__ uint32_t doc_of(const How &m, in
 // products lose; of f16 rows, whose weights are rounded to 2^-11, EXP_CAP_F16).  Else as cap x P(x^2) /
 // Q(x^2), off by 2^-25.5 of itself at most over |x| <= TANH_END, from where on tanh is 1 to 2^-25:
 // degrees and coefficients by least squares reweighted to the least relative error, all of them
-// positive.  In slots of an instruction at full rate 11 and 17 a score.
+// positive.  In slots of an instruction at full rate 11 and 18 a score.
 //   (Measured and left out: where all scores of a wave are under half the cap, the polynomial of
 // tanh alone, 6 or 7: 107 us where one way alone takes 97; and what a row sees made its neighbours' last bits.)
 constexpr float TANH_END = 9.02f, EXP_CAP = 64.f, EXP_CAP_F16 = 1024.f;
@@ -116,7 +116,8 @@ constexpr float TANH_END = 9.02f, EXP_CAP = 64.f, EXP_CAP_F16 = 1024.f;
 __device__ __forceinline__ float over_cap(float sf, const ScoreArgs &how) { return __builtin_amdgcn_fmed3f(sf / how.cap, -0x1p120f, 0x1p120f); }
 template <bool BY_EXP> __device__ __forceinline__ float cap_score(const ScoreArgs &how, float s, float to_x) {
     if constexpr (!BY_EXP) {
-        const float x = __builtin_amdgcn_fmed3f(s * to_x, -TANH_END, TANH_END), u = x * x;
+        // (These two keep a NaN, which the median of three would make a bound.)
+        const float x = __builtin_elementwise_minimum(__builtin_elementwise_maximum(s * to_x, -TANH_END), TANH_END), u = x * x;
         const float p = fmaf(fmaf(fmaf(fmaf(u, 1.33190953e-08f, 2.05835024e-05f), u, 3.49403605e-03f), u, 1.33797193e-01f), u, 9.99999979e-01f);
         const float q = fmaf(fmaf(fmaf(fmaf(u, 7.76203024e-07f, 3.28309512e-04f), u, 2.58710791e-02f), u, 4.67130345e-01f), u, 1.f);
         return how.cap * x * (p * __builtin_amdgcn_rcpf(q));

@@ -271,6 +271,40 @@ def test_non_finite_values_where_nobody_looks(ctx, dtype, x16, hd, value):
                     assert np.isfinite(err).all() and err.max(initial=0) <= most, (which, b)
 
 
+@pytest.mark.parametrize("dtype", [ga.I8, ga.F16], ids=["i8", "f16"])
+@pytest.mark.parametrize("x16", [False, True], ids=["f32rows", "f16rows"])
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("tokens", [True, False], ids=["tokens", "chunks"])
+def test_a_nan_is_not_capped(ctx, dtype, x16, hd, tokens):
+    """A key that is no number makes the heads that see it NaN, one of q its own head, under any cap."""
+    H, hkv, page, bad = 4, 2, 16, 90
+    with Batch(ctx, [(130, 1), (120, 1), (60, 1)] if tokens else [(130, 5), (60, 40), (0, 20)], dtype, hkv, hd, page, row_start=not tokens) as bt:
+        bt.fill()
+        planes = bt.planes()
+        for b in range(3):
+            pg = bt.table[b, bad // page]
+            if pg < 0:
+                continue
+            if dtype == ga.F16:
+                planes[0][pg, bad % page, 1, 7] = np.nan
+            else:
+                planes[2][pg, 1, 0] = 255
+        for d, a in zip((bt.kv.k, bt.kv.v, bt.kv.k_exp, bt.kv.v_exp), planes):
+            ctx.set(d, a)
+        q = rows_of(bt.rng, (bt.n, H, hd), x16)
+        for cap in (0.0, 30.0, 500.0, 5000.0):
+            for slope in (None, np.full(H, 0.01, np.float32)):
+                q[:] = rows_of(bt.rng, (bt.n, H, hd), x16)
+                q[-1, 0, 3] = np.nan
+                got, _ = run(ctx, bt, q, None, dict(cap=cap, slope=slope), scale=hd ** -0.5)
+                want = np.zeros((bt.n, H), bool)
+                for b, (p0, r) in enumerate(bt.seqs):
+                    at = p0 + np.arange(r)
+                    want[bt.start[b]:bt.start[b] + r, H // 2:] = (at >= (bad if dtype == ga.F16 else bad // 16 * 16))[:, None]
+                want[-1, 0] = True
+                assert np.array_equal(np.isnan(got).all(2), want) and np.array_equal(np.isnan(got).any(2), want), (cap, slope is None)
+
+
 def test_masked_pages_that_are_not_there(ctx):
     """Pages before every document, and before the window, may be dropped."""
     for dtype in (ga.I8, ga.F16):
