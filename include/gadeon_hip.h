@@ -109,7 +109,7 @@ int gd_timer_stop(gd_ctx *ctx, float *ms);
  * until it is destroyed: it may outlive its context, and be launched on another one
  * as long as the workspace of the first is not in use at the same time (which GEMMs
  * of f32 rows or split K, gd_gdn_prefill, gd_kv_attn and gd_kv_attn_scored of split keys,
- * gd_kv_reserve of many entries and gd_kv_compact do). */
+ * gd_kv_reserve of many entries and gd_kv_compact of many pages do). */
 typedef struct gd_graph gd_graph;
 int gd_graph_begin(gd_ctx *ctx);
 int gd_graph_end(gd_ctx *ctx, gd_graph **out);
@@ -541,14 +541,15 @@ int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *seq, con
  * sequence's positions pos .. pos + rows - 1 (as far as the table goes) that names no page, or one
  * that others name too, gets a free page, counted once; a shared one's count falls by one, but
  * the last of the entries that share it, in the sequences' order, keeps it if no other than these
- * name it.  The k-th entry, sequence by sequence, gets the k-th lowest page free before the call.  A page replaced that holds
- * positions before pos goes into copies as (from, to): copies[2 n_seq] at most, *n_copies of them
- * (device memory both; the rest of copies stays), for gd_kv_copy_pages before rows are appended.
+ * name it.  The k-th entry, sequence by sequence, gets the k-th lowest page free before the call.
+ * A page replaced that holds positions before pos goes into copies as (from, to): copies[2 n_seq]
+ * at most, *n_copies of them (device memory both; the rest of copies stays), for gd_kv_copy_pages
+ * before rows are appended.
  *   pos_out[n_seq] (may be pos) is pos, or -1 where the free pages do not suffice for all
  * needs up to this sequence's last: it keeps what it had, and the calls that take pos_out leave
  * it alone (also where it needs none but keeps a page that a sequence before it shares).
- * Past 4096 sequences or entries of the rows (a bound of them: n_seq of single rows, else n_rows / page_size + 2 n_seq) it uses the
- * context workspace, 8 bytes a page and 24 an entry. */
+ * Past 4096 sequences or entries of the rows (a bound of them: n_seq of single rows, else
+ * n_rows / page_size + 2 n_seq) it uses the context workspace, 8 bytes a page and 24 an entry. */
 int gd_kv_reserve(gd_ctx *ctx, const gd_kv_pages *pages, const gd_seqs *seqs, int32_t *copies, int32_t *n_copies,
                   int32_t *pos_out);
 
