@@ -48,7 +48,8 @@ class Scores(C.Structure):
 
 class KVPages(C.Structure):
     """Who holds which page of the caches, arrays in device memory (gd_kv_pages)."""
-    _fields_ = [("refs", _vp), ("table", _vp), ("n_pages", _i64), ("n_seq", _i), ("max_pages", _i), ("page_size", _i)]
+    _fields_ = [("refs", _vp), ("table", _vp), ("n_pages", _i64), ("n_seq", _i), ("max_pages", _i), ("page_size", _i),
+                ("keep", _vp)]
 
 
 class StackConfig(C.Structure):

@@ -59,13 +59,16 @@ __global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, cons
 }
 
 // Workgroup (order i, EW entries): sequence seq[i] drops the pages that hold no position of
-// from[i] .. to[i] - 1, but for those that an order before it drops from the same sequence.
-__global__ __launch_bounds__(256) void k_release(Pages pg, const int32_t *seq, const int32_t *from, const int32_t *to) {
+// from[i] .. to[i] - 1, nor one of its first keep[seq[i]] before to[i], but for those that an order
+// before it drops from the same sequence.
+__global__ __launch_bounds__(256) void k_release(Pages pg, const int32_t *keep, const int32_t *seq, const int32_t *from,
+                                                 const int32_t *to) {
     const int i = blockIdx.x, b = seq[i];
     if ((uint32_t)b >= (uint32_t)pg.n_seq) return;
+    const int kept = keep ? keep[b] : 0;
     auto drops = [&](int i, int e) {
         const int64_t p = (int64_t)e * pg.P;
-        return !(p + pg.P > (from ? from[i] : 0) && p < to[i]);
+        return !((p + pg.P > (from ? from[i] : 0) || p < kept) && p < to[i]);
     };
     int32_t *row = pg.row(b);
     const int e0 = blockIdx.y * EW + threadIdx.x;
@@ -678,7 +681,8 @@ int check_pages(gd_ctx *ctx, const char *fn, const gd_kv_pages *pg) {
                pg->max_pages);
     GD_REQUIRE(ctx, pg->page_size > 0 && pg->page_size <= (1 << 24), "%s: page size %d", fn, pg->page_size);
     GD_REQUIRE(ctx, pg->refs && (pg->table || !pg->n_seq), "%s: null refs or table", fn);
-    GD_REQUIRE(ctx, ((uintptr_t)pg->refs | (uintptr_t)pg->table) % 4 == 0, "%s: refs and table must be 4-byte aligned", fn);
+    GD_REQUIRE(ctx, ((uintptr_t)pg->refs | (uintptr_t)pg->table | (uintptr_t)pg->keep) % 4 == 0,
+               "%s: refs, table and keep must be 4-byte aligned", fn);
     return GD_OK;
 }
 Pages pages_of(const gd_kv_pages *pg) {
@@ -721,7 +725,8 @@ extern "C" int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pg, const int32_t *
     GD_CHECK_CTX(ctx);
     if (!n || !pg->n_seq) return GD_OK;
     GD_HIP(ctx, hipSetDevice(ctx->device));
-    hipLaunchKernelGGL(k_release, dim3(n, gd_blocks(pg->max_pages, EW)), dim3(256), 0, ctx->stream, pages_of(pg), seq, from, to);
+    hipLaunchKernelGGL(k_release, dim3(n, gd_blocks(pg->max_pages, EW)), dim3(256), 0, ctx->stream, pages_of(pg), pg->keep,
+                       seq, from, to);
     GD_LAUNCHED(ctx, fn);
     return GD_OK;
 }

@@ -521,6 +521,8 @@ typedef struct gd_kv_pages {
     int32_t *table;              /* [n_seq][max_pages] */
     int64_t n_pages;
     int n_seq, max_pages, page_size;
+    const int32_t *keep;         /* [n_seq] or null: positions at the start of sequence b, keep[b] of them (sinks, a
+                                    prefix), whose pages gd_kv_release leaves it whatever `from` */
 } gd_kv_pages;
 
 /* For i < n (65536 at most; src, dst, len device memory): sequence dst[i] becomes a branch of
@@ -531,10 +533,11 @@ typedef struct gd_kv_pages {
 int gd_kv_fork(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *src, const int32_t *dst, const int32_t *len, int n);
 
 /* For i < n (65536 at most): sequence seq[i] keeps the pages that hold one of its positions
- * from[i] .. to[i]-1 (from null: 0 ..), and its other entries become -1, their pages' counts one
- * less: to = 0 ends it, to = its position takes back pages reserved behind, from = position - window
- * lets go what a window has passed.  A sequence may be named more than once; one outside [0, n_seq)
- * is left out. */
+ * from[i] .. to[i]-1 (from null: 0 ..), or, before to[i], one of its first pages->keep[seq[i]], and its
+ * other entries become -1, their pages' counts one less: to = 0 ends it, to = its position takes back pages
+ * reserved behind, from = position - window lets go what a window has passed.  (Attention sees sinks and a prefix
+ * whatever the window, and passes over pages that are not there: with either, keep is to hold the more of n_sink
+ * and prefix[b].)  A sequence may be named more than once; one outside [0, n_seq) is left out. */
 int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *seq, const int32_t *from, const int32_t *to, int n);
 
 /* Pages for the rows of a call (seqs' table is pages', with as many sequences): every entry of a
