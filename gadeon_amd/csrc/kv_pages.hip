@@ -25,73 +25,78 @@ __device__ __forceinline__ void count(const Pages &pg, int page, int by) {
 
 // ---------------------------------------------------------------- fork, release
 
-constexpr int EW = 1024;                         // entries of a workgroup
+constexpr int EW = 1024;                         // entries that a workgroup works on at once
+constexpr int MOST_WGS = 16384;                  // orders times parts of a row, but for a workgroup an order
 
-// Workgroup (order i, EW entries): row dst[i] takes over src[i]'s entries of the first len[i]
-// positions.  No source is the place of another order, so that rows are only read or only
+// Workgroup (order i, EW entries and every gridDim.y-th of them on): row dst[i] takes over src[i]'s entries
+// of the first len[i] positions.  No source is the place of another order, so that rows are only read or only
 // written; counts are whole numbers, whose order of addition shows nowhere.
 //   The counts bound many orders: 400 of 2048 entries add 138 000 of them in random lines in 11 us (with
-// the ends of 300 others 22 a pass, without any count 12); few are a launch and three loads, 2.4.
+// the ends of 300 others 22 a pass, without any count 12); few are a launch and three loads, 2.4.  Each
+// order looks at all of them, once a workgroup: 8192 rows of 1024 44 us, 65536 2.0 ms.
 __global__ __launch_bounds__(256) void k_fork(Pages pg, const int32_t *src, const int32_t *dst, const int32_t *len, int n) {
     const int i = blockIdx.x, s = src[i], d = dst[i], most = len[i];
     if ((uint32_t)s >= (uint32_t)pg.n_seq || (uint32_t)d >= (uint32_t)pg.n_seq) return;
     const int32_t *from = pg.row(s);
     int32_t *to = pg.row(d);
-    const int e0 = blockIdx.y * EW + threadIdx.x;
-    int old[EW / 256], now[EW / 256];
+    for (int y = blockIdx.y; y * EW < pg.max_pages; y += gridDim.y) {
+        const int e0 = y * EW + threadIdx.x;
+        int old[EW / 256], now[EW / 256];
 #pragma unroll
-    for (int x = 0; x < EW / 256; x++) {
-        const int e = e0 + 256 * x;
-        old[x] = e < pg.max_pages ? to[e] : -1;
-        now[x] = e < pg.max_pages && (int64_t)e * pg.P < most ? from[e] : -1;
-    }
-    bool bad = false;                            // (seen while the rows are on their way)
-    for (int j = threadIdx.x; j < n; j += 256) bad |= src[j] == d || (j > i && dst[j] == d);
-    if (__syncthreads_or(bad)) return;
+        for (int x = 0; x < EW / 256; x++) {
+            const int e = e0 + 256 * x;
+            old[x] = e < pg.max_pages ? to[e] : -1;
+            now[x] = e < pg.max_pages && (int64_t)e * pg.P < most ? from[e] : -1;
+        }
+        if (y == (int)blockIdx.y) {              // (seen while the rows are on their way)
+            bool bad = false;
+            for (int j = threadIdx.x; j < n; j += 256) bad |= src[j] == d || (j > i && dst[j] == d);
+            if (__syncthreads_or(bad)) return;
+        }
 #pragma unroll
-    for (int x = 0; x < EW / 256; x++) {
-        if (!pg.there(now[x])) now[x] = -1;
-        if (old[x] == now[x]) continue;
-        count(pg, old[x], -1);
-        count(pg, now[x], 1);
-        to[e0 + 256 * x] = now[x];
+        for (int x = 0; x < EW / 256; x++) {
+            if (!pg.there(now[x])) now[x] = -1;
+            if (old[x] == now[x]) continue;
+            count(pg, old[x], -1);
+            count(pg, now[x], 1);
+            to[e0 + 256 * x] = now[x];
+        }
     }
 }
 
-// Workgroup (order i, EW entries): sequence seq[i] drops the pages that hold no position of
-// from[i] .. to[i] - 1, nor one of its first keep[seq[i]] before to[i], but for those that an order
-// before it drops from the same sequence.
+// Workgroup (order i, EW entries and on, as k_fork): sequence seq[i] drops the pages that hold no position
+// of from[i] .. to[i] - 1, nor one of its first keep[seq[i]] before to[i].  Other orders may name the
+// sequence too: an entry is counted by the one that exchanges it, and none looks at another (8192 orders of
+// one sequence, rows of 1024, 13 us, 65536 42; each walking those before it 13.8 ms for 8192, and with the square of
+// their number).
 __global__ __launch_bounds__(256) void k_release(Pages pg, const int32_t *keep, const int32_t *seq, const int32_t *from,
                                                  const int32_t *to) {
     const int i = blockIdx.x, b = seq[i];
     if ((uint32_t)b >= (uint32_t)pg.n_seq) return;
     const int kept = keep ? keep[b] : 0;
-    auto drops = [&](int i, int e) {
+    const int first = from ? from[i] : 0, end = to[i];
+    auto drops = [&](int e) {
         const int64_t p = (int64_t)e * pg.P;
-        return !((p + pg.P > (from ? from[i] : 0) || p < kept) && p < to[i]);
+        return !((p + pg.P > first || p < kept) && p < end);
     };
     int32_t *row = pg.row(b);
-    const int e0 = blockIdx.y * EW + threadIdx.x;
-    int old[EW / 256];
+    for (int y = blockIdx.y; y * EW < pg.max_pages; y += gridDim.y) {
+        const int e0 = y * EW + threadIdx.x;
+        int old[EW / 256];
 #pragma unroll
-    for (int x = 0; x < EW / 256; x++) {
-        const int e = e0 + 256 * x;
-        old[x] = e < pg.max_pages && drops(i, e) ? row[e] : -1;
-    }
-    bool before = false;
-    for (int j = threadIdx.x; j < i; j += 256) before |= seq[j] == b;
-    if (__syncthreads_or(before))
-        for (int j = 0; j < i; j++)
-            if (seq[j] == b)
-#pragma unroll
-                for (int x = 0; x < EW / 256; x++)
-                    if (drops(j, e0 + 256 * x)) old[x] = -1;
-#pragma unroll
-    for (int x = 0; x < EW / 256; x++)
-        if (pg.there(old[x])) {
-            row[e0 + 256 * x] = -1;
-            count(pg, old[x], -1);
+        for (int x = 0; x < EW / 256; x++) {
+            const int e = e0 + 256 * x;
+            old[x] = e < pg.max_pages && drops(e) ? row[e] : -1;
         }
+#pragma unroll
+        for (int x = 0; x < EW / 256; x++)
+            if (pg.there(old[x])) {
+                int32_t was = old[x];
+                if (__hip_atomic_compare_exchange_strong(row + e0 + 256 * x, &was, -1, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                                         __HIP_MEMORY_SCOPE_AGENT))
+                    count(pg, old[x], -1);
+            }
+    }
 }
 
 // ---------------------------------------------------------------- reserve
@@ -699,6 +704,9 @@ int check_orders(gd_ctx *ctx, const char *fn, const gd_kv_pages *pg, int n, cons
     GD_REQUIRE(ctx, chunks < 65536 && n * chunks < MAX_WGS, "%s: %d orders over %d pages each", fn, n, pg->max_pages);
     return GD_OK;
 }
+dim3 order_grid(const gd_kv_pages *pg, int n) {
+    return dim3(n, std::min<unsigned>(gd_blocks(pg->max_pages, EW), std::max(1, MOST_WGS / n)));
+}
 
 }  // namespace
 
@@ -713,7 +721,7 @@ extern "C" int gd_kv_fork(gd_ctx *ctx, const gd_kv_pages *pg, const int32_t *src
     GD_CHECK_CTX(ctx);
     if (!n || !pg->n_seq) return GD_OK;
     GD_HIP(ctx, hipSetDevice(ctx->device));
-    hipLaunchKernelGGL(k_fork, dim3(n, gd_blocks(pg->max_pages, EW)), dim3(256), 0, ctx->stream, pages_of(pg), src, dst, len, n);
+    hipLaunchKernelGGL(k_fork, order_grid(pg, n), dim3(256), 0, ctx->stream, pages_of(pg), src, dst, len, n);
     GD_LAUNCHED(ctx, fn);
     return GD_OK;
 }
@@ -725,8 +733,7 @@ extern "C" int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pg, const int32_t *
     GD_CHECK_CTX(ctx);
     if (!n || !pg->n_seq) return GD_OK;
     GD_HIP(ctx, hipSetDevice(ctx->device));
-    hipLaunchKernelGGL(k_release, dim3(n, gd_blocks(pg->max_pages, EW)), dim3(256), 0, ctx->stream, pages_of(pg), pg->keep,
-                       seq, from, to);
+    hipLaunchKernelGGL(k_release, order_grid(pg, n), dim3(256), 0, ctx->stream, pages_of(pg), pg->keep, seq, from, to);
     GD_LAUNCHED(ctx, fn);
     return GD_OK;
 }

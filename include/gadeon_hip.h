@@ -525,7 +525,8 @@ typedef struct gd_kv_pages {
                                     prefix), whose pages gd_kv_release leaves it whatever `from` */
 } gd_kv_pages;
 
-/* For i < n (65536 at most; src, dst, len device memory): sequence dst[i] becomes a branch of
+/* For i < n (65536 at most, which takes 2 ms, with the square of n past some thousands; src, dst, len
+ * device memory): sequence dst[i] becomes a branch of
  * src[i]: its entries those of the pages that hold src's first len[i] positions, the others -1,
  * what it held before released.  No page is copied: gd_kv_reserve does that for the one that
  * either goes on in.  Left out is an order of a sequence outside [0, n_seq), one whose dst is a
