@@ -477,9 +477,15 @@ extern "C" int gd_kv_read(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, void *
     return GD_OK;
 }
 
+int gd_kv_attn_plain(gd_ctx *ctx, const char *fn, const gd_kv *kv, const gd_seqs *s, const void *q, int64_t q_stride,
+                     const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale, int window,
+                     int n_sink) {
+    const AttnArgs a{kv, s, q, q_stride, gate, gate_stride, out, x_dtype, n_head, scale};
+    return attn(ctx, fn, a, window, n_sink, Mask{window, window ? n_sink : 0}, true);
+}
+
 extern "C" int gd_kv_attn(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s, const void *q, int64_t q_stride,
                           const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
                           int window, int n_sink) {
-    const AttnArgs a{kv, s, q, q_stride, gate, gate_stride, out, x_dtype, n_head, scale};
-    return attn(ctx, "gd_kv_attn", a, window, n_sink, Mask{window, window ? n_sink : 0}, true);
+    return gd_kv_attn_plain(ctx, "gd_kv_attn", kv, s, q, q_stride, gate, gate_stride, out, x_dtype, n_head, scale, window, n_sink);
 }

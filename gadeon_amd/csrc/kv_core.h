@@ -229,6 +229,11 @@ Rows rows_of(const gd_kv *kv, const gd_seqs *s) {
 
 }  // namespace
 
+// gd_kv_attn in the name of `fn` (kv_cache.hip, which holds the kernels of plain scores).
+int gd_kv_attn_plain(gd_ctx *ctx, const char *fn, const gd_kv *kv, const gd_seqs *s, const void *q, int64_t q_stride,
+                     const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale, int window,
+                     int n_sink);
+
 // The template of head dim, cache type and row type that a call runs.
 #define GD_KV_PICK(kv, x_dtype, GO) \
     do { \

@@ -16,7 +16,7 @@ extern "C" int gd_kv_attn_scored(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *s,
     const AttnArgs a{kv, s, q, q_stride, gate, gate_stride, out, x_dtype, n_head, scale};
     const int window = how->window, sinks = window ? how->n_sink : 0;
     if (how->cap == 0.f && !how->slope && !how->first && !how->prefix)
-        return gd_kv_attn(ctx, kv, s, q, q_stride, gate, gate_stride, out, x_dtype, n_head, scale, window, how->n_sink);
+        return gd_kv_attn_plain(ctx, fn, kv, s, q, q_stride, gate, gate_stride, out, x_dtype, n_head, scale, window, how->n_sink);
     const ScoreArgs args{window, sinks, how->cap * LOG2E, how->slope, how->first, how->prefix};
     if (how->cap > 0.f && how->cap <= (x_dtype == GD_F32 ? EXP_CAP : EXP_CAP_F16))
         return attn(ctx, fn, a, window, how->n_sink, Scores<true>{args}, !how->prefix);
