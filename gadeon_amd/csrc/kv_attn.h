@@ -103,12 +103,15 @@ template <class How> __device__ __forceinline__ uint32_t doc_of(const How &m, in
     else return 0;
 }
 
-// Scores s capped: cap tanh(x), x = s to_x.  BY_EXP as cap - 2 cap / (1 + e^2x), off by some
-// 2^-23 of the cap: for caps that this is little of, up to EXP_CAP (what the scores' sums of
+// Scores s capped: cap tanh(x), x = s to_x.  BY_EXP as cap - 2 cap / (1 + e^2x), off by 2^-22 of
+// the cap, by 2^-21.3 where the reciprocal is a step off (x so little that e^2x is lost in 1 leaves six
+// half steps of 1): for caps that this is little of, up to EXP_CAP (what the scores' sums of
 // products lose; of f16 rows, whose weights are rounded to 2^-11, EXP_CAP_F16).  Else as cap x P(x^2) /
-// Q(x^2), off by 2^-25.5 of itself at most over |x| <= TANH_END, from where on tanh is 1 to 2^-25:
-// degrees and coefficients by least squares reweighted to the least relative error, all of them
-// positive.  In slots of an instruction at full rate 11 and 18 a score.
+// Q(x^2) over |x| <= TANH_END, from where on tanh is 1 to 2^-25: off by 2^-23.8 of itself in exact
+// arithmetic, by 2^-21.4 as formed, 2^-21 with the reciprocal a step off (twelve half steps of 32 bits at most,
+// 2^-20.4: one each of u, cap x and the last two products, two of each polynomial's last sums, three of the
+// reciprocal, one of the coefficients).  Degrees and coefficients by least squares reweighted to the least
+// relative error, all of them positive.  In slots of an instruction at full rate 11 and 18 a score.
 //   (Measured and left out: where all scores of a wave are under half the cap, the polynomial of
 // tanh alone, 6 or 7: 107 us where one way alone takes 97; and what a row sees made its neighbours' last bits.)
 constexpr float TANH_END = 9.02f, EXP_CAP = 64.f, EXP_CAP_F16 = 1024.f;

@@ -501,8 +501,8 @@ typedef struct gd_scores {
  * t >= first[row] where t <= p and (window == 0, t > p - window or t < n_sink), or t <
  * prefix[b]; out[h] = softmax(score) . v, gated, zeros where it sees nothing.  In all else as
  * gd_kv_attn (and its very results where cap is 0 and the arrays are null): rows, types,
- * alignment, workspace, recording.  Capped scores are off by some 2^-22 of the cap at caps up to
- * 64 (f16 rows of chunks: 1024), and of themselves beyond; a NaN stays one. */
+ * alignment, workspace, recording.  A score is capped to within 2^-20.4 of itself, in chunks (row_start not
+ * null) at caps up to 64 (f16 rows: 1024) to within 2^-21 of the cap; a NaN stays one. */
 int gd_kv_attn_scored(gd_ctx *ctx, const gd_kv *kv, const gd_seqs *seqs, const void *q, int64_t q_stride,
                       const void *gate, int64_t gate_stride, void *out, int x_dtype, int n_head, float scale,
                       const gd_scores *scores);
