@@ -685,8 +685,8 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     // V rows padded so that a transposing read's 32 lanes (MF 32: four rows of 32 dims, else
     // eight of 16) lie in 64 different banks.
     constexpr int KP = HD + 8, VP = HD + (MF == 32 ? 32 : 16), FD = 4;
-    // Dims of the results that LDS holds at once, with rows 16 bytes apart in its banks.
-    constexpr int OD = (size_t)PC * (HD + 4) * 4 <= sizeof(f16) * 2 * AK * (KP + VP) ? HD : HD / 2, OP = OD + 4;
+    constexpr int OP = HD + 4;                   // results' rows, 16 bytes apart in LDS's banks
+    static_assert((size_t)PC * OP * 4 <= sizeof(f16) * 2 * AK * (KP + VP), "results take the tiles' place");
     __shared__ union __attribute__((aligned(16))) {
         struct {
             f16 K[2][AK][KP], V[2][AK][VP];
@@ -1104,15 +1104,14 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
         now = next;
     }
     // Through LDS, each wave its own columns, so that a row is written, and its gate read, in whole lines.
-    constexpr int TPR = OD / 8, RPP = 64 / TPR, PASS = MF / RPP;     // lanes of a row, eight dims each; rows of a pass
+    constexpr int TPR = HD / 8, RPP = 64 / TPR, PASS = MF / RPP;     // lanes of a row, eight dims each; rows of a pass
     const int d = 8 * (lane % TPR), r0 = MF * w + lane / TPR;
-    T8 gates[HD / OD][PASS];
+    T8 gates[PASS];
     if (gate && nz == 1)
 #pragma unroll
-        for (int x = 0; x < HD / OD * PASS; x++) {
-            const int2 row = out_row[r0 + x % PASS * RPP];
-            if (row.y >= 0)
-                gates[x / PASS][x % PASS] = *(const T8 *)(gate + row.x * gate_stride + (row.y - (int64_t)row.x * H) * HD + x / PASS * OD + d);
+        for (int x = 0; x < PASS; x++) {
+            const int2 row = out_row[r0 + x * RPP];
+            if (row.y >= 0) gates[x] = *(const T8 *)(gate + row.x * gate_stride + (row.y - (int64_t)row.x * H) * HD + d);
         }
     if constexpr (MF == 16) l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -1123,39 +1122,34 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     }
     const float inv = nz > 1 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int o = 0; o < HD / OD; o++) {
+    for (int x = 0; x < DT; x++)
 #pragma unroll
-        for (int x = 0; x < OD / MF; x++)
+        for (int v = 0; v < NV; v += 4)
+            *(f32x4 *)&lds.O[MF * w + lc][MF * x + 2 * v + 4 * h] =
+                    f32x4{acc[x][v] * inv, acc[x][v + 1] * inv, acc[x][v + 2] * inv, acc[x][v + 3] * inv};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-            for (int v = 0; v < NV; v += 4) {
-                const Acc &a = acc[o * (OD / MF) + x];
-                *(f32x4 *)&lds.O[MF * w + lc][MF * x + 2 * v + 4 * h] = f32x4{a[v] * inv, a[v + 1] * inv, a[v + 2] * inv, a[v + 3] * inv};
-            }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-        for (int x = 0; x < PASS; x++) {
-            const int r = r0 + x * RPP;
-            const int64_t row = out_row[r].y;
-            if (row < 0) continue;
-            f32x4 y[2] = {*(const f32x4 *)&lds.O[r][d], *(const f32x4 *)&lds.O[r][d + 4]};
-            if (nz > 1) {
-                float *p = part.acc + (row * most + z) * HD + o * OD + d;
-                *(f32x4 *)p = y[0];
-                *(f32x4 *)(p + 4) = y[1];
-                continue;
-            }
-            if (gate)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float g = to_f32<T>(gates[o][x][e]);
-                    y[e / 4][e % 4] *= HL ? gd_sigmoid(g) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * g));
-                }
-            T8 res;
-#pragma unroll
-            for (int e = 0; e < 8; e++) res[e] = from_f32<T>(y[e / 4][e % 4]);
-            *(T8 *)(out + row * HD + o * OD + d) = res;
+    for (int x = 0; x < PASS; x++) {
+        const int r = r0 + x * RPP;
+        const int64_t row = out_row[r].y;
+        if (row < 0) continue;
+        f32x4 y[2] = {*(const f32x4 *)&lds.O[r][d], *(const f32x4 *)&lds.O[r][d + 4]};
+        if (nz > 1) {
+            float *p = part.acc + (row * most + z) * HD + d;
+            *(f32x4 *)p = y[0];
+            *(f32x4 *)(p + 4) = y[1];
+            continue;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (gate)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float g = to_f32<T>(gates[x][e]);
+                y[e / 4][e % 4] *= HL ? gd_sigmoid(g) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * g));
+            }
+        T8 res;
+#pragma unroll
+        for (int e = 0; e < 8; e++) res[e] = from_f32<T>(y[e / 4][e % 4]);
+        *(T8 *)(out + row * HD + d) = res;
     }
 }
 
