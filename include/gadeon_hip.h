@@ -526,19 +526,19 @@ typedef struct gd_kv_pages {
 } gd_kv_pages;
 
 /* For i < n (65536 at most, which takes 2 ms, with the square of n past some thousands; src, dst, len
- * device memory): sequence dst[i] becomes a branch of
- * src[i]: its entries those of the pages that hold src's first len[i] positions, the others -1,
- * what it held before released.  No page is copied: gd_kv_reserve does that for the one that
- * either goes on in.  Left out is an order of a sequence outside [0, n_seq), one whose dst is a
- * src of the call (its own too), and one whose dst a later order names. */
+ * device memory): sequence dst[i] becomes a branch of src[i]: its entries those of the pages that
+ * hold src's first len[i] positions, the others -1, what it held before released.  No page is copied:
+ * gd_kv_reserve does that for the one that either goes on in.  Left out is an order of a sequence outside
+ * [0, n_seq), one whose dst is a src of the call (its own too), and one whose dst a later order names. */
 int gd_kv_fork(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *src, const int32_t *dst, const int32_t *len, int n);
 
 /* For i < n (65536 at most): sequence seq[i] keeps the pages that hold one of its positions
- * from[i] .. to[i]-1 (from null: 0 ..), or, before to[i], one of its first pages->keep[seq[i]], and its
- * other entries become -1, their pages' counts one less: to = 0 ends it, to = its position takes back pages
- * reserved behind, from = position - window lets go what a window has passed.  (Attention sees sinks and a prefix
- * whatever the window, and passes over pages that are not there: with either, keep is to hold the more of n_sink
- * and prefix[b].)  A sequence may be named more than once; one outside [0, n_seq) is left out. */
+ * from[i] .. to[i]-1 (from null: 0 ..; where from is not before to none, but for a page that holds both from
+ * and to - 1), or, before to[i], one of its first pages->keep[seq[i]], and its other entries become -1,
+ * their pages' counts one less: to = 0 ends it, to = its position takes back pages reserved behind, from =
+ * position - window lets go what a window has passed.  (Attention sees sinks and a prefix whatever the window,
+ * and passes over pages that are not there: with either, keep is to hold the more of n_sink and prefix[b].)  A
+ * sequence may be named more than once; one outside [0, n_seq) is left out. */
 int gd_kv_release(gd_ctx *ctx, const gd_kv_pages *pages, const int32_t *seq, const int32_t *from, const int32_t *to, int n);
 
 /* Pages for the rows of a call (seqs' table is pages', with as many sequences): every entry of a

@@ -72,3 +72,15 @@ def test_windows_that_let_go(ctx, dtype, tokens, sinks, prefix):
         assert np.array_equal(attend(), want)
         ctx.gd_kv_release(C.byref(pages), bt.put(np.arange(B, dtype=I32)), None, bt.put(np.zeros(B, I32)), B)
         assert not ctx.get(pages.refs, bt.pages, I32).any()    # ended: the starts too
+
+
+def test_ranges_of_nothing(ctx):
+    """Where from is not before to: one page stays, if it holds both from and to - 1, and else none."""
+    for frm, to, left in ((5, 5, [0]), (5, 1, [0]), (16, 16, []), (17, 16, []), (40, 36, [2]), (40, 20, []), (0, 0, []), (9, -4, [])):
+        with Device(ctx, 1, 4, 16, 4) as d:
+            d.m.table[0], d.m.refs[:] = [3, 1, 2, 0], 1
+            d.set()
+            ctx.gd_kv_release(d.ref, *(d.put(np.array([x], I32)) for x in (0, frm, to)), 1)
+            d.m.release([0], [frm], [to])
+            d.same()
+            assert list(np.flatnonzero(d.m.table[0] >= 0)) == left
