@@ -55,9 +55,10 @@ template <int W> struct KeyBlocks {
     // Window of the query at `first` and on, keys up to `last`.
     __device__ __forceinline__ KeyBlocks(const Mask &m, uint32_t first, uint32_t last) {
         lo = m.window && first >= (uint32_t)m.window ? first - m.window + 1 : 0;
+        lo = min(lo, last + 1);                  // (a window behind the last key there may be: its block may hold sinks)
         sinks = min((uint32_t)m.sinks, lo);
         ns = (int)min((sinks + W - 1) / W, lo / W);
-        n = ns + (lo <= last ? (int)(last / W - lo / W + 1) : 0);
+        n = ns + (int)(last / W + 1 - lo / W);
     }
     __device__ __forceinline__ uint32_t start(int j) const { return (uint32_t)(j < ns ? j : j - ns + (int)(lo / W)) * W; }
     // Splits that these blocks are worked in: of `least` blocks or more, `most` at most.
@@ -71,11 +72,12 @@ template <int W> struct ScoredBlocks {
     int ns, n, from;                             // blocks of sinks, in all; the first of them
     __device__ __forceinline__ ScoredBlocks(const ScoreArgs &m, uint32_t first, uint32_t last, uint32_t prefix, uint32_t doc_) : doc(doc_) {
         lo = m.window && first >= (uint32_t)m.window ? first - m.window + 1 : 0;
+        lo = min(lo, last + 1);
         sinks = min(max((uint32_t)m.sinks, prefix), lo);
         from = (int)(doc / W);
         const uint32_t start = max(lo, doc);
         ns = sinks > doc ? (int)min((sinks + W - 1) / W, start / W) - from : 0;
-        n = ns + (start <= last ? (int)(last / W - start / W + 1) : 0);
+        n = ns + (start <= last + 1 ? (int)(last / W + 1 - start / W) : 0);
         far = (int)(start / W) - ns;
     }
     __device__ __forceinline__ uint32_t start(int j) const { return (uint32_t)(j < ns ? j + from : j + far) * W; }
