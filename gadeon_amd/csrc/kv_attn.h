@@ -24,8 +24,8 @@ struct ScoreArgs {
     const int32_t *first, *prefix;
 };
 // BY_EXP: there is a cap, and an exponential makes it (cap_score); prompt chunks are compiled for
-// that apart, as a branch to the other ways in their loop costs registers (1021 f32 rows after 3003 of 16
-// heads, capped and biased, 97 us; 106 with the branch).
+// that apart (1021 f32 rows after 3003 of 16 heads, capped and biased, 97 us as it was built, 106 with a branch to the
+// other ways in the loop; now 92, not capped 82, by the quotient 102).
 template <bool BY_EXP_> struct Scores : ScoreArgs {
     static constexpr bool SCORED = true, BY_EXP = BY_EXP_;
     using Tokens = Scores<false>;
@@ -153,7 +153,8 @@ struct Part {
 // (one token of 600 positions, us at 4 / 8 / 16 blocks: 40 heads of 128 11.5 / 12.3 / 14.8,
 // 24 of 256 on codes 14.3 / 16.5 / 21, on halves 16.3 / 18.9 / 26; 32 of up to 3000 behind an
 // append, heads of 128, 28.3 / 25.8 / 27.6), for rows 4 (2 rows behind 8191 of codes, at 2 / 4 /
-// 8: 17.3 / 17.3 / 24.1, 16 of 8 sequences 29.2 / 30.7 / 35.0; full chips alike).
+// 8: 17.3 / 17.3 / 24.1, 16 of 8 sequences 29.2 / 30.7 / 35.0; full chips alike; fewer where a
+// document leaves a unit fewer, Units::splits).
 constexpr int token_fewest(int hd) { return 1024 / hd; }
 constexpr int ROWS_FEWEST = 4;
 template <class How> __device__ __forceinline__ Blocks<32, How> token_blocks(const Rows &s, const How &mask, int b, int pos) {
@@ -216,7 +217,9 @@ template <class How> __device__ __forceinline__ int token_least(const Rows &s, c
 //   Two waves a SIMD or more, where halves of head dim 256 (32 KiB of them in flight a wave)
 // take 380 registers and one: us of two with spills / one, 24 heads on 4: one token of 600
 // positions 16.8 / 15.9, 64 of up to 8192 88 / 81, eight 27 / 33.  Codes of 128 at two / three,
-// 64 tokens of up to 8192, 40 heads on 8: 41 / 46; codes of 256, up to 4096, 37 / 51.
+// 64 tokens of up to 8192, 40 heads on 8: 41 / 46; codes of 256, up to 4096, 37 / 51.  Halves of 128 take 168
+// registers, three waves, and scored 173, two: 64 tokens of up to 8191 plain / biased / capped 85.5 / 87.3 / 87.2 us, 32
+// of up to 3000 22.1 / 25.2 / 24.6; codes (139 and 144 registers) 37.1 / 38.4 / 38.9 and 19.7 / 21.1 / 21.3.
 constexpr int TW = 4;                            // waves
 constexpr float LAZY = 7.f;                      // how far (log2) weights may pass the maximum they stand at
                                                  // (0, as ever: 1 to 6% more time)
@@ -579,12 +582,13 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
 // tile that some column does not see whole goes key by key: a mask, and where V holds a NaN or
 // infinity its finite part and, apart, which columns see the others (0 x NaN would reach them all).
 //   512 f16 rows behind 3584 positions of codes, 40 heads of 128 on 8: 67 us, 600 TFLOP/s;
-// 4096 under a window of 1024 127 us, 600; f32 rows (twice the products) of 24 heads of 256
+// 4096 under a window of 1024 124 us, 610; f32 rows (twice the products) of 24 heads of 256
 // on 4 530.  No unit of the CU is full (matrix cores 31% busy, vector ALUs 50%, LDS 31%):
 // with the registers of two waves a SIMD a wave's chain of staging, scores, weights and sums
 // is what lasts, 2.0 to 2.5 us for two waves' tiles, a lone one 1.7.  (f32 rows of 128 take all
-// 256 registers.)  Results leave through LDS, which takes the 16 bytes a lane and line that the
-// products' layout gives (20 mixed f32 chunks 115 -> 107 us, the window's 133 -> 127).  Measured and left out:
+// 256 registers; capped ones keep 21 more in memory on halves, 18 on those of odd pages, 3 on codes; by the
+// quotient or without a cap 5, 7 and none.)  Results leave through LDS, which takes the 16 bytes a lane and line that
+// the products' layout gives (calls of 20 mixed f32 chunks 115 -> 106 us, the window's 132 -> 124).  Measured and left out:
 // units of twice the columns, eight waves to a tile (codes of 256 219 -> 207 us, but f32 rows
 // of chunks 115 -> 122, under a window 133 -> 145); scores formed a tile ahead, beside the
 // weights of the last (143 -> 154, of 256 219 -> 261); tiles of 32 keys and three waves a
@@ -611,16 +615,20 @@ template <int PC, int AK, class How> struct Units {
     __device__ __forceinline__ Blocks<AK, How> blocks(const How &mask, int k, uint32_t doc = 0) const {
         return blocks_of<AK>(mask, pos + first(k), min(last_key(last(k)), cap - 1), prefix, doc);
     }
-    // Splits of each of the units: as the longest, the last, needs them.  (Scored: with the
-    // documents left out, so that it may have fewer blocks than these are made for.)
+    // Splits of each of the units: as the longest, the last, needs them.  Scored: with the
+    // documents left out, so that a unit may have fewer blocks than these are made for, down to one a split, its
+    // start and its partials (us so / keys left whole: 8 chunks of up to 200 rows behind up to 12000, documents of up to
+    // 200, 31.9 / 17.0, 4 of 256 behind 20000, of 300, 30.3 / 23.2; 256 rows behind 20000, of 10000, 87 / 362: a call's
+    // max_len says which).
     __device__ __forceinline__ int splits(const How &mask, int most, int least) const {
         const int longest = blocks(mask, n() - 1).n;
         return longest <= 1.4f * least ? 1 : min(most, (longest + least - 1) / least);
     }
     // Unit k from the last one back, with those first that a document gives over half the most
-    // keys, then a quarter (a workgroup of 20 tiles that starts last is the call's time; 4096 rows of 14
-    // documents, two and a half rounds of workgroups, 116 us in the rows' order, 108 so; of many short ones
-    // 50 and 53).
+    // keys, then a quarter: a workgroup of 20 tiles that starts last is the call's time.  Long documents gain by it
+    // and short ones lose, as every workgroup works the order out, and the documents are not known before (us in the
+    // rows' order / so, 40 heads of 128 on 8: 4096 rows, two and a half rounds of workgroups, of documents of up to
+    // 1500 109 / 100, 300 61.5 / 64.7, 100 53.4 / 59.7, 30 51.3 / 55.4; 3000 of up to 3000 93.4 / 91.5).
     __device__ __forceinline__ int by_document(const How &mask, int k, int r0) const {
         constexpr int MOST = 8;                  // units a lane
         const int lane = threadIdx.x & 63, last_unit = n() - 1;
@@ -1305,7 +1313,8 @@ int attn(gd_ctx *ctx, const char *fn, const AttnArgs &a, int window, int n_sink,
     // Blocks of keys of the longest row, workgroups of a split each, those that the chip
     // holds at once, and the most splits.  The keys are left whole, without a merge's
     // launch, where that is a few rounds of blocks a wave or the workgroups are many; how
-    // finely others are split, the kernels know (token_least, unit_least).
+    // finely others are split, the kernels know (token_least, unit_least).  (Measured below with
+    // plain scores, and taken for all.)
     const int64_t blocks = (keys + width - 1) / width;
     const int64_t slots = (tokens && hd == 256 && kv->dtype == GD_F16 ? 1 : 2) * cus, wgs = units * groups;    // (k_attn_tokens' registers)
     // Rows' partials cost a full chip some 15 us, and a split saves what lets the workgroups
