@@ -105,6 +105,13 @@ template <class How> __device__ __forceinline__ uint32_t doc_of(const How &m, in
     else return 0;
 }
 
+// A head's slope in units of log2, bounded where its products with distances stay numbers (next to a
+// score its next key weighs nothing long before; a NaN stays one).
+constexpr float STEEPEST = 0x1p96f;
+__device__ __forceinline__ float slope_of(const ScoreArgs &m, int head) {
+    return __builtin_elementwise_minimum(__builtin_elementwise_maximum(m.slope[head] * LOG2E, -STEEPEST), STEEPEST);
+}
+
 // Scores s capped: cap tanh(x), x = s to_x.  BY_EXP as cap - 2 cap / (1 + e^2x), off by 2^-22 of
 // the cap, by 2^-21.3 where the reciprocal is a step off (x so little that e^2x is lost in 1 leaves six
 // half steps of 1): for caps that this is little of, up to EXP_CAP (what the scores' sums of
@@ -386,7 +393,7 @@ __global__ __launch_bounds__(64 * TW) __attribute__((amdgpu_waves_per_eu(I8 || H
     // A score over its cap; the units of scores once they are capped, and once they are biased.
     float slope = 0.f, to_x = 0.f, capped = sf, unit = sf;
     if constexpr (How::SCORED) {
-        if (mask.slope) slope = mask.slope[h0 + min(col, nh - 1)] * LOG2E;
+        if (mask.slope) slope = slope_of(mask, h0 + min(col, nh - 1));
         to_x = over_cap(sf, mask);
         if (mask.cap > 0.f) capped = unit = 1.f;
         if (mask.slope) unit = 1.f;
@@ -759,7 +766,7 @@ void k_attn_rows(Cache c, Rows s, const T *q, int64_t q_stride, const T *gate, i
     uint32_t doc = 0, doc0 = 0, doc1 = 0, docs0 = 0, docs1 = 0;      // the column's; the unit's and the wave's first and last
     float slope = 0.f;
     if constexpr (How::SCORED) {
-        if (mask.slope) slope = mask.slope[head] * LOG2E;
+        if (mask.slope) slope = slope_of(mask, head);
         if (mask.first) {
             doc = doc_of(mask, n);
             uint32_t a = doc, z = doc;           // (a wave's columns, then all rows of the unit, of which it has some)

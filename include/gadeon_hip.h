@@ -489,7 +489,8 @@ typedef struct gd_scores {
     float cap;                   /* > 0 (1e-30 .. 1e30): a score s becomes cap tanh(s / cap); 0: stays */
     int window, n_sink;          /* as gd_kv_attn's */
     const float *slope;          /* [n_head] or null: slope[h] |p - t| is taken off the (capped) score of
-                                    the query at position p and the key at t */
+                                    the query at position p and the key at t (infinite, or over 5e28: the
+                                    nearest key is left, or, negative, the farthest) */
     const int32_t *first;        /* [n_rows] or null: a row sees no position before first[row] (where its
                                     document starts; one past its own position, as INT32_MAX: it sees none) */
     const int32_t *prefix;       /* [n_seq] or null: every row of sequence b sees the positions t <
